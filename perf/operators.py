@@ -351,15 +351,17 @@ def work(case):
     if op in ("lookup", "embed"):
         n, h, b = case["tokens"], case["hidden"], DTYPES[case["dtype"]].itemsize
         rows = -(-case["vocab"] // case["shards"])
-        # tokens are spread over the vocabulary's logarithm: the share that falls into this shard, and the rows it hits
-        low, high = math.log(rows * case["at"] + 1), math.log(min(case["vocab"], rows * (case["at"] + 1)) + 1)
-        here = n * (1 - case["pad"]) * (high - low) / math.log(case["vocab"] + 1)
-        if rows * case["at"] <= 3 < rows * (case["at"] + 1):
-            here += n * case["pad"]
-        moved = 8 * n + b * h * (min(here, rows) + n)
+        # row r is a token's with probability ln((r+2)/(r+1)) / ln(vocab+1): the tokens of this shard, and the rows they hit
+        first = rows * case["at"]
+        r = torch.arange(first, max(first, min(case["vocab"], first + rows)), dtype=torch.float64)
+        share = (1 - case["pad"]) * torch.log1p(1 / (r + 1)) / math.log(case["vocab"] + 1)
+        share += case["pad"] * (r == min(3, case["vocab"] - 1))
+        here, hit = n * float(share.sum()), float((1 - (1 - share) ** n).sum())
+        moved = 8 * n + b * h * (hit + n)
         if op == "lookup":
             return {"bytes": moved, "flops": h * here}
-        moved += b * h * here + DTYPES[case["grad"]].itemsize * h * rows * (2 if case["accumulate"] else 1)
+        # an accumulated gradient changes where a token is; a new one is written whole
+        moved += b * h * here + DTYPES[case["grad"]].itemsize * h * (2 * hit if case["accumulate"] else rows)
         return {"bytes": moved, "flops": 2 * h * here}
     n, b = case["rows"] * case["vocab"], DTYPES[case["dtype"]].itemsize
     moved = n * b + case["rows"] * (8 + 12 + 12 * case["top"])

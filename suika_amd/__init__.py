@@ -19,6 +19,7 @@ from .plan import PlanOptions, ReshardPlan, SlotSpec
 from ._lib import PlanError, ReshardError
 from .checkpoint import checkpoint_load, checkpoint_save, migration_load, migration_save
 from .handoff import HandoffError, dummy_migration_IPC_state_dict
+from .optim import ShardAdamW, clip_grads, counted_names, grad_norm, grad_square_sum
 
 __all__ = [
     "CHUNK", "QKV_HEADS", "VOCAB_PAD", "ParamLayout", "TensorMeta", "TransferOp",
@@ -28,4 +29,5 @@ __all__ = [
     "split_model_and_optimizer_state_dict", "PlanOptions", "ReshardPlan", "SlotSpec",
     "PlanError", "ReshardError", "checkpoint_save", "checkpoint_load", "migration_save",
     "migration_load", "forcefully_free_tensor", "cuda_gc", "dummy_migration_IPC_state_dict", "HandoffError",
+    "ShardAdamW", "clip_grads", "counted_names", "grad_norm", "grad_square_sum",
 ]

@@ -77,6 +77,10 @@ EXPORTED_SYMBOLS = (
     "sr_handoff_free",
     "sr_handoff_open",
     "sr_handoff_close",
+    "sr_square_sum_workspace",
+    "sr_square_sum",
+    "sr_clip",
+    "sr_adamw",
 )
 
 # Largest hand-off allocation (SR_HANDOFF_MAX_BYTES, include/suika_handoff.h).

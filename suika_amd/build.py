@@ -8,11 +8,13 @@ present.  Sources: ``reshard.hip`` (plan builder and kernels),
 and its lowering to region moves), ``handoff.cpp`` (exported device
 allocations for the same-GPU state hand-off between processes), ``stage.cpp``
 (sources in host memory packed into device buffers, results copied back to
-host memory, through pinned windows and a host thread pool).
+host memory, through pinned windows and a host thread pool), ``optim.hip``
+(gradient norm, clipping and the AdamW update of a share's state).
 
-``build_host`` compiles ``host_bind.cpp`` into ``suika_amd/lib/_suika_host.so``,
-the CPython extension (on torch's C++ API) that does the drop-in operator's
-per-tensor host work; it is a plain ``g++`` line against the installed torch
+``build_host`` compiles ``host_bind.cpp`` and ``step_bind.cpp`` into
+``suika_amd/lib/_suika_host.so``, the CPython extension (on torch's C++ API)
+that does the drop-in operator's per-tensor host work and takes the
+training-step operators' tensors; it is a plain ``g++`` line against the installed torch
 and the library (whose sr_lower and sr_plan_create it calls), found beside it.
 """
 from __future__ import annotations
@@ -27,11 +29,12 @@ from typing import Tuple
 PKG_DIR = Path(__file__).resolve().parent
 REPO_DIR = PKG_DIR.parent
 SOURCES = [PKG_DIR / "csrc" / "reshard.hip", PKG_DIR / "csrc" / "schedule.cpp",
-           PKG_DIR / "csrc" / "lower.cpp", PKG_DIR / "csrc" / "handoff.cpp", PKG_DIR / "csrc" / "stage.cpp"]
+           PKG_DIR / "csrc" / "lower.cpp", PKG_DIR / "csrc" / "handoff.cpp", PKG_DIR / "csrc" / "stage.cpp",
+           PKG_DIR / "csrc" / "optim.hip"]
 INCLUDE = REPO_DIR / "include"
 LIB_DIR = PKG_DIR / "lib"
 LIB = LIB_DIR / "libsuika_reshard.so"
-HOST_SRC = PKG_DIR / "csrc" / "host_bind.cpp"
+HOST_SOURCES = [PKG_DIR / "csrc" / "host_bind.cpp", PKG_DIR / "csrc" / "step_bind.cpp"]
 HOST_LIB = LIB_DIR / "_suika_host.so"
 
 ARCH = "gfx950"
@@ -124,9 +127,9 @@ def build_host(verbose: bool = False, out: Path = HOST_LIB) -> Path:
            "-DTORCH_EXTENSION_NAME=_suika_host",
            *[f"-I{p}" for p in include_paths()], f"-I{sysconfig.get_paths()['include']}",
            # the library's TensorMeta arithmetic (sr_meta.h) and the headers it uses
-           "-D__HIP_PLATFORM_AMD__", f"-I{INCLUDE}", f"-I{HOST_SRC.parent}",
+           "-D__HIP_PLATFORM_AMD__", f"-I{INCLUDE}", f"-I{HOST_SOURCES[0].parent}",
            f"-I{Path(os.environ.get('ROCM_PATH', '/opt/rocm')) / 'include'}",
-           str(HOST_SRC), *[f"-L{p}" for p in libdirs], *[f"-Wl,-rpath,{p}" for p in libdirs],
+           *map(str, HOST_SOURCES), *[f"-L{p}" for p in libdirs], *[f"-Wl,-rpath,{p}" for p in libdirs],
            "-lc10", "-ltorch", "-ltorch_cpu", "-ltorch_python",
            # the library itself (sr_lower, sr_plan_create), found beside the extension
            f"-L{LIB_DIR}", "-lsuika_reshard", "-Wl,-rpath,$ORIGIN", "-o", str(tmp)]
@@ -184,8 +187,8 @@ def build_sanitized(verbose: bool = False, out_dir: Path = SANITIZE_DIR) -> Tupl
         str(_llvm() / "bin" / "clang++"), *san, "-fsanitize=address,undefined", "-std=c++17", "-fPIC", "-shared",
         "-Wno-braced-scalar-init", f"-D_GLIBCXX_USE_CXX11_ABI={abi}", "-DTORCH_API_INCLUDE_EXTENSION_H",
         "-DTORCH_EXTENSION_NAME=_suika_host", *[f"-I{p}" for p in include_paths()],
-        f"-I{sysconfig.get_paths()['include']}", "-D__HIP_PLATFORM_AMD__", f"-I{INCLUDE}", f"-I{HOST_SRC.parent}",
-        f"-I{Path(os.environ.get('ROCM_PATH', '/opt/rocm')) / 'include'}", str(HOST_SRC),
+        f"-I{sysconfig.get_paths()['include']}", "-D__HIP_PLATFORM_AMD__", f"-I{INCLUDE}", f"-I{HOST_SOURCES[0].parent}",
+        f"-I{Path(os.environ.get('ROCM_PATH', '/opt/rocm')) / 'include'}", *map(str, HOST_SOURCES),
         *[f"-L{p}" for p in libdirs], *[f"-Wl,-rpath,{p}" for p in libdirs],
         "-lc10", "-ltorch", "-ltorch_cpu", "-ltorch_python", f"-L{out_dir}", "-lsuika_reshard",
         "-Wl,-rpath,$ORIGIN", "-o", str(host)]))

@@ -58,6 +58,7 @@
 #include <unordered_map>
 #include <vector>
 
+#include "host_errors.h"
 #include "sr_meta.h"
 #include "suika_planner.h"
 #include "suika_reshard.h"
@@ -1511,35 +1512,7 @@ py::list device_views(uint64_t base, py::list views, int64_t device_index) {
 
 namespace {
 
-PyObject* lib_exception(const char* name) {
-  py::object mod = py::module_::import("suika_amd._lib");
-  py::object cls = mod.attr(name);
-  return cls.release().ptr();   // a new reference, kept for the process
-}
-
-const char* status_name(int rc) {
-  switch (rc) {
-    case SR_OK: return "SR_OK";
-    case SR_EINVAL: return "SR_EINVAL";
-    case SR_EBOUNDS: return "SR_EBOUNDS";
-    case SR_EALIGN: return "SR_EALIGN";
-    case SR_EOVERLAP: return "SR_EOVERLAP";
-    case SR_EHIP: return "SR_EHIP";
-    case SR_ENOMEM: return "SR_ENOMEM";
-    case SR_EDTYPE: return "SR_EDTYPE";
-    default: return nullptr;
-  }
-}
-
-// "<what>: <status>: <message>", as suika_amd._lib.check words it.
-[[noreturn]] void raise_status(int rc, const char* what, const std::string& msg) {
-  static PyObject* plan_error = lib_exception("PlanError");
-  static PyObject* reshard_error = lib_exception("ReshardError");
-  const char* name = status_name(rc);
-  const std::string text = std::string(what) + ": " + (name ? name : std::to_string(rc)) + ": " + msg;
-  PyErr_SetString(rc == SR_EHIP || rc == SR_ENOMEM ? reshard_error : plan_error, text.c_str());
-  throw py::error_already_set();
-}
+using suika_host::raise_status;
 
 // "#<id>" in a library message -> the tensor's name.
 std::string with_names(const char* msg, py::list names) {
@@ -1811,4 +1784,5 @@ PYBIND11_MODULE(_suika_host, m) {
         py::arg("piece_dtype"), py::arg("gather") = false, py::arg("stream") = 0, py::arg("dst_part") = py::none(),
         py::arg("ahead") = py::none(), py::arg("host_ok") = false,
         py::arg("encoding") = static_cast<const Encoded*>(nullptr));
+  suika_host::bind_step(m);
 }

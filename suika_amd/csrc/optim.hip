@@ -1,0 +1,569 @@
+// optim.hip -- the optimizer's part of a training step over a share's
+// tensors (C ABI in include/suika_step.h): the sum of the gradients' squares,
+// clipping, and the AdamW update.
+//
+// Every call works on a list of arrays of any length.  The list goes to the
+// kernels by value, in tables of up to 4 KB of kernel arguments, so nothing is
+// uploaded and nothing is kept between calls; a longer list takes several
+// launches.  Arrays are cut into chunks of a fixed number of elements, numbered
+// through the table; a wave finds the array of a chunk by comparing all first
+// chunks at once, an entry a lane.
+
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+#include <new>
+#include <vector>
+
+#include "suika_step.h"
+#include "sr_step.h"
+
+namespace {
+
+using namespace sr_step;
+
+constexpr int kThreads = 256;
+
+// A table of 4 KB, less the 256 bytes of arguments that the compiler adds.
+constexpr size_t kTableBytes = 3832;
+
+// The entry of a table that chunk `c` lies in: the last one whose first chunk
+// is not behind it.  `first` rises strictly (empty arrays are left out).
+__device__ __forceinline__ int entry_of(const uint32_t* first, int count, uint32_t c) {
+  int found = 0;
+  for (int base = 0; base < count; base += kWave) {
+    const int i = base + int(threadIdx.x % kWave);
+    found += __popcll(__ballot(i < count && first[i] <= c));
+  }
+  return __builtin_amdgcn_readfirstlane(found - 1);
+}
+
+// ------------------------------------------------------------ sum of squares
+
+// sum += x^2 over all elements, in 64 bits: squares of f32 values neither
+// overflow nor vanish there, and each product of two 24-bit numbers is exact.
+constexpr int kSumEntries = 188;
+constexpr uint32_t kSumChunk = 16384;    // elements
+constexpr uint32_t kSumBlocks = 2048;    // workgroups of one launch at most
+
+struct SumTable {
+  uint64_t data[kSumEntries];
+  uint64_t n[kSumEntries];
+  uint32_t first[kSumEntries];
+  int32_t count;
+  uint32_t chunks;
+};
+static_assert(sizeof(SumTable) <= kTableBytes, "kernel arguments");
+
+__device__ __forceinline__ double block_sum(double x) {
+  __shared__ double part[kThreads / kWave];
+  x = wave_sum(x);
+  if (threadIdx.x % kWave == 0) part[threadIdx.x / kWave] = x;
+  __syncthreads();
+  double s = 0;
+#pragma unroll
+  for (int i = 0; i < kThreads / kWave; ++i) s += part[i];
+  return s;
+}
+
+template <typename T>
+__global__ __launch_bounds__(kThreads) void square_sum_kernel(SumTable t, double* partial) {
+  constexpr int N = 16 / sizeof(T);
+  constexpr int kBatch = 4;
+  double sum[4] = {0, 0, 0, 0};
+  for (uint32_t c = blockIdx.x; c < t.chunks; c += gridDim.x) {
+    const int i = entry_of(t.first, t.count, c);
+    const uint64_t at = uint64_t(c - t.first[i]) * kSumChunk;
+    const uint64_t left = t.n[i] - at;
+    const uint32_t n = left < kSumChunk ? uint32_t(left) : kSumChunk;
+    const T* p = reinterpret_cast<const T*>(t.data[i]) + at;
+    uint32_t e = threadIdx.x * N;
+    for (; e + (kBatch - 1) * kThreads * N + N <= n; e += kBatch * kThreads * N) {
+      float x[kBatch][N];
+#pragma unroll
+      for (int b = 0; b < kBatch; ++b) load<T, N>(p + e + b * kThreads * N, x[b]);
+#pragma unroll
+      for (int b = 0; b < kBatch; ++b)
+#pragma unroll
+        for (int k = 0; k < N; ++k) sum[k & 3] = fma(double(x[b][k]), double(x[b][k]), sum[k & 3]);
+    }
+    for (; e + N <= n; e += kThreads * N) {
+      float x[N];
+      load<T, N>(p + e, x);
+#pragma unroll
+      for (int k = 0; k < N; ++k) sum[k & 3] = fma(double(x[k]), double(x[k]), sum[k & 3]);
+    }
+    const uint32_t rest = n - n % N;     // the elements behind the last whole vector, one a lane
+    if (threadIdx.x < n % N) {
+      const double x = double(float(p[rest + threadIdx.x]));
+      sum[0] = fma(x, x, sum[0]);
+    }
+  }
+  const double s = block_sum((sum[0] + sum[1]) + (sum[2] + sum[3]));
+  if (threadIdx.x == 0) partial[blockIdx.x] = s;
+}
+
+__global__ __launch_bounds__(kThreads) void finish_sum_kernel(const double* partial, uint32_t count, double* sum,
+                                                              float* norm) {
+  double x = 0;
+  for (uint32_t i = threadIdx.x; i < count; i += kThreads) x += partial[i];
+  x = block_sum(x);
+  if (threadIdx.x == 0) {
+    *sum = x;
+    if (norm) *norm = float(sqrt(x));
+  }
+}
+
+// ------------------------------------------------------------------ clipping
+
+constexpr int kClipEntries = 128;
+constexpr uint32_t kClipChunk = 4096;
+
+struct ClipTable {
+  uint64_t src[kClipEntries];
+  uint64_t dst[kClipEntries];
+  uint64_t n[kClipEntries];
+  uint32_t first[kClipEntries];
+  int32_t count;
+  float max_norm;
+  const double* square_sum;
+  float* norm;
+};
+static_assert(sizeof(ClipTable) <= kTableBytes, "kernel arguments");
+
+// min(1, max_norm / (norm + 1e-6)); NaN stays NaN.
+__device__ __forceinline__ float clip_factor(double square_sum, float max_norm) {
+  const double f = double(max_norm) / (sqrt(square_sum) + 1e-6);
+  return f > 1.0 ? 1.0f : float(f);
+}
+
+template <typename S, typename D>
+__global__ __launch_bounds__(kThreads) void clip_kernel(ClipTable t) {
+  constexpr int N = 4;
+  constexpr int kBatch = kClipChunk / (kThreads * N);
+  const double q = *t.square_sum;
+  if (t.norm && blockIdx.x == 0 && threadIdx.x == 0) *t.norm = float(sqrt(q));
+  if (t.count == 0) return;
+  const uint32_t c = blockIdx.x;
+  const int i = entry_of(t.first, t.count, c);
+  const float f = clip_factor(q, t.max_norm);
+  if (f == 1.0f && t.dst[i] == t.src[i]) return;
+  const uint64_t at = uint64_t(c - t.first[i]) * kClipChunk;
+  const uint64_t left = t.n[i] - at;
+  const uint32_t n = left < kClipChunk ? uint32_t(left) : kClipChunk;
+  const S* src = reinterpret_cast<const S*>(t.src[i]) + at;
+  D* dst = reinterpret_cast<D*>(t.dst[i]) + at;
+  float x[kBatch][N];
+#pragma unroll
+  for (int b = 0; b < kBatch; ++b) {
+    const uint32_t e = (b * kThreads + threadIdx.x) * N;
+    if (e + N <= n) load<S, N>(src + e, x[b]);
+  }
+#pragma unroll
+  for (int b = 0; b < kBatch; ++b) {
+    const uint32_t e = (b * kThreads + threadIdx.x) * N;
+    if (e + N <= n) {
+#pragma unroll
+      for (int k = 0; k < N; ++k) x[b][k] *= f;
+      store<D, N>(dst + e, x[b]);
+    } else {
+      for (uint32_t k = e; k < n; ++k) dst[k] = D(float(src[k]) * f);
+    }
+  }
+}
+
+// --------------------------------------------------------------------- AdamW
+
+constexpr int kAdamEntries = 78;
+constexpr uint32_t kAdamChunk = 2048;
+
+struct AdamTable {
+  uint64_t weight[kAdamEntries];
+  uint64_t exp_avg[kAdamEntries];
+  uint64_t exp_avg_sq[kAdamEntries];
+  uint64_t param[kAdamEntries];
+  uint64_t grad[kAdamEntries];
+  uint32_t first[kAdamEntries];
+  uint32_t tail[kAdamEntries];    // elements of the last chunk
+  int32_t count;
+  uint32_t chunks;
+  const double* square_sum;
+  float max_norm;
+  float decay;                    // 1 - lr * weight_decay
+  float beta1, rest1, beta2, rest2;
+  float step_size;                // lr / (1 - beta1^step)
+  float root_scale;               // 1 / sqrt(1 - beta2^step)
+  float eps;
+};
+static_assert(sizeof(AdamTable) <= kTableBytes, "kernel arguments");
+
+struct NoCopy {};
+
+// One chunk a workgroup, all of a lane's loads before its first store.
+// W: type of the weight, M: of the moments, G: of the gradient, P: of the
+// weight's copy, or NoCopy.
+template <typename W, typename M, typename G, typename P>
+__global__ __launch_bounds__(kThreads) void adamw_kernel(AdamTable t) {
+  constexpr int N = 4;
+  constexpr int kBatch = kAdamChunk / (kThreads * N);
+  const uint32_t c = blockIdx.x;
+  const int i = entry_of(t.first, t.count, c);
+  const uint32_t next = i + 1 < t.count ? t.first[i + 1] : t.chunks;
+  const uint32_t n = c + 1 == next ? t.tail[i] : kAdamChunk;
+  const uint64_t at = uint64_t(c - t.first[i]) * kAdamChunk;
+  W* weight = reinterpret_cast<W*>(t.weight[i]) + at;
+  M* exp_avg = reinterpret_cast<M*>(t.exp_avg[i]) + at;
+  M* exp_avg_sq = reinterpret_cast<M*>(t.exp_avg_sq[i]) + at;
+  const G* grad = reinterpret_cast<const G*>(t.grad[i]) + at;
+
+  float g[kBatch][N], w[kBatch][N], m[kBatch][N], v[kBatch][N];
+#pragma unroll
+  for (int b = 0; b < kBatch; ++b) {
+    const uint32_t e = (b * kThreads + threadIdx.x) * N;
+    if (e + N <= n) {
+      load<G, N>(grad + e, g[b]);
+      load<W, N>(weight + e, w[b]);
+      load<M, N>(exp_avg + e, m[b]);
+      load<M, N>(exp_avg_sq + e, v[b]);
+    }
+  }
+  const float factor = t.square_sum ? clip_factor(*t.square_sum, t.max_norm) : 1.0f;
+  auto update = [&](float gi, float& wi, float& mi, float& vi) {
+    gi *= factor;
+    mi = fmaf(mi, t.beta1, gi * t.rest1);
+    vi = fmaf(vi, t.beta2, gi * gi * t.rest2);
+    const float root = fmaf(sqrtf(vi), t.root_scale, t.eps);
+    wi = fmaf(wi, t.decay, -(t.step_size * mi) / root);
+  };
+#pragma unroll
+  for (int b = 0; b < kBatch; ++b) {
+    const uint32_t e = (b * kThreads + threadIdx.x) * N;
+    if (e + N <= n) {
+#pragma unroll
+      for (int k = 0; k < N; ++k) update(g[b][k], w[b][k], m[b][k], v[b][k]);
+      store<W, N>(weight + e, w[b]);
+      store<M, N>(exp_avg + e, m[b]);
+      store<M, N>(exp_avg_sq + e, v[b]);
+      if constexpr (!__is_same(P, NoCopy)) store<P, N>(reinterpret_cast<P*>(t.param[i]) + at + e, w[b]);
+    } else {
+      for (uint32_t k = e; k < n; ++k) {
+        float wi = float(weight[k]), mi = float(exp_avg[k]), vi = float(exp_avg_sq[k]);
+        update(float(grad[k]), wi, mi, vi);
+        weight[k] = W(wi);
+        exp_avg[k] = M(mi);
+        exp_avg_sq[k] = M(vi);
+        if constexpr (!__is_same(P, NoCopy)) (reinterpret_cast<P*>(t.param[i]) + at)[k] = P(wi);
+      }
+    }
+  }
+}
+
+// ---------------------------------------------------------------------- host
+
+bool float_dtype(int32_t dt) { return dt == SR_DT_F32 || dt == SR_DT_BF16 || dt == SR_DT_F16; }
+
+int check_arrays(const char* who, const sr_array* a, int32_t count) {
+  if (count < 0 || (count > 0 && a == nullptr)) return fail(SR_EINVAL, "%s: no arrays", who);
+  for (int32_t i = 0; i < count; ++i) {
+    if (a[i].reserved != 0) return fail(SR_EINVAL, "%s: arrays[%d].reserved is not 0", who, i);
+    if (!float_dtype(a[i].dtype)) return fail(SR_EDTYPE, "%s: arrays[%d]: dtype %d", who, i, a[i].dtype);
+    if (a[i].n > SR_STEP_MAX_ELEMENTS)
+      return fail(SR_EBOUNDS, "%s: arrays[%d] has %llu elements", who, i, (unsigned long long)a[i].n);
+    if (a[i].n && a[i].data == nullptr) return fail(SR_EINVAL, "%s: arrays[%d] is null", who, i);
+    if (reinterpret_cast<uintptr_t>(a[i].data) % sr_internal::dtype_size(a[i].dtype))
+      return fail(SR_EALIGN, "%s: arrays[%d] is not aligned to its elements", who, i);
+  }
+  return SR_OK;
+}
+
+uint64_t bytes_of(const sr_array& a) { return a.n * sr_internal::dtype_size(a.dtype); }
+
+// Memory that a call reads or writes.
+struct Span {
+  uintptr_t from, to;
+  bool written;
+};
+
+void add_span(std::vector<Span>& spans, const void* p, uint64_t bytes, bool written) {
+  const uintptr_t a = reinterpret_cast<uintptr_t>(p);
+  if (p && bytes) spans.push_back({a, a + bytes, written});
+}
+
+// Whether anything written overlaps anything else.
+bool clash(std::vector<Span>& spans) {
+  std::sort(spans.begin(), spans.end(), [](const Span& a, const Span& b) { return a.from < b.from; });
+  uintptr_t any = 0, written = 0;    // ends of what came before
+  for (const Span& s : spans) {
+    if (s.from < (s.written ? any : written)) return true;
+    any = std::max(any, s.to);
+    if (s.written) written = std::max(written, s.to);
+  }
+  return false;
+}
+
+// Most chunks of one launch: the grid's threads stay below 2^32.
+constexpr uint32_t kMostChunks = 1u << 23;
+
+constexpr int32_t kFloatTypes[3] = {SR_DT_F32, SR_DT_BF16, SR_DT_F16};
+
+// Launches of a list: the arrays of one type at a time, kSumEntries a table.
+template <typename F>
+int sum_launches(const sr_array* a, int32_t count, F&& launch) {
+  for (int32_t dt : kFloatTypes) {
+    SumTable t;
+    t.count = 0;
+    t.chunks = 0;
+    for (int32_t i = 0; i < count; ++i) {
+      if (a[i].dtype != dt || a[i].n == 0) continue;
+      if (t.count == kSumEntries) {
+        if (int rc = launch(dt, t)) return rc;
+        t.count = 0;
+        t.chunks = 0;
+      }
+      const int k = t.count++;
+      t.data[k] = reinterpret_cast<uint64_t>(a[i].data);
+      t.n[k] = a[i].n;
+      t.first[k] = t.chunks;
+      t.chunks += uint32_t((a[i].n + kSumChunk - 1) / kSumChunk);
+    }
+    if (t.count) {
+      if (int rc = launch(dt, t)) return rc;
+    }
+  }
+  return SR_OK;
+}
+
+uint32_t sum_blocks(const SumTable& t) { return t.chunks < kSumBlocks ? t.chunks : kSumBlocks; }
+
+template <typename S, typename D>
+void launch_clip(const ClipTable& t, uint32_t blocks, hipStream_t stream) {
+  clip_kernel<S, D><<<blocks, kThreads, 0, stream>>>(t);
+}
+
+template <typename S>
+void launch_clip_to(int32_t dst, const ClipTable& t, uint32_t blocks, hipStream_t stream) {
+  if (dst == SR_DT_F32) launch_clip<S, float>(t, blocks, stream);
+  else if (dst == SR_DT_BF16) launch_clip<S, bf16>(t, blocks, stream);
+  else launch_clip<S, f16>(t, blocks, stream);
+}
+
+template <typename W, typename M, typename G>
+void launch_adamw_copy(bool copy, const AdamTable& t, hipStream_t stream) {
+  if constexpr (__is_same(W, float)) {
+    if (copy) {
+      adamw_kernel<W, M, G, bf16><<<t.chunks, kThreads, 0, stream>>>(t);
+      return;
+    }
+  }
+  adamw_kernel<W, M, G, NoCopy><<<t.chunks, kThreads, 0, stream>>>(t);
+}
+
+template <typename W, typename M>
+void launch_adamw_grad(bool wide, bool copy, const AdamTable& t, hipStream_t stream) {
+  if (wide) launch_adamw_copy<W, M, float>(copy, t, stream);
+  else launch_adamw_copy<W, M, bf16>(copy, t, stream);
+}
+
+template <typename W>
+void launch_adamw_moments(bool wide, bool wide_grad, bool copy, const AdamTable& t, hipStream_t stream) {
+  if (wide) launch_adamw_grad<W, float>(wide_grad, copy, t, stream);
+  else launch_adamw_grad<W, bf16>(wide_grad, copy, t, stream);
+}
+
+}  // namespace
+
+extern "C" {
+
+int sr_square_sum_workspace(const sr_array* arrays, int32_t count, uint64_t* bytes) {
+  if (bytes == nullptr) return fail(SR_EINVAL, "sr_square_sum_workspace: null argument");
+  if (int rc = check_arrays("sr_square_sum_workspace", arrays, count)) return rc;
+  uint64_t blocks = 0;
+  sum_launches(arrays, count, [&](int32_t, const SumTable& t) {
+    blocks += sum_blocks(t);
+    return SR_OK;
+  });
+  *bytes = blocks * sizeof(double);
+  return SR_OK;
+}
+
+int sr_square_sum(const sr_array* arrays, int32_t count, void* workspace, uint64_t workspace_bytes, double* sum,
+                  float* norm, hipStream_t stream) {
+  uint64_t need = 0;
+  if (int rc = sr_square_sum_workspace(arrays, count, &need)) return rc;
+  if (sum == nullptr) return fail(SR_EINVAL, "sr_square_sum: sum is null");
+  if (workspace_bytes < need || (need && workspace == nullptr))
+    return fail(SR_EINVAL, "sr_square_sum: a workspace of %llu bytes, %llu are needed",
+                (unsigned long long)workspace_bytes, (unsigned long long)need);
+  if (reinterpret_cast<uintptr_t>(workspace) % 16) return fail(SR_EALIGN, "sr_square_sum: workspace not aligned");
+  double* partial = static_cast<double*>(workspace);
+  uint32_t used = 0;
+  const int rc = sum_launches(arrays, count, [&](int32_t dt, const SumTable& t) {
+    const uint32_t blocks = sum_blocks(t);
+    if (dt == SR_DT_F32) square_sum_kernel<float><<<blocks, kThreads, 0, stream>>>(t, partial + used);
+    else if (dt == SR_DT_BF16) square_sum_kernel<bf16><<<blocks, kThreads, 0, stream>>>(t, partial + used);
+    else square_sum_kernel<f16><<<blocks, kThreads, 0, stream>>>(t, partial + used);
+    used += blocks;
+    return launched("sr_square_sum");
+  });
+  if (rc) return rc;
+  finish_sum_kernel<<<1, kThreads, 0, stream>>>(partial, used, sum, norm);
+  return launched("sr_square_sum");
+}
+
+int sr_clip(const sr_array* src, const sr_array* dst, int32_t count, const double* square_sum, float max_norm,
+            float* norm, hipStream_t stream) try {
+  if (int rc = check_arrays("sr_clip: src", src, count)) return rc;
+  if (dst != nullptr) {
+    if (int rc = check_arrays("sr_clip: dst", dst, count)) return rc;
+  }
+  if (square_sum == nullptr) return fail(SR_EINVAL, "sr_clip: square_sum is null");
+  if (!(max_norm >= 0)) return fail(SR_EINVAL, "sr_clip: max_norm %g", double(max_norm));
+  if (dst == nullptr) dst = src;
+  std::vector<Span> spans;
+  for (int32_t i = 0; i < count; ++i) {
+    if (src[i].n != dst[i].n)
+      return fail(SR_EINVAL, "sr_clip: src[%d] has %llu elements, dst[%d] %llu", i, (unsigned long long)src[i].n, i,
+                  (unsigned long long)dst[i].n);
+    add_span(spans, dst[i].data, bytes_of(dst[i]), true);
+    if (src[i].data != dst[i].data || src[i].dtype != dst[i].dtype)
+      add_span(spans, src[i].data, bytes_of(src[i]), false);
+  }
+  if (clash(spans)) return fail(SR_EOVERLAP, "sr_clip: an array that is written overlaps another");
+  bool any = false;
+  for (int32_t s : kFloatTypes) {
+    for (int32_t d : kFloatTypes) {
+      ClipTable t;
+      t.count = 0;
+      t.max_norm = max_norm;
+      t.square_sum = square_sum;
+      uint32_t chunks = 0;
+      auto launch = [&]() -> int {
+        t.norm = any ? nullptr : norm;
+        any = true;
+        if (s == SR_DT_F32) launch_clip_to<float>(d, t, chunks, stream);
+        else if (s == SR_DT_BF16) launch_clip_to<bf16>(d, t, chunks, stream);
+        else launch_clip_to<f16>(d, t, chunks, stream);
+        t.count = 0;
+        chunks = 0;
+        return launched("sr_clip");
+      };
+      for (int32_t i = 0; i < count; ++i) {
+        if (src[i].dtype != s || dst[i].dtype != d || src[i].n == 0) continue;
+        const uint32_t more = uint32_t((src[i].n + kClipChunk - 1) / kClipChunk);
+        if (t.count == kClipEntries || (t.count && chunks + more > kMostChunks)) {
+          if (int rc = launch()) return rc;
+        }
+        const int k = t.count++;
+        t.src[k] = reinterpret_cast<uint64_t>(src[i].data);
+        t.dst[k] = reinterpret_cast<uint64_t>(dst[i].data);
+        t.n[k] = src[i].n;
+        t.first[k] = chunks;
+        chunks += more;
+      }
+      if (t.count) {
+        if (int rc = launch()) return rc;
+      }
+    }
+  }
+  if (!any && norm != nullptr) {
+    ClipTable t;
+    t.count = 0;
+    t.max_norm = max_norm;
+    t.square_sum = square_sum;
+    t.norm = norm;
+    launch_clip<float, float>(t, 1, stream);
+    return launched("sr_clip");
+  }
+  return SR_OK;
+} catch (const std::bad_alloc&) {
+  return fail(SR_ENOMEM, "sr_clip: out of host memory");
+}
+
+int sr_adamw(const sr_adamw_tensor* tensors, int32_t count, const sr_adamw_options* o, const double* square_sum,
+             hipStream_t stream) try {
+  if (count < 0 || (count > 0 && tensors == nullptr) || o == nullptr)
+    return fail(SR_EINVAL, "sr_adamw: null argument");
+  if (!(o->lr >= 0) || !std::isfinite(o->lr) || !(o->eps >= 0) || !(o->weight_decay >= 0) || !(o->beta1 >= 0) ||
+      !(o->beta1 < 1) || !(o->beta2 >= 0) || !(o->beta2 < 1) || o->step < 1)
+    return fail(SR_EINVAL, "sr_adamw: lr %g, betas %g and %g, eps %g, weight_decay %g, step %lld", o->lr, o->beta1,
+                o->beta2, o->eps, o->weight_decay, (long long)o->step);
+  if (square_sum != nullptr && !(o->max_norm >= 0)) return fail(SR_EINVAL, "sr_adamw: max_norm %g", o->max_norm);
+  std::vector<Span> spans;
+  for (int32_t i = 0; i < count; ++i) {
+    const sr_adamw_tensor& x = tensors[i];
+    if (x.reserved != 0) return fail(SR_EINVAL, "sr_adamw: tensors[%d].reserved is not 0", i);
+    for (int32_t dt : {x.weight_dtype, x.moment_dtype, x.grad_dtype})
+      if (dt != SR_DT_F32 && dt != SR_DT_BF16) return fail(SR_EDTYPE, "sr_adamw: tensors[%d]: dtype %d", i, dt);
+    if (x.param != nullptr && x.weight_dtype != SR_DT_F32)
+      return fail(SR_EDTYPE, "sr_adamw: tensors[%d]: a copy of a weight that is not f32", i);
+    if (x.n > SR_STEP_MAX_ELEMENTS)
+      return fail(SR_EBOUNDS, "sr_adamw: tensors[%d] has %llu elements", i, (unsigned long long)x.n);
+    if (x.n && (!x.weight || !x.exp_avg || !x.exp_avg_sq || !x.grad))
+      return fail(SR_EINVAL, "sr_adamw: tensors[%d]: a field is null", i);
+    const int ws = sr_internal::dtype_size(x.weight_dtype), ms = sr_internal::dtype_size(x.moment_dtype),
+              gs = sr_internal::dtype_size(x.grad_dtype);
+    const struct { const void* p; int size; } field[5] = {
+        {x.weight, ws}, {x.exp_avg, ms}, {x.exp_avg_sq, ms}, {x.param, 2}, {x.grad, gs}};
+    for (int f = 0; f < 5; ++f) {
+      if (reinterpret_cast<uintptr_t>(field[f].p) % field[f].size)
+        return fail(SR_EALIGN, "sr_adamw: tensors[%d]: a field is not aligned to its elements", i);
+      add_span(spans, field[f].p, x.n * field[f].size, f < 4);
+    }
+  }
+  if (clash(spans)) return fail(SR_EOVERLAP, "sr_adamw: a field that is written overlaps another");
+  hipStreamCaptureStatus capturing = hipStreamCaptureStatusNone;
+  SR_STEP_TRY(hipStreamIsCapturing(stream, &capturing));
+  if (capturing != hipStreamCaptureStatusNone)
+    return fail(SR_EINVAL, "sr_adamw: the step number is a host value: the call cannot be captured");
+  AdamTable t;
+  t.square_sum = square_sum;
+  t.max_norm = square_sum ? float(o->max_norm) : 0.0f;
+  t.decay = float(1 - o->lr * o->weight_decay);
+  t.beta1 = float(o->beta1);
+  t.rest1 = float(1 - o->beta1);
+  t.beta2 = float(o->beta2);
+  t.rest2 = float(1 - o->beta2);
+  t.step_size = float(o->lr / (1 - std::pow(o->beta1, double(o->step))));
+  t.root_scale = float(1 / std::sqrt(1 - std::pow(o->beta2, double(o->step))));
+  t.eps = float(o->eps);
+  for (int kind = 0; kind < 16; ++kind) {
+    const bool ww = kind & 1, wm = kind & 2, wg = kind & 4, copy = kind & 8;
+    t.count = 0;
+    t.chunks = 0;
+    auto launch = [&]() -> int {
+      if (ww) launch_adamw_moments<float>(wm, wg, copy, t, stream);
+      else launch_adamw_moments<bf16>(wm, wg, copy, t, stream);
+      t.count = 0;
+      t.chunks = 0;
+      return launched("sr_adamw");
+    };
+    for (int32_t i = 0; i < count; ++i) {
+      const sr_adamw_tensor& x = tensors[i];
+      if (x.n == 0 || (x.weight_dtype == SR_DT_F32) != ww || (x.moment_dtype == SR_DT_F32) != wm ||
+          (x.grad_dtype == SR_DT_F32) != wg || (x.param != nullptr) != copy)
+        continue;
+      const uint64_t chunks = (x.n + kAdamChunk - 1) / kAdamChunk;
+      if (t.count == kAdamEntries || (t.count && t.chunks + chunks > kMostChunks)) {
+        if (int rc = launch()) return rc;
+      }
+      const int k = t.count++;
+      t.weight[k] = reinterpret_cast<uint64_t>(x.weight);
+      t.exp_avg[k] = reinterpret_cast<uint64_t>(x.exp_avg);
+      t.exp_avg_sq[k] = reinterpret_cast<uint64_t>(x.exp_avg_sq);
+      t.param[k] = reinterpret_cast<uint64_t>(x.param);
+      t.grad[k] = reinterpret_cast<uint64_t>(x.grad);
+      t.first[k] = t.chunks;
+      t.tail[k] = uint32_t(x.n - (chunks - 1) * kAdamChunk);
+      t.chunks += uint32_t(chunks);
+    }
+    if (t.count) {
+      if (int rc = launch()) return rc;
+    }
+  }
+  return SR_OK;
+} catch (const std::bad_alloc&) {
+  return fail(SR_ENOMEM, "sr_adamw: out of host memory");
+}
+
+}  // extern "C"

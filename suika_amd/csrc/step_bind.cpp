@@ -1,0 +1,304 @@
+// step_bind.cpp -- the training-step operators (include/suika_step.h) on
+// torch tensors, part of the host extension: argument checks, outputs and
+// workspaces from torch's caching allocator, and the library's calls on the
+// device's current stream.
+
+#include <torch/extension.h>
+#include <c10/core/DeviceGuard.h>
+#include <torch/csrc/DynamicTypes.h>
+
+#include <cstdint>
+#include <string>
+#include <vector>
+
+#include "host_errors.h"
+#include "suika_step.h"
+
+namespace py = pybind11;
+
+namespace {
+
+using suika_host::check;
+using suika_host::plan_error;
+
+std::string indexed(const char* what, size_t i) { return std::string(what) + "[" + std::to_string(i) + "]"; }
+
+int32_t float_code(const at::Tensor& t, const std::string& what) {
+  switch (t.scalar_type()) {
+    case at::kFloat: return SR_DT_F32;
+    case at::kBFloat16: return SR_DT_BF16;
+    case at::kHalf: return SR_DT_F16;
+    default: plan_error(what + ": dtype " + c10::toString(t.scalar_type()) + ", not float32, bfloat16 or float16");
+  }
+}
+
+hipStream_t stream_of(const at::Device& device) {
+  static PyObject* current = [] {
+    py::object f = py::module_::import("torch._C").attr("_cuda_getCurrentRawStream");
+    return f.release().ptr();
+  }();
+  py::object s = py::reinterpret_steal<py::object>(PyObject_CallFunction(current, "i", int(device.index())));
+  if (!s) throw py::error_already_set();
+  return reinterpret_cast<hipStream_t>(PyLong_AsUnsignedLongLong(s.ptr()));
+}
+
+// What the call writes through raw pointers counts as written for autograd.
+void written(const at::Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
+const at::Tensor& tensor_of(PyObject* o, const std::string& what) {
+  if (!THPVariable_Check(o)) plan_error(what + ": not a tensor");
+  return THPVariable_Unpack(o);
+}
+
+// A dense tensor on the GPU; `device` is set by the first one.
+void check_dense(const at::Tensor& t, const std::string& what, c10::optional<at::Device>& device) {
+  if (t.layout() != at::kStrided || !t.is_cuda()) plan_error(what + " is on " + t.device().str() + ", not a dense tensor on the GPU");
+  if (!device) device = t.device();
+  if (t.device() != *device) plan_error(what + " is on " + t.device().str() + ", not on " + device->str());
+  if (!t.is_contiguous()) plan_error(what + " is not contiguous");
+}
+
+// The tensors of a list; None stands for a tensor that is not there.
+class Fast {
+ public:
+  Fast(py::handle list, const char* what) {
+    seq_ = py::reinterpret_steal<py::object>(PySequence_Fast(list.ptr(), "a sequence of tensors is wanted"));
+    if (!seq_) {
+      PyErr_Clear();
+      plan_error(std::string(what) + ": a sequence of tensors is wanted");
+    }
+  }
+  size_t size() const { return size_t(PySequence_Fast_GET_SIZE(seq_.ptr())); }
+  PyObject* operator[](size_t i) const { return PySequence_Fast_GET_ITEM(seq_.ptr(), Py_ssize_t(i)); }
+
+ private:
+  py::object seq_;
+};
+
+sr_array array_of(const at::Tensor& t, const std::string& what) {
+  return {t.data_ptr(), uint64_t(t.numel()), float_code(t, what), 0};
+}
+
+at::Device current_device() {
+  const c10::impl::VirtualGuardImpl impl(at::kCUDA);
+  if (impl.deviceCount() == 0) plan_error("no GPU");
+  return impl.getDevice();
+}
+
+at::TensorOptions on(const at::Device& device, at::ScalarType type) {
+  return at::TensorOptions().device(device).dtype(type);
+}
+
+struct Sum {
+  at::Tensor work;     // the sum, where the caller has no place for it, and the partial sums
+  double* sum = nullptr;
+};
+
+// Launches the sum of squares into `into` (or into memory of its own).
+Sum square_sum_into(const std::vector<sr_array>& a, const at::Device& device, double* into, float* norm) {
+  uint64_t need = 0;
+  check(sr_square_sum_workspace(a.data(), int32_t(a.size()), &need), "sr_square_sum");
+  Sum out;
+  out.work = at::empty({int64_t(need) + 16}, on(device, at::kByte));
+  char* base = static_cast<char*>(out.work.data_ptr());
+  out.sum = into ? into : reinterpret_cast<double*>(base);
+  check(sr_square_sum(a.data(), int32_t(a.size()), base + 16, need, out.sum, norm, stream_of(device)), "sr_square_sum");
+  return out;
+}
+
+std::vector<sr_array> arrays_of(const Fast& list, const char* what, c10::optional<at::Device>& device) {
+  std::vector<sr_array> a;
+  a.reserve(list.size());
+  for (size_t i = 0; i < list.size(); ++i) {
+    if (list[i] == Py_None) continue;
+    const at::Tensor& t = tensor_of(list[i], indexed(what, i));
+    check_dense(t, indexed(what, i), device);
+    a.push_back(array_of(t, indexed(what, i)));
+  }
+  return a;
+}
+
+at::Tensor grad_square_sum(py::object grads) {
+  c10::optional<at::Device> device;
+  const Fast list(grads, "grads");
+  const std::vector<sr_array> a = arrays_of(list, "grads", device);
+  if (!device) device = current_device();
+  const c10::DeviceGuard guard(*device);
+  at::Tensor out = at::empty({}, on(*device, at::kDouble));
+  square_sum_into(a, *device, out.data_ptr<double>(), nullptr);
+  return out;
+}
+
+at::Tensor grad_norm(py::object grads) {
+  c10::optional<at::Device> device;
+  const Fast list(grads, "grads");
+  const std::vector<sr_array> a = arrays_of(list, "grads", device);
+  if (!device) device = current_device();
+  const c10::DeviceGuard guard(*device);
+  at::Tensor norm = at::empty({}, on(*device, at::kFloat));
+  square_sum_into(a, *device, nullptr, norm.data_ptr<float>());
+  return norm;
+}
+
+// A caller's sum of squares (one float64 on the device); null where it is None.
+const double* given_sum(py::handle square_sum, const at::Device& device) {
+  if (square_sum.is_none()) return nullptr;
+  const at::Tensor& t = tensor_of(square_sum.ptr(), "square_sum");
+  if (t.scalar_type() != at::kDouble || t.numel() != 1 || t.device() != device)
+    plan_error("square_sum: one float64 on " + device.str() + " is wanted");
+  return t.data_ptr<double>();
+}
+
+at::Tensor clip_grads(py::object grads, double max_norm, py::object outs, py::object square_sum) {
+  c10::optional<at::Device> device;
+  const Fast list(grads, "grads");
+  std::vector<sr_array> src, dst;
+  std::vector<at::Tensor> to;
+  const bool in_place = outs.is_none();
+  const Fast out_list(in_place ? py::object(py::list()) : outs, "out");
+  if (!in_place && out_list.size() != list.size())
+    plan_error("out has " + std::to_string(out_list.size()) + " tensors, grads " + std::to_string(list.size()));
+  for (size_t i = 0; i < list.size(); ++i) {
+    if (list[i] == Py_None) continue;
+    const at::Tensor& t = tensor_of(list[i], indexed("grads", i));
+    check_dense(t, indexed("grads", i), device);
+    src.push_back(array_of(t, indexed("grads", i)));
+    if (in_place) {
+      to.push_back(t);
+      continue;
+    }
+    const at::Tensor& o = tensor_of(out_list[i], indexed("out", i));
+    check_dense(o, indexed("out", i), device);
+    if (o.sizes() != t.sizes()) plan_error(indexed("out", i) + ": shape differs from the gradient's");
+    dst.push_back(array_of(o, indexed("out", i)));
+    to.push_back(o);
+  }
+  if (!device) device = current_device();
+  const c10::DeviceGuard guard(*device);
+  const double* sum = given_sum(square_sum, *device);
+  at::Tensor norm = at::empty({}, on(*device, at::kFloat));
+  Sum mine;
+  if (!sum) {
+    mine = square_sum_into(src, *device, nullptr, nullptr);
+    sum = mine.sum;
+  }
+  check(sr_clip(src.data(), in_place ? nullptr : dst.data(), int32_t(src.size()), sum, float(max_norm),
+                norm.data_ptr<float>(), stream_of(*device)),
+        "sr_clip");
+  for (const at::Tensor& t : to) written(t);
+  return norm;
+}
+
+// The state that an optimizer steps: the tensors, in the order of its names.
+class AdamWState {
+ public:
+  AdamWState(py::object weight, py::object exp_avg, py::object exp_avg_sq, py::object param, std::vector<std::string> names)
+      : names_(std::move(names)) {
+    const Fast w(weight, "weight"), m(exp_avg, "exp_avg"), v(exp_avg_sq, "exp_avg_sq"), p(param, "param");
+    if (w.size() != names_.size() || m.size() != w.size() || v.size() != w.size() || p.size() != w.size())
+      plan_error("state: lists of different lengths");
+    for (size_t i = 0; i < names_.size(); ++i) {
+      weight_.push_back(field(w[i], i, "weight"));
+      exp_avg_.push_back(field(m[i], i, "exp_avg"));
+      exp_avg_sq_.push_back(field(v[i], i, "exp_avg_sq"));
+      param_.push_back(p[i] == Py_None ? at::Tensor() : field(p[i], i, "param"));
+      for (const at::Tensor* t : {&exp_avg_[i], &exp_avg_sq_[i], &param_[i]})
+        if (t->defined() && t->sizes() != weight_[i].sizes()) plan_error(names_[i] + ": fields of different shapes");
+      const at::ScalarType wt = weight_[i].scalar_type(), mt = exp_avg_[i].scalar_type();
+      if (wt != at::kFloat && wt != at::kBFloat16)
+        plan_error(names_[i] + ": weight of dtype " + c10::toString(wt) + ", not float32 or bfloat16");
+      if ((mt != at::kFloat && mt != at::kBFloat16) || exp_avg_sq_[i].scalar_type() != mt)
+        plan_error(names_[i] + ": moments are both float32 or both bfloat16");
+      if (param_[i].defined() && (wt != at::kFloat || param_[i].scalar_type() != at::kBFloat16))
+        plan_error(names_[i] + ": a master weight is float32 and its param bfloat16");
+    }
+  }
+
+  // One update; the gradients' norm, or None without clipping.
+  py::object step(py::object grads, int64_t step, double lr, double beta1, double beta2, double eps,
+                  double weight_decay, py::object max_norm, py::object square_sum) {
+    const Fast list(grads, "grads");
+    if (list.size() != names_.size())
+      plan_error("grads: " + std::to_string(list.size()) + " tensors for a state of " + std::to_string(names_.size()));
+    std::vector<sr_adamw_tensor> tensors;
+    std::vector<sr_array> arrays;
+    tensors.reserve(names_.size());
+    for (size_t i = 0; i < names_.size(); ++i) {
+      if (list[i] == Py_None) continue;
+      const at::Tensor& g = tensor_of(list[i], "gradient of " + names_[i]);
+      const at::Tensor &w = weight_[i], &m = exp_avg_[i], &v = exp_avg_sq_[i], &p = param_[i];
+      if (g.layout() != at::kStrided || !g.is_contiguous() || g.device() != w.device() || g.sizes() != w.sizes())
+        plan_error("gradient of " + names_[i] + ": a dense tensor like the weight on " + w.device().str() + " is wanted");
+      const at::ScalarType gt = g.scalar_type();
+      if (gt != at::kFloat && gt != at::kBFloat16)
+        plan_error("gradient of " + names_[i] + ": dtype " + c10::toString(gt) + ", not float32 or bfloat16");
+      // storage that was released since the state was taken (forcefully_free_tensor)
+      if (w.numel() && (!w.storage().nbytes() || !m.storage().nbytes() || !v.storage().nbytes()))
+        plan_error(names_[i] + ": a field's storage has been released");
+      const int32_t gc = gt == at::kFloat ? SR_DT_F32 : SR_DT_BF16;
+      tensors.push_back({w.data_ptr(), m.data_ptr(), v.data_ptr(), p.defined() ? p.data_ptr() : nullptr, g.data_ptr(),
+                         uint64_t(w.numel()), w.scalar_type() == at::kFloat ? SR_DT_F32 : SR_DT_BF16,
+                         m.scalar_type() == at::kFloat ? SR_DT_F32 : SR_DT_BF16, gc, 0});
+      if (!max_norm.is_none() && square_sum.is_none()) arrays.push_back({g.data_ptr(), uint64_t(g.numel()), gc, 0});
+    }
+    const at::Device device = device_ ? *device_ : current_device();
+    const c10::DeviceGuard guard(device);
+    sr_adamw_options o{lr, beta1, beta2, eps, weight_decay, step, 0.0};
+    const double* sum = nullptr;
+    Sum mine;
+    at::Tensor norm;
+    if (!max_norm.is_none()) {
+      o.max_norm = max_norm.cast<double>();
+      sum = given_sum(square_sum, device);
+      norm = at::empty({}, on(device, at::kFloat));
+      if (!sum) {
+        mine = square_sum_into(arrays, device, nullptr, norm.data_ptr<float>());
+        sum = mine.sum;
+      } else {
+        check(sr_clip(nullptr, nullptr, 0, sum, float(o.max_norm), norm.data_ptr<float>(), stream_of(device)),
+              "sr_clip");
+      }
+    } else if (!square_sum.is_none()) {
+      plan_error("square_sum is given without max_norm");
+    }
+    check(sr_adamw(tensors.data(), int32_t(tensors.size()), &o, sum, stream_of(device)), "sr_adamw");
+    for (size_t i = 0; i < names_.size(); ++i) {
+      if (list[i] == Py_None) continue;
+      for (const at::Tensor* t : {&weight_[i], &exp_avg_[i], &exp_avg_sq_[i], &param_[i]})
+        if (t->defined()) written(*t);
+    }
+    if (!norm.defined()) return py::none();
+    return py::cast(norm);
+  }
+
+ private:
+  at::Tensor field(PyObject* o, size_t i, const char* what) {
+    const std::string full = names_[i] + "/" + what;
+    const at::Tensor& t = tensor_of(o, full);
+    check_dense(t, full, device_);
+    return t;
+  }
+
+  std::vector<std::string> names_;
+  std::vector<at::Tensor> weight_, exp_avg_, exp_avg_sq_, param_;
+  c10::optional<at::Device> device_;
+};
+
+}  // namespace
+
+namespace suika_host {
+
+void bind_step(py::module_& m) {
+  m.def("grad_square_sum", &grad_square_sum, py::arg("grads"));
+  m.def("grad_norm", &grad_norm, py::arg("grads"));
+  m.def("clip_grads", &clip_grads, py::arg("grads"), py::arg("max_norm"), py::arg("out"), py::arg("square_sum"));
+  py::class_<AdamWState>(m, "AdamWState", "The tensors of a state that AdamW updates in place")
+      .def(py::init<py::object, py::object, py::object, py::object, std::vector<std::string>>(), py::arg("weight"),
+           py::arg("exp_avg"), py::arg("exp_avg_sq"), py::arg("param"), py::arg("names"))
+      .def("step", &AdamWState::step, py::arg("grads"), py::arg("step"), py::arg("lr"), py::arg("beta1"),
+           py::arg("beta2"), py::arg("eps"), py::arg("weight_decay"), py::arg("max_norm"), py::arg("square_sum"));
+}
+
+}  // namespace suika_host

@@ -1,0 +1,161 @@
+"""The optimizer's part of a training step on a share's state.
+
+Between two plan changes a job trains on the state that
+``execute_param_transfer`` returns: ``{name: {"param", "exp_avg",
+"exp_avg_sq"[, "master"][, "step"]}}``.  These operators work on that state as
+it is, whatever allocation its tensors lie in:
+
+* ``grad_norm`` / ``grad_square_sum`` -- the gradients' global 2-norm, or the
+  sum of squares that ranks with other shards add up first;
+* ``clip_grads``  -- the gradients scaled down to a norm;
+* ``ShardAdamW``  -- norm, clipping and the AdamW update of every field.
+
+In the reference this is ``torch.optim.AdamW`` over the model's parameters
+(tasks/task.py:72-73).  The kernels run on the tensors' device, on its current
+stream, behind the C ABI of include/suika_step.h; nothing synchronises with
+the host.  Refused arguments raise ``PlanError`` before anything runs.
+"""
+from __future__ import annotations
+
+from typing import Any, Dict, List, Mapping, Optional, Sequence, Set, Tuple, Union
+
+import torch
+from torch import Tensor
+
+from . import _lib
+from ._lib import PlanError
+from .meta import ParamLayout
+
+Grads = Sequence[Optional[Tensor]]
+
+
+def grad_square_sum(grads: Grads) -> Tensor:
+    """The sum of the squares of all elements of ``grads``, a 0-dim float64
+    tensor on their device.
+
+    ``grads`` are contiguous float32, bfloat16 or float16 tensors of any
+    shapes; ``None`` stands for a parameter without gradient.  Squares and
+    sums are computed in 64 bits, in an order that does not change from run to
+    run.  Of a sharded model, each rank sums the gradients it counts
+    (``counted_names``) and the ranks add their sums up.
+    """
+    return _lib.host().grad_square_sum(grads)
+
+
+def grad_norm(grads: Grads) -> Tensor:
+    """The 2-norm of all elements of ``grads`` together: the root of
+    ``grad_square_sum``, a 0-dim float32 tensor."""
+    return _lib.host().grad_norm(grads)
+
+
+def clip_grads(grads: Grads, max_norm: float, *, out: Optional[Grads] = None,
+               square_sum: Optional[Tensor] = None) -> Tensor:
+    """Scale ``grads`` by ``min(1, max_norm / (norm + 1e-6))`` and return the
+    norm that they had, a 0-dim float32 tensor.
+
+    In place, where a factor of 1 leaves the memory as it is; or into the
+    tensors of ``out``, of the same shapes and of any of the three types
+    (bfloat16 gradients of a model into the float32 ones of its optimizer).
+    ``square_sum`` is the sum to clip by where other ranks have a part in it
+    (a float64 tensor, ``grad_square_sum`` added up over the ranks); by
+    default that of ``grads``.  A norm that is NaN makes every gradient NaN;
+    an infinite one makes the finite gradients 0, as
+    ``torch.nn.utils.clip_grad_norm_`` does.
+    """
+    return _lib.host().clip_grads(grads, float(max_norm), out, square_sum)
+
+
+def counted_names(layout: ParamLayout, rank: int) -> List[str]:
+    """The parameters whose gradients ``rank`` counts in a global norm.
+
+    Every shard is counted once: by the lowest rank that holds it.  So a
+    tensor-parallel shard counts on each rank of its group, a replicated
+    parameter (norms, row-parallel biases, data-parallel copies) on one.
+    """
+    mine = layout.layout[rank]
+    before: Set[Tuple[str, Any]] = set()
+    for r in sorted(layout.layout):
+        if r >= rank:
+            break
+        before.update((n, _shard_of(m)) for n, m in layout.layout[r].items() if n in mine)
+    return [n for n, m in mine.items() if (n, _shard_of(m)) not in before]
+
+
+def _shard_of(meta) -> Any:
+    """What tells a parameter's shards apart: (index, degree), or nothing for a
+    whole one."""
+    return (meta.tp_index(), meta.tp_deg()) if meta.tp_deg() > 1 else None
+
+
+class ShardAdamW:
+    """AdamW on a share's state, in place.
+
+    ``state`` is the dict that ``execute_param_transfer`` returns.  An entry
+    with a float32 ``master`` is updated there and its bfloat16 ``param`` is
+    rounded from it, to nearest even; without a ``master`` the ``param``,
+    float32 or bfloat16, is the weight itself.  The moments are both float32
+    or both bfloat16.  Everything is computed in 32 bits and rounded where it
+    is stored.  The optimizer keeps the tensors (an entry replaced in the dict
+    later is not seen); ``step`` fields, which have to agree, are where it
+    starts to count.
+
+    The update of step t, with g clipped: ``exp_avg = beta1 exp_avg +
+    (1 - beta1) g``; ``exp_avg_sq = beta2 exp_avg_sq + (1 - beta2) g^2``;
+    ``w = w (1 - lr weight_decay) - lr / (1 - beta1^t) exp_avg /
+    (sqrt(exp_avg_sq / (1 - beta2^t)) + eps)``.
+    """
+
+    def __init__(self, state: Dict[str, Dict[str, Tensor]], *, lr: float = 1e-3,
+                 betas: Tuple[float, float] = (0.9, 0.999), eps: float = 1e-8, weight_decay: float = 0.01):
+        self.lr, self.betas, self.eps, self.weight_decay = lr, tuple(betas), eps, weight_decay
+        self.names = list(state)
+        self._state = state
+        steps = set()
+        weight, param = [], []
+        for name, entry in state.items():
+            for f in ("param", "exp_avg", "exp_avg_sq"):
+                if f not in entry:
+                    raise PlanError(f"{name}: no {f} in the state")
+            master = entry.get("master")
+            weight.append(entry["param"] if master is None else master)
+            param.append(None if master is None else entry["param"])
+            if "step" in entry:
+                steps.add(int(entry["step"]))
+        if len(steps) > 1:
+            raise PlanError(f"the state's steps differ: {sorted(steps)}")
+        self.steps = steps.pop() if steps else 0
+        self._native = _lib.host().AdamWState(weight, [e["exp_avg"] for e in state.values()],
+                                              [e["exp_avg_sq"] for e in state.values()], param, self.names)
+
+    def step(self, grads: Union[Grads, Mapping[str, Optional[Tensor]]], *, max_norm: Optional[float] = None,
+             square_sum: Optional[Tensor] = None) -> Optional[Tensor]:
+        """One update by ``grads``: contiguous float32 or bfloat16 tensors in the
+        order of ``names``, or by name; a parameter whose gradient is ``None``
+        or missing keeps its state.
+
+        With ``max_norm`` the gradients count as clipped to it
+        (``clip_grads``; they are not written) and their norm is returned, a
+        0-dim float32 tensor; ``square_sum`` is as for ``clip_grads``.  The
+        number of the step is a host value, so the call refuses to be captured
+        into a graph.
+        """
+        if isinstance(grads, Mapping):
+            unknown = grads.keys() - self._state.keys()
+            if unknown:
+                raise PlanError(f"gradients of unknown parameters: {sorted(unknown)[:4]}")
+            grads = [grads.get(n) for n in self.names]
+        norm = self._native.step(grads, self.steps + 1, self.lr, self.betas[0], self.betas[1], self.eps,
+                                 self.weight_decay, max_norm, square_sum)
+        self.steps += 1
+        return norm
+
+    def state(self) -> Dict[str, Dict[str, Tensor]]:
+        """The state with its ``step`` fields brought up to date: the source of
+        the next ``execute_param_transfer``."""
+        for entry in self._state.values():
+            old = entry.get("step")
+            if isinstance(old, Tensor):
+                old.fill_(self.steps)
+            else:
+                entry["step"] = torch.tensor(float(self.steps))
+        return self._state

@@ -3,14 +3,19 @@
  * (libsuika_reshard.so).
  *
  * Between two plan changes a job trains on the state that a reshard moves:
- * bf16 or f32 parameters, f32 master weights and Adam moments.  These are the parts of a step that work on that state's own
- * layouts:
+ * bf16 or f32 parameters, f32 master weights and Adam moments, with the
+ * vocabulary of the embedding cut over the tensor-parallel ranks.  These are
+ * the parts of a step that work on that state's own layouts:
  *
  *   sr_square_sum, sr_clip, sr_adamw
  *       the gradients' global norm over all tensors of a share, clipping by
  *       it, and the AdamW update of every state field.  In the reference
  *       these are torch.optim.AdamW on the model's parameters
  *       (tasks/task.py:72-73, 94)
+ *   sr_embedding, sr_embedding_grad
+ *       rows of a vocabulary shard for the tokens that lie in it, and the
+ *       gradient of its rows.  In the reference the embedding is an
+ *       nn.Embedding (Suika/models/llama_model.py:108-157)
  *
  * Conventions
  *   - All device memory, workspaces included, belongs to the caller.
@@ -38,9 +43,9 @@
 extern "C" {
 #endif
 
-/* Most elements of one array, and most rows or tokens of one call. */
+/* Most elements of one array; most tokens, rows or columns of one call. */
 #define SR_STEP_MAX_ELEMENTS ((uint64_t)1 << 34)
-#define SR_STEP_MAX_ROWS ((uint64_t)1 << 30)
+#define SR_STEP_MAX_ROWS ((uint64_t)1 << 23)
 
 /* A dense array of n elements (n may be 0). */
 typedef struct sr_array {
@@ -100,6 +105,35 @@ typedef struct sr_adamw_options {
  */
 int sr_adamw(const sr_adamw_tensor* tensors, int32_t count, const sr_adamw_options* options, const double* square_sum,
              hipStream_t stream);
+
+/* The tokens and the shard of an embedding: row r of the shard is token
+ * vocab_start + r.  Tokens outside the shard (negative ones among them) give
+ * rows of zeros and no gradient.  Outputs overlap no inputs (SR_EOVERLAP). */
+typedef struct sr_embedding_shape {
+  const void* tokens;    /* SR_DT_I32 or SR_DT_I64, dense */
+  int32_t token_dtype;
+  int32_t dtype;         /* of the weight and of the outputs' gradient */
+  uint64_t n_tokens;
+  uint64_t rows;         /* of the shard */
+  uint64_t cols;
+  int64_t vocab_start;
+  float scale;
+  int32_t reserved;      /* must be 0 */
+} sr_embedding_shape;
+
+/* out[i] = scale * weight[tokens[i] - vocab_start]; weight's rows are
+ * weight_stride elements apart, out is dense and of the same type. */
+int sr_embedding(const sr_embedding_shape* shape, const void* weight, uint64_t weight_stride, void* out,
+                 hipStream_t stream);
+
+/* grad[r] = scale * sum of grad_out[i] over the tokens of row r, in the order
+ * of i, plus grad[r] where accumulate is not 0.  grad_out's rows are
+ * grad_out_stride elements apart, grad is dense.  workspace:
+ * sr_embedding_grad_workspace bytes. */
+int sr_embedding_grad_workspace(const sr_embedding_shape* shape, uint64_t* bytes);
+int sr_embedding_grad(const sr_embedding_shape* shape, const void* grad_out, uint64_t grad_out_stride, void* grad,
+                      int32_t grad_dtype, int32_t accumulate, void* workspace, uint64_t workspace_bytes,
+                      hipStream_t stream);
 
 #ifdef __cplusplus
 }

@@ -81,6 +81,9 @@ EXPORTED_SYMBOLS = (
     "sr_square_sum",
     "sr_clip",
     "sr_adamw",
+    "sr_embedding",
+    "sr_embedding_grad_workspace",
+    "sr_embedding_grad",
 )
 
 # Largest hand-off allocation (SR_HANDOFF_MAX_BYTES, include/suika_handoff.h).

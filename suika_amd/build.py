@@ -9,7 +9,8 @@ and its lowering to region moves), ``handoff.cpp`` (exported device
 allocations for the same-GPU state hand-off between processes), ``stage.cpp``
 (sources in host memory packed into device buffers, results copied back to
 host memory, through pinned windows and a host thread pool), ``optim.hip``
-(gradient norm, clipping and the AdamW update of a share's state).
+(gradient norm, clipping and the AdamW update of a share's state),
+``embed.hip`` (rows of a vocabulary shard and their gradient).
 
 ``build_host`` compiles ``host_bind.cpp`` and ``step_bind.cpp`` into
 ``suika_amd/lib/_suika_host.so``, the CPython extension (on torch's C++ API)
@@ -30,7 +31,7 @@ PKG_DIR = Path(__file__).resolve().parent
 REPO_DIR = PKG_DIR.parent
 SOURCES = [PKG_DIR / "csrc" / "reshard.hip", PKG_DIR / "csrc" / "schedule.cpp",
            PKG_DIR / "csrc" / "lower.cpp", PKG_DIR / "csrc" / "handoff.cpp", PKG_DIR / "csrc" / "stage.cpp",
-           PKG_DIR / "csrc" / "optim.hip"]
+           PKG_DIR / "csrc" / "optim.hip", PKG_DIR / "csrc" / "embed.hip"]
 INCLUDE = REPO_DIR / "include"
 LIB_DIR = PKG_DIR / "lib"
 LIB = LIB_DIR / "libsuika_reshard.so"

@@ -286,6 +286,94 @@ class AdamWState {
   c10::optional<at::Device> device_;
 };
 
+// ------------------------------------------------------------- vocabulary shard
+
+int32_t index_code(const at::Tensor& t, const char* what) {
+  if (t.scalar_type() == at::kLong) return SR_DT_I64;
+  if (t.scalar_type() == at::kInt) return SR_DT_I32;
+  plan_error(std::string(what) + ": dtype " + c10::toString(t.scalar_type()) + ", not int64 or int32");
+}
+
+// A tensor of rows of `cols` dense elements: their distance in elements.
+uint64_t row_stride(const at::Tensor& t, const std::string& what) {
+  if (t.layout() != at::kStrided || t.dim() < 1) plan_error(what + ": a dense tensor of rows is wanted");
+  const int64_t cols = t.size(-1);
+  if (t.is_contiguous()) return uint64_t(cols);
+  if (t.dim() != 2 || (t.stride(1) != 1 && cols > 1) || (t.stride(0) < cols && t.size(0) > 1))
+    plan_error(what + ": rows of dense elements are wanted, not strides of " + std::to_string(t.stride(-1)));
+  return uint64_t(t.size(0) > 1 ? t.stride(0) : cols);
+}
+
+void check_device(const at::Tensor& t, const char* what, const at::Device& device) {
+  if (t.device() != device) plan_error(std::string(what) + " is on " + t.device().str() + ", not on " + device.str());
+}
+
+sr_embedding_shape embedding_shape(const at::Tensor& tokens, int32_t dtype, int64_t rows, int64_t cols, double scale,
+                                   int64_t vocab_start) {
+  if (!tokens.is_cuda() || !tokens.is_contiguous()) plan_error("tokens: a contiguous tensor on the GPU is wanted");
+  return {tokens.data_ptr(), index_code(tokens, "tokens"), dtype,         uint64_t(tokens.numel()), uint64_t(rows),
+          uint64_t(cols),    vocab_start,                  float(scale), 0};
+}
+
+at::Tensor vocab_embedding(const at::Tensor& tokens, const at::Tensor& weight, double scale, int64_t vocab_start,
+                           const c10::optional<at::Tensor>& out) {
+  if (weight.dim() != 2) plan_error("weight: rows x columns are wanted");
+  const int64_t rows = weight.size(0), cols = weight.size(1);
+  const sr_embedding_shape s =
+      embedding_shape(tokens, float_code(weight, "weight"), rows, cols, scale, vocab_start);
+  check_device(weight, "weight", tokens.device());
+  const uint64_t stride = row_stride(weight, "weight");
+  const c10::DeviceGuard guard(tokens.device());
+  std::vector<int64_t> shape(tokens.sizes().begin(), tokens.sizes().end());
+  shape.push_back(cols);
+  if (out) {
+    check_device(*out, "out", tokens.device());
+    if (out->sizes() != at::IntArrayRef(shape) || !out->is_contiguous() || out->scalar_type() != weight.scalar_type())
+      plan_error("out: a contiguous tensor of the tokens' shape and the weight's columns and dtype is wanted");
+  }
+  at::Tensor to = out ? *out : at::empty(shape, on(tokens.device(), weight.scalar_type()));
+  check(sr_embedding(&s, weight.data_ptr(), stride, to.data_ptr(), stream_of(tokens.device())), "sr_embedding");
+  if (out) written(to);
+  return to;
+}
+
+at::Tensor vocab_embedding_grad(const at::Tensor& tokens, const at::Tensor& grad_output, int64_t rows, double scale,
+                                int64_t vocab_start, py::object dtype, const c10::optional<at::Tensor>& out,
+                                bool accumulate) {
+  if (grad_output.dim() != tokens.dim() + 1 || grad_output.sizes().slice(0, tokens.dim()) != tokens.sizes())
+    plan_error("grad_output: a tensor of the tokens' shape and the columns is wanted");
+  if (rows < 0) plan_error("rows: " + std::to_string(rows));
+  const int64_t cols = grad_output.size(-1);
+  const sr_embedding_shape s =
+      embedding_shape(tokens, float_code(grad_output, "grad_output"), rows, cols, scale, vocab_start);
+  check_device(grad_output, "grad_output", tokens.device());
+  const uint64_t stride = row_stride(grad_output, "grad_output");
+  const c10::DeviceGuard guard(tokens.device());
+  at::Tensor to;
+  if (out) {
+    to = *out;
+    check_device(to, "out", tokens.device());
+    if (to.dim() != 2 || to.size(0) != rows || to.size(1) != cols || !to.is_contiguous())
+      plan_error("out: a contiguous tensor of rows x columns is wanted");
+    if (!dtype.is_none() && torch::python::detail::py_object_to_dtype(dtype) != to.scalar_type())
+      plan_error("out is of another dtype than the one asked for");
+  } else {
+    if (accumulate) plan_error("accumulate goes with out");
+    const at::ScalarType type =
+        dtype.is_none() ? grad_output.scalar_type() : torch::python::detail::py_object_to_dtype(dtype);
+    to = at::empty({rows, cols}, on(tokens.device(), type));
+  }
+  const int32_t code = float_code(to, "the gradient");
+  uint64_t need = 0;
+  check(sr_embedding_grad_workspace(&s, &need), "sr_embedding_grad");
+  const at::Tensor work = at::empty({int64_t(need)}, on(tokens.device(), at::kByte));
+  check(sr_embedding_grad(&s, grad_output.data_ptr(), stride, to.data_ptr(), code, accumulate, work.data_ptr(), need,
+                          stream_of(tokens.device())),
+        "sr_embedding_grad");
+  if (out) written(to);
+  return to;
+}
+
 }  // namespace
 
 namespace suika_host {
@@ -299,6 +387,10 @@ void bind_step(py::module_& m) {
            py::arg("exp_avg"), py::arg("exp_avg_sq"), py::arg("param"), py::arg("names"))
       .def("step", &AdamWState::step, py::arg("grads"), py::arg("step"), py::arg("lr"), py::arg("beta1"),
            py::arg("beta2"), py::arg("eps"), py::arg("weight_decay"), py::arg("max_norm"), py::arg("square_sum"));
+  m.def("vocab_embedding", &vocab_embedding, py::arg("tokens"), py::arg("weight"), py::arg("scale"),
+        py::arg("vocab_start"), py::arg("out"));
+  m.def("vocab_embedding_grad", &vocab_embedding_grad, py::arg("tokens"), py::arg("grad_output"), py::arg("rows"),
+        py::arg("scale"), py::arg("vocab_start"), py::arg("dtype"), py::arg("out"), py::arg("accumulate"));
 }
 
 }  // namespace suika_host

@@ -16,6 +16,9 @@
  *       rows of a vocabulary shard for the tokens that lie in it, and the
  *       gradient of its rows.  In the reference the embedding is an
  *       nn.Embedding (Suika/models/llama_model.py:108-157)
+ *   sr_logprob, sr_logprob_grad
+ *       log probabilities of given tokens, entropy and the best alternatives
+ *       from the head's logits, and the gradient of the logits
  *
  * Conventions
  *   - All device memory, workspaces included, belongs to the caller.
@@ -134,6 +137,46 @@ int sr_embedding_grad_workspace(const sr_embedding_shape* shape, uint64_t* bytes
 int sr_embedding_grad(const sr_embedding_shape* shape, const void* grad_out, uint64_t grad_out_stride, void* grad,
                       int32_t grad_dtype, int32_t accumulate, void* workspace, uint64_t workspace_bytes,
                       hipStream_t stream);
+
+#define SR_LOGPROB_MAX_TOP 64
+
+/* Logits of `rows` positions, `columns` each, of which the first `vocab` are
+ * tokens (the rest pads the head). */
+typedef struct sr_logprob_shape {
+  const void* logits;
+  const void* targets;   /* SR_DT_I32 or SR_DT_I64, dense */
+  int32_t target_dtype;
+  int32_t dtype;         /* SR_DT_F32, SR_DT_BF16 or SR_DT_F16 */
+  uint64_t rows;
+  uint64_t columns;
+  uint64_t vocab;
+  uint64_t stride;       /* elements between rows of logits */
+} sr_logprob_shape;
+
+/*
+ * Per row: lse = ln sum exp(x), logprob = x[target] - lse, entropy, and the
+ * `top` largest log probabilities in falling order with their columns (equal
+ * logits: the lower column first).  A negative target is not scored: logprob
+ * 0.  A target of vocab or more has logprob -inf.  A row whose logits are all
+ * -inf has lse and logprobs -inf and entropy 0.  A row with NaN or +inf has NaN
+ * statistics; its alternatives are ordered with NaN above +inf.  workspace:
+ * sr_logprob_workspace bytes.
+ */
+int sr_logprob_workspace(const sr_logprob_shape* shape, int32_t top, uint64_t* bytes);
+int sr_logprob(const sr_logprob_shape* shape, int32_t top, float* logprob, float* entropy, float* lse,
+               float* top_logprob, int64_t* top_index, void* workspace, uint64_t workspace_bytes, hipStream_t stream);
+
+/*
+ * grad[row][j] = g_logprob[row] * ([j = target] - p_j)
+ *                - g_entropy[row] * p_j * (ln p_j + entropy[row])
+ * with p_j = exp(x_j - lse[row]); 0 in the padded columns, in rows that are
+ * all -inf, and for the first term in rows that are not scored.  g_logprob or
+ * g_entropy may be NULL (0).  grad has the logits' type and rows of
+ * grad_stride elements; it may be the logits themselves, and overlaps no
+ * other input (SR_EOVERLAP).  lse is a float32, so p_j is exact to |lse| 2^-24.
+ */
+int sr_logprob_grad(const sr_logprob_shape* shape, const float* lse, const float* entropy, const float* g_logprob,
+                    const float* g_entropy, void* grad, uint64_t grad_stride, hipStream_t stream);
 
 #ifdef __cplusplus
 }

@@ -20,7 +20,7 @@ from ._lib import PlanError, ReshardError
 from .checkpoint import checkpoint_load, checkpoint_save, migration_load, migration_save
 from .handoff import HandoffError, dummy_migration_IPC_state_dict
 from .optim import ShardAdamW, clip_grads, counted_names, grad_norm, grad_square_sum
-from .vocab import vocab_embedding, vocab_embedding_grad
+from .vocab import TokenLogprobs, token_logprobs, token_logprobs_grad, vocab_embedding, vocab_embedding_grad
 
 __all__ = [
     "CHUNK", "QKV_HEADS", "VOCAB_PAD", "ParamLayout", "TensorMeta", "TransferOp",
@@ -31,5 +31,5 @@ __all__ = [
     "PlanError", "ReshardError", "checkpoint_save", "checkpoint_load", "migration_save",
     "migration_load", "forcefully_free_tensor", "cuda_gc", "dummy_migration_IPC_state_dict", "HandoffError",
     "ShardAdamW", "clip_grads", "counted_names", "grad_norm", "grad_square_sum",
-    "vocab_embedding", "vocab_embedding_grad",
+    "vocab_embedding", "vocab_embedding_grad", "TokenLogprobs", "token_logprobs", "token_logprobs_grad",
 ]

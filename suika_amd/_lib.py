@@ -84,6 +84,9 @@ EXPORTED_SYMBOLS = (
     "sr_embedding",
     "sr_embedding_grad_workspace",
     "sr_embedding_grad",
+    "sr_logprob_workspace",
+    "sr_logprob",
+    "sr_logprob_grad",
 )
 
 # Largest hand-off allocation (SR_HANDOFF_MAX_BYTES, include/suika_handoff.h).

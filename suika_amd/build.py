@@ -10,7 +10,8 @@ allocations for the same-GPU state hand-off between processes), ``stage.cpp``
 (sources in host memory packed into device buffers, results copied back to
 host memory, through pinned windows and a host thread pool), ``optim.hip``
 (gradient norm, clipping and the AdamW update of a share's state),
-``embed.hip`` (rows of a vocabulary shard and their gradient).
+``embed.hip`` (rows of a vocabulary shard and their gradient),
+``logprob.hip`` (token log probabilities and the gradient of the logits).
 
 ``build_host`` compiles ``host_bind.cpp`` and ``step_bind.cpp`` into
 ``suika_amd/lib/_suika_host.so``, the CPython extension (on torch's C++ API)
@@ -31,7 +32,8 @@ PKG_DIR = Path(__file__).resolve().parent
 REPO_DIR = PKG_DIR.parent
 SOURCES = [PKG_DIR / "csrc" / "reshard.hip", PKG_DIR / "csrc" / "schedule.cpp",
            PKG_DIR / "csrc" / "lower.cpp", PKG_DIR / "csrc" / "handoff.cpp", PKG_DIR / "csrc" / "stage.cpp",
-           PKG_DIR / "csrc" / "optim.hip", PKG_DIR / "csrc" / "embed.hip"]
+           PKG_DIR / "csrc" / "optim.hip", PKG_DIR / "csrc" / "embed.hip",
+           PKG_DIR / "csrc" / "logprob.hip"]
 INCLUDE = REPO_DIR / "include"
 LIB_DIR = PKG_DIR / "lib"
 LIB = LIB_DIR / "libsuika_reshard.so"

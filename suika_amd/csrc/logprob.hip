@@ -1,0 +1,574 @@
+// logprob.hip -- log probabilities of given tokens, entropy and the best
+// alternatives from a head's logits, and the gradient of the logits (C ABI in
+// include/suika_step.h).
+//
+// With d = (x - M) log2 e for a running maximum M, one pass over a row keeps
+//   s = sum 2^d   and   w = sum d 2^d,
+// so that lse = M + ln s and entropy = ln s - ln 2 w / s.  When M grows by D
+// (in units of log2), s <- s 2^-D and w <- 2^-D (w - D s).  Every lane keeps
+// its own M, s and w; they are joined once per row.
+//
+// The alternatives come from a second look at few of the logits: the k-th
+// largest of the lane groups' maxima is a bound that at least k logits reach,
+// and only the groups whose maximum reaches it are read again.  The logits that
+// reach it are ranked against each other; equal ones by column.
+//
+// Rows that this arithmetic does not cover (NaN or +inf, a largest logit beyond
+// 1e7 or so, nothing but -inf) are noticed by their sums and go through plain
+// loops over the row instead, and so do alternatives that there is no room to
+// list.
+
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <type_traits>
+#include <utility>
+
+#include "suika_step.h"
+#include "sr_step.h"
+
+namespace {
+
+using namespace sr_step;
+
+constexpr int kThreads = 256;
+constexpr int kWaves = kThreads / kWave;
+constexpr float kLog2e = 1.44269504088896340736f;
+constexpr float kLn2 = 0.69314718055994530942f;
+constexpr float kInf = __builtin_inff();
+constexpr float kLeast = -1e38f;       // start of a running maximum, in log2 units
+constexpr int kMaxTop = SR_LOGPROB_MAX_TOP;
+constexpr uint32_t kCandidates = 1024;
+
+struct Stats {
+  float m;     // largest logit, as it is
+  float M;     // the maximum that s and w go by: max(kLeast, m log2 e)
+  float s, w;
+};
+
+__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+
+__device__ __forceinline__ Stats join(const Stats& a, const Stats& b) {
+  Stats r;
+  r.m = fmaxf(a.m, b.m);
+  r.M = fmaxf(a.M, b.M);
+  const float da = a.M - r.M, db = b.M - r.M;
+  const float ea = exp2_fast(da), eb = exp2_fast(db);
+  r.s = a.s * ea + b.s * eb;
+  // a part without weight has none here either, however far its maximum is off
+  r.w = (a.s > 0 || a.s != a.s ? ea * fmaf(fmaxf(da, -1000.0f), a.s, a.w) : 0) +
+        (b.s > 0 || b.s != b.s ? eb * fmaf(fmaxf(db, -1000.0f), b.s, b.w) : 0);
+  return r;
+}
+
+// Takes N logits into a lane's statistics.
+template <int N>
+__device__ __forceinline__ void take(Stats& t, const float (&x)[N]) {
+  float top = x[0];
+#pragma unroll
+  for (int k = 1; k < N; ++k) top = fmaxf(top, x[k]);
+  if (top > t.m) {
+    t.m = top;
+    const float M = fmaxf(top * kLog2e, kLeast);
+    const float down = t.M - M;
+    const float f = exp2_fast(down);
+    t.w = f * fmaf(fmaxf(down, -1000.0f), t.s, t.w);
+    t.s *= f;
+    t.M = M;
+  }
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    const float d = fmaf(x[k], kLog2e, -t.M);
+    const float e = exp2_fast(d);              // NaN stays NaN
+    t.s += e;
+    t.w = fmaf(fmaxf(d, -160.0f), e, t.w);     // 2^-160 is 0, and so is its part
+  }
+}
+
+__device__ __forceinline__ Stats wave_join(Stats t) {
+#pragma unroll
+  for (int d = kWave / 2; d; d >>= 1) {
+    Stats o;
+    o.m = __shfl_xor(t.m, d);
+    o.M = __shfl_xor(t.M, d);
+    o.s = __shfl_xor(t.s, d);
+    o.w = __shfl_xor(t.w, d);
+    t = join(t, o);
+  }
+  return t;
+}
+
+// Whether the sums say what they should: the largest logit's own part is 1.
+__device__ __forceinline__ bool sound(const Stats& t) {
+  return t.s >= 0.5f && t.s < kInf && t.w > -kInf && t.w < kInf && t.m < kInf;
+}
+
+// Order of logits: NaN above +inf, -0 as 0.  Larger keys come first.
+__device__ __forceinline__ uint32_t key_of(float x) {
+  if (x != x) return 0xffffffffu;
+  const uint32_t b = __float_as_uint(x + 0.0f);
+  return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+
+__device__ __forceinline__ float value_of(uint32_t key) {
+  if (key == 0xffffffffu) return __builtin_nanf("");
+  return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
+}
+
+// A logit and its column, as one number that falls in the order of the
+// alternatives: by value, then by column.
+__device__ __forceinline__ uint64_t candidate(float x, uint32_t column) {
+  return uint64_t(key_of(x)) << 32 | (0xffffffffu - column);
+}
+__device__ __forceinline__ uint32_t column_of(uint64_t c) { return 0xffffffffu - uint32_t(c); }
+
+struct Shared {
+  Stats stats[kWaves];
+  float maxima[kThreads];
+  uint32_t count;
+  float bound;
+  uint64_t list[kCandidates];
+  uint64_t best[kWaves];
+  uint64_t chosen[kMaxTop];
+};
+
+__device__ __forceinline__ Stats block_join(Shared& sh, Stats t) {
+  t = wave_join(t);
+  __syncthreads();
+  if (threadIdx.x % kWave == 0) sh.stats[threadIdx.x / kWave] = t;
+  __syncthreads();
+  Stats all = sh.stats[0];
+#pragma unroll
+  for (int w = 1; w < kWaves; ++w) all = join(all, sh.stats[w]);
+  return all;
+}
+
+__device__ __forceinline__ float block_max(Shared& sh, float x) {
+#pragma unroll
+  for (int d = kWave / 2; d; d >>= 1) x = fmaxf(x, __shfl_xor(x, d));
+  __syncthreads();
+  if (threadIdx.x % kWave == 0) sh.maxima[threadIdx.x / kWave] = x;
+  __syncthreads();
+  float r = sh.maxima[0];
+#pragma unroll
+  for (int w = 1; w < kWaves; ++w) r = fmaxf(r, sh.maxima[w]);
+  return r;
+}
+
+__device__ __forceinline__ float block_add(Shared& sh, float x) {
+  x = wave_sum(x);
+  __syncthreads();
+  if (threadIdx.x % kWave == 0) sh.maxima[threadIdx.x / kWave] = x;
+  __syncthreads();
+  float r = 0;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) r += sh.maxima[w];
+  return r;
+}
+
+__device__ __forceinline__ uint64_t block_best(Shared& sh, uint64_t x) {
+#pragma unroll
+  for (int d = kWave / 2; d; d >>= 1) {
+    const uint64_t o = __shfl_xor((unsigned long long)x, d);
+    x = o > x ? o : x;
+  }
+  __syncthreads();
+  if (threadIdx.x % kWave == 0) sh.best[threadIdx.x / kWave] = x;
+  __syncthreads();
+  uint64_t r = sh.best[0];
+#pragma unroll
+  for (int w = 1; w < kWaves; ++w) r = sh.best[w] > r ? sh.best[w] : r;
+  return r;
+}
+
+// ------------------------------------------------------------------ one row
+
+// N logits from column c on, -inf from column `to` on.
+template <typename T, int N>
+__device__ __forceinline__ void load_or_fill(const T* row, uint32_t c, uint32_t to, float (&x)[N]) {
+  if (c + N <= to) {
+    load<T, N>(row + c, x);
+  } else {
+#pragma unroll
+    for (int k = 0; k < N; ++k) x[k] = c + k < to ? float(row[c + k]) : -kInf;
+  }
+}
+
+// A lane's statistics of columns from..to.
+template <typename T>
+__device__ __forceinline__ Stats row_stats(const T* row, uint32_t from, uint32_t to) {
+  constexpr int N = 16 / sizeof(T);
+  constexpr int kBatch = 4;
+  Stats t{-kInf, kLeast, 0, 0};
+  uint32_t c = from + threadIdx.x * N;
+  for (; c + (kBatch - 1) * kThreads * N + N <= to; c += kBatch * kThreads * N) {
+    float x[kBatch * N];
+#pragma unroll
+    for (int b = 0; b < kBatch; ++b) load<T, N>(row + c + b * kThreads * N, *reinterpret_cast<float(*)[N]>(x + b * N));
+    take<kBatch * N>(t, x);
+  }
+  for (; c < to; c += kThreads * N) {
+    float x[N];
+    load_or_fill<T, N>(row, c, to, x);
+    take<N>(t, x);
+  }
+  return t;
+}
+
+struct Summary {
+  float lse, entropy;
+  float shift;      // logprob = (x - shift) - rest
+  float rest;
+};
+
+// Statistics of a row that the running sums do not cover.
+template <typename T>
+__device__ Summary plain_summary(Shared& sh, const T* row, uint32_t vocab) {
+  float m = -kInf, bad = 0;
+  for (uint32_t c = threadIdx.x; c < vocab; c += kThreads) {
+    const float x = float(row[c]);
+    if (!(x < kInf)) bad = 1;      // NaN, +inf
+    m = fmaxf(m, x);
+  }
+  m = block_max(sh, m);
+  bad = block_max(sh, bad);
+  const float nan = __builtin_nanf("");
+  if (bad > 0) return {nan, nan, nan, nan};
+  if (m == -kInf) return {-kInf, 0, 0, 0};
+  float s = 0, w = 0;
+  for (uint32_t c = threadIdx.x; c < vocab; c += kThreads) {
+    const float d = fmaxf(float(row[c]) - m, -200.0f);
+    const float e = expf(d);
+    s += e;
+    w = fmaf(d, e, w);
+  }
+  s = block_add(sh, s);
+  w = block_add(sh, w);
+  return {m + logf(s), fmaxf(logf(s) - w / s, 0.0f), m, logf(s)};
+}
+
+__device__ __forceinline__ Summary summary_of(const Stats& t) {
+  const float ls = logf(t.s);
+  // the sums go by M, which is m log2 e but for a rounding that 2^M took part in
+  const float slip = fmaf(t.m, kLog2e, -t.M) * kLn2;
+  const float rest = ls - slip;
+  return {t.m + rest, fmaxf(fmaf(-kLn2, t.w / t.s, ls), 0.0f), t.m, rest};
+}
+
+// The k best candidates of the lanes, one after the other: a look at the whole
+// row for each.
+template <typename T>
+__device__ void plain_top(Shared& sh, const T* row, uint32_t from, uint32_t to, int k) {
+  uint64_t last = ~uint64_t(0);
+  for (int i = 0; i < k; ++i) {
+    uint64_t best = 0;
+    for (uint32_t c = from + threadIdx.x; c < to; c += kThreads) {
+      const uint64_t x = candidate(float(row[c]), c);
+      if ((i == 0 || x < last) && x > best) best = x;
+    }
+    last = block_best(sh, best);
+    if (threadIdx.x == 0) sh.chosen[i] = last;
+  }
+  __syncthreads();
+}
+
+// sh.chosen[0..k) = the k largest of n <= kCandidates different numbers in
+// sh.list, in falling order (n >= k).
+__device__ __forceinline__ void rank_list(Shared& sh, uint32_t n, int k) {
+  for (uint32_t i = threadIdx.x; i < n; i += kThreads) {
+    const uint64_t mine = sh.list[i];
+    int before = 0;
+    for (uint32_t j = 0; j < n; ++j) before += sh.list[j] > mine;
+    if (before < k) sh.chosen[before] = mine;
+  }
+  __syncthreads();
+}
+
+// Adds a lane's logits that reach `bound`, or are above it, to the list.
+template <typename T>
+__device__ __forceinline__ void list_reaching(Shared& sh, const T* row, uint32_t from, uint32_t to, float bound,
+                                              bool above) {
+  constexpr int N = 16 / sizeof(T);
+  for (uint32_t c = from + threadIdx.x * N; c < to; c += kThreads * N) {
+    float x[N];
+    load_or_fill<T, N>(row, c, to, x);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      if ((above ? x[i] > bound : x[i] >= bound) && c + i < to) {
+        const uint32_t at = atomicAdd(&sh.count, 1u);
+        if (at < kCandidates) sh.list[at] = candidate(x[i], c + i);
+      }
+    }
+  }
+}
+
+// Adds the first `need` columns whose logit equals `bound` to the list, in
+// their order.
+template <typename T>
+__device__ void list_equal(Shared& sh, const T* row, uint32_t from, uint32_t to, float bound, uint32_t need) {
+  uint32_t* part = reinterpret_cast<uint32_t*>(sh.maxima);
+  const uint32_t lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+  const uint32_t start = sh.count;
+  uint32_t found = 0;
+  for (uint32_t at = from; at < to && found < need; at += kThreads) {
+    const uint32_t c = at + threadIdx.x;
+    const float x = c < to ? float(row[c]) : 0.0f;
+    const bool equal = c < to && x == bound;
+    const uint64_t mask = __ballot(equal);
+    __syncthreads();
+    if (lane == 0) part[wave] = uint32_t(__popcll(mask));
+    __syncthreads();
+    uint32_t place = found + uint32_t(__popcll(mask & ((uint64_t(1) << lane) - 1)));
+    for (uint32_t w = 0; w < kWaves; ++w) {
+      if (w < wave) place += part[w];
+      found += part[w];
+    }
+    if (equal && place < need) sh.list[start + place] = candidate(x, c);
+  }
+  __syncthreads();
+}
+
+// sh.chosen = the k best of columns from..to (at least k columns); `m` is the
+// largest logit of this lane's part, `finite` that there is no NaN.
+template <typename T>
+__device__ void row_top(Shared& sh, const T* row, uint32_t from, uint32_t to, int k, float m, bool finite) {
+  if (!finite) {
+    plain_top(sh, row, from, to, k);
+    return;
+  }
+  __syncthreads();
+  sh.maxima[threadIdx.x] = m;
+  if (threadIdx.x == 0) sh.count = 0;
+  __syncthreads();
+  int before = 0;
+  for (int j = 0; j < kThreads; ++j) {
+    const float o = sh.maxima[j];
+    before += o > m || (o == m && j < int(threadIdx.x));
+  }
+  if (before == k - 1) sh.bound = m;
+  __syncthreads();
+  const float bound = sh.bound;
+  if (m >= bound) list_reaching(sh, row, from, to, bound, false);
+  __syncthreads();
+  uint32_t n = sh.count;
+  if (n > kCandidates) {
+    // many logits equal the bound (a mask's -inf, say): those above it, and the first of the equal ones
+    __syncthreads();
+    if (threadIdx.x == 0) sh.count = 0;
+    __syncthreads();
+    if (m > bound) list_reaching(sh, row, from, to, bound, true);
+    __syncthreads();
+    n = sh.count;
+    if (n > kCandidates - kMaxTop) {
+      plain_top(sh, row, from, to, k);
+      return;
+    }
+    if (n < uint32_t(k)) {
+      list_equal(sh, row, from, to, bound, uint32_t(k) - n);
+      n = uint32_t(k);
+    }
+  }
+  rank_list(sh, n, k);
+}
+
+template <typename I>
+__device__ __forceinline__ int64_t target_at(const I* targets, uint64_t row) { return int64_t(targets[row]); }
+
+struct Outputs {
+  float* logprob;
+  float* entropy;
+  float* lse;
+  float* top_logprob;
+  int64_t* top_index;
+};
+
+__device__ __forceinline__ float logprob_of(float x, const Summary& r) { return (x - r.shift) - r.rest; }
+
+// Writes a row's results; sh.chosen holds the alternatives.
+template <typename T, typename I>
+__device__ __forceinline__ void put(Shared& sh, const T* row, const I* targets, uint64_t i, uint32_t vocab, int k,
+                                    const Summary& r, const Outputs& out) {
+  if (threadIdx.x == 0) {
+    const int64_t target = target_at(targets, i);
+    float lp = 0;
+    if (target >= 0) {
+      lp = -kInf;
+      if (uint64_t(target) < vocab) lp = logprob_of(float(row[target]), r);
+      else if (r.lse != r.lse) lp = r.lse;
+    }
+    out.logprob[i] = lp;
+    out.entropy[i] = r.entropy;
+    out.lse[i] = r.lse;
+  }
+  if (int(threadIdx.x) < k) {
+    const uint64_t c = sh.chosen[threadIdx.x];
+    out.top_logprob[i * k + threadIdx.x] = logprob_of(value_of(uint32_t(c >> 32)), r);
+    out.top_index[i * k + threadIdx.x] = column_of(c);
+  }
+}
+
+template <typename T, typename I>
+__global__ __launch_bounds__(kThreads) void row_kernel(const T* logits, const I* targets, uint64_t stride,
+                                                       uint32_t vocab, int k, Outputs out) {
+  __shared__ Shared sh;
+  const uint64_t i = blockIdx.x;
+  const T* row = logits + i * stride;
+  const Stats mine = row_stats(row, 0, vocab);
+  const Stats all = block_join(sh, mine);
+  const bool ok = sound(all);
+  const Summary r = ok ? summary_of(all) : plain_summary(sh, row, vocab);
+  if (k) row_top(sh, row, 0, vocab, k, mine.m, r.lse == r.lse);
+  put(sh, row, targets, i, vocab, k, r, out);
+}
+
+// ----------------------------------------------------------------- gradient
+
+template <typename T, typename I>
+__global__ __launch_bounds__(kThreads) void grad_kernel(const T* logits, const I* targets, uint64_t stride,
+                                                        uint32_t vocab, uint32_t columns, const float* lse,
+                                                        const float* entropy, const float* g_logprob,
+                                                        const float* g_entropy, T* grad, uint64_t grad_stride) {
+  constexpr int N = 16 / sizeof(T);
+  const uint64_t i = blockIdx.x;
+  const T* row = logits + i * stride;
+  T* to = grad + i * grad_stride;
+  const int64_t target = target_at(targets, i);
+  const float l = lse[i], h = entropy[i];
+  const float gl = g_logprob && target >= 0 ? g_logprob[i] : 0.0f;
+  const float gh = g_entropy ? g_entropy[i] : 0.0f;
+  const float base = fmaf(gh, h, gl);      // grad = [target] gl - p (gl + gh (ln p + h))
+  const bool empty = l == -kInf;
+  auto value = [&](float x, uint32_t c) {
+    const float d = x - l;
+    const float p = exp2_fast(d * kLog2e);             // NaN stays NaN
+    float g = -p * fmaf(gh, fmaxf(d, -200.0f), base);
+    if (int64_t(c) == target) g += gl;
+    return empty || c >= vocab ? 0.0f : g;
+  };
+  for (uint32_t c = blockIdx.y * kThreads * N + threadIdx.x * N; c < columns; c += gridDim.y * kThreads * N) {
+    if (c + N <= columns) {
+      float x[N];
+      load<T, N>(row + c, x);
+#pragma unroll
+      for (int k = 0; k < N; ++k) x[k] = value(x[k], c + k);
+      store<T, N>(to + c, x);
+    } else {
+      for (uint32_t k = c; k < columns; ++k) to[k] = T(value(float(row[k]), k));
+    }
+  }
+}
+
+// ---------------------------------------------------------------------- host
+
+int check_shape(const char* who, const sr_logprob_shape* s) {
+  if (s == nullptr) return fail(SR_EINVAL, "%s: null argument", who);
+  if (s->target_dtype != SR_DT_I32 && s->target_dtype != SR_DT_I64)
+    return fail(SR_EDTYPE, "%s: targets of dtype %d", who, s->target_dtype);
+  if (s->dtype != SR_DT_F32 && s->dtype != SR_DT_BF16 && s->dtype != SR_DT_F16)
+    return fail(SR_EDTYPE, "%s: logits of dtype %d", who, s->dtype);
+  if (s->rows > SR_STEP_MAX_ROWS || s->columns > SR_STEP_MAX_ROWS)
+    return fail(SR_EBOUNDS, "%s: %llu rows of %llu columns", who, (unsigned long long)s->rows,
+                (unsigned long long)s->columns);
+  if (s->vocab < 1 || s->vocab > s->columns)
+    return fail(SR_EINVAL, "%s: a vocabulary of %llu in %llu columns", who, (unsigned long long)s->vocab,
+                (unsigned long long)s->columns);
+  if (s->stride < s->columns || s->stride > SR_STEP_MAX_ELEMENTS)
+    return fail(SR_EINVAL, "%s: rows %llu apart for %llu columns", who, (unsigned long long)s->stride,
+                (unsigned long long)s->columns);
+  if (s->rows && (s->logits == nullptr || s->targets == nullptr)) return fail(SR_EINVAL, "%s: null argument", who);
+  if (reinterpret_cast<uintptr_t>(s->logits) % sr_internal::dtype_size(s->dtype) ||
+      reinterpret_cast<uintptr_t>(s->targets) % sr_internal::dtype_size(s->target_dtype))
+    return fail(SR_EALIGN, "%s: not aligned to the elements", who);
+  return SR_OK;
+}
+
+int check_top(const char* who, const sr_logprob_shape& s, int32_t top) {
+  if (top < 0 || top > kMaxTop || uint64_t(top) > s.vocab)
+    return fail(SR_EINVAL, "%s: the best %d of %llu (at most %d)", who, top, (unsigned long long)s.vocab, kMaxTop);
+  return SR_OK;
+}
+
+// f(logits, targets) with their types.
+template <typename T, typename F>
+void with_targets(const sr_logprob_shape& s, F&& f) {
+  if (s.target_dtype == SR_DT_I64) f(static_cast<const T*>(s.logits), static_cast<const int64_t*>(s.targets));
+  else f(static_cast<const T*>(s.logits), static_cast<const int32_t*>(s.targets));
+}
+
+template <typename F>
+void with_types(const sr_logprob_shape& s, F&& f) {
+  if (s.dtype == SR_DT_F32) with_targets<float>(s, f);
+  else if (s.dtype == SR_DT_BF16) with_targets<bf16>(s, f);
+  else with_targets<f16>(s, f);
+}
+
+}  // namespace
+
+extern "C" {
+
+int sr_logprob_workspace(const sr_logprob_shape* shape, int32_t top, uint64_t* bytes) {
+  if (bytes == nullptr) return fail(SR_EINVAL, "sr_logprob_workspace: null argument");
+  if (int rc = check_shape("sr_logprob_workspace", shape)) return rc;
+  if (int rc = check_top("sr_logprob_workspace", *shape, top)) return rc;
+  *bytes = 0;
+  return SR_OK;
+}
+
+int sr_logprob(const sr_logprob_shape* shape, int32_t top, float* logprob, float* entropy, float* lse,
+               float* top_logprob, int64_t* top_index, void* workspace, uint64_t workspace_bytes, hipStream_t stream) {
+  uint64_t need = 0;
+  if (int rc = sr_logprob_workspace(shape, top, &need)) return rc;
+  const sr_logprob_shape& s = *shape;
+  if (s.rows == 0) return SR_OK;
+  if (!logprob || !entropy || !lse || (top && (!top_logprob || !top_index)))
+    return fail(SR_EINVAL, "sr_logprob: an output is null");
+  for (const float* p : {logprob, entropy, lse, top_logprob})
+    if (reinterpret_cast<uintptr_t>(p) % 4) return fail(SR_EALIGN, "sr_logprob: an output is not aligned");
+  if (reinterpret_cast<uintptr_t>(top_index) % 8) return fail(SR_EALIGN, "sr_logprob: an output is not aligned");
+  if (workspace_bytes < need || (need && workspace == nullptr))
+    return fail(SR_EINVAL, "sr_logprob: a workspace of %llu bytes, %llu are needed", (unsigned long long)workspace_bytes,
+                (unsigned long long)need);
+  if (reinterpret_cast<uintptr_t>(workspace) % 16) return fail(SR_EALIGN, "sr_logprob: workspace not aligned");
+  const Outputs out{logprob, entropy, lse, top_logprob, top_index};
+  with_types(s, [&](auto* logits, auto* targets) {
+    row_kernel<<<uint32_t(s.rows), kThreads, 0, stream>>>(logits, targets, s.stride, uint32_t(s.vocab), int(top), out);
+  });
+  return launched("sr_logprob");
+}
+
+int sr_logprob_grad(const sr_logprob_shape* shape, const float* lse, const float* entropy, const float* g_logprob,
+                    const float* g_entropy, void* grad, uint64_t grad_stride, hipStream_t stream) {
+  if (int rc = check_shape("sr_logprob_grad", shape)) return rc;
+  const sr_logprob_shape& s = *shape;
+  if (s.rows == 0) return SR_OK;
+  if (!lse || !entropy || !grad) return fail(SR_EINVAL, "sr_logprob_grad: null argument");
+  if (grad_stride < s.columns || grad_stride > SR_STEP_MAX_ELEMENTS)
+    return fail(SR_EINVAL, "sr_logprob_grad: rows %llu apart for %llu columns", (unsigned long long)grad_stride,
+                (unsigned long long)s.columns);
+  for (const float* p : {lse, entropy, g_logprob, g_entropy})
+    if (reinterpret_cast<uintptr_t>(p) % 4) return fail(SR_EALIGN, "sr_logprob_grad: not aligned to the elements");
+  const uint64_t size = sr_internal::dtype_size(s.dtype);
+  if (reinterpret_cast<uintptr_t>(grad) % size) return fail(SR_EALIGN, "sr_logprob_grad: not aligned to the elements");
+  auto span = [&](const void* p, uint64_t rows, uint64_t step, uint64_t cols, uint64_t item) {
+    const uintptr_t a = reinterpret_cast<uintptr_t>(p);
+    return std::pair<uintptr_t, uintptr_t>(a, p ? a + ((rows - 1) * step + cols) * item : a);
+  };
+  const auto to = span(grad, s.rows, grad_stride, s.columns, size);
+  auto clash = [&](std::pair<uintptr_t, uintptr_t> o) { return to.first < o.second && o.first < to.second; };
+  const bool in_place = grad == s.logits && grad_stride == s.stride;
+  if ((!in_place && clash(span(s.logits, s.rows, s.stride, s.columns, size))) ||
+      clash(span(s.targets, 1, 0, s.rows, sr_internal::dtype_size(s.target_dtype))) ||
+      clash(span(lse, 1, 0, s.rows, 4)) || clash(span(entropy, 1, 0, s.rows, 4)) ||
+      clash(span(g_logprob, 1, 0, s.rows, 4)) || clash(span(g_entropy, 1, 0, s.rows, 4)))
+    return fail(SR_EOVERLAP, "sr_logprob_grad: the gradient overlaps an input");
+  with_types(s, [&](auto* logits, auto* targets) {
+    typedef typename std::remove_const<typename std::remove_pointer<decltype(logits)>::type>::type T;
+    constexpr uint32_t kSpan = kThreads * 16 / sizeof(T) * 4;
+    const dim3 grid(uint32_t(s.rows), uint32_t(std::min<uint64_t>((s.columns + kSpan - 1) / kSpan, 65535)));
+    grad_kernel<<<grid, kThreads, 0, stream>>>(logits, targets, s.stride, uint32_t(s.vocab), uint32_t(s.columns), lse,
+                                               entropy, g_logprob, g_entropy, static_cast<T*>(grad), grad_stride);
+  });
+  return launched("sr_logprob_grad");
+}
+
+}  // extern "C"

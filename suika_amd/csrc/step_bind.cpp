@@ -374,6 +374,75 @@ at::Tensor vocab_embedding_grad(const at::Tensor& tokens, const at::Tensor& grad
   return to;
 }
 
+sr_logprob_shape logprob_shape(const at::Tensor& logits, const at::Tensor& targets, const c10::optional<int64_t>& vocab) {
+  if (logits.dim() != targets.dim() + 1 || logits.sizes().slice(0, targets.dim()) != targets.sizes())
+    plan_error("logits: a tensor of the targets' shape and the columns is wanted");
+  if (!logits.is_cuda() || !targets.is_contiguous()) plan_error("logits on the GPU and contiguous targets are wanted");
+  check_device(targets, "targets", logits.device());
+  const int64_t columns = logits.size(-1), v = vocab ? *vocab : columns;
+  if (v < 1 || v > columns)
+    plan_error("a vocabulary of " + std::to_string(v) + " in " + std::to_string(columns) + " columns");
+  return {logits.data_ptr(), targets.data_ptr(), index_code(targets, "targets"), float_code(logits, "logits"),
+          uint64_t(targets.numel()), uint64_t(columns), uint64_t(v), row_stride(logits, "logits")};
+}
+
+py::tuple token_logprobs(const at::Tensor& logits, const at::Tensor& targets, int64_t top,
+                         const c10::optional<int64_t>& vocab) {
+  const sr_logprob_shape s = logprob_shape(logits, targets, vocab);
+  if (top < 0 || top > SR_LOGPROB_MAX_TOP || uint64_t(top) > s.vocab)
+    plan_error("top " + std::to_string(top) + " of a vocabulary of " + std::to_string(s.vocab) + " (at most " +
+               std::to_string(SR_LOGPROB_MAX_TOP) + ")");
+  const at::Device device = logits.device();
+  const c10::DeviceGuard guard(device);
+  const at::TensorOptions f32 = on(device, at::kFloat);
+  at::Tensor logprob = at::empty(targets.sizes(), f32), entropy = at::empty(targets.sizes(), f32),
+             lse = at::empty(targets.sizes(), f32), best, index, work;
+  if (top) {
+    std::vector<int64_t> shape(targets.sizes().begin(), targets.sizes().end());
+    shape.push_back(top);
+    best = at::empty(shape, f32);
+    index = at::empty(shape, on(device, at::kLong));
+  }
+  uint64_t need = 0;
+  check(sr_logprob_workspace(&s, int32_t(top), &need), "sr_logprob");
+  if (need) work = at::empty({int64_t(need)}, on(device, at::kByte));
+  check(sr_logprob(&s, int32_t(top), logprob.data_ptr<float>(), entropy.data_ptr<float>(), lse.data_ptr<float>(),
+                   top ? best.data_ptr<float>() : nullptr, top ? index.data_ptr<int64_t>() : nullptr,
+                   need ? work.data_ptr() : nullptr, need, stream_of(device)),
+        "sr_logprob");
+  if (!top) return py::make_tuple(logprob, entropy, lse, py::none(), py::none());
+  return py::make_tuple(logprob, entropy, lse, best, index);
+}
+
+const float* row_values(const at::Tensor& t, const char* what, const at::Tensor& targets) {
+  check_device(t, what, targets.device());
+  if (t.scalar_type() != at::kFloat || t.sizes() != targets.sizes() || !t.is_contiguous())
+    plan_error(std::string(what) + ": a contiguous float32 tensor of the targets' shape is wanted");
+  return t.data_ptr<float>();
+}
+
+at::Tensor token_logprobs_grad(const at::Tensor& logits, const at::Tensor& targets, const at::Tensor& lse,
+                               const at::Tensor& entropy, const c10::optional<at::Tensor>& grad_logprob,
+                               const c10::optional<at::Tensor>& grad_entropy, const c10::optional<int64_t>& vocab,
+                               const c10::optional<at::Tensor>& out) {
+  const sr_logprob_shape s = logprob_shape(logits, targets, vocab);
+  const float* l = row_values(lse, "lse", targets);
+  const float* h = row_values(entropy, "entropy", targets);
+  const float* gl = grad_logprob ? row_values(*grad_logprob, "grad_logprob", targets) : nullptr;
+  const float* gh = grad_entropy ? row_values(*grad_entropy, "grad_entropy", targets) : nullptr;
+  const c10::DeviceGuard guard(logits.device());
+  if (out) {
+    check_device(*out, "out", logits.device());
+    if (out->sizes() != logits.sizes() || out->scalar_type() != logits.scalar_type())
+      plan_error("out: a tensor of the logits' shape and dtype is wanted");
+  }
+  at::Tensor to = out ? *out : at::empty(logits.sizes(), on(logits.device(), logits.scalar_type()));
+  const uint64_t stride = row_stride(to, "out");
+  check(sr_logprob_grad(&s, l, h, gl, gh, to.data_ptr(), stride, stream_of(logits.device())), "sr_logprob_grad");
+  if (out) written(to);
+  return to;
+}
+
 }  // namespace
 
 namespace suika_host {
@@ -391,6 +460,9 @@ void bind_step(py::module_& m) {
         py::arg("vocab_start"), py::arg("out"));
   m.def("vocab_embedding_grad", &vocab_embedding_grad, py::arg("tokens"), py::arg("grad_output"), py::arg("rows"),
         py::arg("scale"), py::arg("vocab_start"), py::arg("dtype"), py::arg("out"), py::arg("accumulate"));
+  m.def("token_logprobs", &token_logprobs, py::arg("logits"), py::arg("targets"), py::arg("top"), py::arg("vocab"));
+  m.def("token_logprobs_grad", &token_logprobs_grad, py::arg("logits"), py::arg("targets"), py::arg("lse"),
+        py::arg("entropy"), py::arg("grad_logprob"), py::arg("grad_entropy"), py::arg("vocab"), py::arg("out"));
 }
 
 }  // namespace suika_host

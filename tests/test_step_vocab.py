@@ -6,7 +6,7 @@ import ctypes
 import pytest
 import torch
 
-from suika_amd import PlanError, vocab_embedding, vocab_embedding_grad
+from suika_amd import PlanError, token_logprobs, vocab_embedding, vocab_embedding_grad
 from suika_amd import _lib
 
 vp, u64 = ctypes.c_void_p, ctypes.c_uint64
@@ -103,3 +103,91 @@ def test_torch_entry_points_refuse():
         vocab_embedding(tokens, weight[0])
     with pytest.raises(PlanError, match="tokens' shape"):
         vocab_embedding_grad(tokens, torch.zeros(2, 8), 4)
+
+
+class LogprobShape(ctypes.Structure):
+    _fields_ = [("logits", vp), ("targets", vp), ("target_dtype", ctypes.c_int32), ("dtype", ctypes.c_int32),
+                ("rows", u64), ("columns", u64), ("vocab", u64), ("stride", u64)]
+
+
+def logprob_shape(**kw):
+    f = dict(logits=BASE, targets=BASE + (1 << 20), target_dtype=I64, dtype=F32, rows=4, columns=16, vocab=15,
+             stride=16)
+    f.update(kw)
+    return LogprobShape(**f)
+
+
+OUT = BASE + (1 << 21)
+
+
+def logprob(top=2, out=(OUT, OUT + 64, OUT + 128, OUT + 192, OUT + 256), work=OUT + 4096, work_bytes=1 << 20, **kw):
+    s = logprob_shape(**kw)
+    return _lib.lib().sr_logprob(ctypes.byref(s), top, *[vp(p) for p in out], vp(work), u64(work_bytes), None)
+
+
+def logprob_grad(lse=OUT, entropy=OUT + 64, gl=OUT + 128, gh=OUT + 192, grad=OUT + 4096, stride=16, **kw):
+    s = logprob_shape(**kw)
+    return _lib.lib().sr_logprob_grad(ctypes.byref(s), vp(lse), vp(entropy), vp(gl), vp(gh), vp(grad), u64(stride),
+                                      None)
+
+
+@pytest.mark.parametrize("shape,code", [
+    (dict(target_dtype=F32), _lib.SR_EDTYPE),
+    (dict(dtype=I64), _lib.SR_EDTYPE),
+    (dict(rows=(1 << 23) + 1), _lib.SR_EBOUNDS),
+    (dict(columns=(1 << 23) + 1, stride=1 << 24), _lib.SR_EBOUNDS),
+    (dict(vocab=0), _lib.SR_EINVAL),
+    (dict(vocab=17), _lib.SR_EINVAL),
+    (dict(stride=15), _lib.SR_EINVAL),
+    (dict(logits=None), _lib.SR_EINVAL),
+    (dict(targets=None), _lib.SR_EINVAL),
+    (dict(logits=BASE + 2), _lib.SR_EALIGN),
+    (dict(targets=BASE + 4), _lib.SR_EALIGN),
+])
+def test_logprob_shapes_refused(shape, code):
+    assert logprob(**shape) == code and _lib.last_error()
+    assert logprob_grad(**shape) == code
+    need = u64()
+    assert _lib.lib().sr_logprob_workspace(ctypes.byref(logprob_shape(**shape)), 2, ctypes.byref(need)) == code
+
+
+@pytest.mark.parametrize("kw,code", [
+    (dict(top=-1), _lib.SR_EINVAL),
+    (dict(top=65, columns=100, vocab=100, stride=100), _lib.SR_EINVAL),
+    (dict(top=16), _lib.SR_EINVAL),                                   # more than the vocabulary
+    (dict(out=(None, OUT, OUT, OUT, OUT)), _lib.SR_EINVAL),
+    (dict(out=(OUT, OUT, OUT, None, OUT)), _lib.SR_EINVAL),
+    (dict(out=(OUT, OUT + 2, OUT, OUT, OUT)), _lib.SR_EALIGN),
+    (dict(out=(OUT, OUT, OUT, OUT, OUT + 4)), _lib.SR_EALIGN),
+    (dict(work=OUT + 8), _lib.SR_EALIGN),
+])
+def test_logprob_refused(kw, code):
+    assert logprob(**kw) == code and "sr_logprob" in _lib.last_error()
+
+
+@pytest.mark.parametrize("kw,code", [
+    (dict(lse=None), _lib.SR_EINVAL),
+    (dict(entropy=None), _lib.SR_EINVAL),
+    (dict(grad=None), _lib.SR_EINVAL),
+    (dict(stride=15), _lib.SR_EINVAL),
+    (dict(grad=OUT + 4098), _lib.SR_EALIGN),
+    (dict(gl=OUT + 130), _lib.SR_EALIGN),
+    (dict(grad=BASE + 4), _lib.SR_EOVERLAP),
+    (dict(grad=BASE, stride=17), _lib.SR_EOVERLAP),
+    (dict(grad=OUT + 8), _lib.SR_EOVERLAP),
+    (dict(grad=BASE + (1 << 20)), _lib.SR_EOVERLAP),
+])
+def test_logprob_grad_refused(kw, code):
+    assert logprob_grad(**kw) == code and "sr_logprob_grad" in _lib.last_error()
+
+
+def test_logprob_of_nothing():
+    assert logprob(rows=0, logits=None, targets=None) == 0
+    assert logprob_grad(rows=0, logits=None, targets=None) == 0
+
+
+def test_token_logprobs_refuses():
+    with pytest.raises(PlanError, match="GPU"):
+        token_logprobs(torch.zeros(3, 5), torch.zeros(3, dtype=torch.int64))
+    with pytest.raises(PlanError, match="targets' shape"):
+        token_logprobs(torch.zeros(3, 5), torch.zeros(4, dtype=torch.int64))

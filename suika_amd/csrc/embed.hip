@@ -6,10 +6,11 @@
 // order in which workgroups run, so the tokens are sorted first (a stable
 // counting sort, one launch) and every row sums its own in that order:
 //
-//   sort    Workgroup b owns a range of rows and reads all tokens, which come
-//           from the L2: it counts those of lower rows, which is where its
-//           own start in the sorted list, and those of each of its rows, and
-//           places them in a second pass.  No workgroup waits for another.
+//   sort    Workgroup b of B owns rows b, b + B, ... (frequent tokens are
+//           neighbours in a vocabulary) and reads all tokens, which come from
+//           the L2: it counts those of the workgroups before it, which is where
+//           its own start in the sorted list, and those of each of its rows,
+//           and places them in a second pass.  No workgroup waits for another.
 //   sum     A group of lanes per row adds up the row's tokens, each lane one
 //           16-byte column block.  A row of many tokens (a space, a filler) is
 //           cut into pieces that are summed side by side, into 32-bit partial
@@ -29,47 +30,60 @@ using namespace sr_step;
 
 constexpr int kThreads = 256;
 
-// Lanes of one row: each takes a 16-byte block of columns, the last one what
-// is left of a row.  Groups of a power of two lanes share a workgroup; rows of
-// more blocks than lanes take several workgroups.
+// The lanes of one row: a group of a power of two, each of them taking every
+// `lanes`-th 16-byte block of the row's columns, U blocks in all; the row's last
+// block may be shorter.  A row of more blocks takes several groups.
 struct Lanes {
   uint32_t blocks;      // column blocks of a row
   uint32_t log2;        // lanes of a group
   uint32_t slices;      // groups along a row
 };
 
-Lanes lanes_of(uint64_t cols, uint32_t per_block) {
+Lanes lanes_of(uint64_t cols, uint32_t per_block, uint32_t most, uint32_t each) {
   Lanes l;
   l.blocks = uint32_t((cols + per_block - 1) / per_block);
   l.log2 = 0;
-  while ((1u << l.log2) < l.blocks && (1u << l.log2) < kThreads) ++l.log2;
-  l.slices = (l.blocks + kThreads - 1) / kThreads;
+  while ((1u << l.log2) * each < l.blocks && (1u << l.log2) < most) ++l.log2;
+  l.slices = (l.blocks + (each << l.log2) - 1) / (each << l.log2);
   return l;
+}
+
+// The first column of this lane's blocks, and from one of them to the next.
+template <int N, int U>
+__device__ __forceinline__ uint64_t first_column(const Lanes& l) {
+  return (uint64_t(blockIdx.y * U << l.log2) + (threadIdx.x & ((1u << l.log2) - 1))) * N;
 }
 
 // --------------------------------------------------------------------- rows
 
-template <typename T, typename I>
+constexpr int kLookupBlocks = 2;      // of a lane
+
+template <typename T, typename I, int U>
 __global__ __launch_bounds__(kThreads) void embedding_kernel(const I* tokens, const T* weight, T* out, uint32_t n_tokens,
                                                              uint64_t rows, uint64_t cols, uint64_t stride,
-                                                             int64_t start, float scale, Lanes l) {
+                                                             uint64_t start, float scale, Lanes l) {
   constexpr int N = 16 / sizeof(T);
   const uint32_t i = (blockIdx.x << (8 - l.log2)) + (threadIdx.x >> l.log2);
-  const uint32_t block = blockIdx.y * kThreads + (threadIdx.x & ((1u << l.log2) - 1));
-  if (i >= n_tokens || block >= l.blocks) return;
-  const int64_t row = int64_t(tokens[i]) - start;
-  const uint64_t c = uint64_t(block) * N;
-  const bool inside = row >= 0 && uint64_t(row) < rows;
-  const T* src = weight + (inside ? uint64_t(row) * stride : 0) + c;
+  if (i >= n_tokens) return;
+  const uint64_t row = uint64_t(int64_t(tokens[i])) - start;
+  const uint64_t c = first_column<N, U>(l), step = uint64_t(N) << l.log2;
+  const bool inside = row < rows;
+  const T* src = weight + (inside ? row * stride : 0) + c;
   T* dst = out + uint64_t(i) * cols + c;
-  if (c + N <= cols) {
-    float x[N] = {};
-    if (inside) load<T, N>(src, x);
+  float x[U][N] = {};
 #pragma unroll
-    for (int k = 0; k < N; ++k) x[k] *= scale;
-    store<T, N>(dst, x);
-  } else {
-    for (uint64_t k = 0; c + k < cols; ++k) dst[k] = inside ? T(float(src[k]) * scale) : T(0.0f);
+  for (int u = 0; u < U; ++u)
+    if (inside && c + u * step + N <= cols) load<T, N>(src + u * step, x[u]);
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const uint64_t at = c + u * step;
+    if (at + N <= cols) {
+#pragma unroll
+      for (int k = 0; k < N; ++k) x[u][k] *= scale;
+      store_stream<T, N>(dst + u * step, x[u]);
+    } else {
+      for (uint64_t k = at; k < cols; ++k) dst[k - c] = inside ? T(float(src[k - c]) * scale) : T(0.0f);
+    }
   }
 }
 
@@ -77,38 +91,56 @@ __global__ __launch_bounds__(kThreads) void embedding_kernel(const I* tokens, co
 
 constexpr int kSortThreads = 1024;
 constexpr int kSortWaves = kSortThreads / kWave;
-constexpr uint32_t kSortRanges = 256;     // workgroups, one a compute unit
-constexpr uint32_t kSortRows = 512;       // most rows of one range
+constexpr uint32_t kSortRows = 512;       // most rows of one workgroup
 
-// A piece of a row's tokens: sorted positions from..to, the k-th of its row.
+// The order in which rows are sorted: by the workgroup that owns them.
+struct Owners {
+  uint32_t log2;     // of the number of workgroups
+  uint32_t range;    // rows of each
+
+};
+
+// One workgroup a compute unit, or more where that many rows have no room.
+Owners owners_of(uint64_t rows) {
+  Owners o{8, 0};
+  while ((rows + (1u << o.log2) - 1) >> o.log2 > kSortRows) ++o.log2;
+  o.range = uint32_t((rows + (1u << o.log2) - 1) >> o.log2);
+  return o;
+}
+
+// A piece of a row's tokens: sorted positions from..to.  The pieces of a row
+// follow one another; the first says how many they are.
 struct alignas(16) Piece {
   uint32_t row;      // kNoPiece: none
   uint32_t from, to;
-  uint32_t k;
+  uint32_t pieces;
 };
 constexpr uint32_t kNoPiece = 0xffffffffu;
 
+// The sorted positions of a row's tokens.
+struct Run {
+  uint32_t from, to;
+};
+
 // What the launches hand on, in the workspace.
 struct Sorted {
-  uint32_t* offset;   // [rows + 1] first sorted position of each row's tokens
+  Run* run;           // [rows]
+  uint32_t* tokens;   // [1] how many lie in the shard
   uint32_t* order;    // [tokens] sorted position -> index of the token
   Piece* piece;       // [slots]
   float* partial;     // [slots][cols]
 };
 
-// The lanes whose tokens are of one row are taken together: f(row, which lanes,
-// the lowest of them, this lane's place among them), row after row.
-template <typename F>
-__device__ __forceinline__ void by_row(bool in, uint32_t row, F&& f) {
-  uint64_t left = __ballot(in);
-  const uint64_t below = (uint64_t(1) << (threadIdx.x % kWave)) - 1;
-  while (left) {
-    const int leader = __ffsll((unsigned long long)left) - 1;
-    const uint32_t r = __builtin_amdgcn_readlane(row, leader);
-    const uint64_t same = __ballot(in && row == r);
-    f(r, same, leader, uint32_t(__popcll(same & below)));
-    left &= ~same;
+// The lanes whose tokens are of the same row as this lane's: of those in `in`,
+// the ones that agree in all `bits` bits of it.
+__device__ __forceinline__ uint64_t same_row(uint64_t in, uint32_t row, uint32_t bits) {
+  uint64_t same = in;
+  for (uint32_t b = 0; b < bits; ++b) {
+    const bool set = row >> b & 1;
+    const uint64_t ones = __ballot(set);
+    same &= set ? ones : ~ones;
   }
+  return same;
 }
 
 __device__ __forceinline__ uint32_t wave_scan(uint32_t x) {   // inclusive
@@ -136,73 +168,122 @@ __device__ __forceinline__ uint32_t block_scan(uint32_t x, uint32_t* part, uint3
   return before + inclusive - x;
 }
 
+// Tokens that a lane reads at once.
+constexpr uint32_t kSortAhead = 8;
+// Tokens of its own that a wave remembers between the passes; a wave that finds
+// more reads its run again.
+constexpr uint32_t kSortKept = 448;
+constexpr uint32_t kOutside = 0xffffffffu;
+
+// A token's row of the shard, kOutside for those of other shards.
 template <typename I>
-__global__ __launch_bounds__(kSortThreads) void sort_kernel(const I* tokens, uint32_t n_tokens, uint64_t rows,
-                                                            int64_t start, uint32_t range, uint32_t piece,
-                                                            Sorted out) {
+__device__ __forceinline__ uint32_t row_of(I token, uint64_t start, uint32_t rows) {
+  const uint64_t row = uint64_t(int64_t(token)) - start;
+  return row < rows ? uint32_t(row) : kOutside;
+}
+
+// f(index, row) for a wave's tokens from..to, 64 at a time in their order; every
+// lane calls it, with kOutside where there is no token.
+template <typename I, typename F>
+__device__ __forceinline__ void for_tokens(const I* tokens, uint32_t from, uint32_t to, uint64_t start, uint32_t rows,
+                                           F&& f) {
+  uint32_t i = from + threadIdx.x % kWave;
+  for (; from + kSortAhead * kWave <= to; from += kSortAhead * kWave) {
+    I t[kSortAhead];
+#pragma unroll
+    for (uint32_t a = 0; a < kSortAhead; ++a) t[a] = tokens[i + a * kWave];
+#pragma unroll
+    for (uint32_t a = 0; a < kSortAhead; ++a) f(i + a * kWave, row_of(t[a], start, rows));
+    i += kSortAhead * kWave;
+  }
+  for (; from < to; from += kWave, i += kWave) f(i, i < to ? row_of(tokens[i], start, rows) : kOutside);
+}
+
+template <typename I>
+__global__ __launch_bounds__(kSortThreads) void sort_kernel(const I* tokens, uint32_t n_tokens, uint32_t rows,
+                                                            uint64_t start, Owners owners, uint32_t bits,
+                                                            uint32_t piece, Sorted out) {
   __shared__ uint32_t count[kSortWaves * kSortRows];
   __shared__ uint32_t part[kSortWaves];
+  __shared__ uint32_t kept[kSortWaves][kSortKept], kept_row[kSortWaves][kSortKept];
   const uint32_t wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
-  const uint64_t first = uint64_t(blockIdx.x) * range;
-  const uint32_t own = uint32_t(rows - first < range ? rows - first : range);
+  const uint64_t below = (uint64_t(1) << lane) - 1;
+  const uint32_t me = blockIdx.x, range = owners.range, mask = (1u << owners.log2) - 1;
   for (uint32_t i = threadIdx.x; i < kSortWaves * range; i += kSortThreads) count[i] = 0;
   __syncthreads();
 
   // Every wave takes a run of the tokens, so waves and lanes are in their order.
   const uint32_t run = (n_tokens + kSortThreads - 1) / kSortThreads * kWave;
-  const uint32_t from = wave * run;
-  const uint32_t to = from < n_tokens ? (n_tokens - from < run ? n_tokens : from + run) : from;
+  const uint32_t from = min(wave * run, n_tokens), to = min(from + run, n_tokens);
   uint32_t* mine = count + wave * range;
-  uint32_t lower = 0;
-  for (uint32_t i = from + lane; i - lane < to; i += kWave) {
-    const int64_t r = i < to ? int64_t(tokens[i]) - start : -1;
-    const bool here = r >= 0 && uint64_t(r) < rows;
-    lower += here && uint64_t(r) < first;
-    const uint64_t local = uint64_t(r) - first;
-    by_row(here && uint64_t(r) >= first && local < own, uint32_t(local),
-           [&](uint32_t row, uint64_t same, int leader, uint32_t) {
-             if (int(lane) == leader) atomicAdd(mine + row, uint32_t(__popcll(same)));
-           });
-  }
+  uint32_t lower = 0, found = 0;
+  for_tokens(tokens, from, to, start, rows, [&](uint32_t i, uint32_t r) {
+    const uint32_t owner = r & mask;
+    lower += r != kOutside && owner < me;
+    const bool own = r != kOutside && owner == me;
+    const uint64_t any = __ballot(own);
+    if (any == 0) return;
+    if (own) {
+      atomicAdd(mine + (r >> owners.log2), 1u);
+      const uint32_t k = found + uint32_t(__popcll(any & below));
+      if (k < kSortKept) {
+        kept[wave][k] = i;
+        kept_row[wave][k] = r >> owners.log2;
+      }
+    }
+    found += uint32_t(__popcll(any));
+  });
   uint32_t base = 0, total = 0, pieces = 0;
-  block_scan(lower, part, &base);      // the sum: where this range starts
+  block_scan(lower, part, &base);      // the sum: where this workgroup's rows start
 
-  // Thread r: the tokens of row r, and where each wave puts its part of them.
+  // Thread q: the tokens of row q of this workgroup, and where each wave puts its part of them.
   uint32_t n = 0;
-  if (threadIdx.x < own)
+  if (threadIdx.x < range)
     for (int w = 0; w < kSortWaves; ++w) n += count[w * range + threadIdx.x];
   const uint32_t at = base + block_scan(n, part, &total);
   const uint32_t cut = n > 2 * piece ? (n + piece - 1) / piece : 0;
   const uint32_t slot = block_scan(cut, part, &pieces);
-  if (threadIdx.x < own) {
+  if (threadIdx.x < range) {
     uint32_t next = at;
     for (int w = 0; w < kSortWaves; ++w) {
       const uint32_t c = count[w * range + threadIdx.x];
       count[w * range + threadIdx.x] = next;
       next += c;
     }
-    out.offset[first + threadIdx.x] = at;
-    if (first + threadIdx.x == rows - 1) out.offset[rows] = base + total;
+    const uint32_t row = (threadIdx.x << owners.log2) + me;
+    if (row < rows) out.run[row] = {at, at + n};
+    if (me == mask && threadIdx.x == 0) *out.tokens = base + total;
   }
-  // A range of `total` tokens has the slots from 2 base / piece on.  A row is
+  // A workgroup of `total` tokens has the slots from 2 base / piece on.  A row is
   // cut where it has more than 2 piece tokens, into at most 3/2 of n / piece
   // pieces, so they fit; the slots left over say that they are empty.
   const uint32_t slot0 = uint32_t(2 * uint64_t(base) / piece);
   const uint32_t slot1 = uint32_t(2 * uint64_t(base + total) / piece);
   for (uint32_t k = 0; k < cut; ++k)
-    out.piece[slot0 + slot + k] = {uint32_t(first + threadIdx.x), at + k * piece, min(at + (k + 1) * piece, at + n), k};
+    out.piece[slot0 + slot + k] = {(threadIdx.x << owners.log2) + me, at + k * piece, min(at + (k + 1) * piece, at + n),
+                                   k ? 0 : cut};
   for (uint32_t s = slot0 + pieces + threadIdx.x; s < slot1; s += kSortThreads) out.piece[s] = {kNoPiece, 0, 0, 0};
   __syncthreads();
 
-  for (uint32_t i = from + lane; i - lane < to; i += kWave) {
-    const int64_t r = i < to ? int64_t(tokens[i]) - start : -1;
-    const uint64_t local = uint64_t(r) - first;
-    const bool in = r >= 0 && uint64_t(r) >= first && local < own;
-    by_row(in, uint32_t(local), [&](uint32_t row, uint64_t same, int leader, uint32_t place) {
-      uint32_t next = 0;
-      if (int(lane) == leader) next = atomicAdd(mine + row, uint32_t(__popcll(same)));
-      next = __builtin_amdgcn_readlane(next, leader);
-      if (in && uint32_t(local) == row) out.order[next + place] = i;
+  // Lanes of one row take consecutive places, in their order, from where the row's last ones ended.
+  auto put = [&](uint32_t i, uint32_t local, bool own) {
+    const uint64_t any = __ballot(own);
+    if (any == 0) return;
+    const uint64_t same = same_row(any, local, bits);
+    const int leader = __ffsll((unsigned long long)same) - 1;
+    uint32_t next = 0;
+    if (own && int(lane) == leader) next = atomicAdd(mine + local, uint32_t(__popcll(same)));
+    next = __shfl(next, leader & (kWave - 1));
+    if (own) out.order[next + uint32_t(__popcll(same & below))] = i;
+  };
+  if (found <= kSortKept) {
+    for (uint32_t k = lane; k - lane < found; k += kWave) {
+      const bool own = k < found;
+      put(own ? kept[wave][k] : 0, own ? kept_row[wave][k] : 0, own);
+    }
+  } else {
+    for_tokens(tokens, from, to, start, rows, [&](uint32_t i, uint32_t r) {
+      put(i, r >> owners.log2, r != kOutside && (r & mask) == me);
     });
   }
 }
@@ -218,19 +299,25 @@ __device__ __forceinline__ void sum_tokens(const T* grad_out, uint64_t stride, c
   if (c + N <= cols) {
     uint32_t i = from;
     for (; i + kAhead <= to; i += kAhead) {
-      float x[kAhead][N];
+      Vec<T, N> x[kAhead];
 #pragma unroll
-      for (uint32_t a = 0; a < kAhead; ++a) load<T, N>(grad_out + order[i + a] * stride + c, x[a]);
+      for (uint32_t a = 0; a < kAhead; ++a)
+        x[a] = __builtin_nontemporal_load(reinterpret_cast<const Vec<T, N>*>(grad_out + order[i + a] * stride + c));
 #pragma unroll
       for (uint32_t a = 0; a < kAhead; ++a)
 #pragma unroll
-        for (int k = 0; k < N; ++k) acc[k] += x[a][k];
+        for (int k = 0; k < N; ++k) acc[k] += float(x[a][k]);
     }
-    for (; i < to; ++i) {
-      float x[N];
-      load<T, N>(grad_out + order[i] * stride + c, x);
+    if (i < to) {
+      Vec<T, N> x[kAhead];
 #pragma unroll
-      for (int k = 0; k < N; ++k) acc[k] += x[k];
+      for (uint32_t a = 0; a < kAhead - 1; ++a)
+        if (i + a < to) x[a] = __builtin_nontemporal_load(reinterpret_cast<const Vec<T, N>*>(grad_out + order[i + a] * stride + c));
+#pragma unroll
+      for (uint32_t a = 0; a < kAhead - 1; ++a)
+        if (i + a < to)
+#pragma unroll
+          for (int k = 0; k < N; ++k) acc[k] += float(x[a][k]);
     }
   } else {
     for (uint32_t i = from; i < to; ++i) {
@@ -251,7 +338,7 @@ __device__ __forceinline__ void put_row(G* grad, uint64_t c, uint64_t cols, floa
     if (accumulate) load<G, N>(grad + c, old);
 #pragma unroll
     for (int k = 0; k < N; ++k) acc[k] = fmaf(acc[k], scale, old[k]);
-    store<G, N>(grad + c, acc);
+    store_stream<G, N>(grad + c, acc);
   } else {
 #pragma unroll
     for (int k = 0; k < N; ++k)
@@ -259,59 +346,69 @@ __device__ __forceinline__ void put_row(G* grad, uint64_t c, uint64_t cols, floa
   }
 }
 
-// Tasks 0..slots are the pieces, the rows follow.
+// Tasks 0..slots are the pieces; the rows follow.
 template <typename T, typename G>
 __global__ __launch_bounds__(kThreads) void sum_kernel(const T* grad_out, uint64_t stride, G* grad, uint64_t rows,
                                                        uint64_t cols, uint32_t slots, uint32_t piece, float scale,
                                                        bool accumulate, Lanes l, Sorted in) {
   constexpr int N = 16 / sizeof(T);
   const uint64_t task = (uint64_t(blockIdx.x) << (8 - l.log2)) + (threadIdx.x >> l.log2);
-  const uint32_t block = blockIdx.y * kThreads + (threadIdx.x & ((1u << l.log2) - 1));
-  if (task >= slots + rows || block >= l.blocks) return;
-  const uint64_t c = uint64_t(block) * N;
+  const uint64_t c = first_column<N, 1>(l);
+  if (c >= cols) return;
   float acc[N] = {};
   if (task < slots) {
-    if (task >= uint32_t(2 * uint64_t(in.offset[rows]) / piece)) return;
+    if (task >= uint32_t(2 * uint64_t(*in.tokens) / piece)) return;
     const Piece p = in.piece[task];
     if (p.row == kNoPiece) return;
     sum_tokens<T, N>(grad_out, stride, in.order, p.from, p.to, c, cols, acc);
-    float* dst = in.partial + task * cols + c;
-#pragma unroll
-    for (int k = 0; k < N; ++k)
-      if (c + k < cols) dst[k] = acc[k];
+    put_row<float, N>(in.partial + task * cols, c, cols, 1.0f, false, acc);
     return;
   }
   const uint64_t row = task - slots;
-  const uint32_t from = in.offset[row], to = in.offset[row + 1];
-  if (to - from > 2 * piece || (accumulate && from == to)) return;
-  sum_tokens<T, N>(grad_out, stride, in.order, from, to, c, cols, acc);
+  if (row >= rows) return;
+  const Run run = in.run[row];
+  const uint32_t n = run.to - run.from;
+  if (n > 2 * piece || (accumulate && n == 0)) return;
+  sum_tokens<T, N>(grad_out, stride, in.order, run.from, run.to, c, cols, acc);
   put_row<G, N>(grad + row * cols, c, cols, scale, accumulate, acc);
 }
 
 template <typename G>
-__global__ __launch_bounds__(kThreads) void join_kernel(G* grad, uint64_t rows, uint64_t cols, uint32_t slots,
-                                                        uint32_t piece, float scale, bool accumulate, Lanes l,
-                                                        Sorted in) {
+__global__ __launch_bounds__(kThreads) void join_kernel(G* grad, uint64_t cols, uint32_t slots, uint32_t piece,
+                                                        float scale, bool accumulate, Lanes l, Sorted in) {
   constexpr int N = 4;
+  constexpr uint32_t kAhead = 8;
   const uint64_t task = (uint64_t(blockIdx.x) << (8 - l.log2)) + (threadIdx.x >> l.log2);
-  const uint32_t block = blockIdx.y * kThreads + (threadIdx.x & ((1u << l.log2) - 1));
-  if (task >= slots || block >= l.blocks || task >= uint32_t(2 * uint64_t(in.offset[rows]) / piece)) return;
+  if (task >= slots || task >= uint32_t(2 * uint64_t(*in.tokens) / piece)) return;
   const Piece p = in.piece[task];
-  if (p.row == kNoPiece || p.k != 0) return;
-  const uint32_t n = in.offset[p.row + 1] - in.offset[p.row];
-  const uint32_t pieces = (n + piece - 1) / piece;
-  const uint64_t c = uint64_t(block) * N;
+  const uint32_t pieces = p.pieces;
+  if (p.row == kNoPiece || pieces == 0) return;
+  const uint64_t c = first_column<N, 1>(l);
+  if (c >= cols) return;
   float acc[N] = {};
   const float* src = in.partial + task * cols + c;
-  for (uint32_t i = 0; i < pieces; ++i) {
-    if (c + N <= cols) {
+  uint32_t i = 0;
+  if (c + N <= cols) {
+    for (; i + kAhead <= pieces; i += kAhead) {
+      float x[kAhead][N];
+#pragma unroll
+      for (uint32_t a = 0; a < kAhead; ++a) load<float, N>(src + (i + a) * cols, x[a]);
+#pragma unroll
+      for (uint32_t a = 0; a < kAhead; ++a)
+#pragma unroll
+        for (int k = 0; k < N; ++k) acc[k] += x[a][k];
+    }
+    for (; i < pieces; ++i) {
       float x[N];
       load<float, N>(src + i * cols, x);
 #pragma unroll
       for (int k = 0; k < N; ++k) acc[k] += x[k];
-    } else {
-      for (int k = 0; c + k < cols; ++k) acc[k] += src[i * cols + k];
     }
+  } else {
+    for (; i < pieces; ++i)
+#pragma unroll
+      for (int k = 0; k < N; ++k)
+        if (c + k < cols) acc[k] += src[i * cols + k];
   }
   put_row<G, N>(grad + uint64_t(p.row) * cols, c, cols, scale, accumulate, acc);
 }
@@ -346,35 +443,38 @@ uint64_t extent(uint64_t rows, uint64_t cols, uint64_t stride, int32_t dt) {
   return rows && cols ? ((rows - 1) * stride + cols) * sr_internal::dtype_size(dt) : 0;
 }
 
-template <typename T>
-void launch_embedding(const sr_embedding_shape& s, const void* weight, uint64_t stride, void* out, hipStream_t stream) {
-  const Lanes l = lanes_of(s.cols, 16 / sizeof(T));
+template <typename T, typename I, int U>
+void launch_embedding_of(const sr_embedding_shape& s, const void* weight, uint64_t stride, void* out,
+                         hipStream_t stream) {
+  const Lanes l = lanes_of(s.cols, 16 / sizeof(T), kThreads, U);
   const uint32_t group = uint32_t(kThreads) >> l.log2;
   const dim3 grid(uint32_t((s.n_tokens + group - 1) / group), l.slices);
-  if (s.token_dtype == SR_DT_I64)
-    embedding_kernel<T, int64_t><<<grid, kThreads, 0, stream>>>(
-        static_cast<const int64_t*>(s.tokens), static_cast<const T*>(weight), static_cast<T*>(out),
-        uint32_t(s.n_tokens), s.rows, s.cols, stride, s.vocab_start, s.scale, l);
-  else
-    embedding_kernel<T, int32_t><<<grid, kThreads, 0, stream>>>(
-        static_cast<const int32_t*>(s.tokens), static_cast<const T*>(weight), static_cast<T*>(out),
-        uint32_t(s.n_tokens), s.rows, s.cols, stride, s.vocab_start, s.scale, l);
+  embedding_kernel<T, I, U><<<grid, kThreads, 0, stream>>>(
+      static_cast<const I*>(s.tokens), static_cast<const T*>(weight), static_cast<T*>(out), uint32_t(s.n_tokens),
+      s.rows, s.cols, stride, uint64_t(s.vocab_start), s.scale, l);
+}
+
+template <typename T>
+void launch_embedding(const sr_embedding_shape& s, const void* weight, uint64_t stride, void* out, hipStream_t stream) {
+  if (s.token_dtype == SR_DT_I64) launch_embedding_of<T, int64_t, kLookupBlocks>(s, weight, stride, out, stream);
+  else launch_embedding_of<T, int32_t, kLookupBlocks>(s, weight, stride, out, stream);
 }
 
 // The parts of the workspace.  Pieces grow with the number of tokens, so that
 // a row of all tokens is joined from 1024 pieces at most.
 struct Layout {
   uint32_t piece, slots;
-  uint64_t order, pieces, partial, bytes;
+  uint64_t count, order, pieces, partial, bytes;
 };
 
 Layout layout_of(const sr_embedding_shape& s) {
   Layout w;
-  w.piece = 32;
-  while (s.n_tokens / w.piece > 512) w.piece *= 2;
+  w.piece = 16;
+  while (s.n_tokens / w.piece > 1024) w.piece *= 2;
   w.slots = uint32_t(2 * s.n_tokens / w.piece);
   auto up = [](uint64_t b) { return (b + 255) / 256 * 256; };
-  w.order = up((s.rows + 1) * 4);
+  w.count = up(s.rows * sizeof(Run));
+  w.order = w.count + 256;
   w.pieces = w.order + up(s.n_tokens * 4);
   w.partial = w.pieces + up(uint64_t(w.slots) * sizeof(Piece));
   w.bytes = w.partial + uint64_t(w.slots) * s.cols * 4;
@@ -384,16 +484,16 @@ Layout layout_of(const sr_embedding_shape& s) {
 template <typename T, typename G>
 void launch_sum(const sr_embedding_shape& s, const Layout& w, const Sorted& sorted, const void* grad_out,
                 uint64_t stride, void* grad, bool accumulate, hipStream_t stream) {
-  const Lanes l = lanes_of(s.cols, 16 / sizeof(T));
+  const Lanes l = lanes_of(s.cols, 16 / sizeof(T), kThreads, 1);
   const uint32_t group = uint32_t(kThreads) >> l.log2;
   const dim3 grid(uint32_t((w.slots + s.rows + group - 1) / group), l.slices);
   sum_kernel<T, G><<<grid, kThreads, 0, stream>>>(static_cast<const T*>(grad_out), stride, static_cast<G*>(grad),
                                                   s.rows, s.cols, w.slots, w.piece, s.scale, accumulate, l, sorted);
   if (s.n_tokens <= 2 * w.piece) return;     // no row is cut
-  const Lanes j = lanes_of(s.cols, 4);
+  const Lanes j = lanes_of(s.cols, 4, kThreads, 1);
   const uint32_t joined = uint32_t(kThreads) >> j.log2;
   const dim3 join_grid((w.slots + joined - 1) / joined, j.slices);
-  join_kernel<G><<<join_grid, kThreads, 0, stream>>>(static_cast<G*>(grad), s.rows, s.cols, w.slots, w.piece, s.scale,
+  join_kernel<G><<<join_grid, kThreads, 0, stream>>>(static_cast<G*>(grad), s.cols, w.slots, w.piece, s.scale,
                                                      accumulate, j, sorted);
 }
 
@@ -460,18 +560,18 @@ int sr_embedding_grad(const sr_embedding_shape* shape, const void* grad_out, uin
       overlap(grad, grad_bytes, workspace, w.bytes))
     return fail(SR_EOVERLAP, "sr_embedding_grad: the gradient overlaps an input");
   char* base = static_cast<char*>(workspace);
-  const Sorted sorted{reinterpret_cast<uint32_t*>(base), reinterpret_cast<uint32_t*>(base + w.order),
+  const Sorted sorted{reinterpret_cast<Run*>(base), reinterpret_cast<uint32_t*>(base + w.count),
+                      reinterpret_cast<uint32_t*>(base + w.order),
                       reinterpret_cast<Piece*>(base + w.pieces), reinterpret_cast<float*>(base + w.partial)};
-  const uint32_t range = uint32_t(std::min<uint64_t>(kSortRows, (s.rows + kSortRanges - 1) / kSortRanges));
-  const uint32_t blocks = uint32_t((s.rows + range - 1) / range);
-  if (s.token_dtype == SR_DT_I64)
-    sort_kernel<int64_t><<<blocks, kSortThreads, 0, stream>>>(static_cast<const int64_t*>(s.tokens),
-                                                             uint32_t(s.n_tokens), s.rows, s.vocab_start, range,
-                                                             w.piece, sorted);
-  else
-    sort_kernel<int32_t><<<blocks, kSortThreads, 0, stream>>>(static_cast<const int32_t*>(s.tokens),
-                                                             uint32_t(s.n_tokens), s.rows, s.vocab_start, range,
-                                                             w.piece, sorted);
+  const Owners owners = owners_of(s.rows);
+  uint32_t bits = 0;
+  while ((1u << bits) < owners.range) ++bits;
+  auto sort = [&](auto* tokens) {
+    sort_kernel<<<1u << owners.log2, kSortThreads, 0, stream>>>(tokens, uint32_t(s.n_tokens), uint32_t(s.rows),
+                                                                uint64_t(s.vocab_start), owners, bits, w.piece, sorted);
+  };
+  if (s.token_dtype == SR_DT_I64) sort(static_cast<const int64_t*>(s.tokens));
+  else sort(static_cast<const int32_t*>(s.tokens));
   if (int rc = launched("sr_embedding_grad: sort")) return rc;
   if (s.dtype == SR_DT_F32) launch_sum_to<float>(grad_dtype, s, w, sorted, grad_out, grad_out_stride, grad, accumulate != 0, stream);
   else if (s.dtype == SR_DT_BF16) launch_sum_to<bf16>(grad_dtype, s, w, sorted, grad_out, grad_out_stride, grad, accumulate != 0, stream);

@@ -33,6 +33,7 @@ using namespace sr_step;
 
 constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / kWave;
+constexpr int kShare = kThreads / kWave;   // lanes of one of the 64 groups that share a maximum
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kLn2 = 0.69314718055994530942f;
 constexpr float kInf = __builtin_inff();
@@ -85,17 +86,18 @@ __device__ __forceinline__ void take(Stats& t, const float (&x)[N]) {
   }
 }
 
+// The wave's statistics, in every lane: the maximum first, then the sums in its
+// units.
 __device__ __forceinline__ Stats wave_join(Stats t) {
+  float m = t.m, M = t.M;
 #pragma unroll
   for (int d = kWave / 2; d; d >>= 1) {
-    Stats o;
-    o.m = __shfl_xor(t.m, d);
-    o.M = __shfl_xor(t.M, d);
-    o.s = __shfl_xor(t.s, d);
-    o.w = __shfl_xor(t.w, d);
-    t = join(t, o);
+    m = fmaxf(m, __shfl_xor(m, d));
+    M = fmaxf(M, __shfl_xor(M, d));
   }
-  return t;
+  const Stats none{m, M, 0, 0};
+  t = join(t, none);
+  return {m, M, wave_sum(t.s), wave_sum(t.w)};
 }
 
 // Whether the sums say what they should: the largest logit's own part is 1.
@@ -124,9 +126,10 @@ __device__ __forceinline__ uint32_t column_of(uint64_t c) { return 0xffffffffu -
 
 struct Shared {
   Stats stats[kWaves];
-  float maxima[kThreads];
-  uint32_t count;
+  float maxima[kWave];
+  uint32_t group[kWave];
   float bound;
+  uint32_t count;
   uint64_t list[kCandidates];
   uint64_t best[kWaves];
   uint64_t chosen[kMaxTop];
@@ -194,17 +197,32 @@ __device__ __forceinline__ void load_or_fill(const T* row, uint32_t c, uint32_t 
   }
 }
 
-// A lane's statistics of columns from..to.
+template <typename T, int N, int B>
+__device__ __forceinline__ void load_batch(const T* p, Vec<T, N> (&x)[B]) {
+#pragma unroll
+  for (int b = 0; b < B; ++b) x[b] = __builtin_nontemporal_load(reinterpret_cast<const Vec<T, N>*>(p + b * kThreads * N));
+}
+
+// A lane's statistics of columns from..to.  The next batch is on its way while
+// one is taken in.
 template <typename T>
 __device__ __forceinline__ Stats row_stats(const T* row, uint32_t from, uint32_t to) {
   constexpr int N = 16 / sizeof(T);
   constexpr int kBatch = 4;
+  constexpr uint32_t kStep = kBatch * kThreads * N;
   Stats t{-kInf, kLeast, 0, 0};
   uint32_t c = from + threadIdx.x * N;
-  for (; c + (kBatch - 1) * kThreads * N + N <= to; c += kBatch * kThreads * N) {
+  auto whole = [&](uint32_t at) { return at + (kBatch - 1) * kThreads * N + N <= to; };
+  Vec<T, N> ahead[kBatch];
+  if (whole(c)) load_batch<T, N, kBatch>(row + c, ahead);
+  while (whole(c)) {
     float x[kBatch * N];
 #pragma unroll
-    for (int b = 0; b < kBatch; ++b) load<T, N>(row + c + b * kThreads * N, *reinterpret_cast<float(*)[N]>(x + b * N));
+    for (int b = 0; b < kBatch; ++b)
+#pragma unroll
+      for (int k = 0; k < N; ++k) x[b * N + k] = float(ahead[b][k]);
+    c += kStep;
+    if (whole(c)) load_batch<T, N, kBatch>(row + c, ahead);
     take<kBatch * N>(t, x);
   }
   for (; c < to; c += kThreads * N) {
@@ -284,19 +302,50 @@ __device__ __forceinline__ void rank_list(Shared& sh, uint32_t n, int k) {
   __syncthreads();
 }
 
-// Adds a lane's logits that reach `bound`, or are above it, to the list.
+// Adds the logits of the groups in `groups` that reach `bound`, or are above
+// it, to the list.  The groups' vectors are dealt out to all lanes, neighbours
+// of a group to neighbouring lanes, and several loads of a lane are on their
+// way at once.
 template <typename T>
-__device__ __forceinline__ void list_reaching(Shared& sh, const T* row, uint32_t from, uint32_t to, float bound,
-                                              bool above) {
-  constexpr int N = 16 / sizeof(T);
-  for (uint32_t c = from + threadIdx.x * N; c < to; c += kThreads * N) {
-    float x[N];
-    load_or_fill<T, N>(row, c, to, x);
+__device__ __forceinline__ void list_reaching(Shared& sh, const T* row, uint32_t from, uint32_t to, uint64_t groups,
+                                              float bound, bool above) {
+  constexpr uint32_t N = 16 / sizeof(T), kAhead = 4;
+  const uint32_t lane = threadIdx.x % kWave;
+  __syncthreads();
+  if (threadIdx.x < kWave && (groups >> lane & 1)) sh.group[__popcll(groups & ((uint64_t(1) << lane) - 1))] = lane;
+  __syncthreads();
+  // Quads of lanes take (group, round) pairs, 64 of them at a time.
+  const uint32_t rounds = (to - from + kThreads * N - 1) / (kThreads * N);
+  const uint32_t all = uint32_t(__popcll(groups)), step = kThreads / kShare;
+  const uint32_t g_step = step / rounds, r_step = step % rounds;
+  uint32_t g = threadIdx.x / kShare / rounds, r = threadIdx.x / kShare % rounds;
+  while (__ballot(g < all)) {
+    float x[kAhead][N];
+    uint32_t c[kAhead];
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      if ((above ? x[i] > bound : x[i] >= bound) && c + i < to) {
-        const uint32_t at = atomicAdd(&sh.count, 1u);
-        if (at < kCandidates) sh.list[at] = candidate(x[i], c + i);
+    for (uint32_t a = 0; a < kAhead; ++a) {
+      c[a] = g < all ? from + (sh.group[g] * kShare + threadIdx.x % kShare + r * kThreads) * N : to;
+      load_or_fill<T, N>(row, c[a], to, x[a]);
+      g += g_step;
+      r += r_step;
+      if (r >= rounds) {
+        r -= rounds;
+        ++g;
+      }
+    }
+#pragma unroll
+    for (uint32_t a = 0; a < kAhead; ++a) {
+      float top = x[a][0];
+#pragma unroll
+      for (uint32_t k = 1; k < N; ++k) top = fmaxf(top, x[a][k]);
+      if (above ? top > bound : top >= bound) {
+#pragma unroll
+        for (uint32_t k = 0; k < N; ++k) {
+          if ((above ? x[a][k] > bound : x[a][k] >= bound) && c[a] + k < to) {
+            const uint32_t at = atomicAdd(&sh.count, 1u);
+            if (at < kCandidates) sh.list[at] = candidate(x[a][k], c[a] + k);
+          }
+        }
       }
     }
   }
@@ -328,27 +377,36 @@ __device__ void list_equal(Shared& sh, const T* row, uint32_t from, uint32_t to,
   __syncthreads();
 }
 
-// sh.chosen = the k best of columns from..to (at least k columns); `m` is the
-// largest logit of this lane's part, `finite` that there is no NaN.
+// sh.chosen = the k best of columns from..to (at least k columns, k <= 64); `m`
+// is the largest logit of this lane's part, `finite` that there is no NaN.
 template <typename T>
 __device__ void row_top(Shared& sh, const T* row, uint32_t from, uint32_t to, int k, float m, bool finite) {
+  static_assert(kMaxTop <= kWave, "as many groups as alternatives");
   if (!finite) {
     plain_top(sh, row, from, to, k);
     return;
   }
+  // Lanes are taken in 64 groups.  The k-th largest of the groups' maxima is
+  // the bound: k groups have a logit that reaches it.
+#pragma unroll
+  for (int d = 1; d < kShare; d <<= 1) m = fmaxf(m, __shfl_xor(m, d));
   __syncthreads();
-  sh.maxima[threadIdx.x] = m;
+  if (threadIdx.x % kShare == 0) sh.maxima[threadIdx.x / kShare] = m;
   if (threadIdx.x == 0) sh.count = 0;
   __syncthreads();
-  int before = 0;
-  for (int j = 0; j < kThreads; ++j) {
-    const float o = sh.maxima[j];
-    before += o > m || (o == m && j < int(threadIdx.x));
+  const float mine = sh.maxima[threadIdx.x % kWave];
+  if (threadIdx.x < kWave) {
+    int before = 0;
+#pragma unroll
+    for (int j = 0; j < kWave; ++j) {
+      const float o = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(mine), j));
+      before += o > mine || (o == mine && j < int(threadIdx.x));
+    }
+    if (before == k - 1) sh.bound = mine;
   }
-  if (before == k - 1) sh.bound = m;
   __syncthreads();
   const float bound = sh.bound;
-  if (m >= bound) list_reaching(sh, row, from, to, bound, false);
+  list_reaching(sh, row, from, to, __ballot(mine >= bound), bound, false);
   __syncthreads();
   uint32_t n = sh.count;
   if (n > kCandidates) {
@@ -356,7 +414,7 @@ __device__ void row_top(Shared& sh, const T* row, uint32_t from, uint32_t to, in
     __syncthreads();
     if (threadIdx.x == 0) sh.count = 0;
     __syncthreads();
-    if (m > bound) list_reaching(sh, row, from, to, bound, true);
+    list_reaching(sh, row, from, to, __ballot(mine > bound), bound, true);
     __syncthreads();
     n = sh.count;
     if (n > kCandidates - kMaxTop) {
@@ -374,6 +432,19 @@ __device__ void row_top(Shared& sh, const T* row, uint32_t from, uint32_t to, in
 template <typename I>
 __device__ __forceinline__ int64_t target_at(const I* targets, uint64_t row) { return int64_t(targets[row]); }
 
+// A row's target and its logit, read ahead of the row.
+struct Target {
+  bool scored, inside;
+  float x;
+};
+
+template <typename T, typename I>
+__device__ __forceinline__ Target target_of(const T* row, const I* targets, uint64_t i, uint32_t vocab) {
+  const int64_t t = target_at(targets, i);
+  const bool inside = t >= 0 && uint64_t(t) < vocab;
+  return {t >= 0, inside, inside ? float(row[t]) : 0.0f};
+}
+
 struct Outputs {
   float* logprob;
   float* entropy;
@@ -385,17 +456,11 @@ struct Outputs {
 __device__ __forceinline__ float logprob_of(float x, const Summary& r) { return (x - r.shift) - r.rest; }
 
 // Writes a row's results; sh.chosen holds the alternatives.
-template <typename T, typename I>
-__device__ __forceinline__ void put(Shared& sh, const T* row, const I* targets, uint64_t i, uint32_t vocab, int k,
-                                    const Summary& r, const Outputs& out) {
+__device__ __forceinline__ void put(Shared& sh, const Target& t, uint64_t i, int k, const Summary& r,
+                                    const Outputs& out) {
   if (threadIdx.x == 0) {
-    const int64_t target = target_at(targets, i);
     float lp = 0;
-    if (target >= 0) {
-      lp = -kInf;
-      if (uint64_t(target) < vocab) lp = logprob_of(float(row[target]), r);
-      else if (r.lse != r.lse) lp = r.lse;
-    }
+    if (t.scored) lp = t.inside ? logprob_of(t.x, r) : r.lse != r.lse ? r.lse : -kInf;
     out.logprob[i] = lp;
     out.entropy[i] = r.entropy;
     out.lse[i] = r.lse;
@@ -407,31 +472,119 @@ __device__ __forceinline__ void put(Shared& sh, const T* row, const I* targets, 
   }
 }
 
-template <typename T, typename I>
+template <bool TOP, typename T, typename I>
 __global__ __launch_bounds__(kThreads) void row_kernel(const T* logits, const I* targets, uint64_t stride,
                                                        uint32_t vocab, int k, Outputs out) {
   __shared__ Shared sh;
   const uint64_t i = blockIdx.x;
   const T* row = logits + i * stride;
+  const Target target = target_of(row, targets, i, vocab);
   const Stats mine = row_stats(row, 0, vocab);
   const Stats all = block_join(sh, mine);
-  const bool ok = sound(all);
-  const Summary r = ok ? summary_of(all) : plain_summary(sh, row, vocab);
-  if (k) row_top(sh, row, 0, vocab, k, mine.m, r.lse == r.lse);
-  put(sh, row, targets, i, vocab, k, r, out);
+  const Summary r = sound(all) ? summary_of(all) : plain_summary(sh, row, vocab);
+  if constexpr (TOP) row_top(sh, row, 0, vocab, k, mine.m, r.lse == r.lse);
+  put(sh, target, i, TOP ? k : 0, r, out);
+}
+
+// ---------------------------------------------------------------- split rows
+
+// Few rows do not fill the GPU with a workgroup each, so each is cut into parts
+// of `length` columns that leave their statistics and their best k candidates
+// in the workspace; a second launch joins them.
+struct Parts {
+  uint32_t parts, length;
+  Stats* stats;         // [rows][parts]
+  uint64_t* best;       // [rows][parts][k], falling; 0 where a part has fewer
+};
+
+template <bool TOP, typename T>
+__global__ __launch_bounds__(kThreads) void part_kernel(const T* logits, uint64_t stride, uint32_t vocab, int k,
+                                                        Parts out) {
+  __shared__ Shared sh;
+  const uint32_t part = blockIdx.x;
+  const uint64_t i = blockIdx.y;
+  const T* row = logits + i * stride;
+  const uint32_t from = part * out.length, to = min(from + out.length, vocab);
+  const Stats mine = row_stats(row, from, to);
+  const Stats all = block_join(sh, mine);
+  const uint64_t at = i * out.parts + part;
+  if (threadIdx.x == 0) out.stats[at] = all;
+  if constexpr (TOP) {
+    const int own = min(k, int(to - from));
+    row_top(sh, row, from, to, own, mine.m, all.s == all.s);
+    if (int(threadIdx.x) < k) out.best[at * k + threadIdx.x] = int(threadIdx.x) < own ? sh.chosen[threadIdx.x] : 0;
+  }
+}
+
+// sh.chosen = the k best of the parts' candidates.  The k-th best of what each
+// part has in front bounds them from below.
+__device__ void parts_top(Shared& sh, const uint64_t* best, uint32_t parts, int k) {
+  uint32_t front = (2 * uint32_t(k) + parts - 1) / parts;
+  front = front < uint32_t(k) ? front : uint32_t(k);
+  const uint32_t n = parts * front;
+  __syncthreads();
+  for (uint32_t i = threadIdx.x; i < n; i += kThreads) sh.list[i] = best[i / front * k + i % front];
+  if (threadIdx.x == 0) sh.count = 0;
+  __syncthreads();
+  rank_list(sh, n, k);
+  const uint64_t bound = sh.chosen[k - 1];
+  __syncthreads();
+  for (uint32_t i = threadIdx.x; i < parts * k; i += kThreads) {
+    const uint64_t x = best[i];
+    if (x >= bound) {
+      const uint32_t at = atomicAdd(&sh.count, 1u);
+      if (at < kCandidates) sh.list[at] = x;
+    }
+  }
+  __syncthreads();
+  if (sh.count <= kCandidates) {
+    rank_list(sh, sh.count, k);
+    return;
+  }
+  uint64_t last = ~uint64_t(0);
+  for (int i = 0; i < k; ++i) {
+    uint64_t top = 0;
+    for (uint32_t j = threadIdx.x; j < parts * k; j += kThreads) {
+      const uint64_t x = best[j];
+      if ((i == 0 || x < last) && x > top) top = x;
+    }
+    last = block_best(sh, top);
+    if (threadIdx.x == 0) sh.chosen[i] = last;
+  }
+  __syncthreads();
+}
+
+template <typename T, typename I>
+__global__ __launch_bounds__(kThreads) void parts_kernel(const T* logits, const I* targets, uint64_t stride,
+                                                         uint32_t vocab, int k, Parts in, Outputs out) {
+  __shared__ Shared sh;
+  const uint64_t i = blockIdx.x;
+  const T* row = logits + i * stride;
+  const Target target = target_of(row, targets, i, vocab);
+  const Stats mine = threadIdx.x < in.parts ? in.stats[i * in.parts + threadIdx.x] : Stats{-kInf, kLeast, 0, 0};
+  const Stats all = block_join(sh, mine);
+  const Summary r = sound(all) ? summary_of(all) : plain_summary(sh, row, vocab);
+  if (k) parts_top(sh, in.best + i * in.parts * k, in.parts, k);
+  put(sh, target, i, k, r, out);
 }
 
 // ----------------------------------------------------------------- gradient
 
+// One vector a lane, in the order of memory.
 template <typename T, typename I>
 __global__ __launch_bounds__(kThreads) void grad_kernel(const T* logits, const I* targets, uint64_t stride,
-                                                        uint32_t vocab, uint32_t columns, const float* lse,
-                                                        const float* entropy, const float* g_logprob,
-                                                        const float* g_entropy, T* grad, uint64_t grad_stride) {
+                                                        uint32_t vocab, uint32_t columns, uint32_t spans,
+                                                        const float* lse, const float* entropy,
+                                                        const float* g_logprob, const float* g_entropy, T* grad,
+                                                        uint64_t grad_stride) {
   constexpr int N = 16 / sizeof(T);
-  const uint64_t i = blockIdx.x;
+  const uint32_t i = blockIdx.x / spans;
+  const uint32_t c = ((blockIdx.x - i * spans) * kThreads + threadIdx.x) * N;
   const T* row = logits + i * stride;
   T* to = grad + i * grad_stride;
+  const bool whole = c + N <= columns;
+  Vec<T, N> x;
+  if (whole) x = __builtin_nontemporal_load(reinterpret_cast<const Vec<T, N>*>(row + c));
   const int64_t target = target_at(targets, i);
   const float l = lse[i], h = entropy[i];
   const float gl = g_logprob && target >= 0 ? g_logprob[i] : 0.0f;
@@ -445,16 +598,13 @@ __global__ __launch_bounds__(kThreads) void grad_kernel(const T* logits, const I
     if (int64_t(c) == target) g += gl;
     return empty || c >= vocab ? 0.0f : g;
   };
-  for (uint32_t c = blockIdx.y * kThreads * N + threadIdx.x * N; c < columns; c += gridDim.y * kThreads * N) {
-    if (c + N <= columns) {
-      float x[N];
-      load<T, N>(row + c, x);
+  if (whole) {
+    float g[N];
 #pragma unroll
-      for (int k = 0; k < N; ++k) x[k] = value(x[k], c + k);
-      store<T, N>(to + c, x);
-    } else {
-      for (uint32_t k = c; k < columns; ++k) to[k] = T(value(float(row[k]), k));
-    }
+    for (int k = 0; k < N; ++k) g[k] = value(float(x[k]), c + k);
+    store_region<kThrough, T, N>(region(to, uint32_t(columns * sizeof(T))), uint32_t(c * sizeof(T)), g);
+  } else {
+    for (uint32_t k = c; k < columns; ++k) to[k] = T(value(float(row[k]), k));
   }
 }
 
@@ -488,6 +638,26 @@ int check_top(const char* who, const sr_logprob_shape& s, int32_t top) {
   return SR_OK;
 }
 
+// How rows are cut: into as many parts as give every compute unit eight
+// workgroups, of 2048 columns or more.
+struct Cut {
+  uint32_t parts, length;
+  uint64_t best, bytes;
+};
+
+Cut parts_of(const sr_logprob_shape& s, int32_t top) {
+  constexpr uint64_t kFill = 2048, kLeastColumns = 2048, kMostParts = 128;
+  Cut c{1, uint32_t(s.vocab), 0, 0};
+  if (s.rows == 0) return c;
+  const uint64_t parts = std::min({kFill / s.rows, s.vocab / kLeastColumns, kMostParts});
+  if (parts < 2) return c;
+  c.length = uint32_t((s.vocab + parts - 1) / parts + 7) / 8 * 8;      // whole vectors
+  c.parts = uint32_t((s.vocab + c.length - 1) / c.length);
+  c.best = (s.rows * c.parts * sizeof(Stats) + 255) / 256 * 256;
+  c.bytes = c.best + s.rows * c.parts * uint64_t(top) * sizeof(uint64_t);
+  return c;
+}
+
 // f(logits, targets) with their types.
 template <typename T, typename F>
 void with_targets(const sr_logprob_shape& s, F&& f) {
@@ -510,7 +680,7 @@ int sr_logprob_workspace(const sr_logprob_shape* shape, int32_t top, uint64_t* b
   if (bytes == nullptr) return fail(SR_EINVAL, "sr_logprob_workspace: null argument");
   if (int rc = check_shape("sr_logprob_workspace", shape)) return rc;
   if (int rc = check_top("sr_logprob_workspace", *shape, top)) return rc;
-  *bytes = 0;
+  *bytes = parts_of(*shape, top).bytes;
   return SR_OK;
 }
 
@@ -530,8 +700,20 @@ int sr_logprob(const sr_logprob_shape* shape, int32_t top, float* logprob, float
                 (unsigned long long)need);
   if (reinterpret_cast<uintptr_t>(workspace) % 16) return fail(SR_EALIGN, "sr_logprob: workspace not aligned");
   const Outputs out{logprob, entropy, lse, top_logprob, top_index};
+  const Cut cut = parts_of(s, top);
+  char* base = static_cast<char*>(workspace);
+  const Parts parts{cut.parts, cut.length, reinterpret_cast<Stats*>(base), reinterpret_cast<uint64_t*>(base + cut.best)};
   with_types(s, [&](auto* logits, auto* targets) {
-    row_kernel<<<uint32_t(s.rows), kThreads, 0, stream>>>(logits, targets, s.stride, uint32_t(s.vocab), int(top), out);
+    const uint32_t rows = uint32_t(s.rows), vocab = uint32_t(s.vocab);
+    if (cut.parts == 1) {
+      if (top) row_kernel<true><<<rows, kThreads, 0, stream>>>(logits, targets, s.stride, vocab, int(top), out);
+      else row_kernel<false><<<rows, kThreads, 0, stream>>>(logits, targets, s.stride, vocab, 0, out);
+      return;
+    }
+    const dim3 grid(cut.parts, rows);
+    if (top) part_kernel<true><<<grid, kThreads, 0, stream>>>(logits, s.stride, vocab, int(top), parts);
+    else part_kernel<false><<<grid, kThreads, 0, stream>>>(logits, s.stride, vocab, 0, parts);
+    parts_kernel<<<rows, kThreads, 0, stream>>>(logits, targets, s.stride, vocab, int(top), parts, out);
   });
   return launched("sr_logprob");
 }
@@ -561,12 +743,15 @@ int sr_logprob_grad(const sr_logprob_shape* shape, const float* lse, const float
       clash(span(lse, 1, 0, s.rows, 4)) || clash(span(entropy, 1, 0, s.rows, 4)) ||
       clash(span(g_logprob, 1, 0, s.rows, 4)) || clash(span(g_entropy, 1, 0, s.rows, 4)))
     return fail(SR_EOVERLAP, "sr_logprob_grad: the gradient overlaps an input");
+  const uint64_t step = kThreads * 16 / size, spans = (s.columns + step - 1) / step, blocks = s.rows * spans;
+  if (blocks >= uint64_t(1) << 24)     // the grid's threads stay below 2^32
+    return fail(SR_EBOUNDS, "sr_logprob_grad: %llu rows of %llu columns", (unsigned long long)s.rows,
+                (unsigned long long)s.columns);
   with_types(s, [&](auto* logits, auto* targets) {
     typedef typename std::remove_const<typename std::remove_pointer<decltype(logits)>::type>::type T;
-    constexpr uint32_t kSpan = kThreads * 16 / sizeof(T) * 4;
-    const dim3 grid(uint32_t(s.rows), uint32_t(std::min<uint64_t>((s.columns + kSpan - 1) / kSpan, 65535)));
-    grad_kernel<<<grid, kThreads, 0, stream>>>(logits, targets, s.stride, uint32_t(s.vocab), uint32_t(s.columns), lse,
-                                               entropy, g_logprob, g_entropy, static_cast<T*>(grad), grad_stride);
+    grad_kernel<<<uint32_t(blocks), kThreads, 0, stream>>>(
+        logits, targets, s.stride, uint32_t(s.vocab), uint32_t(s.columns), uint32_t(spans), lse, entropy, g_logprob,
+        g_entropy, static_cast<T*>(grad), grad_stride);
   });
   return launched("sr_logprob_grad");
 }

@@ -44,8 +44,12 @@ __device__ __forceinline__ int entry_of(const uint32_t* first, int count, uint32
 // sum += x^2 over all elements, in 64 bits: squares of f32 values neither
 // overflow nor vanish there, and each product of two 24-bit numbers is exact.
 constexpr int kSumEntries = 188;
-constexpr uint32_t kSumChunk = 16384;    // elements
-constexpr uint32_t kSumBlocks = 2048;    // workgroups of one launch at most
+constexpr uint32_t kSumChunk = 32768;      // elements
+constexpr uint32_t kSumBlocks = 16384;     // workgroups of one launch at most
+#ifndef SUM_CACHED
+#define SUM_CACHED (uint64_t(1) << 30)
+#endif
+constexpr uint64_t kSumCached = SUM_CACHED;
 
 struct SumTable {
   uint64_t data[kSumEntries];
@@ -56,23 +60,27 @@ struct SumTable {
 };
 static_assert(sizeof(SumTable) <= kTableBytes, "kernel arguments");
 
+constexpr int kFinishThreads = 1024;
+
+template <int THREADS>
 __device__ __forceinline__ double block_sum(double x) {
-  __shared__ double part[kThreads / kWave];
+  __shared__ double part[THREADS / kWave];
   x = wave_sum(x);
   if (threadIdx.x % kWave == 0) part[threadIdx.x / kWave] = x;
   __syncthreads();
   double s = 0;
 #pragma unroll
-  for (int i = 0; i < kThreads / kWave; ++i) s += part[i];
+  for (int i = 0; i < THREADS / kWave; ++i) s += part[i];
   return s;
 }
 
-template <typename T>
-__global__ __launch_bounds__(kThreads) void square_sum_kernel(SumTable t, double* partial) {
+template <typename T, bool STREAM>
+__global__ __launch_bounds__(kThreads) void square_sum_kernel(SumTable t, uint32_t run, double* partial) {
   constexpr int N = 16 / sizeof(T);
-  constexpr int kBatch = 4;
+  constexpr int kBatch = 8;
   double sum[4] = {0, 0, 0, 0};
-  for (uint32_t c = blockIdx.x; c < t.chunks; c += gridDim.x) {
+  const uint32_t end = min((blockIdx.x + 1) * run, t.chunks);
+  for (uint32_t c = blockIdx.x * run; c < end; ++c) {
     const int i = entry_of(t.first, t.count, c);
     const uint64_t at = uint64_t(c - t.first[i]) * kSumChunk;
     const uint64_t left = t.n[i] - at;
@@ -80,13 +88,19 @@ __global__ __launch_bounds__(kThreads) void square_sum_kernel(SumTable t, double
     const T* p = reinterpret_cast<const T*>(t.data[i]) + at;
     uint32_t e = threadIdx.x * N;
     for (; e + (kBatch - 1) * kThreads * N + N <= n; e += kBatch * kThreads * N) {
-      float x[kBatch][N];
+      Vec<T, N> x[kBatch];
 #pragma unroll
-      for (int b = 0; b < kBatch; ++b) load<T, N>(p + e + b * kThreads * N, x[b]);
+      for (int b = 0; b < kBatch; ++b) {
+        const Vec<T, N>* v = reinterpret_cast<const Vec<T, N>*>(p + e + b * kThreads * N);
+        x[b] = STREAM ? __builtin_nontemporal_load(v) : *v;
+      }
 #pragma unroll
       for (int b = 0; b < kBatch; ++b)
 #pragma unroll
-        for (int k = 0; k < N; ++k) sum[k & 3] = fma(double(x[b][k]), double(x[b][k]), sum[k & 3]);
+        for (int k = 0; k < N; ++k) {
+          const double d = double(float(x[b][k]));
+          sum[k & 3] = fma(d, d, sum[k & 3]);
+        }
     }
     for (; e + N <= n; e += kThreads * N) {
       float x[N];
@@ -100,15 +114,24 @@ __global__ __launch_bounds__(kThreads) void square_sum_kernel(SumTable t, double
       sum[0] = fma(x, x, sum[0]);
     }
   }
-  const double s = block_sum((sum[0] + sum[1]) + (sum[2] + sum[3]));
+  const double s = block_sum<kThreads>((sum[0] + sum[1]) + (sum[2] + sum[3]));
   if (threadIdx.x == 0) partial[blockIdx.x] = s;
 }
 
-__global__ __launch_bounds__(kThreads) void finish_sum_kernel(const double* partial, uint32_t count, double* sum,
-                                                              float* norm) {
+__global__ __launch_bounds__(kFinishThreads) void finish_sum_kernel(const double* partial, uint32_t count, double* sum,
+                                                                    float* norm) {
+  constexpr uint32_t kAhead = 4;
   double x = 0;
-  for (uint32_t i = threadIdx.x; i < count; i += kThreads) x += partial[i];
-  x = block_sum(x);
+  uint32_t i = threadIdx.x;
+  for (; i + (kAhead - 1) * kFinishThreads < count; i += kAhead * kFinishThreads) {
+    double p[kAhead];
+#pragma unroll
+    for (uint32_t a = 0; a < kAhead; ++a) p[a] = partial[i + a * kFinishThreads];
+#pragma unroll
+    for (uint32_t a = 0; a < kAhead; ++a) x += p[a];
+  }
+  for (; i < count; i += kFinishThreads) x += partial[i];
+  x = block_sum<kFinishThreads>(x);
   if (threadIdx.x == 0) {
     *sum = x;
     if (norm) *norm = float(sqrt(x));
@@ -158,7 +181,7 @@ __global__ __launch_bounds__(kThreads) void clip_kernel(ClipTable t) {
 #pragma unroll
   for (int b = 0; b < kBatch; ++b) {
     const uint32_t e = (b * kThreads + threadIdx.x) * N;
-    if (e + N <= n) load<S, N>(src + e, x[b]);
+    if (e + N <= n) load_stream<S, N>(src + e, x[b]);
   }
 #pragma unroll
   for (int b = 0; b < kBatch; ++b) {
@@ -166,7 +189,7 @@ __global__ __launch_bounds__(kThreads) void clip_kernel(ClipTable t) {
     if (e + N <= n) {
 #pragma unroll
       for (int k = 0; k < N; ++k) x[b][k] *= f;
-      store<D, N>(dst + e, x[b]);
+      store_stream<D, N>(dst + e, x[b]);
     } else {
       for (uint32_t k = e; k < n; ++k) dst[k] = D(float(src[k]) * f);
     }
@@ -176,6 +199,7 @@ __global__ __launch_bounds__(kThreads) void clip_kernel(ClipTable t) {
 // --------------------------------------------------------------------- AdamW
 
 constexpr int kAdamEntries = 78;
+constexpr int kAdamThreads = 512;
 constexpr uint32_t kAdamChunk = 2048;
 
 struct AdamTable {
@@ -204,10 +228,10 @@ struct NoCopy {};
 // W: type of the weight, M: of the moments, G: of the gradient, P: of the
 // weight's copy, or NoCopy.
 template <typename W, typename M, typename G, typename P>
-__global__ __launch_bounds__(kThreads) void adamw_kernel(AdamTable t) {
-  constexpr int N = 4;
-  constexpr int kBatch = kAdamChunk / (kThreads * N);
-  const uint32_t c = blockIdx.x;
+__global__ __launch_bounds__(kAdamThreads) void adamw_kernel(AdamTable t) {
+  constexpr int N = kAdamChunk / kAdamThreads;
+    const uint32_t c = xcd_order(blockIdx.x, t.chunks);
+  if (c >= t.chunks) return;
   const int i = entry_of(t.first, t.count, c);
   const uint32_t next = i + 1 < t.count ? t.first[i + 1] : t.chunks;
   const uint32_t n = c + 1 == next ? t.tail[i] : kAdamChunk;
@@ -217,16 +241,14 @@ __global__ __launch_bounds__(kThreads) void adamw_kernel(AdamTable t) {
   M* exp_avg_sq = reinterpret_cast<M*>(t.exp_avg_sq[i]) + at;
   const G* grad = reinterpret_cast<const G*>(t.grad[i]) + at;
 
-  float g[kBatch][N], w[kBatch][N], m[kBatch][N], v[kBatch][N];
-#pragma unroll
-  for (int b = 0; b < kBatch; ++b) {
-    const uint32_t e = (b * kThreads + threadIdx.x) * N;
-    if (e + N <= n) {
-      load<G, N>(grad + e, g[b]);
-      load<W, N>(weight + e, w[b]);
-      load<M, N>(exp_avg + e, m[b]);
-      load<M, N>(exp_avg_sq + e, v[b]);
-    }
+  const uint32_t e = threadIdx.x * N;
+  const bool whole = e + N <= n;
+  float g[N], w[N], m[N], v[N];
+  if (whole) {
+    load_stream<G, N>(grad + e, g);
+    load_stream<W, N>(weight + e, w);
+    load_stream<M, N>(exp_avg + e, m);
+    load_stream<M, N>(exp_avg_sq + e, v);
   }
   const float factor = t.square_sum ? clip_factor(*t.square_sum, t.max_norm) : 1.0f;
   auto update = [&](float gi, float& wi, float& mi, float& vi) {
@@ -236,25 +258,21 @@ __global__ __launch_bounds__(kThreads) void adamw_kernel(AdamTable t) {
     const float root = fmaf(sqrtf(vi), t.root_scale, t.eps);
     wi = fmaf(wi, t.decay, -(t.step_size * mi) / root);
   };
+  if (whole) {
 #pragma unroll
-  for (int b = 0; b < kBatch; ++b) {
-    const uint32_t e = (b * kThreads + threadIdx.x) * N;
-    if (e + N <= n) {
-#pragma unroll
-      for (int k = 0; k < N; ++k) update(g[b][k], w[b][k], m[b][k], v[b][k]);
-      store<W, N>(weight + e, w[b]);
-      store<M, N>(exp_avg + e, m[b]);
-      store<M, N>(exp_avg_sq + e, v[b]);
-      if constexpr (!__is_same(P, NoCopy)) store<P, N>(reinterpret_cast<P*>(t.param[i]) + at + e, w[b]);
-    } else {
-      for (uint32_t k = e; k < n; ++k) {
-        float wi = float(weight[k]), mi = float(exp_avg[k]), vi = float(exp_avg_sq[k]);
-        update(float(grad[k]), wi, mi, vi);
-        weight[k] = W(wi);
-        exp_avg[k] = M(mi);
-        exp_avg_sq[k] = M(vi);
-        if constexpr (!__is_same(P, NoCopy)) (reinterpret_cast<P*>(t.param[i]) + at)[k] = P(wi);
-      }
+    for (int k = 0; k < N; ++k) update(g[k], w[k], m[k], v[k]);
+    store_stream<W, N>(weight + e, w);
+    store_stream<M, N>(exp_avg + e, m);
+    store_stream<M, N>(exp_avg_sq + e, v);
+    if constexpr (!__is_same(P, NoCopy)) store_stream<P, N>(reinterpret_cast<P*>(t.param[i]) + at + e, w);
+  } else {
+    for (uint32_t k = e; k < n; ++k) {
+      float wi = float(weight[k]), mi = float(exp_avg[k]), vi = float(exp_avg_sq[k]);
+      update(float(grad[k]), wi, mi, vi);
+      weight[k] = W(wi);
+      exp_avg[k] = M(mi);
+      exp_avg_sq[k] = M(vi);
+      if constexpr (!__is_same(P, NoCopy)) (reinterpret_cast<P*>(t.param[i]) + at)[k] = P(wi);
     }
   }
 }
@@ -334,7 +352,16 @@ int sum_launches(const sr_array* a, int32_t count, F&& launch) {
   return SR_OK;
 }
 
-uint32_t sum_blocks(const SumTable& t) { return t.chunks < kSumBlocks ? t.chunks : kSumBlocks; }
+// Consecutive chunks of one workgroup, and the workgroups.
+uint32_t sum_run(const SumTable& t) { return (t.chunks + kSumBlocks - 1) / kSumBlocks; }
+uint32_t sum_blocks(const SumTable& t) { return (t.chunks + sum_run(t) - 1) / sum_run(t); }
+
+template <typename T>
+void launch_sum(const SumTable& t, uint32_t run, uint32_t blocks, bool stream_loads, double* partial,
+                hipStream_t stream) {
+  if (stream_loads) square_sum_kernel<T, true><<<blocks, kThreads, 0, stream>>>(t, run, partial);
+  else square_sum_kernel<T, false><<<blocks, kThreads, 0, stream>>>(t, run, partial);
+}
 
 template <typename S, typename D>
 void launch_clip(const ClipTable& t, uint32_t blocks, hipStream_t stream) {
@@ -352,11 +379,11 @@ template <typename W, typename M, typename G>
 void launch_adamw_copy(bool copy, const AdamTable& t, hipStream_t stream) {
   if constexpr (__is_same(W, float)) {
     if (copy) {
-      adamw_kernel<W, M, G, bf16><<<t.chunks, kThreads, 0, stream>>>(t);
+      adamw_kernel<W, M, G, bf16><<<xcd_blocks(t.chunks), kAdamThreads, 0, stream>>>(t);
       return;
     }
   }
-  adamw_kernel<W, M, G, NoCopy><<<t.chunks, kThreads, 0, stream>>>(t);
+  adamw_kernel<W, M, G, NoCopy><<<xcd_blocks(t.chunks), kAdamThreads, 0, stream>>>(t);
 }
 
 template <typename W, typename M>
@@ -398,16 +425,19 @@ int sr_square_sum(const sr_array* arrays, int32_t count, void* workspace, uint64
   if (reinterpret_cast<uintptr_t>(workspace) % 16) return fail(SR_EALIGN, "sr_square_sum: workspace not aligned");
   double* partial = static_cast<double*>(workspace);
   uint32_t used = 0;
+  uint64_t bytes = 0;
+  for (int32_t i = 0; i < count; ++i) bytes += bytes_of(arrays[i]);
+  const bool stream_loads = bytes > kSumCached;
   const int rc = sum_launches(arrays, count, [&](int32_t dt, const SumTable& t) {
-    const uint32_t blocks = sum_blocks(t);
-    if (dt == SR_DT_F32) square_sum_kernel<float><<<blocks, kThreads, 0, stream>>>(t, partial + used);
-    else if (dt == SR_DT_BF16) square_sum_kernel<bf16><<<blocks, kThreads, 0, stream>>>(t, partial + used);
-    else square_sum_kernel<f16><<<blocks, kThreads, 0, stream>>>(t, partial + used);
+    const uint32_t blocks = sum_blocks(t), run = sum_run(t);
+    if (dt == SR_DT_F32) launch_sum<float>(t, run, blocks, stream_loads, partial + used, stream);
+    else if (dt == SR_DT_BF16) launch_sum<bf16>(t, run, blocks, stream_loads, partial + used, stream);
+    else launch_sum<f16>(t, run, blocks, stream_loads, partial + used, stream);
     used += blocks;
     return launched("sr_square_sum");
   });
   if (rc) return rc;
-  finish_sum_kernel<<<1, kThreads, 0, stream>>>(partial, used, sum, norm);
+  finish_sum_kernel<<<1, kFinishThreads, 0, stream>>>(partial, used, sum, norm);
   return launched("sr_square_sum");
 }
 

@@ -64,11 +64,52 @@ __device__ __forceinline__ void store_stream(T* p, const float (&f)[N]) {
   __builtin_nontemporal_store(v, reinterpret_cast<Vec<T, N>*>(p));
 }
 
+// Memory from an address on as a buffer resource, for stores with a cache
+// policy: 32-bit offsets, and what lies outside `bytes` is dropped.
+typedef __amdgpu_buffer_rsrc_t Region;
+
+__device__ __forceinline__ Region region(void* p, uint32_t bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc(p, 0, int(bytes), 0x00027000);
+}
+
+constexpr int kThrough = 16;     // sc1: whole lines go through the L2
+
+template <int POLICY, typename T, int N>
+__device__ __forceinline__ void store_region(Region r, uint32_t at, const float (&f)[N]) {
+  typename VecAt<T, N>::packed v;
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = static_cast<T>(f[i]);
+  typedef unsigned int u32;
+  typedef u32 u32x2 __attribute__((ext_vector_type(2)));
+  typedef u32 u32x4 __attribute__((ext_vector_type(4)));
+  constexpr int kBytes = N * sizeof(T);
+  static_assert(kBytes == 8 || kBytes == 16 || kBytes == 32, "whole vectors");
+  if constexpr (kBytes == 8) {
+    __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, v), r, at, 0, POLICY);
+  } else if constexpr (kBytes == 16) {
+    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), r, at, 0, POLICY);
+  } else {
+    struct Two { u32x4 a, b; };
+    const Two t = __builtin_bit_cast(Two, v);
+    __builtin_amdgcn_raw_buffer_store_b128(t.a, r, at, 0, POLICY);
+    __builtin_amdgcn_raw_buffer_store_b128(t.b, r, at + 16, 0, POLICY);
+  }
+}
+
 template <typename T>
 __device__ __forceinline__ T wave_sum(T x) {
 #pragma unroll
   for (int d = kWave / 2; d; d >>= 1) x += __shfl_xor(x, d);
   return x;
+}
+
+// Work items in the order of memory, an eighth of them for each of the 8 dies
+// that workgroups go to in turn: the items in flight then come from 8 distant
+// regions.  A grid of xcd_blocks(items), of which some have no item.
+constexpr uint32_t kXcds = 8;
+__host__ __device__ inline uint32_t xcd_blocks(uint32_t items) { return (items + kXcds - 1) / kXcds * kXcds; }
+__device__ __forceinline__ uint32_t xcd_order(uint32_t block, uint32_t items) {
+  return block % kXcds * ((items + kXcds - 1) / kXcds) + block / kXcds;
 }
 
 inline int launched(const char* what) {

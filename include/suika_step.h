@@ -64,8 +64,8 @@ typedef struct sr_array {
  * their sums before clipping.  workspace: sr_square_sum_workspace bytes.
  */
 int sr_square_sum_workspace(const sr_array* arrays, int32_t count, uint64_t* bytes);
-int sr_square_sum(const sr_array* arrays, int32_t count, void* workspace, uint64_t workspace_bytes, double* sum,
-                  float* norm, hipStream_t stream);
+int sr_square_sum(const sr_array* arrays, int32_t count, int32_t read_again, void* workspace, uint64_t workspace_bytes,
+                  double* sum, float* norm, hipStream_t stream);
 
 /*
  * dst[i] = src[i] * min(1, max_norm / (sqrt(*square_sum) + 1e-6)), array by

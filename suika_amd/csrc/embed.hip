@@ -117,9 +117,11 @@ struct alignas(16) Piece {
 };
 constexpr uint32_t kNoPiece = 0xffffffffu;
 
-// The sorted positions of a row's tokens.
-struct Run {
+// The sorted positions of a row's tokens, and the first two tokens: most rows
+// have no more, and these are one load less away.
+struct alignas(16) Run {
   uint32_t from, to;
+  uint32_t token[2];
 };
 
 // What the launches hand on, in the workspace.
@@ -204,7 +206,7 @@ __global__ __launch_bounds__(kSortThreads) void sort_kernel(const I* tokens, uin
                                                             uint64_t start, Owners owners, uint32_t bits,
                                                             uint32_t piece, Sorted out) {
   __shared__ uint32_t count[kSortWaves * kSortRows];
-  __shared__ uint32_t part[kSortWaves];
+  __shared__ uint32_t part[kSortWaves], start_of[kSortRows];
   __shared__ uint32_t kept[kSortWaves][kSortKept], kept_row[kSortWaves][kSortKept];
   const uint32_t wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
   const uint64_t below = (uint64_t(1) << lane) - 1;
@@ -251,7 +253,11 @@ __global__ __launch_bounds__(kSortThreads) void sort_kernel(const I* tokens, uin
       next += c;
     }
     const uint32_t row = (threadIdx.x << owners.log2) + me;
-    if (row < rows) out.run[row] = {at, at + n};
+    start_of[threadIdx.x] = at;
+    if (row < rows) {
+      out.run[row].from = at;
+      out.run[row].to = at + n;
+    }
     if (me == mask && threadIdx.x == 0) *out.tokens = base + total;
   }
   // A workgroup of `total` tokens has the slots from 2 base / piece on.  A row is
@@ -274,7 +280,11 @@ __global__ __launch_bounds__(kSortThreads) void sort_kernel(const I* tokens, uin
     uint32_t next = 0;
     if (own && int(lane) == leader) next = atomicAdd(mine + local, uint32_t(__popcll(same)));
     next = __shfl(next, leader & (kWave - 1));
-    if (own) out.order[next + uint32_t(__popcll(same & below))] = i;
+    if (own) {
+      const uint32_t p = next + uint32_t(__popcll(same & below)), nth = p - start_of[local];
+      out.order[p] = i;
+      if (nth < 2) out.run[(local << owners.log2) + me].token[nth] = i;
+    }
   };
   if (found <= kSortKept) {
     for (uint32_t k = lane; k - lane < found; k += kWave) {
@@ -369,7 +379,20 @@ __global__ __launch_bounds__(kThreads) void sum_kernel(const T* grad_out, uint64
   const Run run = in.run[row];
   const uint32_t n = run.to - run.from;
   if (n > 2 * piece || (accumulate && n == 0)) return;
-  sum_tokens<T, N>(grad_out, stride, in.order, run.from, run.to, c, cols, acc);
+  uint32_t from = run.from;
+  if (c + N <= cols) {
+    Vec<T, N> x[2];
+#pragma unroll
+    for (uint32_t a = 0; a < 2; ++a)
+      if (a < n) x[a] = __builtin_nontemporal_load(reinterpret_cast<const Vec<T, N>*>(grad_out + run.token[a] * stride + c));
+#pragma unroll
+    for (uint32_t a = 0; a < 2; ++a)
+      if (a < n)
+#pragma unroll
+        for (int k = 0; k < N; ++k) acc[k] += float(x[a][k]);
+    from += n < 2 ? n : 2;
+  }
+  sum_tokens<T, N>(grad_out, stride, in.order, from, run.to, c, cols, acc);
   put_row<G, N>(grad + row * cols, c, cols, scale, accumulate, acc);
 }
 

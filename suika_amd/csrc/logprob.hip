@@ -127,8 +127,7 @@ __device__ __forceinline__ uint32_t column_of(uint64_t c) { return 0xffffffffu -
 struct Shared {
   Stats stats[kWaves];
   float maxima[kWave];
-  uint32_t group[kWave];
-  float bound;
+  uint32_t group[kWave], place[kWave];
   uint32_t count;
   uint64_t list[kCandidates];
   uint64_t best[kWaves];
@@ -241,7 +240,7 @@ struct Summary {
 
 // Statistics of a row that the running sums do not cover.
 template <typename T>
-__device__ Summary plain_summary(Shared& sh, const T* row, uint32_t vocab) {
+__device__ __forceinline__ Summary plain_summary(Shared& sh, const T* row, uint32_t vocab) {
   float m = -kInf, bad = 0;
   for (uint32_t c = threadIdx.x; c < vocab; c += kThreads) {
     const float x = float(row[c]);
@@ -276,7 +275,7 @@ __device__ __forceinline__ Summary summary_of(const Stats& t) {
 // The k best candidates of the lanes, one after the other: a look at the whole
 // row for each.
 template <typename T>
-__device__ void plain_top(Shared& sh, const T* row, uint32_t from, uint32_t to, int k) {
+__device__ __forceinline__ void plain_top(Shared& sh, const T* row, uint32_t from, uint32_t to, int k) {
   uint64_t last = ~uint64_t(0);
   for (int i = 0; i < k; ++i) {
     uint64_t best = 0;
@@ -303,7 +302,8 @@ __device__ __forceinline__ void rank_list(Shared& sh, uint32_t n, int k) {
 }
 
 // Adds the logits of the groups in `groups` that reach `bound`, or are above
-// it, to the list.  The groups' vectors are dealt out to all lanes, neighbours
+// it, to the list (its count was set, and the groups' list is free, before a
+// barrier).  The groups' vectors are dealt out to all lanes, neighbours
 // of a group to neighbouring lanes, and several loads of a lane are on their
 // way at once.
 template <typename T>
@@ -311,7 +311,6 @@ __device__ __forceinline__ void list_reaching(Shared& sh, const T* row, uint32_t
                                               float bound, bool above) {
   constexpr uint32_t N = 16 / sizeof(T), kAhead = 4;
   const uint32_t lane = threadIdx.x % kWave;
-  __syncthreads();
   if (threadIdx.x < kWave && (groups >> lane & 1)) sh.group[__popcll(groups & ((uint64_t(1) << lane) - 1))] = lane;
   __syncthreads();
   // Quads of lanes take (group, round) pairs, 64 of them at a time.
@@ -319,13 +318,18 @@ __device__ __forceinline__ void list_reaching(Shared& sh, const T* row, uint32_t
   const uint32_t all = uint32_t(__popcll(groups)), step = kThreads / kShare;
   const uint32_t g_step = step / rounds, r_step = step % rounds;
   uint32_t g = threadIdx.x / kShare / rounds, r = threadIdx.x / kShare % rounds;
+  auto reaches = [&](float x) { return above ? x > bound : x >= bound; };
+  auto add = [&](float x, uint32_t c) {
+    const uint32_t at = atomicAdd(&sh.count, 1u);
+    if (at < kCandidates) sh.list[at] = candidate(x, c);
+  };
   while (__ballot(g < all)) {
-    float x[kAhead][N];
+    Vec<T, N> x[kAhead];
     uint32_t c[kAhead];
 #pragma unroll
     for (uint32_t a = 0; a < kAhead; ++a) {
       c[a] = g < all ? from + (sh.group[g] * kShare + threadIdx.x % kShare + r * kThreads) * N : to;
-      load_or_fill<T, N>(row, c[a], to, x[a]);
+      if (c[a] + N <= to) x[a] = *reinterpret_cast<const Vec<T, N>*>(row + c[a]);
       g += g_step;
       r += r_step;
       if (r >= rounds) {
@@ -335,17 +339,17 @@ __device__ __forceinline__ void list_reaching(Shared& sh, const T* row, uint32_t
     }
 #pragma unroll
     for (uint32_t a = 0; a < kAhead; ++a) {
-      float top = x[a][0];
+      if (c[a] + N <= to) {
+        float top = float(x[a][0]);
 #pragma unroll
-      for (uint32_t k = 1; k < N; ++k) top = fmaxf(top, x[a][k]);
-      if (above ? top > bound : top >= bound) {
+        for (uint32_t k = 1; k < N; ++k) top = fmaxf(top, float(x[a][k]));
+        if (!reaches(top)) continue;
 #pragma unroll
-        for (uint32_t k = 0; k < N; ++k) {
-          if ((above ? x[a][k] > bound : x[a][k] >= bound) && c[a] + k < to) {
-            const uint32_t at = atomicAdd(&sh.count, 1u);
-            if (at < kCandidates) sh.list[at] = candidate(x[a][k], c[a] + k);
-          }
-        }
+        for (uint32_t k = 0; k < N; ++k)
+          if (reaches(float(x[a][k]))) add(float(x[a][k]), c[a] + k);
+      } else {
+        for (uint32_t k = c[a]; k < to; ++k)
+          if (reaches(float(row[k]))) add(float(row[k]), k);
       }
     }
   }
@@ -354,7 +358,7 @@ __device__ __forceinline__ void list_reaching(Shared& sh, const T* row, uint32_t
 // Adds the first `need` columns whose logit equals `bound` to the list, in
 // their order.
 template <typename T>
-__device__ void list_equal(Shared& sh, const T* row, uint32_t from, uint32_t to, float bound, uint32_t need) {
+__device__ __forceinline__ void list_equal(Shared& sh, const T* row, uint32_t from, uint32_t to, float bound, uint32_t need) {
   uint32_t* part = reinterpret_cast<uint32_t*>(sh.maxima);
   const uint32_t lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
   const uint32_t start = sh.count;
@@ -380,7 +384,7 @@ __device__ void list_equal(Shared& sh, const T* row, uint32_t from, uint32_t to,
 // sh.chosen = the k best of columns from..to (at least k columns, k <= 64); `m`
 // is the largest logit of this lane's part, `finite` that there is no NaN.
 template <typename T>
-__device__ void row_top(Shared& sh, const T* row, uint32_t from, uint32_t to, int k, float m, bool finite) {
+__device__ __forceinline__ void row_top(Shared& sh, const T* row, uint32_t from, uint32_t to, int k, float m, bool finite) {
   static_assert(kMaxTop <= kWave, "as many groups as alternatives");
   if (!finite) {
     plain_top(sh, row, from, to, k);
@@ -392,20 +396,24 @@ __device__ void row_top(Shared& sh, const T* row, uint32_t from, uint32_t to, in
   for (int d = 1; d < kShare; d <<= 1) m = fmaxf(m, __shfl_xor(m, d));
   __syncthreads();
   if (threadIdx.x % kShare == 0) sh.maxima[threadIdx.x / kShare] = m;
+  if (threadIdx.x < kWave) sh.place[threadIdx.x] = 0;
   if (threadIdx.x == 0) sh.count = 0;
   __syncthreads();
-  const float mine = sh.maxima[threadIdx.x % kWave];
-  if (threadIdx.x < kWave) {
-    int before = 0;
+  // Every wave compares with a quarter of the groups, so that the counts add up
+  // to a group's place.
+  const uint32_t lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+  const float mine = sh.maxima[lane];
+  uint32_t before = 0;
 #pragma unroll
-    for (int j = 0; j < kWave; ++j) {
-      const float o = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(mine), j));
-      before += o > mine || (o == mine && j < int(threadIdx.x));
-    }
-    if (before == k - 1) sh.bound = mine;
+  for (uint32_t j = 0; j < kWave / kWaves; ++j) {
+    const uint32_t other = wave * (kWave / kWaves) + j;
+    const float o = sh.maxima[other];
+    before += o > mine || (o == mine && other < lane);
   }
+  atomicAdd(&sh.place[lane], before);
   __syncthreads();
-  const float bound = sh.bound;
+  const int at = __ffsll((unsigned long long)__ballot(sh.place[lane] == uint32_t(k - 1))) - 1;
+  const float bound = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(mine), at));
   list_reaching(sh, row, from, to, __ballot(mine >= bound), bound, false);
   __syncthreads();
   uint32_t n = sh.count;
@@ -516,35 +524,51 @@ __global__ __launch_bounds__(kThreads) void part_kernel(const T* logits, uint64_
   }
 }
 
-// sh.chosen = the k best of the parts' candidates.  The k-th best of what each
-// part has in front bounds them from below.
-__device__ void parts_top(Shared& sh, const uint64_t* best, uint32_t parts, int k) {
-  uint32_t front = (2 * uint32_t(k) + parts - 1) / parts;
-  front = front < uint32_t(k) ? front : uint32_t(k);
-  const uint32_t n = parts * front;
+// sh.chosen = the k best of n candidates, of which `most` is the best of this
+// lane's (every kThreads-th).  As in a row: the k-th largest of the lane groups'
+// maxima bounds them from below.
+__device__ __forceinline__ void parts_top(Shared& sh, const uint64_t* best, uint32_t n, uint64_t most, int k) {
+#pragma unroll
+  for (int d = 1; d < kShare; d <<= 1) {
+    const uint64_t o = __shfl_xor((unsigned long long)most, d);
+    most = o > most ? o : most;
+  }
   __syncthreads();
-  for (uint32_t i = threadIdx.x; i < n; i += kThreads) sh.list[i] = best[i / front * k + i % front];
+  if (threadIdx.x % kShare == 0) sh.list[threadIdx.x / kShare] = most;
+  if (threadIdx.x < kWave) sh.place[threadIdx.x] = 0;
   if (threadIdx.x == 0) sh.count = 0;
   __syncthreads();
-  rank_list(sh, n, k);
-  const uint64_t bound = sh.chosen[k - 1];
+  const uint32_t lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+  const uint64_t mine = sh.list[lane];
+  uint32_t before = 0;
+#pragma unroll
+  for (uint32_t j = 0; j < kWave / kWaves; ++j) {
+    const uint32_t other = wave * (kWave / kWaves) + j;
+    const uint64_t o = sh.list[other];
+    before += o > mine || (o == mine && other < lane);
+  }
+  atomicAdd(&sh.place[lane], before);
   __syncthreads();
-  for (uint32_t i = threadIdx.x; i < parts * k; i += kThreads) {
+  const int at = __ffsll((unsigned long long)__ballot(sh.place[lane] == uint32_t(k - 1))) - 1;
+  const uint64_t bound = __shfl((unsigned long long)mine, at);
+  __syncthreads();
+  for (uint32_t i = threadIdx.x; i < n; i += kThreads) {
     const uint64_t x = best[i];
-    if (x >= bound) {
-      const uint32_t at = atomicAdd(&sh.count, 1u);
-      if (at < kCandidates) sh.list[at] = x;
+    if (x >= bound && x != 0) {
+      const uint32_t to = atomicAdd(&sh.count, 1u);
+      if (to < kCandidates) sh.list[to] = x;
     }
   }
   __syncthreads();
-  if (sh.count <= kCandidates) {
-    rank_list(sh, sh.count, k);
+  const uint32_t listed = sh.count;
+  if (listed <= kCandidates) {
+    rank_list(sh, listed, k);
     return;
   }
   uint64_t last = ~uint64_t(0);
   for (int i = 0; i < k; ++i) {
     uint64_t top = 0;
-    for (uint32_t j = threadIdx.x; j < parts * k; j += kThreads) {
+    for (uint32_t j = threadIdx.x; j < n; j += kThreads) {
       const uint64_t x = best[j];
       if ((i == 0 || x < last) && x > top) top = x;
     }
@@ -562,9 +586,13 @@ __global__ __launch_bounds__(kThreads) void parts_kernel(const T* logits, const 
   const T* row = logits + i * stride;
   const Target target = target_of(row, targets, i, vocab);
   const Stats mine = threadIdx.x < in.parts ? in.stats[i * in.parts + threadIdx.x] : Stats{-kInf, kLeast, 0, 0};
+  const uint32_t n = in.parts * uint32_t(k);
+  const uint64_t* best = in.best + i * n;
+  uint64_t most = 0;
+  for (uint32_t j = threadIdx.x; j < n; j += kThreads) most = best[j] > most ? best[j] : most;
   const Stats all = block_join(sh, mine);
   const Summary r = sound(all) ? summary_of(all) : plain_summary(sh, row, vocab);
-  if (k) parts_top(sh, in.best + i * in.parts * k, in.parts, k);
+  if (k) parts_top(sh, best, n, most, k);
   put(sh, target, i, k, r, out);
 }
 

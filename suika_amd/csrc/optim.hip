@@ -6,14 +6,18 @@
 // kernels by value, in tables of up to 4 KB of kernel arguments, so nothing is
 // uploaded and nothing is kept between calls; a longer list takes several
 // launches.  Arrays are cut into chunks of a fixed number of elements, numbered
-// through the table; a wave finds the array of a chunk by comparing all first
-// chunks at once, an entry a lane.
+// through the table.  A wave finds the array of a chunk by comparing all first
+// chunks at once, a few of them a lane: one vector load on the way to the
+// addresses.  (Scalar loads from an index by the chunk's number take longer, as
+// each waits for the one before: AdamW of 8 arrays of 112 M elements in mixed
+// precision 4.31 ms, with the comparison LOOKUP_MS.)
 
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
 #include <cmath>
 #include <new>
+#include <type_traits>
 #include <vector>
 
 #include "suika_step.h"
@@ -28,35 +32,87 @@ constexpr int kThreads = 256;
 // A table of 4 KB, less the 256 bytes of arguments that the compiler adds.
 constexpr size_t kTableBytes = 3832;
 
-// The entry of a table that chunk `c` lies in: the last one whose first chunk
-// is not behind it.  `first` rises strictly (empty arrays are left out).
-__device__ __forceinline__ int entry_of(const uint32_t* first, int count, uint32_t c) {
-  int found = 0;
-  for (int base = 0; base < count; base += kWave) {
-    const int i = base + int(threadIdx.x % kWave);
-    found += __popcll(__ballot(i < count && first[i] <= c));
+// Most chunks of one launch: the grid's threads stay below 2^32.
+constexpr uint32_t kMostChunks = 1u << 23;
+static_assert(SR_STEP_MAX_ELEMENTS / 2048 <= kMostChunks, "an array fits into a launch");
+
+// Where the chunks of a table's entries start.
+template <int ENTRIES>
+struct Chunks {
+  static constexpr int kEach = (ENTRIES + kWave - 1) / kWave;     // entries of a lane
+  static_assert(ENTRIES % kEach == 0, "a lane's entries are loaded together");
+
+  uint32_t first[ENTRIES];       // rises strictly: empty arrays are left out
+  uint32_t count;                // entries
+  uint32_t chunks;
+
+  void clear() {
+    count = chunks = 0;
+    for (uint32_t& f : first) f = 0xffffffffu;
   }
-  return __builtin_amdgcn_readfirstlane(found - 1);
-}
+  bool room(uint64_t n, uint32_t chunk) const {
+    return count < ENTRIES && (count == 0 || chunks + (n + chunk - 1) / chunk <= kMostChunks);
+  }
+  // Takes an array of n elements; returns its entry.
+  uint32_t add(uint64_t n, uint32_t chunk) {
+    first[count] = chunks;
+    chunks += uint32_t((n + chunk - 1) / chunk);
+    return count++;
+  }
+
+  // The entry of chunk c, and where it and the next one start.
+  struct Found {
+    uint32_t entry, from, to;
+  };
+
+  __device__ __forceinline__ Found find(uint32_t c) const {
+    const int lane = threadIdx.x % kWave;
+    const bool in = lane < ENTRIES / kEach;
+    uint32_t f[kEach];
+#pragma unroll
+    for (int k = 0; k < kEach; ++k) f[k] = first[(in ? lane : 0) * kEach + k];
+    uint32_t n = 0;
+#pragma unroll
+    for (int k = 0; k < kEach; ++k) n += uint32_t(__popcll(__ballot(in && f[k] <= c)));
+    Found r;
+    r.entry = __builtin_amdgcn_readfirstlane(n) - 1;
+    r.from = at(f, r.entry);
+    r.to = r.entry + 1 < ENTRIES ? at(f, r.entry + 1) : 0xffffffffu;
+    r.to = r.to < chunks ? r.to : chunks;
+    return r;
+  }
+
+ private:
+  __device__ __forceinline__ static uint32_t at(const uint32_t (&f)[kEach], uint32_t i) {
+    uint32_t x = 0;
+#pragma unroll
+    for (int k = 0; k < kEach; ++k) {
+      const uint32_t y = __builtin_amdgcn_readlane(f[k], i / kEach);
+      x = i % kEach == k ? y : x;
+    }
+    return x;
+  }
+};
 
 // ------------------------------------------------------------ sum of squares
 
 // sum += x^2 over all elements, in 64 bits: squares of f32 values neither
 // overflow nor vanish there, and each product of two 24-bit numbers is exact.
-constexpr int kSumEntries = 188;
+constexpr int kSumEntries = 189;
 constexpr uint32_t kSumChunk = 32768;      // elements
 constexpr uint32_t kSumBlocks = 16384;     // workgroups of one launch at most
-#ifndef SUM_CACHED
-#define SUM_CACHED (uint64_t(1) << 30)
-#endif
-constexpr uint64_t kSumCached = SUM_CACHED;
+
+// Loads stream past the caches (2.56 GB of bf16 372 us, cached 422; 320 MB of
+// f32 51.5, cached 58), unless the arrays are read again soon and are not much
+// more than the 256 MB memory-side cache: then the next reader finds part of
+// them there (clipping 320 MB of f32 into other tensors, norm included, 151 us
+// with cached loads, 159 with streamed ones; 640 MB 307 and 310; 1.28 GB 627
+// and 618).
+constexpr uint64_t kSumCached = uint64_t(1) << 30;
 
 struct SumTable {
-  uint64_t data[kSumEntries];
-  uint64_t n[kSumEntries];
-  uint32_t first[kSumEntries];
-  int32_t count;
-  uint32_t chunks;
+  struct Entry { uint64_t data, n; } entry[kSumEntries];
+  Chunks<kSumEntries> at;
 };
 static_assert(sizeof(SumTable) <= kTableBytes, "kernel arguments");
 
@@ -75,17 +131,19 @@ __device__ __forceinline__ double block_sum(double x) {
 }
 
 template <typename T, bool STREAM>
-__global__ __launch_bounds__(kThreads) void square_sum_kernel(SumTable t, uint32_t run, double* partial) {
+__global__ __launch_bounds__(kThreads) void square_sum_kernel(uint32_t run, uint32_t chunks, double* partial,
+                                                             SumTable t) {
   constexpr int N = 16 / sizeof(T);
   constexpr int kBatch = 8;
   double sum[4] = {0, 0, 0, 0};
-  const uint32_t end = min((blockIdx.x + 1) * run, t.chunks);
+  const uint32_t end = min((blockIdx.x + 1) * run, chunks);
   for (uint32_t c = blockIdx.x * run; c < end; ++c) {
-    const int i = entry_of(t.first, t.count, c);
-    const uint64_t at = uint64_t(c - t.first[i]) * kSumChunk;
-    const uint64_t left = t.n[i] - at;
+    const auto found = t.at.find(c);
+    const uint32_t i = found.entry;
+    const uint64_t at = uint64_t(c - found.from) * kSumChunk;
+    const uint64_t left = t.entry[i].n - at;
     const uint32_t n = left < kSumChunk ? uint32_t(left) : kSumChunk;
-    const T* p = reinterpret_cast<const T*>(t.data[i]) + at;
+    const T* p = global<const T>(t.entry[i].data) + at;
     uint32_t e = threadIdx.x * N;
     for (; e + (kBatch - 1) * kThreads * N + N <= n; e += kBatch * kThreads * N) {
       Vec<T, N> x[kBatch];
@@ -144,11 +202,8 @@ constexpr int kClipEntries = 128;
 constexpr uint32_t kClipChunk = 4096;
 
 struct ClipTable {
-  uint64_t src[kClipEntries];
-  uint64_t dst[kClipEntries];
-  uint64_t n[kClipEntries];
-  uint32_t first[kClipEntries];
-  int32_t count;
+  struct Entry { uint64_t src, dst, n; } entry[kClipEntries];
+  Chunks<kClipEntries> at;
   float max_norm;
   const double* square_sum;
   float* norm;
@@ -167,16 +222,17 @@ __global__ __launch_bounds__(kThreads) void clip_kernel(ClipTable t) {
   constexpr int kBatch = kClipChunk / (kThreads * N);
   const double q = *t.square_sum;
   if (t.norm && blockIdx.x == 0 && threadIdx.x == 0) *t.norm = float(sqrt(q));
-  if (t.count == 0) return;
+  if (t.at.count == 0) return;
   const uint32_t c = blockIdx.x;
-  const int i = entry_of(t.first, t.count, c);
+  const auto found = t.at.find(c);
+  const uint32_t i = found.entry;
   const float f = clip_factor(q, t.max_norm);
-  if (f == 1.0f && t.dst[i] == t.src[i]) return;
-  const uint64_t at = uint64_t(c - t.first[i]) * kClipChunk;
-  const uint64_t left = t.n[i] - at;
+  if (f == 1.0f && t.entry[i].dst == t.entry[i].src) return;
+  const uint64_t at = uint64_t(c - found.from) * kClipChunk;
+  const uint64_t left = t.entry[i].n - at;
   const uint32_t n = left < kClipChunk ? uint32_t(left) : kClipChunk;
-  const S* src = reinterpret_cast<const S*>(t.src[i]) + at;
-  D* dst = reinterpret_cast<D*>(t.dst[i]) + at;
+  const S* src = global<const S>(t.entry[i].src) + at;
+  D* dst = global<D>(t.entry[i].dst) + at;
   float x[kBatch][N];
 #pragma unroll
   for (int b = 0; b < kBatch; ++b) {
@@ -198,20 +254,20 @@ __global__ __launch_bounds__(kThreads) void clip_kernel(ClipTable t) {
 
 // --------------------------------------------------------------------- AdamW
 
-constexpr int kAdamEntries = 78;
 constexpr int kAdamThreads = 512;
 constexpr uint32_t kAdamChunk = 2048;
 
+// What a table holds of one parameter; without a copy of the weight, one
+// address less.
+template <bool COPY> struct AdamEntry { uint64_t weight, exp_avg, exp_avg_sq, grad, param; };
+template <> struct AdamEntry<false> { uint64_t weight, exp_avg, exp_avg_sq, grad; };
+
+template <bool COPY>
 struct AdamTable {
-  uint64_t weight[kAdamEntries];
-  uint64_t exp_avg[kAdamEntries];
-  uint64_t exp_avg_sq[kAdamEntries];
-  uint64_t param[kAdamEntries];
-  uint64_t grad[kAdamEntries];
-  uint32_t first[kAdamEntries];
-  uint32_t tail[kAdamEntries];    // elements of the last chunk
-  int32_t count;
-  uint32_t chunks;
+  static constexpr int kEntries = COPY ? 80 : 96;
+  AdamEntry<COPY> entry[kEntries];
+  Chunks<kEntries> at;
+  uint16_t tail[kEntries];        // elements of the last chunk
   const double* square_sum;
   float max_norm;
   float decay;                    // 1 - lr * weight_decay
@@ -220,7 +276,7 @@ struct AdamTable {
   float root_scale;               // 1 / sqrt(1 - beta2^step)
   float eps;
 };
-static_assert(sizeof(AdamTable) <= kTableBytes, "kernel arguments");
+static_assert(sizeof(AdamTable<true>) <= kTableBytes && sizeof(AdamTable<false>) <= kTableBytes, "kernel arguments");
 
 struct NoCopy {};
 
@@ -228,18 +284,19 @@ struct NoCopy {};
 // W: type of the weight, M: of the moments, G: of the gradient, P: of the
 // weight's copy, or NoCopy.
 template <typename W, typename M, typename G, typename P>
-__global__ __launch_bounds__(kAdamThreads) void adamw_kernel(AdamTable t) {
+__global__ __launch_bounds__(kAdamThreads) void adamw_kernel(uint32_t chunks,
+                                                             AdamTable<!__is_same(P, NoCopy)> t) {
   constexpr int N = kAdamChunk / kAdamThreads;
-    const uint32_t c = xcd_order(blockIdx.x, t.chunks);
-  if (c >= t.chunks) return;
-  const int i = entry_of(t.first, t.count, c);
-  const uint32_t next = i + 1 < t.count ? t.first[i + 1] : t.chunks;
-  const uint32_t n = c + 1 == next ? t.tail[i] : kAdamChunk;
-  const uint64_t at = uint64_t(c - t.first[i]) * kAdamChunk;
-  W* weight = reinterpret_cast<W*>(t.weight[i]) + at;
-  M* exp_avg = reinterpret_cast<M*>(t.exp_avg[i]) + at;
-  M* exp_avg_sq = reinterpret_cast<M*>(t.exp_avg_sq[i]) + at;
-  const G* grad = reinterpret_cast<const G*>(t.grad[i]) + at;
+    const uint32_t c = xcd_order(blockIdx.x, chunks);
+  if (c >= chunks) return;
+  const auto found = t.at.find(c);
+  const uint32_t i = found.entry;
+  const uint32_t n = c + 1 == found.to ? t.tail[i] : kAdamChunk;
+  const uint64_t at = uint64_t(c - found.from) * kAdamChunk;
+  W* weight = global<W>(t.entry[i].weight) + at;
+  M* exp_avg = global<M>(t.entry[i].exp_avg) + at;
+  M* exp_avg_sq = global<M>(t.entry[i].exp_avg_sq) + at;
+  const G* grad = global<const G>(t.entry[i].grad) + at;
 
   const uint32_t e = threadIdx.x * N;
   const bool whole = e + N <= n;
@@ -264,7 +321,7 @@ __global__ __launch_bounds__(kAdamThreads) void adamw_kernel(AdamTable t) {
     store_stream<W, N>(weight + e, w);
     store_stream<M, N>(exp_avg + e, m);
     store_stream<M, N>(exp_avg_sq + e, v);
-    if constexpr (!__is_same(P, NoCopy)) store_stream<P, N>(reinterpret_cast<P*>(t.param[i]) + at + e, w);
+    if constexpr (!__is_same(P, NoCopy)) store_stream<P, N>(global<P>(t.entry[i].param) + at + e, w);
   } else {
     for (uint32_t k = e; k < n; ++k) {
       float wi = float(weight[k]), mi = float(exp_avg[k]), vi = float(exp_avg_sq[k]);
@@ -272,7 +329,7 @@ __global__ __launch_bounds__(kAdamThreads) void adamw_kernel(AdamTable t) {
       weight[k] = W(wi);
       exp_avg[k] = M(mi);
       exp_avg_sq[k] = M(vi);
-      if constexpr (!__is_same(P, NoCopy)) (reinterpret_cast<P*>(t.param[i]) + at)[k] = P(wi);
+      if constexpr (!__is_same(P, NoCopy)) (global<P>(t.entry[i].param) + at)[k] = P(wi);
     }
   }
 }
@@ -320,82 +377,115 @@ bool clash(std::vector<Span>& spans) {
   return false;
 }
 
-// Most chunks of one launch: the grid's threads stay below 2^32.
-constexpr uint32_t kMostChunks = 1u << 23;
 
 constexpr int32_t kFloatTypes[3] = {SR_DT_F32, SR_DT_BF16, SR_DT_F16};
 
-// Launches of a list: the arrays of one type at a time, kSumEntries a table.
+// Launches of a list: the arrays of one type at a time, as many as a table takes.
 template <typename F>
 int sum_launches(const sr_array* a, int32_t count, F&& launch) {
   for (int32_t dt : kFloatTypes) {
     SumTable t;
-    t.count = 0;
-    t.chunks = 0;
+    t.at.clear();
+    auto flush = [&]() -> int {
+      if (t.at.count == 0) return SR_OK;
+      const int rc = launch(dt, t);
+      t.at.clear();
+      return rc;
+    };
     for (int32_t i = 0; i < count; ++i) {
       if (a[i].dtype != dt || a[i].n == 0) continue;
-      if (t.count == kSumEntries) {
-        if (int rc = launch(dt, t)) return rc;
-        t.count = 0;
-        t.chunks = 0;
+      if (!t.at.room(a[i].n, kSumChunk)) {
+        if (int rc = flush()) return rc;
       }
-      const int k = t.count++;
-      t.data[k] = reinterpret_cast<uint64_t>(a[i].data);
-      t.n[k] = a[i].n;
-      t.first[k] = t.chunks;
-      t.chunks += uint32_t((a[i].n + kSumChunk - 1) / kSumChunk);
+      t.entry[t.at.add(a[i].n, kSumChunk)] = {reinterpret_cast<uint64_t>(a[i].data), a[i].n};
     }
-    if (t.count) {
-      if (int rc = launch(dt, t)) return rc;
-    }
+    if (int rc = flush()) return rc;
   }
   return SR_OK;
 }
 
 // Consecutive chunks of one workgroup, and the workgroups.
-uint32_t sum_run(const SumTable& t) { return (t.chunks + kSumBlocks - 1) / kSumBlocks; }
-uint32_t sum_blocks(const SumTable& t) { return (t.chunks + sum_run(t) - 1) / sum_run(t); }
+uint32_t sum_run(const SumTable& t) { return (t.at.chunks + kSumBlocks - 1) / kSumBlocks; }
+uint32_t sum_blocks(const SumTable& t) { return (t.at.chunks + sum_run(t) - 1) / sum_run(t); }
 
 template <typename T>
 void launch_sum(const SumTable& t, uint32_t run, uint32_t blocks, bool stream_loads, double* partial,
                 hipStream_t stream) {
-  if (stream_loads) square_sum_kernel<T, true><<<blocks, kThreads, 0, stream>>>(t, run, partial);
-  else square_sum_kernel<T, false><<<blocks, kThreads, 0, stream>>>(t, run, partial);
+  if (stream_loads) square_sum_kernel<T, true><<<blocks, kThreads, 0, stream>>>(run, t.at.chunks, partial, t);
+  else square_sum_kernel<T, false><<<blocks, kThreads, 0, stream>>>(run, t.at.chunks, partial, t);
 }
 
 template <typename S, typename D>
-void launch_clip(const ClipTable& t, uint32_t blocks, hipStream_t stream) {
-  clip_kernel<S, D><<<blocks, kThreads, 0, stream>>>(t);
+void launch_clip(const ClipTable& t, hipStream_t stream) {
+  clip_kernel<S, D><<<t.at.chunks, kThreads, 0, stream>>>(t);
 }
 
 template <typename S>
-void launch_clip_to(int32_t dst, const ClipTable& t, uint32_t blocks, hipStream_t stream) {
-  if (dst == SR_DT_F32) launch_clip<S, float>(t, blocks, stream);
-  else if (dst == SR_DT_BF16) launch_clip<S, bf16>(t, blocks, stream);
-  else launch_clip<S, f16>(t, blocks, stream);
+void launch_clip_to(int32_t dst, const ClipTable& t, hipStream_t stream) {
+  if (dst == SR_DT_F32) launch_clip<S, float>(t, stream);
+  else if (dst == SR_DT_BF16) launch_clip<S, bf16>(t, stream);
+  else launch_clip<S, f16>(t, stream);
 }
 
-template <typename W, typename M, typename G>
-void launch_adamw_copy(bool copy, const AdamTable& t, hipStream_t stream) {
-  if constexpr (__is_same(W, float)) {
-    if (copy) {
-      adamw_kernel<W, M, G, bf16><<<xcd_blocks(t.chunks), kAdamThreads, 0, stream>>>(t);
-      return;
+template <typename W, typename M, typename G, bool COPY>
+void launch_adamw_of(const AdamTable<COPY>& t, hipStream_t stream) {
+  typedef typename std::conditional<COPY, bf16, NoCopy>::type P;
+  adamw_kernel<W, M, G, P><<<xcd_blocks(t.at.chunks), kAdamThreads, 0, stream>>>(t.at.chunks, t);
+}
+
+// The tensors whose fields have the types W, M and G, and a copy or none.
+template <typename W, typename M, typename G, bool COPY>
+int adamw_launches(const sr_adamw_tensor* tensors, int32_t count, AdamTable<COPY> t, hipStream_t stream) {
+  auto code = [](bool wide) { return wide ? SR_DT_F32 : SR_DT_BF16; };
+  const int32_t weight = code(__is_same(W, float)), moment = code(__is_same(M, float)), grad = code(__is_same(G, float));
+  t.at.clear();
+  auto flush = [&]() -> int {
+    if (t.at.count == 0) return SR_OK;
+    launch_adamw_of<W, M, G, COPY>(t, stream);
+    t.at.clear();
+    return launched("sr_adamw");
+  };
+  for (int32_t i = 0; i < count; ++i) {
+    const sr_adamw_tensor& x = tensors[i];
+    if (x.n == 0 || x.weight_dtype != weight || x.moment_dtype != moment || x.grad_dtype != grad ||
+        (x.param != nullptr) != COPY)
+      continue;
+    if (!t.at.room(x.n, kAdamChunk)) {
+      if (int rc = flush()) return rc;
     }
+    const uint32_t k = t.at.add(x.n, kAdamChunk);
+    auto& e = t.entry[k];
+    e.weight = reinterpret_cast<uint64_t>(x.weight);
+    e.exp_avg = reinterpret_cast<uint64_t>(x.exp_avg);
+    e.exp_avg_sq = reinterpret_cast<uint64_t>(x.exp_avg_sq);
+    e.grad = reinterpret_cast<uint64_t>(x.grad);
+    if constexpr (COPY) e.param = reinterpret_cast<uint64_t>(x.param);
+    t.tail[k] = uint16_t(x.n - (x.n - 1) / kAdamChunk * kAdamChunk);
   }
-  adamw_kernel<W, M, G, NoCopy><<<xcd_blocks(t.chunks), kAdamThreads, 0, stream>>>(t);
+  return flush();
 }
 
-template <typename W, typename M>
-void launch_adamw_grad(bool wide, bool copy, const AdamTable& t, hipStream_t stream) {
-  if (wide) launch_adamw_copy<W, M, float>(copy, t, stream);
-  else launch_adamw_copy<W, M, bf16>(copy, t, stream);
+// Without launches for the types that no tensor has.
+template <typename W, bool COPY>
+int adamw_types(const sr_adamw_tensor* tensors, int32_t count, const AdamTable<COPY>& t, hipStream_t stream) {
+  if (int rc = adamw_launches<W, float, float, COPY>(tensors, count, t, stream)) return rc;
+  if (int rc = adamw_launches<W, float, bf16, COPY>(tensors, count, t, stream)) return rc;
+  if (int rc = adamw_launches<W, bf16, float, COPY>(tensors, count, t, stream)) return rc;
+  return adamw_launches<W, bf16, bf16, COPY>(tensors, count, t, stream);
 }
 
-template <typename W>
-void launch_adamw_moments(bool wide, bool wide_grad, bool copy, const AdamTable& t, hipStream_t stream) {
-  if (wide) launch_adamw_grad<W, float>(wide_grad, copy, t, stream);
-  else launch_adamw_grad<W, bf16>(wide_grad, copy, t, stream);
+template <bool COPY>
+void adamw_scalars(AdamTable<COPY>& t, const sr_adamw_options& o, const double* square_sum) {
+  t.square_sum = square_sum;
+  t.max_norm = square_sum ? float(o.max_norm) : 0.0f;
+  t.decay = float(1 - o.lr * o.weight_decay);
+  t.beta1 = float(o.beta1);
+  t.rest1 = float(1 - o.beta1);
+  t.beta2 = float(o.beta2);
+  t.rest2 = float(1 - o.beta2);
+  t.step_size = float(o.lr / (1 - std::pow(o.beta1, double(o.step))));
+  t.root_scale = float(1 / std::sqrt(1 - std::pow(o.beta2, double(o.step))));
+  t.eps = float(o.eps);
 }
 
 }  // namespace
@@ -414,8 +504,8 @@ int sr_square_sum_workspace(const sr_array* arrays, int32_t count, uint64_t* byt
   return SR_OK;
 }
 
-int sr_square_sum(const sr_array* arrays, int32_t count, void* workspace, uint64_t workspace_bytes, double* sum,
-                  float* norm, hipStream_t stream) {
+int sr_square_sum(const sr_array* arrays, int32_t count, int32_t read_again, void* workspace, uint64_t workspace_bytes,
+                  double* sum, float* norm, hipStream_t stream) {
   uint64_t need = 0;
   if (int rc = sr_square_sum_workspace(arrays, count, &need)) return rc;
   if (sum == nullptr) return fail(SR_EINVAL, "sr_square_sum: sum is null");
@@ -427,7 +517,7 @@ int sr_square_sum(const sr_array* arrays, int32_t count, void* workspace, uint64
   uint32_t used = 0;
   uint64_t bytes = 0;
   for (int32_t i = 0; i < count; ++i) bytes += bytes_of(arrays[i]);
-  const bool stream_loads = bytes > kSumCached;
+  const bool stream_loads = read_again == 0 || bytes > kSumCached;
   const int rc = sum_launches(arrays, count, [&](int32_t dt, const SumTable& t) {
     const uint32_t blocks = sum_blocks(t), run = sum_run(t);
     if (dt == SR_DT_F32) launch_sum<float>(t, run, blocks, stream_loads, partial + used, stream);
@@ -464,45 +554,38 @@ int sr_clip(const sr_array* src, const sr_array* dst, int32_t count, const doubl
   for (int32_t s : kFloatTypes) {
     for (int32_t d : kFloatTypes) {
       ClipTable t;
-      t.count = 0;
+      t.at.clear();
       t.max_norm = max_norm;
       t.square_sum = square_sum;
-      uint32_t chunks = 0;
-      auto launch = [&]() -> int {
-        t.norm = any ? nullptr : norm;
+      auto flush = [&]() -> int {
+        if (t.at.count == 0) return SR_OK;
+          t.norm = any ? nullptr : norm;
         any = true;
-        if (s == SR_DT_F32) launch_clip_to<float>(d, t, chunks, stream);
-        else if (s == SR_DT_BF16) launch_clip_to<bf16>(d, t, chunks, stream);
-        else launch_clip_to<f16>(d, t, chunks, stream);
-        t.count = 0;
-        chunks = 0;
+        if (s == SR_DT_F32) launch_clip_to<float>(d, t, stream);
+        else if (s == SR_DT_BF16) launch_clip_to<bf16>(d, t, stream);
+        else launch_clip_to<f16>(d, t, stream);
+        t.at.clear();
         return launched("sr_clip");
       };
       for (int32_t i = 0; i < count; ++i) {
         if (src[i].dtype != s || dst[i].dtype != d || src[i].n == 0) continue;
-        const uint32_t more = uint32_t((src[i].n + kClipChunk - 1) / kClipChunk);
-        if (t.count == kClipEntries || (t.count && chunks + more > kMostChunks)) {
-          if (int rc = launch()) return rc;
+        if (!t.at.room(src[i].n, kClipChunk)) {
+          if (int rc = flush()) return rc;
         }
-        const int k = t.count++;
-        t.src[k] = reinterpret_cast<uint64_t>(src[i].data);
-        t.dst[k] = reinterpret_cast<uint64_t>(dst[i].data);
-        t.n[k] = src[i].n;
-        t.first[k] = chunks;
-        chunks += more;
+        t.entry[t.at.add(src[i].n, kClipChunk)] = {reinterpret_cast<uint64_t>(src[i].data),
+                                                   reinterpret_cast<uint64_t>(dst[i].data), src[i].n};
       }
-      if (t.count) {
-        if (int rc = launch()) return rc;
-      }
+      if (int rc = flush()) return rc;
     }
   }
   if (!any && norm != nullptr) {
-    ClipTable t;
-    t.count = 0;
+    ClipTable t;       // nothing to clip: the norm alone
+    t.at.clear();
+    t.at.chunks = 1;
     t.max_norm = max_norm;
     t.square_sum = square_sum;
     t.norm = norm;
-    launch_clip<float, float>(t, 1, stream);
+    launch_clip<float, float>(t, stream);
     return launched("sr_clip");
   }
   return SR_OK;
@@ -546,52 +629,13 @@ int sr_adamw(const sr_adamw_tensor* tensors, int32_t count, const sr_adamw_optio
   SR_STEP_TRY(hipStreamIsCapturing(stream, &capturing));
   if (capturing != hipStreamCaptureStatusNone)
     return fail(SR_EINVAL, "sr_adamw: the step number is a host value: the call cannot be captured");
-  AdamTable t;
-  t.square_sum = square_sum;
-  t.max_norm = square_sum ? float(o->max_norm) : 0.0f;
-  t.decay = float(1 - o->lr * o->weight_decay);
-  t.beta1 = float(o->beta1);
-  t.rest1 = float(1 - o->beta1);
-  t.beta2 = float(o->beta2);
-  t.rest2 = float(1 - o->beta2);
-  t.step_size = float(o->lr / (1 - std::pow(o->beta1, double(o->step))));
-  t.root_scale = float(1 / std::sqrt(1 - std::pow(o->beta2, double(o->step))));
-  t.eps = float(o->eps);
-  for (int kind = 0; kind < 16; ++kind) {
-    const bool ww = kind & 1, wm = kind & 2, wg = kind & 4, copy = kind & 8;
-    t.count = 0;
-    t.chunks = 0;
-    auto launch = [&]() -> int {
-      if (ww) launch_adamw_moments<float>(wm, wg, copy, t, stream);
-      else launch_adamw_moments<bf16>(wm, wg, copy, t, stream);
-      t.count = 0;
-      t.chunks = 0;
-      return launched("sr_adamw");
-    };
-    for (int32_t i = 0; i < count; ++i) {
-      const sr_adamw_tensor& x = tensors[i];
-      if (x.n == 0 || (x.weight_dtype == SR_DT_F32) != ww || (x.moment_dtype == SR_DT_F32) != wm ||
-          (x.grad_dtype == SR_DT_F32) != wg || (x.param != nullptr) != copy)
-        continue;
-      const uint64_t chunks = (x.n + kAdamChunk - 1) / kAdamChunk;
-      if (t.count == kAdamEntries || (t.count && t.chunks + chunks > kMostChunks)) {
-        if (int rc = launch()) return rc;
-      }
-      const int k = t.count++;
-      t.weight[k] = reinterpret_cast<uint64_t>(x.weight);
-      t.exp_avg[k] = reinterpret_cast<uint64_t>(x.exp_avg);
-      t.exp_avg_sq[k] = reinterpret_cast<uint64_t>(x.exp_avg_sq);
-      t.param[k] = reinterpret_cast<uint64_t>(x.param);
-      t.grad[k] = reinterpret_cast<uint64_t>(x.grad);
-      t.first[k] = t.chunks;
-      t.tail[k] = uint32_t(x.n - (chunks - 1) * kAdamChunk);
-      t.chunks += uint32_t(chunks);
-    }
-    if (t.count) {
-      if (int rc = launch()) return rc;
-    }
-  }
-  return SR_OK;
+  AdamTable<true> with_copy;
+  AdamTable<false> alone;
+  adamw_scalars(with_copy, *o, square_sum);
+  adamw_scalars(alone, *o, square_sum);
+  if (int rc = adamw_types<float, true>(tensors, count, with_copy, stream)) return rc;
+  if (int rc = adamw_types<float, false>(tensors, count, alone, stream)) return rc;
+  return adamw_types<bf16, false>(tensors, count, alone, stream);
 } catch (const std::bad_alloc&) {
   return fail(SR_ENOMEM, "sr_adamw: out of host memory");
 }

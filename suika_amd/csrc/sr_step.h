@@ -25,6 +25,14 @@ constexpr int kWave = 64;
 typedef __bf16 bf16;
 typedef _Float16 f16;
 
+// A device address out of a table of kernel arguments: known to be global
+// memory, which a flat access would not be.
+template <typename T>
+__device__ __forceinline__ T* global(uint64_t address) {
+  typedef __attribute__((address_space(1))) T* Global;
+  return (T*)(Global)address;
+}
+
 // Vectors of N elements that are aligned as one element is: the hardware takes
 // 16-byte accesses at any address.
 template <typename T, int N> struct VecAt {

@@ -96,15 +96,18 @@ struct Sum {
   double* sum = nullptr;
 };
 
-// Launches the sum of squares into `into` (or into memory of its own).
-Sum square_sum_into(const std::vector<sr_array>& a, const at::Device& device, double* into, float* norm) {
+// Launches the sum of squares into `into` (or into memory of its own);
+// `read_again`: the arrays are read again right after.
+Sum square_sum_into(const std::vector<sr_array>& a, const at::Device& device, bool read_again, double* into,
+                    float* norm) {
   uint64_t need = 0;
   check(sr_square_sum_workspace(a.data(), int32_t(a.size()), &need), "sr_square_sum");
   Sum out;
   out.work = at::empty({int64_t(need) + 16}, on(device, at::kByte));
   char* base = static_cast<char*>(out.work.data_ptr());
   out.sum = into ? into : reinterpret_cast<double*>(base);
-  check(sr_square_sum(a.data(), int32_t(a.size()), base + 16, need, out.sum, norm, stream_of(device)), "sr_square_sum");
+  check(sr_square_sum(a.data(), int32_t(a.size()), read_again, base + 16, need, out.sum, norm, stream_of(device)),
+        "sr_square_sum");
   return out;
 }
 
@@ -127,7 +130,7 @@ at::Tensor grad_square_sum(py::object grads) {
   if (!device) device = current_device();
   const c10::DeviceGuard guard(*device);
   at::Tensor out = at::empty({}, on(*device, at::kDouble));
-  square_sum_into(a, *device, out.data_ptr<double>(), nullptr);
+  square_sum_into(a, *device, false, out.data_ptr<double>(), nullptr);
   return out;
 }
 
@@ -138,7 +141,7 @@ at::Tensor grad_norm(py::object grads) {
   if (!device) device = current_device();
   const c10::DeviceGuard guard(*device);
   at::Tensor norm = at::empty({}, on(*device, at::kFloat));
-  square_sum_into(a, *device, nullptr, norm.data_ptr<float>());
+  square_sum_into(a, *device, false, nullptr, norm.data_ptr<float>());
   return norm;
 }
 
@@ -181,7 +184,7 @@ at::Tensor clip_grads(py::object grads, double max_norm, py::object outs, py::ob
   at::Tensor norm = at::empty({}, on(*device, at::kFloat));
   Sum mine;
   if (!sum) {
-    mine = square_sum_into(src, *device, nullptr, nullptr);
+    mine = square_sum_into(src, *device, true, nullptr, nullptr);
     sum = mine.sum;
   }
   check(sr_clip(src.data(), in_place ? nullptr : dst.data(), int32_t(src.size()), sum, float(max_norm),
@@ -254,7 +257,7 @@ class AdamWState {
       sum = given_sum(square_sum, device);
       norm = at::empty({}, on(device, at::kFloat));
       if (!sum) {
-        mine = square_sum_into(arrays, device, nullptr, norm.data_ptr<float>());
+        mine = square_sum_into(arrays, device, true, nullptr, norm.data_ptr<float>());
         sum = mine.sum;
       } else {
         check(sr_clip(nullptr, nullptr, 0, sum, float(o.max_norm), norm.data_ptr<float>(), stream_of(device)),

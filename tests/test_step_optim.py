@@ -64,10 +64,10 @@ def test_square_sum_workspace():
     assert L.sr_square_sum_workspace(arrays(), -1, ctypes.byref(need)) == _lib.SR_EINVAL
     assert L.sr_square_sum_workspace(None, 1, ctypes.byref(need)) == _lib.SR_EINVAL
     one = arrays((BASE, 5, F32, 0))
-    assert L.sr_square_sum(one, 1, vp(BASE), ctypes.c_uint64(0), vp(BASE), None, None) == _lib.SR_EINVAL
-    assert L.sr_square_sum(one, 1, None, ctypes.c_uint64(1 << 20), vp(BASE), None, None) == _lib.SR_EINVAL
-    assert L.sr_square_sum(one, 1, vp(BASE + 8), ctypes.c_uint64(1 << 20), vp(BASE), None, None) == _lib.SR_EALIGN
-    assert L.sr_square_sum(one, 1, vp(BASE), ctypes.c_uint64(1 << 20), None, None, None) == _lib.SR_EINVAL
+    assert L.sr_square_sum(one, 1, 0, vp(BASE), ctypes.c_uint64(0), vp(BASE), None, None) == _lib.SR_EINVAL
+    assert L.sr_square_sum(one, 1, 0, None, ctypes.c_uint64(1 << 20), vp(BASE), None, None) == _lib.SR_EINVAL
+    assert L.sr_square_sum(one, 1, 0, vp(BASE + 8), ctypes.c_uint64(1 << 20), vp(BASE), None, None) == _lib.SR_EALIGN
+    assert L.sr_square_sum(one, 1, 0, vp(BASE), ctypes.c_uint64(1 << 20), None, None, None) == _lib.SR_EINVAL
 
 
 def test_clip_refusals():

@@ -196,6 +196,35 @@ __global__ __launch_bounds__(kFinishThreads) void finish_sum_kernel(const double
   }
 }
 
+// The whole sum of few elements in one workgroup and one launch: its waves take
+// the arrays in turn.
+constexpr uint64_t kSmallElements = 32768;
+
+template <typename T>
+__global__ __launch_bounds__(kFinishThreads) void small_sum_kernel(double* sum, float* norm, SumTable t) {
+  constexpr int N = 16 / sizeof(T);
+  double x = 0;
+  for (uint32_t i = threadIdx.x / kWave; i < t.at.count; i += kFinishThreads / kWave) {
+    const T* p = global<const T>(t.entry[i].data);
+    const uint32_t n = uint32_t(t.entry[i].n);
+    for (uint32_t e = threadIdx.x % kWave * N; e < n; e += kWave * N) {
+      if (e + N <= n) {
+        float v[N];
+        load<T, N>(p + e, v);
+#pragma unroll
+        for (int k = 0; k < N; ++k) x = fma(double(v[k]), double(v[k]), x);
+      } else {
+        for (uint32_t k = e; k < n; ++k) x = fma(double(float(p[k])), double(float(p[k])), x);
+      }
+    }
+  }
+  x = block_sum<kFinishThreads>(x);
+  if (threadIdx.x == 0) {
+    *sum = x;
+    if (norm) *norm = float(sqrt(x));
+  }
+}
+
 // ------------------------------------------------------------------ clipping
 
 constexpr int kClipEntries = 128;
@@ -517,8 +546,24 @@ int sr_square_sum(const sr_array* arrays, int32_t count, int32_t read_again, voi
   uint32_t used = 0;
   uint64_t bytes = 0;
   for (int32_t i = 0; i < count; ++i) bytes += bytes_of(arrays[i]);
+  uint64_t elements = 0;
+  int32_t tables = 0;
+  for (int32_t i = 0; i < count; ++i) elements += arrays[i].n;
   const bool stream_loads = read_again == 0 || bytes > kSumCached;
+  if (elements <= kSmallElements) {
+    sum_launches(arrays, count, [&](int32_t, const SumTable&) {
+      ++tables;
+      return SR_OK;
+    });
+  }
+  const bool small = tables == 1;
   const int rc = sum_launches(arrays, count, [&](int32_t dt, const SumTable& t) {
+    if (small) {
+      if (dt == SR_DT_F32) small_sum_kernel<float><<<1, kFinishThreads, 0, stream>>>(sum, norm, t);
+      else if (dt == SR_DT_BF16) small_sum_kernel<bf16><<<1, kFinishThreads, 0, stream>>>(sum, norm, t);
+      else small_sum_kernel<f16><<<1, kFinishThreads, 0, stream>>>(sum, norm, t);
+      return launched("sr_square_sum");
+    }
     const uint32_t blocks = sum_blocks(t), run = sum_run(t);
     if (dt == SR_DT_F32) launch_sum<float>(t, run, blocks, stream_loads, partial + used, stream);
     else if (dt == SR_DT_BF16) launch_sum<bf16>(t, run, blocks, stream_loads, partial + used, stream);
@@ -526,7 +571,7 @@ int sr_square_sum(const sr_array* arrays, int32_t count, int32_t read_again, voi
     used += blocks;
     return launched("sr_square_sum");
   });
-  if (rc) return rc;
+  if (rc || small) return rc;
   finish_sum_kernel<<<1, kFinishThreads, 0, stream>>>(partial, used, sum, norm);
   return launched("sr_square_sum");
 }

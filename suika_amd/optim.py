@@ -139,7 +139,7 @@ class ShardAdamW:
         number of the step is a host value, so the call refuses to be captured
         into a graph.
         """
-        if isinstance(grads, Mapping):
+        if not isinstance(grads, (list, tuple)) and isinstance(grads, Mapping):
             unknown = grads.keys() - self._state.keys()
             if unknown:
                 raise PlanError(f"gradients of unknown parameters: {sorted(unknown)[:4]}")

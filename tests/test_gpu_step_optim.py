@@ -37,7 +37,7 @@ def square_sum64(grads):
 
 
 LENGTHS = [[], [0], [1], [7], [0, 3, 0, 1], [255, 256, 257], [16383], [16384], [16385], [2 ** 20 + 13],
-           [5] * 189, [64, 1] * 200, [100003, 17, 2 ** 18, 0, 31]]
+           [5] * 189, [5] * 190, [64, 1] * 200, [32768], [32769], [40000] * 190, [100003, 17, 2 ** 18, 0, 31]]
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])
@@ -213,7 +213,7 @@ def copy_of(state):
 
 @pytest.mark.parametrize("fields,grad", [("f32", F32), ("f32", BF16), ("master", BF16), ("master", F32),
                                          ("bf16", BF16), ("bf16", F32)])
-@pytest.mark.parametrize("lengths", [[1], [0, 3], [2047, 2048, 2049], [7] * 79, [100003, 1, 4096]],
+@pytest.mark.parametrize("lengths", [[1], [0, 3], [2047, 2048, 2049], [7] * 203, [100003, 1, 4096]],
                          ids=lambda v: f"{len(v)}x{max(v)}")
 @pytest.mark.parametrize("shift", [0, 1])
 @pytest.mark.parametrize("max_norm", [None, 0.01])

@@ -1,6 +1,10 @@
 // embed.hip -- rows of a vocabulary shard for given tokens, and the gradient
 // of those rows (C ABI in include/suika_step.h).
 //
+// The lookup is a copy with a table of rows: HBM bounds it (16384 tokens of 4096
+// bf16 columns, 186 MB with the rows they hit, 29.5 us, 6.3 TB/s).  Outputs are
+// streamed, the table's rows are cached: frequent tokens read the same ones.
+//
 // The gradient of row r is the sum of the outputs' gradients at the tokens
 // that are r.  Adding them with atomics would make the result depend on the
 // order in which workgroups run, so the tokens are sorted first (a stable
@@ -11,11 +15,17 @@
 //           the L2: it counts those of the workgroups before it, which is where
 //           its own start in the sorted list, and those of each of its rows,
 //           and places them in a second pass.  No workgroup waits for another.
-//   sum     A group of lanes per row adds up the row's tokens, each lane one
-//           16-byte column block.  A row of many tokens (a space, a filler) is
+//           Its time is a chain of loads, scans and barriers: 12.5 us for 16384
+//           tokens, 20 for 30011.  (Ranges of neighbouring rows: 24 and 43 us,
+//           as the range of the frequent tokens is one workgroup's.)
+//   sum     A group of lanes per row adds up the row's tokens, each lane two
+//           16-byte column blocks.  A row of many tokens (a space, a filler) is
 //           cut into pieces that are summed side by side, into 32-bit partial
-//           sums.
-//   join    The partial sums of such rows, added in order.
+//           sums.  Rows in the order of memory, gradients read and written
+//           past the caches: 51.7 us for 256 MB (5 TB/s; one block a lane
+//           55.0, four 68; with cached accesses 73; rows in the sort's order
+//           78).  What is left is the chain from a row's tokens to its sum.
+//   join    The partial sums of such rows, added in order: 12 us.
 
 #include <hip/hip_runtime.h>
 
@@ -357,21 +367,28 @@ __device__ __forceinline__ void put_row(G* grad, uint64_t c, uint64_t cols, floa
 }
 
 // Tasks 0..slots are the pieces; the rows follow.
+constexpr int kSumBlocks = 2;         // of a lane
+
 template <typename T, typename G>
 __global__ __launch_bounds__(kThreads) void sum_kernel(const T* grad_out, uint64_t stride, G* grad, uint64_t rows,
                                                        uint64_t cols, uint32_t slots, uint32_t piece, float scale,
                                                        bool accumulate, Lanes l, Sorted in) {
-  constexpr int N = 16 / sizeof(T);
+  constexpr int N = 16 / sizeof(T), U = kSumBlocks;
   const uint64_t task = (uint64_t(blockIdx.x) << (8 - l.log2)) + (threadIdx.x >> l.log2);
-  const uint64_t c = first_column<N, 1>(l);
+  const uint64_t c = first_column<N, U>(l), step = uint64_t(N) << l.log2;
   if (c >= cols) return;
-  float acc[N] = {};
   if (task < slots) {
     if (task >= uint32_t(2 * uint64_t(*in.tokens) / piece)) return;
     const Piece p = in.piece[task];
     if (p.row == kNoPiece) return;
-    sum_tokens<T, N>(grad_out, stride, in.order, p.from, p.to, c, cols, acc);
-    put_row<float, N>(in.partial + task * cols, c, cols, 1.0f, false, acc);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const uint64_t at = c + u * step;
+      if (at >= cols) break;
+      float acc[N] = {};
+      sum_tokens<T, N>(grad_out, stride, in.order, p.from, p.to, at, cols, acc);
+      put_row<float, N>(in.partial + task * cols, at, cols, 1.0f, false, acc);
+    }
     return;
   }
   const uint64_t row = task - slots;
@@ -379,21 +396,30 @@ __global__ __launch_bounds__(kThreads) void sum_kernel(const T* grad_out, uint64
   const Run run = in.run[row];
   const uint32_t n = run.to - run.from;
   if (n > 2 * piece || (accumulate && n == 0)) return;
-  uint32_t from = run.from;
-  if (c + N <= cols) {
-    Vec<T, N> x[2];
+  Vec<T, N> x[U][2];
+#pragma unroll
+  for (int u = 0; u < U; ++u)
 #pragma unroll
     for (uint32_t a = 0; a < 2; ++a)
-      if (a < n) x[a] = __builtin_nontemporal_load(reinterpret_cast<const Vec<T, N>*>(grad_out + run.token[a] * stride + c));
+      if (a < n && c + u * step + N <= cols)
+        x[u][a] = __builtin_nontemporal_load(reinterpret_cast<const Vec<T, N>*>(grad_out + run.token[a] * stride + c + u * step));
 #pragma unroll
-    for (uint32_t a = 0; a < 2; ++a)
-      if (a < n)
+  for (int u = 0; u < U; ++u) {
+    const uint64_t at = c + u * step;
+    if (at >= cols) break;
+    float acc[N] = {};
+    uint32_t from = run.from;
+    if (at + N <= cols) {
 #pragma unroll
-        for (int k = 0; k < N; ++k) acc[k] += float(x[a][k]);
-    from += n < 2 ? n : 2;
+      for (uint32_t a = 0; a < 2; ++a)
+        if (a < n)
+#pragma unroll
+          for (int k = 0; k < N; ++k) acc[k] += float(x[u][a][k]);
+      from += n < 2 ? n : 2;
+    }
+    sum_tokens<T, N>(grad_out, stride, in.order, from, run.to, at, cols, acc);
+    put_row<G, N>(grad + row * cols, at, cols, scale, accumulate, acc);
   }
-  sum_tokens<T, N>(grad_out, stride, in.order, from, run.to, c, cols, acc);
-  put_row<G, N>(grad + row * cols, c, cols, scale, accumulate, acc);
 }
 
 template <typename G>
@@ -456,9 +482,8 @@ int check_shape(const char* who, const sr_embedding_shape* s) {
   return SR_OK;
 }
 
-bool overlap(const void* a, uint64_t na, const void* b, uint64_t nb) {
-  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
-  return na && nb && x < y + nb && y < x + na;
+Extent tokens_of(const sr_embedding_shape& s) {
+  return {s.tokens, s.n_tokens * sr_internal::dtype_size(s.token_dtype)};
 }
 
 // Bytes from the first element of a matrix to behind its last.
@@ -507,7 +532,7 @@ Layout layout_of(const sr_embedding_shape& s) {
 template <typename T, typename G>
 void launch_sum(const sr_embedding_shape& s, const Layout& w, const Sorted& sorted, const void* grad_out,
                 uint64_t stride, void* grad, bool accumulate, hipStream_t stream) {
-  const Lanes l = lanes_of(s.cols, 16 / sizeof(T), kThreads, 1);
+  const Lanes l = lanes_of(s.cols, 16 / sizeof(T), kThreads, kSumBlocks);
   const uint32_t group = uint32_t(kThreads) >> l.log2;
   const dim3 grid(uint32_t((w.slots + s.rows + group - 1) / group), l.slices);
   sum_kernel<T, G><<<grid, kThreads, 0, stream>>>(static_cast<const T*>(grad_out), stride, static_cast<G*>(grad),
@@ -542,9 +567,8 @@ int sr_embedding(const sr_embedding_shape* shape, const void* weight, uint64_t w
     return fail(SR_EINVAL, "sr_embedding: rows %llu apart for %llu columns", (unsigned long long)weight_stride,
                 (unsigned long long)s.cols);
   if (!aligned(weight, s.dtype) || !aligned(out, s.dtype)) return fail(SR_EALIGN, "sr_embedding: not aligned to the elements");
-  const uint64_t out_bytes = extent(s.n_tokens, s.cols, s.cols, s.dtype);
-  if (overlap(out, out_bytes, weight, extent(s.rows, s.cols, weight_stride, s.dtype)) ||
-      overlap(out, out_bytes, s.tokens, s.n_tokens * sr_internal::dtype_size(s.token_dtype)))
+  const Extent to{out, extent(s.n_tokens, s.cols, s.cols, s.dtype)};
+  if (to.meets({weight, extent(s.rows, s.cols, weight_stride, s.dtype)}) || to.meets(tokens_of(s)))
     return fail(SR_EOVERLAP, "sr_embedding: the output overlaps an input");
   if (s.dtype == SR_DT_F32) launch_embedding<float>(s, weight, weight_stride, out, stream);
   else if (s.dtype == SR_DT_BF16) launch_embedding<bf16>(s, weight, weight_stride, out, stream);
@@ -577,11 +601,10 @@ int sr_embedding_grad(const sr_embedding_shape* shape, const void* grad_out, uin
     return fail(SR_EINVAL, "sr_embedding_grad: a workspace of %llu bytes, %llu are needed",
                 (unsigned long long)workspace_bytes, (unsigned long long)w.bytes);
   if (reinterpret_cast<uintptr_t>(workspace) % 16) return fail(SR_EALIGN, "sr_embedding_grad: workspace not aligned");
-  const uint64_t grad_bytes = extent(s.rows, s.cols, s.cols, grad_dtype);
-  if (overlap(grad, grad_bytes, grad_out, extent(s.n_tokens, s.cols, grad_out_stride, s.dtype)) ||
-      overlap(grad, grad_bytes, s.tokens, s.n_tokens * sr_internal::dtype_size(s.token_dtype)) ||
-      overlap(grad, grad_bytes, workspace, w.bytes))
-    return fail(SR_EOVERLAP, "sr_embedding_grad: the gradient overlaps an input");
+  const Extent to{grad, extent(s.rows, s.cols, s.cols, grad_dtype)}, work{workspace, w.bytes};
+  const Extent from{grad_out, extent(s.n_tokens, s.cols, grad_out_stride, s.dtype)};
+  if (to.meets(from) || to.meets(tokens_of(s)) || to.meets(work) || work.meets(from) || work.meets(tokens_of(s)))
+    return fail(SR_EOVERLAP, "sr_embedding_grad: the gradient or the workspace overlaps an input");
   char* base = static_cast<char*>(workspace);
   const Sorted sorted{reinterpret_cast<Run*>(base), reinterpret_cast<uint32_t*>(base + w.count),
                       reinterpret_cast<uint32_t*>(base + w.order),

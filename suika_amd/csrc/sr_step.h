@@ -120,6 +120,17 @@ __device__ __forceinline__ uint32_t xcd_order(uint32_t block, uint32_t items) {
   return block % kXcds * ((items + kXcds - 1) / kXcds) + block / kXcds;
 }
 
+// Memory that a call reads or writes.
+struct Extent {
+  const void* p;
+  uint64_t bytes;
+
+  bool meets(const Extent& o) const {
+    const uintptr_t a = reinterpret_cast<uintptr_t>(p), b = reinterpret_cast<uintptr_t>(o.p);
+    return p && o.p && bytes && o.bytes && a < b + o.bytes && b < a + bytes;
+  }
+};
+
 inline int launched(const char* what) {
   const hipError_t e = hipGetLastError();
   return e == hipSuccess ? SR_OK : fail(SR_EHIP, "%s: launch failed: %s", what, hipGetErrorString(e));

@@ -68,6 +68,8 @@ def test_square_sum_workspace():
     assert L.sr_square_sum(one, 1, 0, None, ctypes.c_uint64(1 << 20), vp(BASE), None, None) == _lib.SR_EINVAL
     assert L.sr_square_sum(one, 1, 0, vp(BASE + 8), ctypes.c_uint64(1 << 20), vp(BASE), None, None) == _lib.SR_EALIGN
     assert L.sr_square_sum(one, 1, 0, vp(BASE), ctypes.c_uint64(1 << 20), None, None, None) == _lib.SR_EINVAL
+    assert L.sr_square_sum(one, 1, 0, vp(BASE), ctypes.c_uint64(1 << 20), vp(BASE + 4), None, None) == _lib.SR_EALIGN
+    assert L.sr_square_sum(one, 1, 0, vp(BASE), ctypes.c_uint64(1 << 20), vp(BASE), vp(BASE + 2), None) == _lib.SR_EALIGN
 
 
 def test_clip_refusals():
@@ -77,6 +79,7 @@ def test_clip_refusals():
     def clip(src, dst, n, q=vp(BASE), max_norm=1.0):
         return L.sr_clip(src, dst, n, q, ctypes.c_float(max_norm), None, None)
     assert clip(one, None, 1, q=None) == _lib.SR_EINVAL
+    assert clip(one, None, 1, q=vp(BASE + 4)) == _lib.SR_EALIGN
     assert clip(one, None, 1, max_norm=-1.0) == _lib.SR_EINVAL
     assert clip(one, None, 1, max_norm=float("nan")) == _lib.SR_EINVAL
     assert clip(one, arrays((BASE + 64, 7, F32, 0)), 1) == _lib.SR_EINVAL           # other length

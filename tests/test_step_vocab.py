@@ -81,6 +81,8 @@ def test_embedding_refused(kw, code):
     (dict(grad=BASE + 4096 + 4 * 64 - 4), _lib.SR_EOVERLAP),
     (dict(grad=BASE), _lib.SR_EOVERLAP),
     (dict(work=BASE + 65536 + 16), _lib.SR_EOVERLAP),
+    (dict(work=BASE + 4096 + 16), _lib.SR_EOVERLAP),
+    (dict(work=BASE + 16), _lib.SR_EOVERLAP),
 ])
 def test_embedding_grad_refused(kw, code):
     assert embedding_grad(**kw) == code and "sr_embedding_grad" in _lib.last_error()
@@ -160,6 +162,10 @@ def test_logprob_shapes_refused(shape, code):
     (dict(out=(OUT, OUT + 2, OUT, OUT, OUT)), _lib.SR_EALIGN),
     (dict(out=(OUT, OUT, OUT, OUT, OUT + 4)), _lib.SR_EALIGN),
     (dict(work=OUT + 8), _lib.SR_EALIGN),
+    (dict(out=(OUT, OUT + 12, OUT + 128, OUT + 192, OUT + 256)), _lib.SR_EOVERLAP),      # two outputs
+    (dict(out=(OUT, OUT + 64, OUT + 128, OUT + 192, OUT + 208)), _lib.SR_EOVERLAP),
+    (dict(out=(BASE + 4, OUT + 64, OUT + 128, OUT + 192, OUT + 256)), _lib.SR_EOVERLAP), # the logits
+    (dict(out=(OUT, OUT + 64, OUT + 128, OUT + 192, BASE + (1 << 20) + 8)), _lib.SR_EOVERLAP),
 ])
 def test_logprob_refused(kw, code):
     assert logprob(**kw) == code and "sr_logprob" in _lib.last_error()

@@ -84,24 +84,12 @@ constexpr int kThrough = 16;     // sc1: whole lines go through the L2
 
 template <int POLICY, typename T, int N>
 __device__ __forceinline__ void store_region(Region r, uint32_t at, const float (&f)[N]) {
+  static_assert(N * sizeof(T) == 16, "a whole vector");
   typename VecAt<T, N>::packed v;
 #pragma unroll
   for (int i = 0; i < N; ++i) v[i] = static_cast<T>(f[i]);
-  typedef unsigned int u32;
-  typedef u32 u32x2 __attribute__((ext_vector_type(2)));
-  typedef u32 u32x4 __attribute__((ext_vector_type(4)));
-  constexpr int kBytes = N * sizeof(T);
-  static_assert(kBytes == 8 || kBytes == 16 || kBytes == 32, "whole vectors");
-  if constexpr (kBytes == 8) {
-    __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, v), r, at, 0, POLICY);
-  } else if constexpr (kBytes == 16) {
-    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), r, at, 0, POLICY);
-  } else {
-    struct Two { u32x4 a, b; };
-    const Two t = __builtin_bit_cast(Two, v);
-    __builtin_amdgcn_raw_buffer_store_b128(t.a, r, at, 0, POLICY);
-    __builtin_amdgcn_raw_buffer_store_b128(t.b, r, at + 16, 0, POLICY);
-  }
+  typedef unsigned int Words __attribute__((ext_vector_type(4)));
+  __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(Words, v), r, at, 0, POLICY);
 }
 
 template <typename T>

@@ -127,6 +127,13 @@ struct alignas(16) Piece {
 };
 constexpr uint32_t kNoPiece = 0xffffffffu;
 
+// The tokens of a piece of a row of n: `least` or, of long rows, as many as the
+// row then has pieces, so that adding up a piece and joining them take the same
+// number of steps.
+__device__ __forceinline__ uint32_t piece_of(uint32_t n, uint32_t least) {
+  return max(least, (uint32_t(sqrtf(float(n))) + 3) / 4 * 4);
+}
+
 // The sorted positions of a row's tokens, and the first two tokens: most rows
 // have no more, and these are one load less away.
 struct alignas(16) Run {
@@ -253,7 +260,8 @@ __global__ __launch_bounds__(kSortThreads) void sort_kernel(const I* tokens, uin
   if (threadIdx.x < range)
     for (int w = 0; w < kSortWaves; ++w) n += count[w * range + threadIdx.x];
   const uint32_t at = base + block_scan(n, part, &total);
-  const uint32_t cut = n > 2 * piece ? (n + piece - 1) / piece : 0;
+  const uint32_t each = piece_of(n, piece);
+  const uint32_t cut = n > 2 * piece ? (n + each - 1) / each : 0;
   const uint32_t slot = block_scan(cut, part, &pieces);
   if (threadIdx.x < range) {
     uint32_t next = at;
@@ -271,12 +279,12 @@ __global__ __launch_bounds__(kSortThreads) void sort_kernel(const I* tokens, uin
     if (me == mask && threadIdx.x == 0) *out.tokens = base + total;
   }
   // A workgroup of `total` tokens has the slots from 2 base / piece on.  A row is
-  // cut where it has more than 2 piece tokens, into at most 3/2 of n / piece
-  // pieces, so they fit; the slots left over say that they are empty.
+  // cut where it has more than 2 piece tokens, into pieces of `piece` or more: at
+  // most 3/2 of n / piece, so they fit; the slots left over say that they are empty.
   const uint32_t slot0 = uint32_t(2 * uint64_t(base) / piece);
   const uint32_t slot1 = uint32_t(2 * uint64_t(base + total) / piece);
   for (uint32_t k = 0; k < cut; ++k)
-    out.piece[slot0 + slot + k] = {(threadIdx.x << owners.log2) + me, at + k * piece, min(at + (k + 1) * piece, at + n),
+    out.piece[slot0 + slot + k] = {(threadIdx.x << owners.log2) + me, at + k * each, min(at + (k + 1) * each, at + n),
                                    k ? 0 : cut};
   for (uint32_t s = slot0 + pieces + threadIdx.x; s < slot1; s += kSortThreads) out.piece[s] = {kNoPiece, 0, 0, 0};
   __syncthreads();

@@ -60,8 +60,8 @@ Lanes lanes_of(uint64_t cols, uint32_t per_block, uint32_t most, uint32_t each) 
 
 // The first column of this lane's blocks, and from one of them to the next.
 template <int N, int U>
-__device__ __forceinline__ uint64_t first_column(const Lanes& l) {
-  return (uint64_t(blockIdx.y * U << l.log2) + (threadIdx.x & ((1u << l.log2) - 1))) * N;
+__device__ __forceinline__ uint32_t first_column(const Lanes& l) {
+  return ((blockIdx.y * U << l.log2) + (threadIdx.x & ((1u << l.log2) - 1))) * N;
 }
 
 // --------------------------------------------------------------------- rows
@@ -318,19 +318,52 @@ __global__ __launch_bounds__(kSortThreads) void sort_kernel(const I* tokens, uin
 
 // ---------------------------------------------------------------------- sum
 
+// Where a lane loads the block of columns from c on: a row's last, shorter block
+// from N columns before its end, so that it is a vector as the others.
+template <int N>
+__device__ __forceinline__ uint32_t block_at(uint32_t c, uint32_t cols) {
+  return c + N <= cols || cols < N ? c : cols - N;
+}
+
+// A lane group's place in a grid of groups.  Where a group is whole waves
+// (kWhole), it is known to be the same in all lanes, and with it what is read
+// there: the addresses of rows need no vector registers.
+template <bool kWhole>
+__device__ __forceinline__ uint32_t task_of(const Lanes& l) {
+  const uint32_t group = threadIdx.x >> l.log2;
+  return (blockIdx.x << (8 - l.log2)) + (kWhole ? __builtin_amdgcn_readfirstlane(group) : group);
+}
+
+// What the launches before have written.
+template <bool kWhole, typename V>
+__device__ __forceinline__ V written(const V* p) {
+  typedef uint32_t Words __attribute__((ext_vector_type(sizeof(V) / 4)));
+  typedef const __attribute__((address_space(4))) Words* Constant;
+  if constexpr (kWhole) return __builtin_bit_cast(V, *(Constant)(uintptr_t)p);
+  else return *p;
+}
+
 // Adds columns c.. of the tokens at sorted positions from..to to `acc`, in
-// their order; N of them, or `cols - c` at a row's end.
-template <typename T, int N>
+// their order; N of them, or `cols - c` of a row that has no N columns.
+constexpr uint32_t kAhead = 8;        // tokens that a lane loads at once
+
+template <bool kWhole, typename T, int N>
 __device__ __forceinline__ void sum_tokens(const T* grad_out, uint64_t stride, const uint32_t* order, uint32_t from,
-                                           uint32_t to, uint64_t c, uint64_t cols, float (&acc)[N]) {
-  constexpr uint32_t kAhead = 4;
+                                           uint32_t to, uint32_t c, uint32_t cols, float (&acc)[N]) {
+  typedef const Vec<T, N>* Vector;
   if (c + N <= cols) {
+    uint32_t token[kAhead];
+#pragma unroll
+    for (uint32_t a = 0; a < kAhead; ++a) token[a] = from + a < to ? written<kWhole>(order + from + a) : 0;
     uint32_t i = from;
     for (; i + kAhead <= to; i += kAhead) {
       Vec<T, N> x[kAhead];
 #pragma unroll
       for (uint32_t a = 0; a < kAhead; ++a)
-        x[a] = __builtin_nontemporal_load(reinterpret_cast<const Vec<T, N>*>(grad_out + order[i + a] * stride + c));
+        x[a] = __builtin_nontemporal_load(Vector(grad_out + token[a] * stride + c));
+#pragma unroll
+      for (uint32_t a = 0; a < kAhead; ++a)
+        token[a] = i + kAhead + a < to ? written<kWhole>(order + i + kAhead + a) : 0;
 #pragma unroll
       for (uint32_t a = 0; a < kAhead; ++a)
 #pragma unroll
@@ -340,7 +373,7 @@ __device__ __forceinline__ void sum_tokens(const T* grad_out, uint64_t stride, c
       Vec<T, N> x[kAhead];
 #pragma unroll
       for (uint32_t a = 0; a < kAhead - 1; ++a)
-        if (i + a < to) x[a] = __builtin_nontemporal_load(reinterpret_cast<const Vec<T, N>*>(grad_out + order[i + a] * stride + c));
+        if (i + a < to) x[a] = __builtin_nontemporal_load(Vector(grad_out + token[a] * stride + c));
 #pragma unroll
       for (uint32_t a = 0; a < kAhead - 1; ++a)
         if (i + a < to)
@@ -349,7 +382,7 @@ __device__ __forceinline__ void sum_tokens(const T* grad_out, uint64_t stride, c
     }
   } else {
     for (uint32_t i = from; i < to; ++i) {
-      const T* p = grad_out + order[i] * stride + c;
+      const T* p = grad_out + written<kWhole>(order + i) * stride + c;
 #pragma unroll
       for (int k = 0; k < N; ++k)
         if (c + k < cols) acc[k] += float(p[k]);
@@ -357,51 +390,53 @@ __device__ __forceinline__ void sum_tokens(const T* grad_out, uint64_t stride, c
   }
 }
 
-// grad[c..] = scale * acc, plus what is there.
+// grad[c..] = scale * acc, plus what is there; acc holds the columns from `at`
+// = block_at(c) on.  Blocks of more than 16 bytes take two stores that each leave
+// gaps, for the L2 to merge: streamed, 50304 rows of 768 f32 took 56 us, not 39.
 template <typename G, int N>
-__device__ __forceinline__ void put_row(G* grad, uint64_t c, uint64_t cols, float scale, bool accumulate,
+__device__ __forceinline__ void put_row(G* grad, uint32_t c, uint32_t at, uint32_t cols, float scale, bool accumulate,
                                         float (&acc)[N]) {
   if (c + N <= cols) {
     float old[N] = {};
     if (accumulate) load<G, N>(grad + c, old);
 #pragma unroll
     for (int k = 0; k < N; ++k) acc[k] = fmaf(acc[k], scale, old[k]);
-    store_stream<G, N>(grad + c, acc);
+    if constexpr (N * sizeof(G) > 16) store<G, N>(grad + c, acc);
+    else store_stream<G, N>(grad + c, acc);
   } else {
 #pragma unroll
     for (int k = 0; k < N; ++k)
-      if (c + k < cols) grad[c + k] = G(fmaf(acc[k], scale, accumulate ? float(grad[c + k]) : 0.0f));
+      if (at + k >= c && at + k < cols)
+        grad[at + k] = G(fmaf(acc[k], scale, accumulate ? float(grad[at + k]) : 0.0f));
   }
 }
 
-// Tasks 0..slots are the pieces; the rows follow.
+// Tasks 0..slots * U are the pieces, each of a lane's U blocks apart: they are the
+// longest; the rows follow.
 constexpr int kSumBlocks = 2;         // of a lane
 
-template <typename T, typename G>
-__global__ __launch_bounds__(kThreads) void sum_kernel(const T* grad_out, uint64_t stride, G* grad, uint64_t rows,
-                                                       uint64_t cols, uint32_t slots, uint32_t piece, float scale,
+template <typename T, typename G, bool kWhole>
+__global__ __launch_bounds__(kThreads) void sum_kernel(const T* grad_out, uint64_t stride, G* grad, uint32_t rows,
+                                                       uint32_t cols, uint32_t slots, uint32_t piece, float scale,
                                                        bool accumulate, Lanes l, Sorted in) {
   constexpr int N = 16 / sizeof(T), U = kSumBlocks;
-  const uint64_t task = (uint64_t(blockIdx.x) << (8 - l.log2)) + (threadIdx.x >> l.log2);
-  const uint64_t c = first_column<N, U>(l), step = uint64_t(N) << l.log2;
-  if (c >= cols) return;
-  if (task < slots) {
-    if (task >= uint32_t(2 * uint64_t(*in.tokens) / piece)) return;
-    const Piece p = in.piece[task];
-    if (p.row == kNoPiece) return;
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const uint64_t at = c + u * step;
-      if (at >= cols) break;
-      float acc[N] = {};
-      sum_tokens<T, N>(grad_out, stride, in.order, p.from, p.to, at, cols, acc);
-      put_row<float, N>(in.partial + task * cols, at, cols, 1.0f, false, acc);
-    }
+  typedef const Vec<T, N>* Vector;
+  const uint32_t task = task_of<kWhole>(l);
+  const uint32_t c = first_column<N, U>(l), step = uint32_t(N) << l.log2;
+  if (task < slots * U) {
+    const uint32_t slot = task / U;
+    const Piece p = written<kWhole>(in.piece + slot);
+    if (slot >= uint32_t(2 * uint64_t(*in.tokens) / piece) || p.row == kNoPiece) return;
+    const uint32_t own = c + task % U * step, at = block_at<N>(own, cols);
+    if (own >= cols) return;
+    float acc[N] = {};
+    sum_tokens<kWhole, T, N>(grad_out, stride, in.order, p.from, p.to, at, cols, acc);
+    put_row<float, N>(in.partial + uint64_t(slot) * cols, own, at, cols, 1.0f, false, acc);
     return;
   }
-  const uint64_t row = task - slots;
-  if (row >= rows) return;
-  const Run run = in.run[row];
+  const uint32_t row = task - slots * U;
+  if (row >= rows || c >= cols) return;
+  const Run run = written<kWhole>(in.run + row);
   const uint32_t n = run.to - run.from;
   if (n > 2 * piece || (accumulate && n == 0)) return;
   Vec<T, N> x[U][2];
@@ -409,15 +444,15 @@ __global__ __launch_bounds__(kThreads) void sum_kernel(const T* grad_out, uint64
   for (int u = 0; u < U; ++u)
 #pragma unroll
     for (uint32_t a = 0; a < 2; ++a)
-      if (a < n && c + u * step + N <= cols)
-        x[u][a] = __builtin_nontemporal_load(reinterpret_cast<const Vec<T, N>*>(grad_out + run.token[a] * stride + c + u * step));
+      if (a < n && c + u * step < cols && N <= cols)
+        x[u][a] = __builtin_nontemporal_load(Vector(grad_out + run.token[a] * stride + block_at<N>(c + u * step, cols)));
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    const uint64_t at = c + u * step;
-    if (at >= cols) break;
+    const uint32_t own = c + u * step, at = block_at<N>(own, cols);
+    if (own >= cols) break;
     float acc[N] = {};
     uint32_t from = run.from;
-    if (at + N <= cols) {
+    if (N <= cols) {
 #pragma unroll
       for (uint32_t a = 0; a < 2; ++a)
         if (a < n)
@@ -425,31 +460,31 @@ __global__ __launch_bounds__(kThreads) void sum_kernel(const T* grad_out, uint64
           for (int k = 0; k < N; ++k) acc[k] += float(x[u][a][k]);
       from += n < 2 ? n : 2;
     }
-    sum_tokens<T, N>(grad_out, stride, in.order, from, run.to, at, cols, acc);
-    put_row<G, N>(grad + row * cols, at, cols, scale, accumulate, acc);
+    sum_tokens<kWhole, T, N>(grad_out, stride, in.order, from, run.to, at, cols, acc);
+    put_row<G, N>(grad + uint64_t(row) * cols, own, at, cols, scale, accumulate, acc);
   }
 }
 
 template <typename G>
-__global__ __launch_bounds__(kThreads) void join_kernel(G* grad, uint64_t cols, uint32_t slots, uint32_t piece,
+__global__ __launch_bounds__(kThreads) void join_kernel(G* grad, uint32_t cols, uint32_t slots, uint32_t piece,
                                                         float scale, bool accumulate, Lanes l, Sorted in) {
   constexpr int N = 4;
   constexpr uint32_t kAhead = 8;
-  const uint64_t task = (uint64_t(blockIdx.x) << (8 - l.log2)) + (threadIdx.x >> l.log2);
+  const uint32_t task = (blockIdx.x << (8 - l.log2)) + (threadIdx.x >> l.log2);
   if (task >= slots || task >= uint32_t(2 * uint64_t(*in.tokens) / piece)) return;
   const Piece p = in.piece[task];
   const uint32_t pieces = p.pieces;
   if (p.row == kNoPiece || pieces == 0) return;
-  const uint64_t c = first_column<N, 1>(l);
+  const uint32_t c = first_column<N, 1>(l), at = block_at<N>(c, cols);
   if (c >= cols) return;
   float acc[N] = {};
-  const float* src = in.partial + task * cols + c;
+  const float* src = in.partial + uint64_t(task) * cols + at;
   uint32_t i = 0;
-  if (c + N <= cols) {
+  if (N <= cols) {
     for (; i + kAhead <= pieces; i += kAhead) {
       float x[kAhead][N];
 #pragma unroll
-      for (uint32_t a = 0; a < kAhead; ++a) load<float, N>(src + (i + a) * cols, x[a]);
+      for (uint32_t a = 0; a < kAhead; ++a) load<float, N>(src + uint64_t(i + a) * cols, x[a]);
 #pragma unroll
       for (uint32_t a = 0; a < kAhead; ++a)
 #pragma unroll
@@ -457,7 +492,7 @@ __global__ __launch_bounds__(kThreads) void join_kernel(G* grad, uint64_t cols, 
     }
     for (; i < pieces; ++i) {
       float x[N];
-      load<float, N>(src + i * cols, x);
+      load<float, N>(src + uint64_t(i) * cols, x);
 #pragma unroll
       for (int k = 0; k < N; ++k) acc[k] += x[k];
     }
@@ -465,9 +500,9 @@ __global__ __launch_bounds__(kThreads) void join_kernel(G* grad, uint64_t cols, 
     for (; i < pieces; ++i)
 #pragma unroll
       for (int k = 0; k < N; ++k)
-        if (c + k < cols) acc[k] += src[i * cols + k];
+        if (at + k < cols) acc[k] += src[uint64_t(i) * cols + k];
   }
-  put_row<G, N>(grad + uint64_t(p.row) * cols, c, cols, scale, accumulate, acc);
+  put_row<G, N>(grad + uint64_t(p.row) * cols, c, at, cols, scale, accumulate, acc);
 }
 
 // ---------------------------------------------------------------------- host
@@ -542,14 +577,16 @@ void launch_sum(const sr_embedding_shape& s, const Layout& w, const Sorted& sort
                 uint64_t stride, void* grad, bool accumulate, hipStream_t stream) {
   const Lanes l = lanes_of(s.cols, 16 / sizeof(T), kThreads, kSumBlocks);
   const uint32_t group = uint32_t(kThreads) >> l.log2;
-  const dim3 grid(uint32_t((w.slots + s.rows + group - 1) / group), l.slices);
-  sum_kernel<T, G><<<grid, kThreads, 0, stream>>>(static_cast<const T*>(grad_out), stride, static_cast<G*>(grad),
-                                                  s.rows, s.cols, w.slots, w.piece, s.scale, accumulate, l, sorted);
+  const dim3 grid(uint32_t((uint64_t(w.slots) * kSumBlocks + s.rows + group - 1) / group), l.slices);
+  auto* kernel = l.log2 >= 6 ? sum_kernel<T, G, true> : sum_kernel<T, G, false>;
+  kernel<<<grid, kThreads, 0, stream>>>(static_cast<const T*>(grad_out), stride, static_cast<G*>(grad),
+                                        uint32_t(s.rows), uint32_t(s.cols), w.slots, w.piece, s.scale, accumulate, l,
+                                        sorted);
   if (s.n_tokens <= 2 * w.piece) return;     // no row is cut
   const Lanes j = lanes_of(s.cols, 4, kThreads, 1);
   const uint32_t joined = uint32_t(kThreads) >> j.log2;
   const dim3 join_grid((w.slots + joined - 1) / joined, j.slices);
-  join_kernel<G><<<join_grid, kThreads, 0, stream>>>(static_cast<G*>(grad), s.cols, w.slots, w.piece, s.scale,
+  join_kernel<G><<<join_grid, kThreads, 0, stream>>>(static_cast<G*>(grad), uint32_t(s.cols), w.slots, w.piece, s.scale,
                                                      accumulate, j, sorted);
 }
 

@@ -413,13 +413,11 @@ __device__ __forceinline__ void put_row(G* grad, uint32_t c, uint32_t at, uint32
 
 // Tasks 0..slots * U are the pieces, each of a lane's U blocks apart: they are the
 // longest; the rows follow.
-constexpr int kSumBlocks = 2;         // of a lane
-
-template <typename T, typename G, bool kWhole>
+template <typename T, typename G, int U, bool kWhole>
 __global__ __launch_bounds__(kThreads) void sum_kernel(const T* grad_out, uint64_t stride, G* grad, uint32_t rows,
                                                        uint32_t cols, uint32_t slots, uint32_t piece, float scale,
                                                        bool accumulate, Lanes l, Sorted in) {
-  constexpr int N = 16 / sizeof(T), U = kSumBlocks;
+  constexpr int N = 16 / sizeof(T);
   typedef const Vec<T, N>* Vector;
   const uint32_t task = task_of<kWhole>(l);
   const uint32_t c = first_column<N, U>(l), step = uint32_t(N) << l.log2;
@@ -572,13 +570,21 @@ Layout layout_of(const sr_embedding_shape& s) {
   return w;
 }
 
+// A lane takes one block of columns, or two where a row has more of them than a
+// workgroup has lanes: 30011 tokens of 3584 bf16 columns 136 us with two, 141
+// with one (of two workgroups a row), but 65536 tokens of 1984 columns 151 and
+// 141, and 4096 tokens of 768 f32 columns 31 and 28.
 template <typename T, typename G>
 void launch_sum(const sr_embedding_shape& s, const Layout& w, const Sorted& sorted, const void* grad_out,
                 uint64_t stride, void* grad, bool accumulate, hipStream_t stream) {
-  const Lanes l = lanes_of(s.cols, 16 / sizeof(T), kThreads, kSumBlocks);
+  constexpr uint32_t N = 16 / sizeof(T);
+  const int each = s.cols > uint64_t(N) * kThreads ? 2 : 1;
+  const Lanes l = lanes_of(s.cols, N, kThreads, each);
   const uint32_t group = uint32_t(kThreads) >> l.log2;
-  const dim3 grid(uint32_t((uint64_t(w.slots) * kSumBlocks + s.rows + group - 1) / group), l.slices);
-  auto* kernel = l.log2 >= 6 ? sum_kernel<T, G, true> : sum_kernel<T, G, false>;
+  const dim3 grid(uint32_t((uint64_t(w.slots) * each + s.rows + group - 1) / group), l.slices);
+  auto* kernel = each == 2     ? sum_kernel<T, G, 2, true>
+                 : l.log2 >= 6 ? sum_kernel<T, G, 1, true>
+                               : sum_kernel<T, G, 1, false>;
   kernel<<<grid, kThreads, 0, stream>>>(static_cast<const T*>(grad_out), stride, static_cast<G*>(grad),
                                         uint32_t(s.rows), uint32_t(s.cols), w.slots, w.piece, s.scale, accumulate, l,
                                         sorted);

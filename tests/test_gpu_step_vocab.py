@@ -155,6 +155,25 @@ def test_grad_accumulates(grad_dtype):
     assert_near(out, want, off)
 
 
+@pytest.mark.parametrize("cols", [5, 511, 999, 2047, 2053, 4100])
+@pytest.mark.parametrize("dtype,grad_dtype", [(BF16, F32), (F16, F16), (F32, F32)])
+def test_grad_of_wide_rows_and_their_ends(cols, dtype, grad_dtype):
+    """Rows that take part of a wave, whole waves or a workgroup twice over, with
+    a last block that is not whole; short, long and cut, added to what is there."""
+    g = gen(8)
+    lengths = torch.tensor([0, 1, 2, 3, 9, 10, 17, 32, 33, 300, 900], device=DEV)
+    tokens = torch.repeat_interleave(torch.arange(len(lengths), device=DEV), lengths)
+    tokens = tokens[torch.randperm(len(tokens), generator=g, device=DEV)]
+    grad_out = randn(g, len(tokens), cols, dtype=dtype)
+    out = randn(g, len(lengths), cols, dtype=grad_dtype)
+    old = out.double()
+    want, off = grad64(tokens, grad_out, len(lengths), 0.5, 0)
+    vocab_embedding_grad(tokens, grad_out, len(lengths), scale=0.5, out=out, accumulate=True)
+    assert_near(out, want + old, off + u * (want.abs() + old.abs()))
+    vocab_embedding_grad(tokens, grad_out, len(lengths), scale=0.5, out=out)
+    assert_near(out, want, off)
+
+
 def test_grad_strides_and_shapes():
     g = gen(7)
     wide = randn(g, 90, 70, dtype=BF16)

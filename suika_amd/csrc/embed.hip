@@ -15,17 +15,21 @@
 //           the L2: it counts those of the workgroups before it, which is where
 //           its own start in the sorted list, and those of each of its rows,
 //           and places them in a second pass.  No workgroup waits for another.
-//           Its time is a chain of loads, scans and barriers: 12.5 us for 16384
-//           tokens, 20 for 30011.  (Ranges of neighbouring rows: 24 and 43 us,
-//           as the range of the frequent tokens is one workgroup's.)
-//   sum     A group of lanes per row adds up the row's tokens, each lane two
-//           16-byte column blocks.  A row of many tokens (a space, a filler) is
-//           cut into pieces that are summed side by side, into 32-bit partial
-//           sums.  Rows in the order of memory, gradients read and written
-//           past the caches: 51.7 us for 256 MB (5 TB/s; one block a lane
-//           55.0, four 68; with cached accesses 73; rows in the sort's order
-//           78).  What is left is the chain from a row's tokens to its sum.
-//   join    The partial sums of such rows, added in order: 12 us.
+//           Its time is a chain of loads, scans and barriers: 11.2 us for 16384
+//           tokens, 18 for 30011; 28 where one row has 9800 of 16384, which is
+//           one workgroup's.  (Ranges of neighbouring rows: 24 and 43 us, as
+//           the range of the frequent tokens is one workgroup's.)
+//   sum     A group of lanes per row adds up the row's tokens, each lane one or
+//           two 16-byte column blocks.  A row of many tokens (a space, a filler)
+//           is cut into pieces that are summed side by side, into 32-bit partial
+//           sums.  A chain of tokens bounds it where rows have many, so eight
+//           are loaded at once and the indices of the next eight beside them;
+//           groups of whole waves keep the rows' addresses in scalar registers,
+//           which leaves room for that at full occupancy.  Rows in the order of
+//           memory, gradients read and written past the caches: 48.2 us for
+//           256 MB (5.3 TB/s; four tokens at once and indices as they are
+//           needed 51.8; with cached accesses 73; rows in the sort's order 78).
+//   join    The partial sums of such rows, added in order: 6.7 us.
 
 #include <hip/hip_runtime.h>
 
@@ -129,7 +133,7 @@ constexpr uint32_t kNoPiece = 0xffffffffu;
 
 // The tokens of a piece of a row of n: `least` or, of long rows, as many as the
 // row then has pieces, so that adding up a piece and joining them take the same
-// number of steps.
+// number of steps (with `least` for all: the join 11.8 us, not 8.9).
 __device__ __forceinline__ uint32_t piece_of(uint32_t n, uint32_t least) {
   return max(least, (uint32_t(sqrtf(float(n))) + 3) / 4 * 4);
 }

@@ -52,12 +52,28 @@ const at::Tensor& tensor_of(PyObject* o, const std::string& what) {
   return THPVariable_Unpack(o);
 }
 
+// Whether a tensor's storage holds its elements: it does not once it was
+// released (forcefully_free_tensor), and then a view's address is its offset
+// alone.
+bool stored(const at::Tensor& t) {
+  if (t.numel() == 0) return true;
+  if (!t.has_storage()) return false;
+  uint64_t last = uint64_t(t.storage_offset());
+  for (int64_t d = 0; d < t.dim(); ++d) last += uint64_t((t.size(d) - 1) * t.stride(d));
+  return (last + 1) * t.element_size() <= t.storage().nbytes();
+}
+
+void check_stored(const at::Tensor& t, const char* what) {
+  if (!stored(t)) plan_error(std::string(what) + ": its storage has been released");
+}
+
 // A dense tensor on the GPU; `device` is set by the first one.
 void check_dense(const at::Tensor& t, const std::string& what, c10::optional<at::Device>& device) {
   if (t.layout() != at::kStrided || !t.is_cuda()) plan_error(what + " is on " + t.device().str() + ", not a dense tensor on the GPU");
   if (!device) device = t.device();
   if (t.device() != *device) plan_error(what + " is on " + t.device().str() + ", not on " + device->str());
   if (!t.is_contiguous()) plan_error(what + " is not contiguous");
+  if (!stored(t)) plan_error(what + ": its storage has been released");
 }
 
 // The tensors of a list; None stands for a tensor that is not there.
@@ -151,6 +167,7 @@ const double* given_sum(py::handle square_sum, const at::Device& device) {
   const at::Tensor& t = tensor_of(square_sum.ptr(), "square_sum");
   if (t.scalar_type() != at::kDouble || t.numel() != 1 || t.device() != device)
     plan_error("square_sum: one float64 on " + device.str() + " is wanted");
+  check_stored(t, "square_sum");
   return t.data_ptr<double>();
 }
 
@@ -237,8 +254,10 @@ class AdamWState {
       const at::ScalarType gt = g.scalar_type();
       if (gt != at::kFloat && gt != at::kBFloat16)
         plan_error("gradient of " + names_[i] + ": dtype " + c10::toString(gt) + ", not float32 or bfloat16");
-      // storage that was released since the state was taken (forcefully_free_tensor)
-      if (w.numel() && (!w.storage().nbytes() || !m.storage().nbytes() || !v.storage().nbytes()))
+      if (!stored(g)) plan_error("gradient of " + names_[i] + ": its storage has been released");
+      // fields whose storage was released since the state was taken; the address of a param without storage may be
+      // null, which would mean that there is none
+      if (!stored(w) || !stored(m) || !stored(v) || (p.defined() && !stored(p)))
         plan_error(names_[i] + ": a field's storage has been released");
       const int32_t gc = gt == at::kFloat ? SR_DT_F32 : SR_DT_BF16;
       tensors.push_back({w.data_ptr(), m.data_ptr(), v.data_ptr(), p.defined() ? p.data_ptr() : nullptr, g.data_ptr(),
@@ -300,6 +319,7 @@ int32_t index_code(const at::Tensor& t, const char* what) {
 // A tensor of rows of `cols` dense elements: their distance in elements.
 uint64_t row_stride(const at::Tensor& t, const std::string& what) {
   if (t.layout() != at::kStrided || t.dim() < 1) plan_error(what + ": a dense tensor of rows is wanted");
+  if (!stored(t)) plan_error(what + ": its storage has been released");
   const int64_t cols = t.size(-1);
   if (t.is_contiguous()) return uint64_t(cols);
   if (t.dim() != 2 || (t.stride(1) != 1 && cols > 1) || (t.stride(0) < cols && t.size(0) > 1))
@@ -314,6 +334,7 @@ void check_device(const at::Tensor& t, const char* what, const at::Device& devic
 sr_embedding_shape embedding_shape(const at::Tensor& tokens, int32_t dtype, int64_t rows, int64_t cols, double scale,
                                    int64_t vocab_start) {
   if (!tokens.is_cuda() || !tokens.is_contiguous()) plan_error("tokens: a contiguous tensor on the GPU is wanted");
+  check_stored(tokens, "tokens");
   return {tokens.data_ptr(), index_code(tokens, "tokens"), dtype,         uint64_t(tokens.numel()), uint64_t(rows),
           uint64_t(cols),    vocab_start,                  float(scale), 0};
 }
@@ -333,6 +354,7 @@ at::Tensor vocab_embedding(const at::Tensor& tokens, const at::Tensor& weight, d
     check_device(*out, "out", tokens.device());
     if (out->sizes() != at::IntArrayRef(shape) || !out->is_contiguous() || out->scalar_type() != weight.scalar_type())
       plan_error("out: a contiguous tensor of the tokens' shape and the weight's columns and dtype is wanted");
+    check_stored(*out, "out");
   }
   at::Tensor to = out ? *out : at::empty(shape, on(tokens.device(), weight.scalar_type()));
   check(sr_embedding(&s, weight.data_ptr(), stride, to.data_ptr(), stream_of(tokens.device())), "sr_embedding");
@@ -358,6 +380,7 @@ at::Tensor vocab_embedding_grad(const at::Tensor& tokens, const at::Tensor& grad
     check_device(to, "out", tokens.device());
     if (to.dim() != 2 || to.size(0) != rows || to.size(1) != cols || !to.is_contiguous())
       plan_error("out: a contiguous tensor of rows x columns is wanted");
+    check_stored(to, "out");
     if (!dtype.is_none() && torch::python::detail::py_object_to_dtype(dtype) != to.scalar_type())
       plan_error("out is of another dtype than the one asked for");
   } else {
@@ -382,6 +405,7 @@ sr_logprob_shape logprob_shape(const at::Tensor& logits, const at::Tensor& targe
     plan_error("logits: a tensor of the targets' shape and the columns is wanted");
   if (!logits.is_cuda() || !targets.is_contiguous()) plan_error("logits on the GPU and contiguous targets are wanted");
   check_device(targets, "targets", logits.device());
+  check_stored(targets, "targets");
   const int64_t columns = logits.size(-1), v = vocab ? *vocab : columns;
   if (v < 1 || v > columns)
     plan_error("a vocabulary of " + std::to_string(v) + " in " + std::to_string(columns) + " columns");
@@ -421,6 +445,7 @@ const float* row_values(const at::Tensor& t, const char* what, const at::Tensor&
   check_device(t, what, targets.device());
   if (t.scalar_type() != at::kFloat || t.sizes() != targets.sizes() || !t.is_contiguous())
     plan_error(std::string(what) + ": a contiguous float32 tensor of the targets' shape is wanted");
+  check_stored(t, what);
   return t.data_ptr<float>();
 }
 

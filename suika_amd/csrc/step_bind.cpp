@@ -67,6 +67,11 @@ void check_stored(const at::Tensor& t, const char* what) {
   if (!stored(t)) plan_error(std::string(what) + ": its storage has been released");
 }
 
+// Whether a tensor is what check_dense wants, but for its storage.
+bool dense(const at::Tensor& t, const c10::optional<at::Device>& device) {
+  return t.layout() == at::kStrided && t.is_cuda() && device && t.device() == *device && t.is_contiguous();
+}
+
 // A dense tensor on the GPU; `device` is set by the first one.
 void check_dense(const at::Tensor& t, const std::string& what, c10::optional<at::Device>& device) {
   if (t.layout() != at::kStrided || !t.is_cuda()) plan_error(what + " is on " + t.device().str() + ", not a dense tensor on the GPU");
@@ -220,19 +225,11 @@ class AdamWState {
     if (w.size() != names_.size() || m.size() != w.size() || v.size() != w.size() || p.size() != w.size())
       plan_error("state: lists of different lengths");
     for (size_t i = 0; i < names_.size(); ++i) {
-      weight_.push_back(field(w[i], i, "weight"));
-      exp_avg_.push_back(field(m[i], i, "exp_avg"));
-      exp_avg_sq_.push_back(field(v[i], i, "exp_avg_sq"));
-      param_.push_back(p[i] == Py_None ? at::Tensor() : field(p[i], i, "param"));
-      for (const at::Tensor* t : {&exp_avg_[i], &exp_avg_sq_[i], &param_[i]})
-        if (t->defined() && t->sizes() != weight_[i].sizes()) plan_error(names_[i] + ": fields of different shapes");
-      const at::ScalarType wt = weight_[i].scalar_type(), mt = exp_avg_[i].scalar_type();
-      if (wt != at::kFloat && wt != at::kBFloat16)
-        plan_error(names_[i] + ": weight of dtype " + c10::toString(wt) + ", not float32 or bfloat16");
-      if ((mt != at::kFloat && mt != at::kBFloat16) || exp_avg_sq_[i].scalar_type() != mt)
-        plan_error(names_[i] + ": moments are both float32 or both bfloat16");
-      if (param_[i].defined() && (wt != at::kFloat || param_[i].scalar_type() != at::kBFloat16))
-        plan_error(names_[i] + ": a master weight is float32 and its param bfloat16");
+      weight_.push_back(tensor_of(w[i], names_[i] + "/weight"));
+      exp_avg_.push_back(tensor_of(m[i], names_[i] + "/exp_avg"));
+      exp_avg_sq_.push_back(tensor_of(v[i], names_[i] + "/exp_avg_sq"));
+      param_.push_back(p[i] == Py_None ? at::Tensor() : tensor_of(p[i], names_[i] + "/param"));
+      check_fields(i);
     }
   }
 
@@ -247,18 +244,16 @@ class AdamWState {
     tensors.reserve(names_.size());
     for (size_t i = 0; i < names_.size(); ++i) {
       if (list[i] == Py_None) continue;
-      const at::Tensor& g = tensor_of(list[i], "gradient of " + names_[i]);
+      if (!THPVariable_Check(list[i])) plan_error("gradient of " + names_[i] + ": not a tensor");
+      const at::Tensor& g = THPVariable_Unpack(list[i]);
       const at::Tensor &w = weight_[i], &m = exp_avg_[i], &v = exp_avg_sq_[i], &p = param_[i];
+      check_fields(i);
       if (g.layout() != at::kStrided || !g.is_contiguous() || g.device() != w.device() || g.sizes() != w.sizes())
         plan_error("gradient of " + names_[i] + ": a dense tensor like the weight on " + w.device().str() + " is wanted");
       const at::ScalarType gt = g.scalar_type();
       if (gt != at::kFloat && gt != at::kBFloat16)
         plan_error("gradient of " + names_[i] + ": dtype " + c10::toString(gt) + ", not float32 or bfloat16");
       if (!stored(g)) plan_error("gradient of " + names_[i] + ": its storage has been released");
-      // fields whose storage was released since the state was taken; the address of a param without storage may be
-      // null, which would mean that there is none
-      if (!stored(w) || !stored(m) || !stored(v) || (p.defined() && !stored(p)))
-        plan_error(names_[i] + ": a field's storage has been released");
       const int32_t gc = gt == at::kFloat ? SR_DT_F32 : SR_DT_BF16;
       tensors.push_back({w.data_ptr(), m.data_ptr(), v.data_ptr(), p.defined() ? p.data_ptr() : nullptr, g.data_ptr(),
                          uint64_t(w.numel()), w.scalar_type() == at::kFloat ? SR_DT_F32 : SR_DT_BF16,
@@ -296,11 +291,26 @@ class AdamWState {
   }
 
  private:
-  at::Tensor field(PyObject* o, size_t i, const char* what) {
-    const std::string full = names_[i] + "/" + what;
-    const at::Tensor& t = tensor_of(o, full);
-    check_dense(t, full, device_);
-    return t;
+  // The fields of parameter i as they are now: a tensor's memory, shape and type
+  // can be replaced (`.data`, set_) or its storage released since the state was
+  // taken, and the kernels go by the weight's size.
+  void check_fields(size_t i) {
+    const at::Tensor &w = weight_[i], &m = exp_avg_[i], &v = exp_avg_sq_[i], &p = param_[i];
+    const struct { const at::Tensor& t; const char* what; } field[4] = {
+        {w, "weight"}, {m, "exp_avg"}, {v, "exp_avg_sq"}, {p, "param"}};
+    for (const auto& f : field) {
+      if (!f.t.defined()) continue;
+      if (!dense(f.t, device_)) check_dense(f.t, names_[i] + "/" + f.what, device_);     // says what is wrong
+      if (!stored(f.t)) plan_error(names_[i] + ": a field's storage has been released");
+      if (f.t.sizes() != w.sizes()) plan_error(names_[i] + ": fields of different shapes");
+    }
+    const at::ScalarType wt = w.scalar_type(), mt = m.scalar_type();
+    if (wt != at::kFloat && wt != at::kBFloat16)
+      plan_error(names_[i] + ": weight of dtype " + c10::toString(wt) + ", not float32 or bfloat16");
+    if ((mt != at::kFloat && mt != at::kBFloat16) || v.scalar_type() != mt)
+      plan_error(names_[i] + ": moments are both float32 or both bfloat16");
+    if (p.defined() && (wt != at::kFloat || p.scalar_type() != at::kBFloat16))
+      plan_error(names_[i] + ": a master weight is float32 and its param bfloat16");
   }
 
   std::vector<std::string> names_;

@@ -17,7 +17,7 @@ the host.  Refused arguments raise ``PlanError`` before anything runs.
 """
 from __future__ import annotations
 
-from typing import Any, Dict, List, Mapping, Optional, Sequence, Set, Tuple, Union
+from typing import Dict, List, Mapping, Optional, Sequence, Tuple, Union
 
 import torch
 from torch import Tensor
@@ -68,23 +68,28 @@ def clip_grads(grads: Grads, max_norm: float, *, out: Optional[Grads] = None,
 def counted_names(layout: ParamLayout, rank: int) -> List[str]:
     """The parameters whose gradients ``rank`` counts in a global norm.
 
-    Every shard is counted once: by the lowest rank that holds it.  So a
-    tensor-parallel shard counts on each rank of its group, a replicated
-    parameter (norms, row-parallel biases, data-parallel copies) on one.
+    Every element of a parameter is counted once.  Of its holders, those of one
+    tensor-parallel degree count, each shard on the lowest rank that has it: so
+    a tensor-parallel shard counts on each rank of one group, a replicated
+    parameter (norms, row-parallel biases, data-parallel copies) on one rank.
+    Where replicas hold a parameter at different degrees, the degree is that of
+    the lowest rank whose degree's shards are all there.
     """
     mine = layout.layout[rank]
-    before: Set[Tuple[str, Any]] = set()
+    holders: Dict[str, List[Tuple[int, int, int]]] = {n: [] for n in mine}     # (degree, index, rank), by rank
     for r in sorted(layout.layout):
-        if r >= rank:
-            break
-        before.update((n, _shard_of(m)) for n, m in layout.layout[r].items() if n in mine)
-    return [n for n, m in mine.items() if (n, _shard_of(m)) not in before]
+        for n, m in layout.layout[r].items():
+            if n in mine:
+                holders[n].append((m.tp_deg(), m.tp_index(), r))
+    return [n for n in mine if _counts(holders[n], rank)]
 
 
-def _shard_of(meta) -> Any:
-    """What tells a parameter's shards apart: (index, degree), or nothing for a
-    whole one."""
-    return (meta.tp_index(), meta.tp_deg()) if meta.tp_deg() > 1 else None
+def _counts(holders: List[Tuple[int, int, int]], rank: int) -> bool:
+    first: Dict[int, Dict[int, int]] = {}      # degree -> index -> the lowest rank that holds it
+    for deg, index, r in holders:
+        first.setdefault(deg, {}).setdefault(index, r)
+    whole = [shards for deg, shards in first.items() if len(shards) == deg]
+    return rank in (whole or list(first.values()))[0].values()
 
 
 class ShardAdamW:

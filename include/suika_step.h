@@ -7,7 +7,7 @@
  * vocabulary of the embedding cut over the tensor-parallel ranks.  These are
  * the parts of a step that work on that state's own layouts:
  *
- *   sr_square_sum, sr_clip, sr_adamw
+ *   sr_square_sum, sr_clip, sr_clip_norm, sr_adamw, sr_adamw_norm
  *       the gradients' global norm over all tensors of a share, clipping by
  *       it, and the AdamW update of every state field.  In the reference
  *       these are torch.optim.AdamW on the model's parameters
@@ -24,8 +24,8 @@
  *   - All device memory, workspaces included, belongs to the caller.
  *   - Calls are asynchronous and stream-ordered, allocate nothing, and keep
  *     nothing from one call for the next.  They launch kernels only, so they
- *     can be captured into a HIP graph; sr_adamw refuses (SR_EINVAL), because
- *     its step number is a host value.
+ *     can be captured into a HIP graph; sr_adamw and sr_adamw_norm refuse
+ *     (SR_EINVAL), because their step number is a host value.
  *   - Data may be aligned to its element size only.  Workspaces are aligned
  *     to 16 bytes.
  *   - Sums, statistics and updates are computed in 32 bits or more and
@@ -76,6 +76,22 @@ int sr_square_sum(const sr_array* arrays, int32_t count, int32_t read_again, voi
 int sr_clip(const sr_array* src, const sr_array* dst, int32_t count, const double* square_sum, float max_norm,
             float* norm, hipStream_t stream);
 
+/* The norm that gradients are clipped by: of a sum of squares on the device
+ * (square_sum; sum and workspace are not used then), or, where square_sum is
+ * NULL, of the call's own gradients, whose sum goes to *sum. */
+typedef struct sr_norm {
+  const double* square_sum;
+  double* sum;
+  void* workspace;          /* sr_square_sum_workspace bytes of the gradients */
+  uint64_t workspace_bytes;
+  float* norm;              /* gets the sum's root; may be NULL */
+} sr_norm;
+
+/* sr_clip by such a norm: the gradients' sum of squares and the clipping in one
+ * call, whose arguments are all checked before the first launch. */
+int sr_clip_norm(const sr_array* src, const sr_array* dst, int32_t count, float max_norm, const sr_norm* norm,
+                 hipStream_t stream);
+
 /* One parameter's fields.  param is the bf16 copy of an f32 weight (master),
  * NULL where the weight is the parameter itself. */
 typedef struct sr_adamw_tensor {
@@ -98,7 +114,7 @@ typedef struct sr_adamw_options {
   double eps;
   double weight_decay;
   int64_t step;          /* number of this update, from 1 */
-  double max_norm;       /* with square_sum: the gradients are clipped to it */
+  double max_norm;       /* with square_sum or norm: the gradients are clipped to it */
 } sr_adamw_options;
 
 /*
@@ -108,6 +124,11 @@ typedef struct sr_adamw_options {
  */
 int sr_adamw(const sr_adamw_tensor* tensors, int32_t count, const sr_adamw_options* options, const double* square_sum,
              hipStream_t stream);
+
+/* The same with the norm in the call: clipped by `norm`, or not where it is
+ * NULL.  All arguments are checked before the first launch. */
+int sr_adamw_norm(const sr_adamw_tensor* tensors, int32_t count, const sr_adamw_options* options, const sr_norm* norm,
+                  hipStream_t stream);
 
 /* The tokens and the shard of an embedding: row r of the shard is token
  * vocab_start + r.  Tokens outside the shard (negative ones among them) give

@@ -80,7 +80,9 @@ EXPORTED_SYMBOLS = (
     "sr_square_sum_workspace",
     "sr_square_sum",
     "sr_clip",
+    "sr_clip_norm",
     "sr_adamw",
+    "sr_adamw_norm",
     "sr_embedding",
     "sr_embedding_grad_workspace",
     "sr_embedding_grad",

@@ -532,33 +532,34 @@ void adamw_scalars(AdamTable<COPY>& t, const sr_adamw_options& o, const double* 
   t.eps = float(o.eps);
 }
 
-}  // namespace
+// ------------------------------------------------------- checks, then launches
 
-extern "C" {
-
-int sr_square_sum_workspace(const sr_array* arrays, int32_t count, uint64_t* bytes) {
-  if (bytes == nullptr) return fail(SR_EINVAL, "sr_square_sum_workspace: null argument");
-  if (int rc = check_arrays("sr_square_sum_workspace", arrays, count)) return rc;
+// The bytes of a workspace for the sum of checked arrays.
+uint64_t sum_workspace(const sr_array* arrays, int32_t count) {
   uint64_t blocks = 0;
   sum_launches(arrays, count, [&](int32_t, const SumTable& t) {
     blocks += sum_blocks(t);
     return SR_OK;
   });
-  *bytes = blocks * sizeof(double);
+  return blocks * sizeof(double);
+}
+
+int check_sum(const char* who, const sr_array* arrays, int32_t count, const void* workspace, uint64_t workspace_bytes,
+              const double* sum, const float* norm) {
+  if (int rc = check_arrays(who, arrays, count)) return rc;
+  const uint64_t need = sum_workspace(arrays, count);
+  if (sum == nullptr) return fail(SR_EINVAL, "%s: sum is null", who);
+  if (workspace_bytes < need || (need && workspace == nullptr))
+    return fail(SR_EINVAL, "%s: a workspace of %llu bytes, %llu are needed", who, (unsigned long long)workspace_bytes,
+                (unsigned long long)need);
+  if (reinterpret_cast<uintptr_t>(workspace) % 16 || reinterpret_cast<uintptr_t>(sum) % 8 ||
+      reinterpret_cast<uintptr_t>(norm) % 4)
+    return fail(SR_EALIGN, "%s: the workspace or a result is not aligned", who);
   return SR_OK;
 }
 
-int sr_square_sum(const sr_array* arrays, int32_t count, int32_t read_again, void* workspace, uint64_t workspace_bytes,
-                  double* sum, float* norm, hipStream_t stream) {
-  uint64_t need = 0;
-  if (int rc = sr_square_sum_workspace(arrays, count, &need)) return rc;
-  if (sum == nullptr) return fail(SR_EINVAL, "sr_square_sum: sum is null");
-  if (workspace_bytes < need || (need && workspace == nullptr))
-    return fail(SR_EINVAL, "sr_square_sum: a workspace of %llu bytes, %llu are needed",
-                (unsigned long long)workspace_bytes, (unsigned long long)need);
-  if (reinterpret_cast<uintptr_t>(workspace) % 16 || reinterpret_cast<uintptr_t>(sum) % 8 ||
-      reinterpret_cast<uintptr_t>(norm) % 4)
-    return fail(SR_EALIGN, "sr_square_sum: the workspace or a result is not aligned");
+int launch_square_sum(const sr_array* arrays, int32_t count, bool read_again, void* workspace, double* sum, float* norm,
+                      hipStream_t stream) {
   double* partial = static_cast<double*>(workspace);
   uint32_t used = 0;
   uint64_t bytes = 0;
@@ -566,7 +567,7 @@ int sr_square_sum(const sr_array* arrays, int32_t count, int32_t read_again, voi
   uint64_t elements = 0;
   int32_t tables = 0;
   for (int32_t i = 0; i < count; ++i) elements += arrays[i].n;
-  const bool stream_loads = read_again == 0 || bytes > kSumCached;
+  const bool stream_loads = !read_again || bytes > kSumCached;
   if (elements <= kSmallElements) {
     sum_launches(arrays, count, [&](int32_t, const SumTable&) {
       ++tables;
@@ -593,27 +594,50 @@ int sr_square_sum(const sr_array* arrays, int32_t count, int32_t read_again, voi
   return launched("sr_square_sum");
 }
 
-int sr_clip(const sr_array* src, const sr_array* dst, int32_t count, const double* square_sum, float max_norm,
-            float* norm, hipStream_t stream) try {
-  if (int rc = check_arrays("sr_clip: src", src, count)) return rc;
+// What a norm takes: the sum that is given, or the place and the workspace for that of the gradients.
+int check_norm(const char* who, const sr_norm& n, const sr_array* grads, int32_t count) {
+  if (n.square_sum == nullptr) return check_sum(who, grads, count, n.workspace, n.workspace_bytes, n.sum, n.norm);
+  if (reinterpret_cast<uintptr_t>(n.square_sum) % 8 || reinterpret_cast<uintptr_t>(n.norm) % 4)
+    return fail(SR_EALIGN, "%s: square_sum or norm is not aligned", who);
+  return SR_OK;
+}
+
+// *norm = sqrt(*square_sum), with nothing to clip.
+int launch_norm(const char* who, const double* square_sum, float* norm, hipStream_t stream) {
+  ClipTable t;
+  t.at.clear();
+  t.at.chunks = 1;
+  t.max_norm = 0;
+  t.square_sum = square_sum;
+  t.norm = norm;
+  launch_clip<float, float>(t, stream);
+  return launched(who);
+}
+
+int clip(const char* who, const sr_array* src, const sr_array* dst, int32_t count, float max_norm, const sr_norm& n,
+         hipStream_t stream) try {
+  if (int rc = check_arrays(who, src, count)) return rc;
   if (dst != nullptr) {
-    if (int rc = check_arrays("sr_clip: dst", dst, count)) return rc;
+    if (int rc = check_arrays(who, dst, count)) return rc;
   }
-  if (square_sum == nullptr) return fail(SR_EINVAL, "sr_clip: square_sum is null");
-  if (reinterpret_cast<uintptr_t>(square_sum) % 8 || reinterpret_cast<uintptr_t>(norm) % 4)
-    return fail(SR_EALIGN, "sr_clip: square_sum or norm is not aligned");
-  if (!(max_norm >= 0)) return fail(SR_EINVAL, "sr_clip: max_norm %g", double(max_norm));
+  if (int rc = check_norm(who, n, src, count)) return rc;
+  if (!(max_norm >= 0)) return fail(SR_EINVAL, "%s: max_norm %g", who, double(max_norm));
   if (dst == nullptr) dst = src;
   std::vector<Span> spans;
   for (int32_t i = 0; i < count; ++i) {
     if (src[i].n != dst[i].n)
-      return fail(SR_EINVAL, "sr_clip: src[%d] has %llu elements, dst[%d] %llu", i, (unsigned long long)src[i].n, i,
+      return fail(SR_EINVAL, "%s: src[%d] has %llu elements, dst[%d] %llu", who, i, (unsigned long long)src[i].n, i,
                   (unsigned long long)dst[i].n);
     add_span(spans, dst[i].data, bytes_of(dst[i]), true);
     if (src[i].data != dst[i].data || src[i].dtype != dst[i].dtype)
       add_span(spans, src[i].data, bytes_of(src[i]), false);
   }
-  if (clash(spans)) return fail(SR_EOVERLAP, "sr_clip: an array that is written overlaps another");
+  if (clash(spans)) return fail(SR_EOVERLAP, "%s: an array that is written overlaps another", who);
+  const double* square_sum = n.square_sum;
+  if (square_sum == nullptr) {
+    if (int rc = launch_square_sum(src, count, true, n.workspace, n.sum, nullptr, stream)) return rc;
+    square_sum = n.sum;
+  }
   bool any = false;
   for (int32_t s : kFloatTypes) {
     for (int32_t d : kFloatTypes) {
@@ -623,13 +647,13 @@ int sr_clip(const sr_array* src, const sr_array* dst, int32_t count, const doubl
       t.square_sum = square_sum;
       auto flush = [&]() -> int {
         if (t.at.count == 0) return SR_OK;
-          t.norm = any ? nullptr : norm;
+        t.norm = any ? nullptr : n.norm;
         any = true;
         if (s == SR_DT_F32) launch_clip_to<float>(d, t, stream);
         else if (s == SR_DT_BF16) launch_clip_to<bf16>(d, t, stream);
         else launch_clip_to<f16>(d, t, stream);
         t.at.clear();
-        return launched("sr_clip");
+        return launched(who);
       };
       for (int32_t i = 0; i < count; ++i) {
         if (src[i].dtype != s || dst[i].dtype != d || src[i].n == 0) continue;
@@ -642,58 +666,63 @@ int sr_clip(const sr_array* src, const sr_array* dst, int32_t count, const doubl
       if (int rc = flush()) return rc;
     }
   }
-  if (!any && norm != nullptr) {
-    ClipTable t;       // nothing to clip: the norm alone
-    t.at.clear();
-    t.at.chunks = 1;
-    t.max_norm = max_norm;
-    t.square_sum = square_sum;
-    t.norm = norm;
-    launch_clip<float, float>(t, stream);
-    return launched("sr_clip");
-  }
-  return SR_OK;
+  return any || n.norm == nullptr ? int(SR_OK) : launch_norm(who, square_sum, n.norm, stream);
 } catch (const std::bad_alloc&) {
-  return fail(SR_ENOMEM, "sr_clip: out of host memory");
+  return fail(SR_ENOMEM, "%s: out of host memory", who);
 }
 
-int sr_adamw(const sr_adamw_tensor* tensors, int32_t count, const sr_adamw_options* o, const double* square_sum,
-             hipStream_t stream) try {
-  if (count < 0 || (count > 0 && tensors == nullptr) || o == nullptr)
-    return fail(SR_EINVAL, "sr_adamw: null argument");
+int adamw(const char* who, const sr_adamw_tensor* tensors, int32_t count, const sr_adamw_options* o, const sr_norm* n,
+          hipStream_t stream) try {
+  if (count < 0 || (count > 0 && tensors == nullptr) || o == nullptr) return fail(SR_EINVAL, "%s: null argument", who);
   if (!(o->lr >= 0) || !std::isfinite(o->lr) || !(o->eps >= 0) || !(o->weight_decay >= 0) || !(o->beta1 >= 0) ||
       !(o->beta1 < 1) || !(o->beta2 >= 0) || !(o->beta2 < 1) || o->step < 1)
-    return fail(SR_EINVAL, "sr_adamw: lr %g, betas %g and %g, eps %g, weight_decay %g, step %lld", o->lr, o->beta1,
+    return fail(SR_EINVAL, "%s: lr %g, betas %g and %g, eps %g, weight_decay %g, step %lld", who, o->lr, o->beta1,
                 o->beta2, o->eps, o->weight_decay, (long long)o->step);
-  if (square_sum != nullptr && !(o->max_norm >= 0)) return fail(SR_EINVAL, "sr_adamw: max_norm %g", o->max_norm);
-  if (reinterpret_cast<uintptr_t>(square_sum) % 8) return fail(SR_EALIGN, "sr_adamw: square_sum is not aligned");
+  if (n != nullptr && !(o->max_norm >= 0)) return fail(SR_EINVAL, "%s: max_norm %g", who, o->max_norm);
   std::vector<Span> spans;
+  std::vector<sr_array> grads;      // where their sum of squares is formed here
+  const bool own_sum = n != nullptr && n->square_sum == nullptr;
   for (int32_t i = 0; i < count; ++i) {
     const sr_adamw_tensor& x = tensors[i];
-    if (x.reserved != 0) return fail(SR_EINVAL, "sr_adamw: tensors[%d].reserved is not 0", i);
+    if (x.reserved != 0) return fail(SR_EINVAL, "%s: tensors[%d].reserved is not 0", who, i);
     for (int32_t dt : {x.weight_dtype, x.moment_dtype, x.grad_dtype})
-      if (dt != SR_DT_F32 && dt != SR_DT_BF16) return fail(SR_EDTYPE, "sr_adamw: tensors[%d]: dtype %d", i, dt);
+      if (dt != SR_DT_F32 && dt != SR_DT_BF16) return fail(SR_EDTYPE, "%s: tensors[%d]: dtype %d", who, i, dt);
     if (x.param != nullptr && x.weight_dtype != SR_DT_F32)
-      return fail(SR_EDTYPE, "sr_adamw: tensors[%d]: a copy of a weight that is not f32", i);
+      return fail(SR_EDTYPE, "%s: tensors[%d]: a copy of a weight that is not f32", who, i);
     if (x.n > SR_STEP_MAX_ELEMENTS)
-      return fail(SR_EBOUNDS, "sr_adamw: tensors[%d] has %llu elements", i, (unsigned long long)x.n);
+      return fail(SR_EBOUNDS, "%s: tensors[%d] has %llu elements", who, i, (unsigned long long)x.n);
     if (x.n && (!x.weight || !x.exp_avg || !x.exp_avg_sq || !x.grad))
-      return fail(SR_EINVAL, "sr_adamw: tensors[%d]: a field is null", i);
+      return fail(SR_EINVAL, "%s: tensors[%d]: a field is null", who, i);
     const int ws = sr_internal::dtype_size(x.weight_dtype), ms = sr_internal::dtype_size(x.moment_dtype),
               gs = sr_internal::dtype_size(x.grad_dtype);
     const struct { const void* p; int size; } field[5] = {
         {x.weight, ws}, {x.exp_avg, ms}, {x.exp_avg_sq, ms}, {x.param, 2}, {x.grad, gs}};
     for (int f = 0; f < 5; ++f) {
       if (reinterpret_cast<uintptr_t>(field[f].p) % field[f].size)
-        return fail(SR_EALIGN, "sr_adamw: tensors[%d]: a field is not aligned to its elements", i);
+        return fail(SR_EALIGN, "%s: tensors[%d]: a field is not aligned to its elements", who, i);
       add_span(spans, field[f].p, x.n * field[f].size, f < 4);
     }
+    if (own_sum) grads.push_back({const_cast<void*>(x.grad), x.n, x.grad_dtype, 0});
   }
-  if (clash(spans)) return fail(SR_EOVERLAP, "sr_adamw: a field that is written overlaps another");
+  if (n != nullptr) {
+    if (int rc = check_norm(who, *n, grads.data(), int32_t(grads.size()))) return rc;
+  }
+  if (clash(spans)) return fail(SR_EOVERLAP, "%s: a field that is written overlaps another", who);
   hipStreamCaptureStatus capturing = hipStreamCaptureStatusNone;
   SR_STEP_TRY(hipStreamIsCapturing(stream, &capturing));
   if (capturing != hipStreamCaptureStatusNone)
-    return fail(SR_EINVAL, "sr_adamw: the step number is a host value: the call cannot be captured");
+    return fail(SR_EINVAL, "%s: the step number is a host value: the call cannot be captured", who);
+  const double* square_sum = nullptr;
+  if (own_sum) {
+    square_sum = n->sum;
+    if (int rc = launch_square_sum(grads.data(), int32_t(grads.size()), true, n->workspace, n->sum, n->norm, stream))
+      return rc;
+  } else if (n != nullptr) {
+    square_sum = n->square_sum;
+    if (n->norm != nullptr) {
+      if (int rc = launch_norm(who, square_sum, n->norm, stream)) return rc;
+    }
+  }
   AdamTable<true> with_copy;
   AdamTable<false> alone;
   adamw_scalars(with_copy, *o, square_sum);
@@ -702,7 +731,48 @@ int sr_adamw(const sr_adamw_tensor* tensors, int32_t count, const sr_adamw_optio
   if (int rc = adamw_types<float, false>(tensors, count, alone, stream)) return rc;
   return adamw_types<bf16, false>(tensors, count, alone, stream);
 } catch (const std::bad_alloc&) {
-  return fail(SR_ENOMEM, "sr_adamw: out of host memory");
+  return fail(SR_ENOMEM, "%s: out of host memory", who);
+}
+
+}  // namespace
+
+extern "C" {
+
+int sr_square_sum_workspace(const sr_array* arrays, int32_t count, uint64_t* bytes) {
+  if (bytes == nullptr) return fail(SR_EINVAL, "sr_square_sum_workspace: null argument");
+  if (int rc = check_arrays("sr_square_sum_workspace", arrays, count)) return rc;
+  *bytes = sum_workspace(arrays, count);
+  return SR_OK;
+}
+
+int sr_square_sum(const sr_array* arrays, int32_t count, int32_t read_again, void* workspace, uint64_t workspace_bytes,
+                  double* sum, float* norm, hipStream_t stream) {
+  if (int rc = check_sum("sr_square_sum", arrays, count, workspace, workspace_bytes, sum, norm)) return rc;
+  return launch_square_sum(arrays, count, read_again != 0, workspace, sum, norm, stream);
+}
+
+int sr_clip(const sr_array* src, const sr_array* dst, int32_t count, const double* square_sum, float max_norm,
+            float* norm, hipStream_t stream) {
+  if (square_sum == nullptr) return fail(SR_EINVAL, "sr_clip: square_sum is null");
+  const sr_norm given{square_sum, nullptr, nullptr, 0, norm};
+  return clip("sr_clip", src, dst, count, max_norm, given, stream);
+}
+
+int sr_clip_norm(const sr_array* src, const sr_array* dst, int32_t count, float max_norm, const sr_norm* norm,
+                 hipStream_t stream) {
+  if (norm == nullptr) return fail(SR_EINVAL, "sr_clip_norm: norm is null");
+  return clip("sr_clip_norm", src, dst, count, max_norm, *norm, stream);
+}
+
+int sr_adamw(const sr_adamw_tensor* tensors, int32_t count, const sr_adamw_options* o, const double* square_sum,
+             hipStream_t stream) {
+  const sr_norm given{square_sum, nullptr, nullptr, 0, nullptr};
+  return adamw("sr_adamw", tensors, count, o, square_sum ? &given : nullptr, stream);
+}
+
+int sr_adamw_norm(const sr_adamw_tensor* tensors, int32_t count, const sr_adamw_options* o, const sr_norm* norm,
+                  hipStream_t stream) {
+  return adamw("sr_adamw_norm", tensors, count, o, norm, stream);
 }
 
 }  // extern "C"

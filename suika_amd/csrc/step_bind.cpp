@@ -112,24 +112,34 @@ at::TensorOptions on(const at::Device& device, at::ScalarType type) {
   return at::TensorOptions().device(device).dtype(type);
 }
 
-struct Sum {
-  at::Tensor work;     // the sum, where the caller has no place for it, and the partial sums
-  double* sum = nullptr;
+// The memory that a sum of squares takes: the sum, and the parts of it.
+struct SumWork {
+  at::Tensor memory;
+  uint64_t bytes = 0;      // of the parts
+
+  SumWork(const std::vector<sr_array>& a, const at::Device& device) {
+    check(sr_square_sum_workspace(a.data(), int32_t(a.size()), &bytes), "sr_square_sum");
+    memory = at::empty({int64_t(bytes) + 16}, on(device, at::kByte));
+  }
+  double* sum() const { return static_cast<double*>(memory.data_ptr()); }
+  void* parts() const { return static_cast<char*>(memory.data_ptr()) + 16; }
 };
 
-// Launches the sum of squares into `into` (or into memory of its own);
-// `read_again`: the arrays are read again right after.
-Sum square_sum_into(const std::vector<sr_array>& a, const at::Device& device, bool read_again, double* into,
-                    float* norm) {
-  uint64_t need = 0;
-  check(sr_square_sum_workspace(a.data(), int32_t(a.size()), &need), "sr_square_sum");
-  Sum out;
-  out.work = at::empty({int64_t(need) + 16}, on(device, at::kByte));
-  char* base = static_cast<char*>(out.work.data_ptr());
-  out.sum = into ? into : reinterpret_cast<double*>(base);
-  check(sr_square_sum(a.data(), int32_t(a.size()), read_again, base + 16, need, out.sum, norm, stream_of(device)),
+// Launches the sum of squares into `into`, or into memory of its own.
+void square_sum_into(const std::vector<sr_array>& a, const at::Device& device, double* into, float* norm) {
+  const SumWork work(a, device);
+  check(sr_square_sum(a.data(), int32_t(a.size()), 0, work.parts(), work.bytes, into ? into : work.sum(), norm,
+                      stream_of(device)),
         "sr_square_sum");
-  return out;
+}
+
+// The norm that gradients are clipped by: of a given sum, or of `grads`, with
+// the memory for it.
+sr_norm norm_of(const double* given, const std::vector<sr_array>& grads, const at::Device& device, float* norm,
+                c10::optional<SumWork>& work) {
+  if (given) return {given, nullptr, nullptr, 0, norm};
+  work.emplace(grads, device);
+  return {nullptr, work->sum(), work->parts(), work->bytes, norm};
 }
 
 std::vector<sr_array> arrays_of(const Fast& list, const char* what, c10::optional<at::Device>& device) {
@@ -151,7 +161,7 @@ at::Tensor grad_square_sum(py::object grads) {
   if (!device) device = current_device();
   const c10::DeviceGuard guard(*device);
   at::Tensor out = at::empty({}, on(*device, at::kDouble));
-  square_sum_into(a, *device, false, out.data_ptr<double>(), nullptr);
+  square_sum_into(a, *device, out.data_ptr<double>(), nullptr);
   return out;
 }
 
@@ -162,7 +172,7 @@ at::Tensor grad_norm(py::object grads) {
   if (!device) device = current_device();
   const c10::DeviceGuard guard(*device);
   at::Tensor norm = at::empty({}, on(*device, at::kFloat));
-  square_sum_into(a, *device, false, nullptr, norm.data_ptr<float>());
+  square_sum_into(a, *device, nullptr, norm.data_ptr<float>());
   return norm;
 }
 
@@ -204,14 +214,11 @@ at::Tensor clip_grads(py::object grads, double max_norm, py::object outs, py::ob
   const c10::DeviceGuard guard(*device);
   const double* sum = given_sum(square_sum, *device);
   at::Tensor norm = at::empty({}, on(*device, at::kFloat));
-  Sum mine;
-  if (!sum) {
-    mine = square_sum_into(src, *device, true, nullptr, nullptr);
-    sum = mine.sum;
-  }
-  check(sr_clip(src.data(), in_place ? nullptr : dst.data(), int32_t(src.size()), sum, float(max_norm),
-                norm.data_ptr<float>(), stream_of(*device)),
-        "sr_clip");
+  c10::optional<SumWork> work;
+  const sr_norm by = norm_of(sum, src, *device, norm.data_ptr<float>(), work);
+  check(sr_clip_norm(src.data(), in_place ? nullptr : dst.data(), int32_t(src.size()), float(max_norm), &by,
+                     stream_of(*device)),
+        "sr_clip_norm");
   for (const at::Tensor& t : to) written(t);
   return norm;
 }
@@ -263,24 +270,20 @@ class AdamWState {
     const at::Device device = device_ ? *device_ : current_device();
     const c10::DeviceGuard guard(device);
     sr_adamw_options o{lr, beta1, beta2, eps, weight_decay, step, 0.0};
-    const double* sum = nullptr;
-    Sum mine;
+    c10::optional<SumWork> work;
+    sr_norm by{};
     at::Tensor norm;
     if (!max_norm.is_none()) {
       o.max_norm = max_norm.cast<double>();
-      sum = given_sum(square_sum, device);
+      const double* sum = given_sum(square_sum, device);
       norm = at::empty({}, on(device, at::kFloat));
-      if (!sum) {
-        mine = square_sum_into(arrays, device, true, nullptr, norm.data_ptr<float>());
-        sum = mine.sum;
-      } else {
-        check(sr_clip(nullptr, nullptr, 0, sum, float(o.max_norm), norm.data_ptr<float>(), stream_of(device)),
-              "sr_clip");
-      }
+      by = norm_of(sum, arrays, device, norm.data_ptr<float>(), work);
     } else if (!square_sum.is_none()) {
       plan_error("square_sum is given without max_norm");
     }
-    check(sr_adamw(tensors.data(), int32_t(tensors.size()), &o, sum, stream_of(device)), "sr_adamw");
+    check(sr_adamw_norm(tensors.data(), int32_t(tensors.size()), &o, max_norm.is_none() ? nullptr : &by,
+                        stream_of(device)),
+          "sr_adamw_norm");
     for (size_t i = 0; i < names_.size(); ++i) {
       if (list[i] == Py_None) continue;
       for (const at::Tensor* t : {&weight_[i], &exp_avg_[i], &exp_avg_sq_[i], &param_[i]})

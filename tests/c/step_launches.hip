@@ -1,0 +1,163 @@
+// The optimizer operators' host code over a model of the HIP runtime, on the
+// CPU: which launches a call makes, with which grids and tables, and that a
+// refused call makes none.  The kernels themselves do not run.
+//
+// Usage: step_launches SCENARIO; prints "ok" and exits 0, or says what differs.
+#include "../../suika_amd/csrc/optim.hip"
+
+#include <cstdarg>
+#include <cstdio>
+#include <cstdlib>
+#include <cstring>
+
+namespace sr_internal {
+
+char message[512];
+
+int fail(int code, const char* fmt, ...) {
+  va_list ap;
+  va_start(ap, fmt);
+  std::vsnprintf(message, sizeof message, fmt, ap);
+  va_end(ap);
+  return code;
+}
+
+int dtype_size(int32_t dt) { return dt == SR_DT_F32 ? 4 : dt == SR_DT_BF16 || dt == SR_DT_F16 ? 2 : 8; }
+
+}  // namespace sr_internal
+
+namespace model {
+
+[[noreturn]] void die(const char* what) {
+  std::printf("FAILED: %s (%s)\n", what, sr_internal::message);
+  std::exit(1);
+}
+
+struct Launch {
+  const void* fn;
+  uint64_t blocks, threads;         // of the grid, of a block
+  std::vector<unsigned char> table; // the last argument's bytes, where it is a table of the AdamW kernels
+};
+std::vector<Launch> launches;
+bool capturing = false;
+
+const void* const kCopies[] = {reinterpret_cast<const void*>(adamw_kernel<float, float, float, bf16>),
+                               reinterpret_cast<const void*>(adamw_kernel<float, float, bf16, bf16>)};
+const void* const kAlone[] = {reinterpret_cast<const void*>(adamw_kernel<float, float, float, NoCopy>),
+                              reinterpret_cast<const void*>(adamw_kernel<float, float, bf16, NoCopy>),
+                              reinterpret_cast<const void*>(adamw_kernel<bf16, bf16, bf16, NoCopy>)};
+
+template <typename T>
+std::vector<unsigned char> bytes_at(void* p) {
+  std::vector<unsigned char> b(sizeof(T));
+  std::memcpy(b.data(), p, sizeof(T));
+  return b;
+}
+
+}  // namespace model
+
+extern "C" {
+
+hipError_t hipGetLastError() { return hipSuccess; }
+const char* hipGetErrorString(hipError_t) { return "error of the model"; }
+hipError_t hipStreamIsCapturing(hipStream_t, hipStreamCaptureStatus* c) {
+  return *c = model::capturing ? hipStreamCaptureStatusActive : hipStreamCaptureStatusNone, hipSuccess;
+}
+hipError_t hipLaunchKernel(const void* fn, dim3 grid, dim3 block, void** args, size_t, hipStream_t) {
+  model::Launch l{fn, uint64_t(grid.x), uint64_t(block.x), {}};
+  for (const void* f : model::kCopies)
+    if (f == fn) l.table = model::bytes_at<AdamTable<true>>(args[1]);
+  for (const void* f : model::kAlone)
+    if (f == fn) l.table = model::bytes_at<AdamTable<false>>(args[1]);
+  model::launches.push_back(l);
+  return hipSuccess;
+}
+
+static struct {
+  dim3 grid, block;
+  size_t shmem;
+  hipStream_t stream;
+} g_call;
+hipError_t __hipPushCallConfiguration(dim3 g, dim3 b, size_t m, hipStream_t s) {
+  return g_call = {g, b, m, s}, hipSuccess;
+}
+hipError_t __hipPopCallConfiguration(dim3* g, dim3* b, size_t* m, hipStream_t* s) {
+  return *g = g_call.grid, *b = g_call.block, *m = g_call.shmem, *s = g_call.stream, hipSuccess;
+}
+void** __hipRegisterFatBinary(const void*) { return nullptr; }
+void __hipRegisterFunction(void**, const void*, char*, const char*, unsigned, void*, void*, void*, void*, int*) {}
+void __hipRegisterVar(void**, void*, char*, char*, int, size_t, int, int) {}
+void __hipUnregisterFatBinary(void**) {}
+
+}  // extern "C"
+
+// ------------------------------------------------------------------ scenarios
+
+namespace {
+
+using model::die;
+using model::launches;
+
+constexpr uint64_t kBase = uint64_t(1) << 40;       // addresses that nothing reads
+void* at(uint64_t offset) { return reinterpret_cast<void*>(kBase + offset); }
+
+const sr_adamw_options kOptions = {1e-3, 0.9, 0.99, 1e-8, 0.1, 1, 1.0};
+
+sr_norm own_norm() { return {nullptr, static_cast<double*>(at(64)), at(128), 1 << 20, static_cast<float*>(at(96))}; }
+
+void expect(int rc, int want, size_t n, const char* what) {
+  if (rc != want || launches.size() != n) {
+    std::printf("status %d, %zu launches; wanted %d and %zu\n", rc, launches.size(), want, n);
+    die(what);
+  }
+  launches.clear();
+}
+
+// Calls that form the sum themselves refuse before it is launched.
+void refusals() {
+  const uint64_t M = 1 << 24;
+  const sr_norm norm = own_norm();
+  const sr_array good[2] = {{at(M), 100000, SR_DT_F32, 0}, {at(2 * M), 8, SR_DT_BF16, 0}};
+  const sr_array twice[2] = {good[0], good[0]};
+  expect(sr_clip_norm(good, nullptr, 2, 1.0f, &norm, nullptr), SR_OK, 5, "clip");
+  expect(sr_clip_norm(twice, nullptr, 2, 1.0f, &norm, nullptr), SR_EOVERLAP, 0, "clip: listed twice");
+  expect(sr_clip_norm(good, nullptr, 2, -1.0f, &norm, nullptr), SR_EINVAL, 0, "clip: max_norm");
+  expect(sr_clip_norm(good, nullptr, 2, 1.0f, nullptr, nullptr), SR_EINVAL, 0, "clip: no norm");
+  sr_norm small = norm;
+  small.workspace_bytes = 8;
+  expect(sr_clip_norm(good, nullptr, 2, 1.0f, &small, nullptr), SR_EINVAL, 0, "clip: workspace");
+  small = norm;
+  small.sum = nullptr;
+  expect(sr_clip_norm(good, nullptr, 2, 1.0f, &small, nullptr), SR_EINVAL, 0, "clip: no place for the sum");
+
+  sr_adamw_tensor t{at(M), at(2 * M), at(3 * M), nullptr, at(4 * M), 100000, SR_DT_F32, SR_DT_F32, SR_DT_F32, 0};
+  expect(sr_adamw_norm(&t, 1, &kOptions, &norm, nullptr), SR_OK, 3, "adamw");
+  expect(sr_adamw_norm(&t, 1, &kOptions, nullptr, nullptr), SR_OK, 1, "adamw without clipping");
+  sr_norm given = {static_cast<const double*>(at(64)), nullptr, nullptr, 0, static_cast<float*>(at(96))};
+  expect(sr_adamw_norm(&t, 1, &kOptions, &given, nullptr), SR_OK, 2, "adamw by a given sum");
+  given.norm = nullptr;
+  expect(sr_adamw_norm(&t, 1, &kOptions, &given, nullptr), SR_OK, 1, "adamw by a given sum alone");
+  expect(sr_adamw_norm(&t, 1, &kOptions, &small, nullptr), SR_EINVAL, 0, "adamw: no place for the sum");
+  sr_adamw_options o = kOptions;
+  o.lr = -1;
+  expect(sr_adamw_norm(&t, 1, &o, &norm, nullptr), SR_EINVAL, 0, "adamw: lr");
+  o = kOptions;
+  o.max_norm = -1;
+  expect(sr_adamw_norm(&t, 1, &o, &norm, nullptr), SR_EINVAL, 0, "adamw: max_norm");
+  o.max_norm = 1;
+  const sr_adamw_tensor both[2] = {t, t};
+  expect(sr_adamw_norm(both, 2, &o, &norm, nullptr), SR_EOVERLAP, 0, "adamw: listed twice");
+  model::capturing = true;
+  expect(sr_adamw_norm(&t, 1, &o, &norm, nullptr), SR_EINVAL, 0, "adamw: captured");
+  expect(sr_clip_norm(good, nullptr, 2, 1.0f, &norm, nullptr), SR_OK, 5, "clip: captured");
+}
+
+}  // namespace
+
+int main(int argc, char** argv) {
+  const char* scenario = argc > 1 ? argv[1] : "";
+  if (!std::strcmp(scenario, "refusals")) refusals();
+  else die("no such scenario");
+  std::printf("ok\n");
+  return 0;
+}

@@ -126,9 +126,11 @@ int sr_adamw(const sr_adamw_tensor* tensors, int32_t count, const sr_adamw_optio
              hipStream_t stream);
 
 /* The same with the norm in the call: clipped by `norm`, or not where it is
- * NULL.  All arguments are checked before the first launch. */
-int sr_adamw_norm(const sr_adamw_tensor* tensors, int32_t count, const sr_adamw_options* options, const sr_norm* norm,
-                  hipStream_t stream);
+ * NULL.  steps[i] is the number of tensors[i]'s update (a parameter that had no
+ * gradient for a while has had fewer); steps NULL: options->step for all.  All
+ * arguments are checked before the first launch. */
+int sr_adamw_norm(const sr_adamw_tensor* tensors, const int64_t* steps, int32_t count,
+                  const sr_adamw_options* options, const sr_norm* norm, hipStream_t stream);
 
 /* The tokens and the shard of an embedding: row r of the shard is token
  * vocab_start + r.  Tokens outside the shard (negative ones among them) give

@@ -18,6 +18,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <functional>
 #include <new>
 #include <type_traits>
 #include <vector>
@@ -519,7 +520,7 @@ int adamw_types(const sr_adamw_tensor* tensors, int32_t count, const AdamTable<C
 }
 
 template <bool COPY>
-void adamw_scalars(AdamTable<COPY>& t, const sr_adamw_options& o, const double* square_sum) {
+void adamw_scalars(AdamTable<COPY>& t, const sr_adamw_options& o, int64_t step, const double* square_sum) {
   t.square_sum = square_sum;
   t.max_norm = square_sum ? float(o.max_norm) : 0.0f;
   t.decay = float(1 - o.lr * o.weight_decay);
@@ -527,8 +528,8 @@ void adamw_scalars(AdamTable<COPY>& t, const sr_adamw_options& o, const double* 
   t.rest1 = float(1 - o.beta1);
   t.beta2 = float(o.beta2);
   t.rest2 = float(1 - o.beta2);
-  t.step_size = float(o.lr / (1 - std::pow(o.beta1, double(o.step))));
-  t.root_scale = float(1 / std::sqrt(1 - std::pow(o.beta2, double(o.step))));
+  t.step_size = float(o.lr / (1 - std::pow(o.beta1, double(step))));
+  t.root_scale = float(1 / std::sqrt(1 - std::pow(o.beta2, double(step))));
   t.eps = float(o.eps);
 }
 
@@ -671,11 +672,23 @@ int clip(const char* who, const sr_array* src, const sr_array* dst, int32_t coun
   return fail(SR_ENOMEM, "%s: out of host memory", who);
 }
 
-int adamw(const char* who, const sr_adamw_tensor* tensors, int32_t count, const sr_adamw_options* o, const sr_norm* n,
-          hipStream_t stream) try {
+// One update of checked tensors, all of the same step.
+int launch_adamw(const sr_adamw_tensor* tensors, int32_t count, const sr_adamw_options& o, int64_t step,
+                 const double* square_sum, hipStream_t stream) {
+  AdamTable<true> with_copy;
+  AdamTable<false> alone;
+  adamw_scalars(with_copy, o, step, square_sum);
+  adamw_scalars(alone, o, step, square_sum);
+  if (int rc = adamw_types<float, true>(tensors, count, with_copy, stream)) return rc;
+  if (int rc = adamw_types<float, false>(tensors, count, alone, stream)) return rc;
+  return adamw_types<bf16, false>(tensors, count, alone, stream);
+}
+
+int adamw(const char* who, const sr_adamw_tensor* tensors, const int64_t* steps, int32_t count,
+          const sr_adamw_options* o, const sr_norm* n, hipStream_t stream) try {
   if (count < 0 || (count > 0 && tensors == nullptr) || o == nullptr) return fail(SR_EINVAL, "%s: null argument", who);
   if (!(o->lr >= 0) || !std::isfinite(o->lr) || !(o->eps >= 0) || !(o->weight_decay >= 0) || !(o->beta1 >= 0) ||
-      !(o->beta1 < 1) || !(o->beta2 >= 0) || !(o->beta2 < 1) || o->step < 1)
+      !(o->beta1 < 1) || !(o->beta2 >= 0) || !(o->beta2 < 1) || (steps == nullptr && o->step < 1))
     return fail(SR_EINVAL, "%s: lr %g, betas %g and %g, eps %g, weight_decay %g, step %lld", who, o->lr, o->beta1,
                 o->beta2, o->eps, o->weight_decay, (long long)o->step);
   if (n != nullptr && !(o->max_norm >= 0)) return fail(SR_EINVAL, "%s: max_norm %g", who, o->max_norm);
@@ -685,6 +698,7 @@ int adamw(const char* who, const sr_adamw_tensor* tensors, int32_t count, const 
   for (int32_t i = 0; i < count; ++i) {
     const sr_adamw_tensor& x = tensors[i];
     if (x.reserved != 0) return fail(SR_EINVAL, "%s: tensors[%d].reserved is not 0", who, i);
+    if (steps != nullptr && steps[i] < 1) return fail(SR_EINVAL, "%s: steps[%d] is %lld", who, i, (long long)steps[i]);
     for (int32_t dt : {x.weight_dtype, x.moment_dtype, x.grad_dtype})
       if (dt != SR_DT_F32 && dt != SR_DT_BF16) return fail(SR_EDTYPE, "%s: tensors[%d]: dtype %d", who, i, dt);
     if (x.param != nullptr && x.weight_dtype != SR_DT_F32)
@@ -723,13 +737,20 @@ int adamw(const char* who, const sr_adamw_tensor* tensors, int32_t count, const 
       if (int rc = launch_norm(who, square_sum, n->norm, stream)) return rc;
     }
   }
-  AdamTable<true> with_copy;
-  AdamTable<false> alone;
-  adamw_scalars(with_copy, *o, square_sum);
-  adamw_scalars(alone, *o, square_sum);
-  if (int rc = adamw_types<float, true>(tensors, count, with_copy, stream)) return rc;
-  if (int rc = adamw_types<float, false>(tensors, count, alone, stream)) return rc;
-  return adamw_types<bf16, false>(tensors, count, alone, stream);
+  if (steps == nullptr) return launch_adamw(tensors, count, *o, o->step, square_sum, stream);
+  if (std::adjacent_find(steps, steps + count, std::not_equal_to<int64_t>()) == steps + count)
+    return count ? launch_adamw(tensors, count, *o, steps[0], square_sum, stream) : int(SR_OK);
+  // the tensors of one step after those of another, each in launches of its own
+  std::vector<int32_t> order(size_t(count), 0);
+  for (int32_t i = 0; i < count; ++i) order[i] = i;
+  std::stable_sort(order.begin(), order.end(), [&](int32_t a, int32_t b) { return steps[a] < steps[b]; });
+  std::vector<sr_adamw_tensor> sorted;
+  for (int32_t i : order) sorted.push_back(tensors[i]);
+  for (int32_t from = 0, to; from < count; from = to) {
+    for (to = from; to < count && steps[order[to]] == steps[order[from]];) ++to;
+    if (int rc = launch_adamw(&sorted[from], to - from, *o, steps[order[from]], square_sum, stream)) return rc;
+  }
+  return SR_OK;
 } catch (const std::bad_alloc&) {
   return fail(SR_ENOMEM, "%s: out of host memory", who);
 }
@@ -767,12 +788,12 @@ int sr_clip_norm(const sr_array* src, const sr_array* dst, int32_t count, float 
 int sr_adamw(const sr_adamw_tensor* tensors, int32_t count, const sr_adamw_options* o, const double* square_sum,
              hipStream_t stream) {
   const sr_norm given{square_sum, nullptr, nullptr, 0, nullptr};
-  return adamw("sr_adamw", tensors, count, o, square_sum ? &given : nullptr, stream);
+  return adamw("sr_adamw", tensors, nullptr, count, o, square_sum ? &given : nullptr, stream);
 }
 
-int sr_adamw_norm(const sr_adamw_tensor* tensors, int32_t count, const sr_adamw_options* o, const sr_norm* norm,
-                  hipStream_t stream) {
-  return adamw("sr_adamw_norm", tensors, count, o, norm, stream);
+int sr_adamw_norm(const sr_adamw_tensor* tensors, const int64_t* steps, int32_t count, const sr_adamw_options* o,
+                  const sr_norm* norm, hipStream_t stream) {
+  return adamw("sr_adamw_norm", tensors, steps, count, o, norm, stream);
 }
 
 }  // extern "C"

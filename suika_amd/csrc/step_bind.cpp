@@ -9,6 +9,7 @@
 
 #include <cstdint>
 #include <string>
+#include <unordered_map>
 #include <vector>
 
 #include "host_errors.h"
@@ -226,7 +227,9 @@ at::Tensor clip_grads(py::object grads, double max_norm, py::object outs, py::ob
 // The state that an optimizer steps: the tensors, in the order of its names.
 class AdamWState {
  public:
-  AdamWState(py::object weight, py::object exp_avg, py::object exp_avg_sq, py::object param, std::vector<std::string> names)
+  // `steps`: how many updates each parameter has had.
+  AdamWState(py::object weight, py::object exp_avg, py::object exp_avg_sq, py::object param, std::vector<std::string> names,
+             std::vector<int64_t> steps)
       : names_(std::move(names)) {
     const Fast w(weight, "weight"), m(exp_avg, "exp_avg"), v(exp_avg_sq, "exp_avg_sq"), p(param, "param");
     if (w.size() != names_.size() || m.size() != w.size() || v.size() != w.size() || p.size() != w.size())
@@ -238,17 +241,34 @@ class AdamWState {
       param_.push_back(p[i] == Py_None ? at::Tensor() : tensor_of(p[i], names_[i] + "/param"));
       check_fields(i);
     }
+    // names of one tensor count its updates together
+    std::unordered_map<const void*, size_t> first;
+    for (size_t i = 0; i < names_.size(); ++i)
+      counted_.push_back(first.emplace(weight_[i].unsafeGetTensorImpl(), i).first->second);
+    set_steps(std::move(steps));
+  }
+
+  std::vector<int64_t> steps() const {
+    std::vector<int64_t> all;
+    for (size_t i : counted_) all.push_back(steps_[i]);
+    return all;
+  }
+  void set_steps(std::vector<int64_t> steps) {
+    if (steps.size() != names_.size()) plan_error("steps: one of each parameter is wanted");
+    steps_ = std::move(steps);
   }
 
   // One update; the gradients' norm, or None without clipping.
-  py::object step(py::object grads, int64_t step, double lr, double beta1, double beta2, double eps,
+  py::object step(py::object grads, double lr, double beta1, double beta2, double eps,
                   double weight_decay, py::object max_norm, py::object square_sum) {
     const Fast list(grads, "grads");
     if (list.size() != names_.size())
       plan_error("grads: " + std::to_string(list.size()) + " tensors for a state of " + std::to_string(names_.size()));
     std::vector<sr_adamw_tensor> tensors;
     std::vector<sr_array> arrays;
+    std::vector<int64_t> numbers;
     tensors.reserve(names_.size());
+    numbers.reserve(names_.size());
     for (size_t i = 0; i < names_.size(); ++i) {
       if (list[i] == Py_None) continue;
       if (!THPVariable_Check(list[i])) plan_error("gradient of " + names_[i] + ": not a tensor");
@@ -265,11 +285,12 @@ class AdamWState {
       tensors.push_back({w.data_ptr(), m.data_ptr(), v.data_ptr(), p.defined() ? p.data_ptr() : nullptr, g.data_ptr(),
                          uint64_t(w.numel()), w.scalar_type() == at::kFloat ? SR_DT_F32 : SR_DT_BF16,
                          m.scalar_type() == at::kFloat ? SR_DT_F32 : SR_DT_BF16, gc, 0});
+      numbers.push_back(steps_[counted_[i]] + 1);
       if (!max_norm.is_none() && square_sum.is_none()) arrays.push_back({g.data_ptr(), uint64_t(g.numel()), gc, 0});
     }
     const at::Device device = device_ ? *device_ : current_device();
     const c10::DeviceGuard guard(device);
-    sr_adamw_options o{lr, beta1, beta2, eps, weight_decay, step, 0.0};
+    sr_adamw_options o{lr, beta1, beta2, eps, weight_decay, 1, 0.0};     // the tensors have their own numbers
     c10::optional<SumWork> work;
     sr_norm by{};
     at::Tensor norm;
@@ -281,11 +302,12 @@ class AdamWState {
     } else if (!square_sum.is_none()) {
       plan_error("square_sum is given without max_norm");
     }
-    check(sr_adamw_norm(tensors.data(), int32_t(tensors.size()), &o, max_norm.is_none() ? nullptr : &by,
-                        stream_of(device)),
+    check(sr_adamw_norm(tensors.data(), numbers.data(), int32_t(tensors.size()), &o,
+                        max_norm.is_none() ? nullptr : &by, stream_of(device)),
           "sr_adamw_norm");
     for (size_t i = 0; i < names_.size(); ++i) {
       if (list[i] == Py_None) continue;
+      ++steps_[counted_[i]];
       for (const at::Tensor* t : {&weight_[i], &exp_avg_[i], &exp_avg_sq_[i], &param_[i]})
         if (t->defined()) written(*t);
     }
@@ -318,6 +340,8 @@ class AdamWState {
 
   std::vector<std::string> names_;
   std::vector<at::Tensor> weight_, exp_avg_, exp_avg_sq_, param_;
+  std::vector<size_t> counted_;     // the first parameter that has this one's weight
+  std::vector<int64_t> steps_;      // updates so far, of counted_[i]
   c10::optional<at::Device> device_;
 };
 
@@ -493,9 +517,11 @@ void bind_step(py::module_& m) {
   m.def("grad_norm", &grad_norm, py::arg("grads"));
   m.def("clip_grads", &clip_grads, py::arg("grads"), py::arg("max_norm"), py::arg("out"), py::arg("square_sum"));
   py::class_<AdamWState>(m, "AdamWState", "The tensors of a state that AdamW updates in place")
-      .def(py::init<py::object, py::object, py::object, py::object, std::vector<std::string>>(), py::arg("weight"),
-           py::arg("exp_avg"), py::arg("exp_avg_sq"), py::arg("param"), py::arg("names"))
-      .def("step", &AdamWState::step, py::arg("grads"), py::arg("step"), py::arg("lr"), py::arg("beta1"),
+      .def(py::init<py::object, py::object, py::object, py::object, std::vector<std::string>, std::vector<int64_t>>(),
+           py::arg("weight"), py::arg("exp_avg"), py::arg("exp_avg_sq"), py::arg("param"), py::arg("names"),
+           py::arg("steps"))
+      .def_property("steps", &AdamWState::steps, &AdamWState::set_steps)
+      .def("step", &AdamWState::step, py::arg("grads"), py::arg("lr"), py::arg("beta1"),
            py::arg("beta2"), py::arg("eps"), py::arg("weight_decay"), py::arg("max_norm"), py::arg("square_sum"));
   m.def("vocab_embedding", &vocab_embedding, py::arg("tokens"), py::arg("weight"), py::arg("scale"),
         py::arg("vocab_start"), py::arg("out"));

@@ -101,10 +101,14 @@ class ShardAdamW:
     float32 or bfloat16, is the weight itself.  The moments are both float32
     or both bfloat16.  Everything is computed in 32 bits and rounded where it
     is stored.  The optimizer keeps the tensors (an entry replaced in the dict
-    later is not seen); ``step`` fields, which have to agree, are where it
-    starts to count.
+    later is not seen).
 
-    The update of step t, with g clipped: ``exp_avg = beta1 exp_avg +
+    Every parameter counts its own updates, from its ``step`` field on (where
+    it has none: from the others' if they agree, else from 0), and one that
+    gets no gradient does not count, as in ``torch.optim.AdamW``.  Names of one
+    tensor count together, so their ``step`` fields have to agree.
+
+    A parameter's update t, with g clipped: ``exp_avg = beta1 exp_avg +
     (1 - beta1) g``; ``exp_avg_sq = beta2 exp_avg_sq + (1 - beta2) g^2``;
     ``w = w (1 - lr weight_decay) - lr / (1 - beta1^t) exp_avg /
     (sqrt(exp_avg_sq / (1 - beta2^t)) + eps)``.
@@ -115,8 +119,8 @@ class ShardAdamW:
         self.lr, self.betas, self.eps, self.weight_decay = lr, tuple(betas), eps, weight_decay
         self.names = list(state)
         self._state = state
-        steps = set()
         weight, param = [], []
+        counts: Dict[int, Tuple[str, int]] = {}      # of a tensor: a name of it, and its updates
         for name, entry in state.items():
             for f in ("param", "exp_avg", "exp_avg_sq"):
                 if f not in entry:
@@ -125,18 +129,30 @@ class ShardAdamW:
             weight.append(entry["param"] if master is None else master)
             param.append(None if master is None else entry["param"])
             if "step" in entry:
-                steps.add(int(entry["step"]))
-        if len(steps) > 1:
-            raise PlanError(f"the state's steps differ: {sorted(steps)}")
-        self.steps = steps.pop() if steps else 0
+                step = int(entry["step"])
+                other, count = counts.setdefault(id(weight[-1]), (name, step))
+                if count != step:
+                    raise PlanError(f"{other} and {name} are one tensor, but their steps differ: {count} and {step}")
+        known = {count for _, count in counts.values()}
+        rest = ("", known.pop() if len(known) == 1 else 0)
         self._native = _lib.host().AdamWState(weight, [e["exp_avg"] for e in state.values()],
-                                              [e["exp_avg_sq"] for e in state.values()], param, self.names)
+                                              [e["exp_avg_sq"] for e in state.values()], param, self.names,
+                                              [counts.get(id(w), rest)[1] for w in weight])
+
+    @property
+    def steps(self) -> int:
+        """The most updates that a parameter has had; setting it sets all."""
+        return max(self._native.steps, default=0)
+
+    @steps.setter
+    def steps(self, count: int) -> None:
+        self._native.steps = [count] * len(self.names)
 
     def step(self, grads: Union[Grads, Mapping[str, Optional[Tensor]]], *, max_norm: Optional[float] = None,
              square_sum: Optional[Tensor] = None) -> Optional[Tensor]:
         """One update by ``grads``: contiguous float32 or bfloat16 tensors in the
         order of ``names``, or by name; a parameter whose gradient is ``None``
-        or missing keeps its state.
+        or missing keeps its state, its step included.
 
         With ``max_norm`` the gradients count as clipped to it
         (``clip_grads``; they are not written) and their norm is returned, a
@@ -149,18 +165,20 @@ class ShardAdamW:
             if unknown:
                 raise PlanError(f"gradients of unknown parameters: {sorted(unknown)[:4]}")
             grads = [grads.get(n) for n in self.names]
-        norm = self._native.step(grads, self.steps + 1, self.lr, self.betas[0], self.betas[1], self.eps,
-                                 self.weight_decay, max_norm, square_sum)
-        self.steps += 1
-        return norm
+        return self._native.step(grads, self.lr, self.betas[0], self.betas[1], self.eps, self.weight_decay, max_norm,
+                                 square_sum)
 
     def state(self) -> Dict[str, Dict[str, Tensor]]:
-        """The state with its ``step`` fields brought up to date: the source of
-        the next ``execute_param_transfer``."""
-        for entry in self._state.values():
+        """The state with its ``step`` fields brought up to date, each to its
+        parameter's count: the source of the next ``execute_param_transfer``."""
+        written: Dict[int, int] = {}
+        for name, count in zip(self.names, self._native.steps):
+            entry = self._state[name]
             old = entry.get("step")
-            if isinstance(old, Tensor):
-                old.fill_(self.steps)
-            else:
-                entry["step"] = torch.tensor(float(self.steps))
+            if not isinstance(old, Tensor):
+                entry["step"] = torch.tensor(float(count))
+            elif written.setdefault(id(old), count) == count:
+                old.fill_(count)
+            else:       # the same tensor as another entry's, which has had other updates
+                entry["step"] = torch.full_like(old, count)
         return self._state

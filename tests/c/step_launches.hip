@@ -131,25 +131,71 @@ void refusals() {
   expect(sr_clip_norm(good, nullptr, 2, 1.0f, &small, nullptr), SR_EINVAL, 0, "clip: no place for the sum");
 
   sr_adamw_tensor t{at(M), at(2 * M), at(3 * M), nullptr, at(4 * M), 100000, SR_DT_F32, SR_DT_F32, SR_DT_F32, 0};
-  expect(sr_adamw_norm(&t, 1, &kOptions, &norm, nullptr), SR_OK, 3, "adamw");
-  expect(sr_adamw_norm(&t, 1, &kOptions, nullptr, nullptr), SR_OK, 1, "adamw without clipping");
+  expect(sr_adamw_norm(&t, nullptr, 1, &kOptions, &norm, nullptr), SR_OK, 3, "adamw");
+  expect(sr_adamw_norm(&t, nullptr, 1, &kOptions, nullptr, nullptr), SR_OK, 1, "adamw without clipping");
   sr_norm given = {static_cast<const double*>(at(64)), nullptr, nullptr, 0, static_cast<float*>(at(96))};
-  expect(sr_adamw_norm(&t, 1, &kOptions, &given, nullptr), SR_OK, 2, "adamw by a given sum");
+  expect(sr_adamw_norm(&t, nullptr, 1, &kOptions, &given, nullptr), SR_OK, 2, "adamw by a given sum");
   given.norm = nullptr;
-  expect(sr_adamw_norm(&t, 1, &kOptions, &given, nullptr), SR_OK, 1, "adamw by a given sum alone");
-  expect(sr_adamw_norm(&t, 1, &kOptions, &small, nullptr), SR_EINVAL, 0, "adamw: no place for the sum");
+  expect(sr_adamw_norm(&t, nullptr, 1, &kOptions, &given, nullptr), SR_OK, 1, "adamw by a given sum alone");
+  expect(sr_adamw_norm(&t, nullptr, 1, &kOptions, &small, nullptr), SR_EINVAL, 0, "adamw: no place for the sum");
   sr_adamw_options o = kOptions;
   o.lr = -1;
-  expect(sr_adamw_norm(&t, 1, &o, &norm, nullptr), SR_EINVAL, 0, "adamw: lr");
+  expect(sr_adamw_norm(&t, nullptr, 1, &o, &norm, nullptr), SR_EINVAL, 0, "adamw: lr");
   o = kOptions;
   o.max_norm = -1;
-  expect(sr_adamw_norm(&t, 1, &o, &norm, nullptr), SR_EINVAL, 0, "adamw: max_norm");
+  expect(sr_adamw_norm(&t, nullptr, 1, &o, &norm, nullptr), SR_EINVAL, 0, "adamw: max_norm");
   o.max_norm = 1;
   const sr_adamw_tensor both[2] = {t, t};
-  expect(sr_adamw_norm(both, 2, &o, &norm, nullptr), SR_EOVERLAP, 0, "adamw: listed twice");
+  expect(sr_adamw_norm(both, nullptr, 2, &o, &norm, nullptr), SR_EOVERLAP, 0, "adamw: listed twice");
   model::capturing = true;
-  expect(sr_adamw_norm(&t, 1, &o, &norm, nullptr), SR_EINVAL, 0, "adamw: captured");
+  expect(sr_adamw_norm(&t, nullptr, 1, &o, &norm, nullptr), SR_EINVAL, 0, "adamw: captured");
   expect(sr_clip_norm(good, nullptr, 2, 1.0f, &norm, nullptr), SR_OK, 5, "clip: captured");
+}
+
+template <bool COPY>
+const AdamTable<COPY>& table(size_t i) { return *reinterpret_cast<const AdamTable<COPY>*>(launches[i].table.data()); }
+
+bool near(float got, double want) { return std::fabs(got - want) <= std::fabs(want) * 1e-7; }
+
+// Tensors of other update numbers get their own bias corrections: launches by
+// number, within one by type.
+void steps() {
+  const uint64_t M = 1 << 24;
+  std::vector<sr_adamw_tensor> t;
+  const int64_t numbers[6] = {7, 1, 7, 1000, 1, 7};
+  for (int i = 0; i < 6; ++i) {
+    const uint64_t b = uint64_t(i + 1) * M;
+    t.push_back({at(b), at(b + 65536), at(b + 131072), i == 2 ? at(b + 196608) : nullptr, at(b + 262144), uint64_t(100 + i),
+                 SR_DT_F32, SR_DT_F32, SR_DT_F32, 0});
+  }
+  if (sr_adamw_norm(t.data(), numbers, 6, &kOptions, nullptr, nullptr) != SR_OK) die("steps");
+  // 1: two tensors; 7: one with a copy, two without; 1000: one
+  const struct { int64_t step; std::vector<int> tensors; } want[4] = {{1, {1, 4}}, {7, {2}}, {7, {0, 5}}, {1000, {3}}};
+  if (launches.size() != 4) die("launches by number and type");
+  for (int k = 0; k < 4; ++k) {
+    const double c1 = 1 - std::pow(0.9, double(want[k].step)), c2 = 1 - std::pow(0.99, double(want[k].step));
+    const auto check = [&](const auto& tab) {
+      if (!near(tab.step_size, 1e-3 / c1) || !near(tab.root_scale, 1 / std::sqrt(c2))) die("bias corrections");
+      if (tab.at.count != want[k].tensors.size()) die("tensors of a launch");
+      for (size_t j = 0; j < want[k].tensors.size(); ++j) {
+        const sr_adamw_tensor& x = t[size_t(want[k].tensors[j])];
+        if (tab.entry[j].weight != reinterpret_cast<uint64_t>(x.weight) || tab.tail[j] != x.n) die("another tensor");
+      }
+    };
+    if (k == 1) check(table<true>(1));
+    else check(table<false>(size_t(k)));
+  }
+  launches.clear();
+  const int64_t same[6] = {7, 7, 7, 7, 7, 7};
+  expect(sr_adamw_norm(t.data(), same, 6, &kOptions, nullptr, nullptr), SR_OK, 2, "one number");
+  const int64_t none[6] = {7, 7, 0, 7, 7, 7};
+  expect(sr_adamw_norm(t.data(), none, 6, &kOptions, nullptr, nullptr), SR_EINVAL, 0, "a number below 1");
+  sr_adamw_options o = kOptions;
+  o.step = 0;       // not used beside numbers
+  expect(sr_adamw_norm(t.data(), same, 6, &o, nullptr, nullptr), SR_OK, 2, "numbers alone");
+  expect(sr_adamw_norm(t.data(), nullptr, 6, &o, nullptr, nullptr), SR_EINVAL, 0, "no number");
+  expect(sr_adamw_norm(nullptr, nullptr, 0, &kOptions, nullptr, nullptr), SR_OK, 0, "nothing");
+  expect(sr_adamw_norm(nullptr, none, 0, &kOptions, nullptr, nullptr), SR_OK, 0, "nothing, with numbers");
 }
 
 }  // namespace
@@ -157,6 +203,7 @@ void refusals() {
 int main(int argc, char** argv) {
   const char* scenario = argc > 1 ? argv[1] : "";
   if (!std::strcmp(scenario, "refusals")) refusals();
+  else if (!std::strcmp(scenario, "steps")) steps();
   else die("no such scenario");
   std::printf("ok\n");
   return 0;

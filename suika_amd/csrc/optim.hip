@@ -35,9 +35,9 @@ constexpr int kThreads = 256;
 // A table of 4 KB, less the 256 bytes of arguments that the compiler adds.
 constexpr size_t kTableBytes = 3832;
 
-// Most chunks of one launch: the grid's threads stay below 2^32.
-constexpr uint32_t kMostChunks = 1u << 23;
-static_assert(SR_STEP_MAX_ELEMENTS / 2048 <= kMostChunks, "an array fits into a launch");
+// Most chunks of one launch: a grid has fewer than 2^32 threads, with 512 of
+// them a chunk and chunks rounded up to the dies half of that.
+constexpr uint32_t kMostChunks = 1u << 22;
 
 // Where the chunks of a table's entries start.
 template <int ENTRIES>
@@ -122,6 +122,7 @@ struct SumTable {
   Chunks<kSumEntries> at;
 };
 static_assert(sizeof(SumTable) <= kTableBytes, "kernel arguments");
+static_assert(SR_STEP_MAX_ELEMENTS / kSumChunk <= kMostChunks, "an array fits into a launch");
 
 constexpr int kFinishThreads = 1024;
 
@@ -248,6 +249,8 @@ struct ClipTable {
   float* norm;
 };
 static_assert(sizeof(ClipTable) <= kTableBytes, "kernel arguments");
+static_assert(SR_STEP_MAX_ELEMENTS / kClipChunk <= kMostChunks, "an array fits into a launch");
+static_assert(uint64_t(kMostChunks) * kThreads < uint64_t(1) << 32, "a grid's threads");
 
 // min(1, max_norm / (norm + 1e-6)); NaN stays NaN.
 __device__ __forceinline__ float clip_factor(double square_sum, float max_norm) {
@@ -295,6 +298,8 @@ __global__ __launch_bounds__(kThreads) void clip_kernel(ClipTable t) {
 
 constexpr int kAdamThreads = 512;
 constexpr uint32_t kAdamChunk = 2048;
+constexpr uint64_t kAdamPart = uint64_t(kMostChunks) * kAdamChunk;     // elements of one entry: longer arrays have several
+static_assert(uint64_t(kMostChunks + kXcds) * kAdamThreads < uint64_t(1) << 32, "a grid's threads");
 
 // What a table holds of one parameter; without a copy of the weight, one
 // address less.
@@ -495,17 +500,20 @@ int adamw_launches(const sr_adamw_tensor* tensors, int32_t count, AdamTable<COPY
     if (x.n == 0 || x.weight_dtype != weight || x.moment_dtype != moment || x.grad_dtype != grad ||
         (x.param != nullptr) != COPY)
       continue;
-    if (!t.at.room(x.n, kAdamChunk)) {
-      if (int rc = flush()) return rc;
+    for (uint64_t from = 0; from < x.n; from += kAdamPart) {
+      const uint64_t n = std::min(x.n - from, kAdamPart);
+      if (!t.at.room(n, kAdamChunk)) {
+        if (int rc = flush()) return rc;
+      }
+      const uint32_t k = t.at.add(n, kAdamChunk);
+      auto& e = t.entry[k];
+      e.weight = reinterpret_cast<uint64_t>(x.weight) + from * sizeof(W);
+      e.exp_avg = reinterpret_cast<uint64_t>(x.exp_avg) + from * sizeof(M);
+      e.exp_avg_sq = reinterpret_cast<uint64_t>(x.exp_avg_sq) + from * sizeof(M);
+      e.grad = reinterpret_cast<uint64_t>(x.grad) + from * sizeof(G);
+      if constexpr (COPY) e.param = reinterpret_cast<uint64_t>(x.param) + from * sizeof(bf16);
+      t.tail[k] = uint16_t(n - (n - 1) / kAdamChunk * kAdamChunk);
     }
-    const uint32_t k = t.at.add(x.n, kAdamChunk);
-    auto& e = t.entry[k];
-    e.weight = reinterpret_cast<uint64_t>(x.weight);
-    e.exp_avg = reinterpret_cast<uint64_t>(x.exp_avg);
-    e.exp_avg_sq = reinterpret_cast<uint64_t>(x.exp_avg_sq);
-    e.grad = reinterpret_cast<uint64_t>(x.grad);
-    if constexpr (COPY) e.param = reinterpret_cast<uint64_t>(x.param);
-    t.tail[k] = uint16_t(x.n - (x.n - 1) / kAdamChunk * kAdamChunk);
   }
   return flush();
 }

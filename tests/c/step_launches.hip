@@ -103,7 +103,11 @@ void* at(uint64_t offset) { return reinterpret_cast<void*>(kBase + offset); }
 
 const sr_adamw_options kOptions = {1e-3, 0.9, 0.99, 1e-8, 0.1, 1, 1.0};
 
-sr_norm own_norm() { return {nullptr, static_cast<double*>(at(64)), at(128), 1 << 20, static_cast<float*>(at(96))}; }
+// The sum, the norm and a workspace, below all arrays.
+const uint64_t kSum = -(uint64_t(1) << 21) + 64, kNorm = kSum + 32, kWork = kSum + 64;
+sr_norm own_norm() {
+  return {nullptr, static_cast<double*>(at(kSum)), at(kWork), 1 << 20, static_cast<float*>(at(kNorm))};
+}
 
 void expect(int rc, int want, size_t n, const char* what) {
   if (rc != want || launches.size() != n) {
@@ -133,7 +137,7 @@ void refusals() {
   sr_adamw_tensor t{at(M), at(2 * M), at(3 * M), nullptr, at(4 * M), 100000, SR_DT_F32, SR_DT_F32, SR_DT_F32, 0};
   expect(sr_adamw_norm(&t, nullptr, 1, &kOptions, &norm, nullptr), SR_OK, 3, "adamw");
   expect(sr_adamw_norm(&t, nullptr, 1, &kOptions, nullptr, nullptr), SR_OK, 1, "adamw without clipping");
-  sr_norm given = {static_cast<const double*>(at(64)), nullptr, nullptr, 0, static_cast<float*>(at(96))};
+  sr_norm given = {norm.sum, nullptr, nullptr, 0, norm.norm};
   expect(sr_adamw_norm(&t, nullptr, 1, &kOptions, &given, nullptr), SR_OK, 2, "adamw by a given sum");
   given.norm = nullptr;
   expect(sr_adamw_norm(&t, nullptr, 1, &kOptions, &given, nullptr), SR_OK, 1, "adamw by a given sum alone");
@@ -198,12 +202,69 @@ void steps() {
   expect(sr_adamw_norm(nullptr, none, 0, &kOptions, nullptr, nullptr), SR_OK, 0, "nothing, with numbers");
 }
 
+// Launches of the largest arrays: grids stay below 2^32 threads, and the tables
+// name every element once.
+void expect_grids(const char* what) {
+  for (const model::Launch& l : launches)
+    if (l.blocks == 0 || l.blocks * l.threads >= uint64_t(1) << 32) {
+      std::printf("a grid of %llu blocks of %llu\n", (unsigned long long)l.blocks, (unsigned long long)l.threads);
+      die(what);
+    }
+}
+
+void grids() {
+  const uint64_t most = SR_STEP_MAX_ELEMENTS, far = uint64_t(1) << 37;
+  const std::vector<std::vector<uint64_t>> lists = {
+      {most}, {most - 1}, {most - 2048 * 7}, {most - 2048 * 8}, {most / 2}, {most / 2 + 1}, {5, most, 2049},
+      {most / 2 - 1, most / 2}, std::vector<uint64_t>(16, most / 16), std::vector<uint64_t>(17, most / 16)};
+  for (const auto& list : lists) {
+    std::vector<sr_adamw_tensor> t;
+    std::vector<sr_array> a;
+    for (uint64_t n : list) {
+      const uint64_t b = 4 * far * t.size();
+      t.push_back({at(b), at(b + far), at(b + 2 * far), nullptr, at(b + 3 * far), n, SR_DT_BF16, SR_DT_BF16, SR_DT_BF16, 0});
+      a.push_back({at(b), n, SR_DT_F32, 0});
+    }
+    const int32_t count = int32_t(t.size());
+    launches.clear();
+    if (sr_adamw(t.data(), count, &kOptions, nullptr, nullptr) != SR_OK) die("adamw");
+    expect_grids("adamw");
+    size_t tensor = 0;
+    uint64_t done = 0;        // elements of it that were named
+    for (size_t l = 0; l < launches.size(); ++l) {
+      const AdamTable<false>& tab = table<false>(l);
+      if (launches[l].blocks < tab.at.chunks) die("fewer workgroups than chunks");
+      for (uint32_t e = 0; e < tab.at.count; ++e) {
+        const uint32_t to = e + 1 < tab.at.count ? tab.at.first[e + 1] : tab.at.chunks;
+        const uint64_t n = uint64_t(to - tab.at.first[e] - 1) * kAdamChunk + tab.tail[e];
+        const sr_adamw_tensor& x = t[tensor];
+        const uint64_t shift = done * 2;
+        if (tab.entry[e].weight != reinterpret_cast<uint64_t>(x.weight) + shift ||
+            tab.entry[e].exp_avg != reinterpret_cast<uint64_t>(x.exp_avg) + shift ||
+            tab.entry[e].exp_avg_sq != reinterpret_cast<uint64_t>(x.exp_avg_sq) + shift ||
+            tab.entry[e].grad != reinterpret_cast<uint64_t>(x.grad) + shift || tab.tail[e] > kAdamChunk)
+          die("another place");
+        done += n;
+        if (done > x.n) die("beyond a tensor");
+        if (done == x.n) ++tensor, done = 0;
+      }
+    }
+    if (tensor != t.size() || done) die("elements that no launch takes");
+    launches.clear();
+    const sr_norm norm = own_norm();
+    if (sr_clip_norm(a.data(), nullptr, count, 1.0f, &norm, nullptr) != SR_OK) die("clip");
+    expect_grids("clip");
+    launches.clear();
+  }
+}
+
 }  // namespace
 
 int main(int argc, char** argv) {
   const char* scenario = argc > 1 ? argv[1] : "";
   if (!std::strcmp(scenario, "refusals")) refusals();
   else if (!std::strcmp(scenario, "steps")) steps();
+  else if (!std::strcmp(scenario, "grids")) grids();
   else die("no such scenario");
   std::printf("ok\n");
   return 0;

@@ -22,7 +22,7 @@ def model(tmp_path_factory):
     return out / "model"
 
 
-@pytest.mark.parametrize("scenario", ["refusals", "steps"])
+@pytest.mark.parametrize("scenario", ["refusals", "steps", "grids"])
 def test_scenario(model, scenario):
     res = subprocess.run([str(model), scenario], capture_output=True, text=True, timeout=60)
     assert res.returncode == 0 and res.stdout.endswith("ok\n"), res.stdout + res.stderr

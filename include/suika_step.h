@@ -16,7 +16,7 @@
  *       rows of a vocabulary shard for the tokens that lie in it, and the
  *       gradient of its rows.  In the reference the embedding is an
  *       nn.Embedding (Suika/models/llama_model.py:108-157)
- *   sr_logprob, sr_logprob_grad
+ *   sr_logprob, sr_logprob_grad, sr_logprob_pair, sr_logprob_pair_grad
  *       log probabilities of given tokens, entropy and the best alternatives
  *       from the head's logits, and the gradient of the logits
  *
@@ -196,10 +196,24 @@ int sr_logprob(const sr_logprob_shape* shape, int32_t top, float* logprob, float
  * all -inf, and for the first term in rows that are not scored.  g_logprob or
  * g_entropy may be NULL (0).  grad has the logits' type and rows of
  * grad_stride elements; it may be the logits themselves, and overlaps no
- * other input (SR_EOVERLAP).  lse is a float32, so p_j is exact to |lse| 2^-24.
+ * other input (SR_EOVERLAP).  lse is rounded to a float32: beside the error of
+ * the sum and of the exponential, p_j is off by up to |lse| 2^-24 of itself, so
+ * logits of a large common offset want the pair below.
  */
 int sr_logprob_grad(const sr_logprob_shape* shape, const float* lse, const float* entropy, const float* g_logprob,
                     const float* g_entropy, void* grad, uint64_t grad_stride, hipStream_t stream);
+
+/*
+ * The same with the log of the sum as two floats: lse_low is what the rounding
+ * of lse lost (0 where lse is not finite), and p_j = exp((x_j - lse) - lse_low)
+ * does not depend on a common offset of the logits.
+ */
+int sr_logprob_pair(const sr_logprob_shape* shape, int32_t top, float* logprob, float* entropy, float* lse,
+                    float* lse_low, float* top_logprob, int64_t* top_index, void* workspace, uint64_t workspace_bytes,
+                    hipStream_t stream);
+int sr_logprob_pair_grad(const sr_logprob_shape* shape, const float* lse, const float* lse_low, const float* entropy,
+                         const float* g_logprob, const float* g_entropy, void* grad, uint64_t grad_stride,
+                         hipStream_t stream);
 
 #ifdef __cplusplus
 }

@@ -89,6 +89,8 @@ EXPORTED_SYMBOLS = (
     "sr_logprob_workspace",
     "sr_logprob",
     "sr_logprob_grad",
+    "sr_logprob_pair",
+    "sr_logprob_pair_grad",
 )
 
 # Largest hand-off allocation (SR_HANDOFF_MAX_BYTES, include/suika_handoff.h).

@@ -464,11 +464,21 @@ struct Outputs {
   float* logprob;
   float* entropy;
   float* lse;
+  float* lse_low;       // or null
   float* top_logprob;
   int64_t* top_index;
 };
 
 __device__ __forceinline__ float logprob_of(float x, const Summary& r) { return (x - r.shift) - r.rest; }
+
+// What the rounding of lse = shift + rest lost, exactly (the two-sum of Knuth):
+// of logits that are large together, lse alone knows the probabilities to
+// |lse| 2^-24 of themselves only.
+__device__ __forceinline__ float low_of(const Summary& r) {
+  const float b = r.lse - r.shift;
+  const float low = (r.shift - (r.lse - b)) + (r.rest - b);
+  return fabsf(r.lse) < kInf ? low : 0.0f;
+}
 
 // Writes a row's results; sh.chosen holds the alternatives.
 __device__ __forceinline__ void put(Shared& sh, const Target& t, uint64_t i, int k, const Summary& r,
@@ -479,6 +489,7 @@ __device__ __forceinline__ void put(Shared& sh, const Target& t, uint64_t i, int
     out.logprob[i] = lp;
     out.entropy[i] = r.entropy;
     out.lse[i] = r.lse;
+    if (out.lse_low) out.lse_low[i] = low_of(r);
   }
   if (int(threadIdx.x) < k) {
     const uint64_t c = sh.chosen[threadIdx.x];
@@ -614,7 +625,7 @@ __global__ __launch_bounds__(kThreads) void parts_kernel(const T* logits, const 
 template <typename T, typename I>
 __global__ __launch_bounds__(kThreads) void grad_kernel(const T* logits, const I* targets, uint64_t stride,
                                                         uint32_t vocab, uint32_t columns, uint32_t spans,
-                                                        const float* lse, const float* entropy,
+                                                        const float* lse, const float* lse_low, const float* entropy,
                                                         const float* g_logprob, const float* g_entropy, T* grad,
                                                         uint64_t grad_stride) {
   constexpr int N = 16 / sizeof(T);
@@ -626,14 +637,16 @@ __global__ __launch_bounds__(kThreads) void grad_kernel(const T* logits, const I
   Vec<T, N> x;
   if (whole) x = __builtin_nontemporal_load(reinterpret_cast<const Vec<T, N>*>(row + c));
   const int64_t target = target_at(targets, i);
-  const float l = lse[i], h = entropy[i];
+  const float l = lse[i], low = lse_low ? lse_low[i] : 0.0f, h = entropy[i];
   const float gl = g_logprob && target >= 0 ? g_logprob[i] : 0.0f;
   const float gh = g_entropy ? g_entropy[i] : 0.0f;
-  const float base = fmaf(gh, h, gl);      // grad = [target] gl - p (gl + gh (ln p + h))
+  // grad = [target] gl - p (gl + gh (ln p + h)) with ln p = d - low; d = x - l is exact where x is within a factor
+  // of two of l
+  const float base = fmaf(-gh, low, fmaf(gh, h, gl)), low2 = low * kLog2e;
   const bool empty = l == -kInf;
   auto value = [&](float x, uint32_t c) {
     const float d = x - l;
-    const float p = exp2_fast(d * kLog2e);             // NaN stays NaN
+    const float p = exp2_fast(fmaf(d, kLog2e, -low2));             // NaN stays NaN
     float g = -p * fmaf(gh, fmaxf(d, -200.0f), base);
     if (int64_t(c) == target) g += gl;
     return empty || c >= vocab ? 0.0f : g;
@@ -712,45 +725,34 @@ void with_types(const sr_logprob_shape& s, F&& f) {
   else with_targets<f16>(s, f);
 }
 
-}  // namespace
-
-extern "C" {
-
-int sr_logprob_workspace(const sr_logprob_shape* shape, int32_t top, uint64_t* bytes) {
-  if (bytes == nullptr) return fail(SR_EINVAL, "sr_logprob_workspace: null argument");
-  if (int rc = check_shape("sr_logprob_workspace", shape)) return rc;
-  if (int rc = check_top("sr_logprob_workspace", *shape, top)) return rc;
-  *bytes = parts_of(*shape, top).bytes;
-  return SR_OK;
-}
-
-int sr_logprob(const sr_logprob_shape* shape, int32_t top, float* logprob, float* entropy, float* lse,
-               float* top_logprob, int64_t* top_index, void* workspace, uint64_t workspace_bytes, hipStream_t stream) {
-  uint64_t need = 0;
-  if (int rc = sr_logprob_workspace(shape, top, &need)) return rc;
+int logprobs(const char* who, const sr_logprob_shape* shape, int32_t top, const Outputs& out, bool pair, void* workspace,
+             uint64_t workspace_bytes, hipStream_t stream) {
+  if (int rc = check_shape(who, shape)) return rc;
+  if (int rc = check_top(who, *shape, top)) return rc;
+  const uint64_t need = parts_of(*shape, top).bytes;
   const sr_logprob_shape& s = *shape;
   if (s.rows == 0) return SR_OK;
-  if (!logprob || !entropy || !lse || (top && (!top_logprob || !top_index)))
-    return fail(SR_EINVAL, "sr_logprob: an output is null");
-  for (const float* p : {logprob, entropy, lse, top_logprob})
-    if (reinterpret_cast<uintptr_t>(p) % 4) return fail(SR_EALIGN, "sr_logprob: an output is not aligned");
-  if (reinterpret_cast<uintptr_t>(top_index) % 8) return fail(SR_EALIGN, "sr_logprob: an output is not aligned");
+  if (!out.logprob || !out.entropy || !out.lse || (pair && !out.lse_low) ||
+      (top && (!out.top_logprob || !out.top_index)))
+    return fail(SR_EINVAL, "%s: an output is null", who);
+  for (const float* p : {out.logprob, out.entropy, out.lse, out.lse_low, out.top_logprob})
+    if (reinterpret_cast<uintptr_t>(p) % 4) return fail(SR_EALIGN, "%s: an output is not aligned", who);
+  if (reinterpret_cast<uintptr_t>(out.top_index) % 8) return fail(SR_EALIGN, "%s: an output is not aligned", who);
   if (workspace_bytes < need || (need && workspace == nullptr))
-    return fail(SR_EINVAL, "sr_logprob: a workspace of %llu bytes, %llu are needed", (unsigned long long)workspace_bytes,
+    return fail(SR_EINVAL, "%s: a workspace of %llu bytes, %llu are needed", who, (unsigned long long)workspace_bytes,
                 (unsigned long long)need);
-  if (reinterpret_cast<uintptr_t>(workspace) % 16) return fail(SR_EALIGN, "sr_logprob: workspace not aligned");
-  const Extent written[] = {{logprob, s.rows * 4}, {entropy, s.rows * 4}, {lse, s.rows * 4},
-                            {top_logprob, top ? s.rows * top * 4 : 0}, {top_index, top ? s.rows * top * 8 : 0},
-                            {workspace, need}};
+  if (reinterpret_cast<uintptr_t>(workspace) % 16) return fail(SR_EALIGN, "%s: workspace not aligned", who);
+  const Extent written[] = {{out.logprob, s.rows * 4}, {out.entropy, s.rows * 4}, {out.lse, s.rows * 4},
+                            {out.lse_low, s.rows * 4}, {out.top_logprob, top ? s.rows * top * 4 : 0},
+                            {out.top_index, top ? s.rows * top * 8 : 0}, {workspace, need}};
   const Extent read[] = {{s.logits, ((s.rows - 1) * s.stride + s.columns) * sr_internal::dtype_size(s.dtype)},
                          {s.targets, s.rows * sr_internal::dtype_size(s.target_dtype)}};
   for (const Extent& w : written) {
     for (const Extent& o : written)
-      if (&o != &w && w.meets(o)) return fail(SR_EOVERLAP, "sr_logprob: two outputs overlap");
+      if (&o != &w && w.meets(o)) return fail(SR_EOVERLAP, "%s: two outputs overlap", who);
     for (const Extent& o : read)
-      if (w.meets(o)) return fail(SR_EOVERLAP, "sr_logprob: an output overlaps an input");
+      if (w.meets(o)) return fail(SR_EOVERLAP, "%s: an output overlaps an input", who);
   }
-  const Outputs out{logprob, entropy, lse, top_logprob, top_index};
   const Cut cut = parts_of(s, top);
   char* base = static_cast<char*>(workspace);
   const Parts parts{cut.parts, cut.length, reinterpret_cast<Stats*>(base), reinterpret_cast<uint64_t*>(base + cut.best)};
@@ -766,40 +768,80 @@ int sr_logprob(const sr_logprob_shape* shape, int32_t top, float* logprob, float
     else part_kernel<false><<<grid, kThreads, 0, stream>>>(logits, s.stride, vocab, 0, parts);
     parts_kernel<<<rows, kThreads, 0, stream>>>(logits, targets, s.stride, vocab, int(top), parts, out);
   });
-  return launched("sr_logprob");
+  return launched(who);
 }
 
-int sr_logprob_grad(const sr_logprob_shape* shape, const float* lse, const float* entropy, const float* g_logprob,
-                    const float* g_entropy, void* grad, uint64_t grad_stride, hipStream_t stream) {
-  if (int rc = check_shape("sr_logprob_grad", shape)) return rc;
+int logprobs_grad(const char* who, const sr_logprob_shape* shape, const float* lse, const float* lse_low, bool pair,
+                  const float* entropy, const float* g_logprob, const float* g_entropy, void* grad,
+                  uint64_t grad_stride, hipStream_t stream) {
+  if (int rc = check_shape(who, shape)) return rc;
   const sr_logprob_shape& s = *shape;
   if (s.rows == 0) return SR_OK;
-  if (!lse || !entropy || !grad) return fail(SR_EINVAL, "sr_logprob_grad: null argument");
+  if (!lse || (pair && !lse_low) || !entropy || !grad) return fail(SR_EINVAL, "%s: null argument", who);
   if (grad_stride < s.columns || grad_stride > SR_STEP_MAX_ELEMENTS)
-    return fail(SR_EINVAL, "sr_logprob_grad: rows %llu apart for %llu columns", (unsigned long long)grad_stride,
+    return fail(SR_EINVAL, "%s: rows %llu apart for %llu columns", who, (unsigned long long)grad_stride,
                 (unsigned long long)s.columns);
-  for (const float* p : {lse, entropy, g_logprob, g_entropy})
-    if (reinterpret_cast<uintptr_t>(p) % 4) return fail(SR_EALIGN, "sr_logprob_grad: not aligned to the elements");
+  for (const float* p : {lse, lse_low, entropy, g_logprob, g_entropy})
+    if (reinterpret_cast<uintptr_t>(p) % 4) return fail(SR_EALIGN, "%s: not aligned to the elements", who);
   const uint64_t size = sr_internal::dtype_size(s.dtype);
-  if (reinterpret_cast<uintptr_t>(grad) % size) return fail(SR_EALIGN, "sr_logprob_grad: not aligned to the elements");
+  if (reinterpret_cast<uintptr_t>(grad) % size) return fail(SR_EALIGN, "%s: not aligned to the elements", who);
   const Extent to{grad, ((s.rows - 1) * grad_stride + s.columns) * size};
   const Extent logits{s.logits, ((s.rows - 1) * s.stride + s.columns) * size};
   const bool in_place = grad == s.logits && grad_stride == s.stride;
   if ((!in_place && to.meets(logits)) ||
       to.meets({s.targets, s.rows * sr_internal::dtype_size(s.target_dtype)}) || to.meets({lse, s.rows * 4}) ||
-      to.meets({entropy, s.rows * 4}) || to.meets({g_logprob, s.rows * 4}) || to.meets({g_entropy, s.rows * 4}))
-    return fail(SR_EOVERLAP, "sr_logprob_grad: the gradient overlaps an input");
+      to.meets({lse_low, s.rows * 4}) || to.meets({entropy, s.rows * 4}) || to.meets({g_logprob, s.rows * 4}) ||
+      to.meets({g_entropy, s.rows * 4}))
+    return fail(SR_EOVERLAP, "%s: the gradient overlaps an input", who);
   const uint64_t step = kThreads * 16 / size, spans = (s.columns + step - 1) / step, blocks = s.rows * spans;
   if (blocks >= uint64_t(1) << 24)     // the grid's threads stay below 2^32
-    return fail(SR_EBOUNDS, "sr_logprob_grad: %llu rows of %llu columns", (unsigned long long)s.rows,
+    return fail(SR_EBOUNDS, "%s: %llu rows of %llu columns", who, (unsigned long long)s.rows,
                 (unsigned long long)s.columns);
   with_types(s, [&](const auto* logits, const auto* targets) {
     typedef typename std::remove_cv<typename std::remove_reference<decltype(*logits)>::type>::type T;
     grad_kernel<<<uint32_t(blocks), kThreads, 0, stream>>>(
-        logits, targets, s.stride, uint32_t(s.vocab), uint32_t(s.columns), uint32_t(spans), lse, entropy, g_logprob,
-        g_entropy, static_cast<T*>(grad), grad_stride);
+        logits, targets, s.stride, uint32_t(s.vocab), uint32_t(s.columns), uint32_t(spans), lse, lse_low,
+        entropy, g_logprob, g_entropy, static_cast<T*>(grad), grad_stride);
   });
-  return launched("sr_logprob_grad");
+  return launched(who);
+}
+
+}  // namespace
+
+extern "C" {
+
+int sr_logprob_workspace(const sr_logprob_shape* shape, int32_t top, uint64_t* bytes) {
+  if (bytes == nullptr) return fail(SR_EINVAL, "sr_logprob_workspace: null argument");
+  if (int rc = check_shape("sr_logprob_workspace", shape)) return rc;
+  if (int rc = check_top("sr_logprob_workspace", *shape, top)) return rc;
+  *bytes = parts_of(*shape, top).bytes;
+  return SR_OK;
+}
+
+int sr_logprob(const sr_logprob_shape* shape, int32_t top, float* logprob, float* entropy, float* lse,
+               float* top_logprob, int64_t* top_index, void* workspace, uint64_t workspace_bytes, hipStream_t stream) {
+  return logprobs("sr_logprob", shape, top, {logprob, entropy, lse, nullptr, top_logprob, top_index}, false, workspace,
+                  workspace_bytes, stream);
+}
+
+int sr_logprob_pair(const sr_logprob_shape* shape, int32_t top, float* logprob, float* entropy, float* lse,
+                    float* lse_low, float* top_logprob, int64_t* top_index, void* workspace, uint64_t workspace_bytes,
+                    hipStream_t stream) {
+  return logprobs("sr_logprob_pair", shape, top, {logprob, entropy, lse, lse_low, top_logprob, top_index}, true,
+                  workspace, workspace_bytes, stream);
+}
+
+int sr_logprob_grad(const sr_logprob_shape* shape, const float* lse, const float* entropy, const float* g_logprob,
+                    const float* g_entropy, void* grad, uint64_t grad_stride, hipStream_t stream) {
+  return logprobs_grad("sr_logprob_grad", shape, lse, nullptr, false, entropy, g_logprob, g_entropy, grad, grad_stride,
+                       stream);
+}
+
+int sr_logprob_pair_grad(const sr_logprob_shape* shape, const float* lse, const float* lse_low, const float* entropy,
+                         const float* g_logprob, const float* g_entropy, void* grad, uint64_t grad_stride,
+                         hipStream_t stream) {
+  return logprobs_grad("sr_logprob_pair_grad", shape, lse, lse_low, true, entropy, g_logprob, g_entropy, grad,
+                       grad_stride, stream);
 }
 
 }  // extern "C"

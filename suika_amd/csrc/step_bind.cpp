@@ -460,7 +460,7 @@ py::tuple token_logprobs(const at::Tensor& logits, const at::Tensor& targets, in
   const c10::DeviceGuard guard(device);
   const at::TensorOptions f32 = on(device, at::kFloat);
   at::Tensor logprob = at::empty(targets.sizes(), f32), entropy = at::empty(targets.sizes(), f32),
-             lse = at::empty(targets.sizes(), f32), best, index, work;
+             lse = at::empty(targets.sizes(), f32), lse_low = at::empty(targets.sizes(), f32), best, index, work;
   if (top) {
     std::vector<int64_t> shape(targets.sizes().begin(), targets.sizes().end());
     shape.push_back(top);
@@ -470,12 +470,13 @@ py::tuple token_logprobs(const at::Tensor& logits, const at::Tensor& targets, in
   uint64_t need = 0;
   check(sr_logprob_workspace(&s, int32_t(top), &need), "sr_logprob");
   if (need) work = at::empty({int64_t(need)}, on(device, at::kByte));
-  check(sr_logprob(&s, int32_t(top), logprob.data_ptr<float>(), entropy.data_ptr<float>(), lse.data_ptr<float>(),
-                   top ? best.data_ptr<float>() : nullptr, top ? index.data_ptr<int64_t>() : nullptr,
-                   need ? work.data_ptr() : nullptr, need, stream_of(device)),
-        "sr_logprob");
-  if (!top) return py::make_tuple(logprob, entropy, lse, py::none(), py::none());
-  return py::make_tuple(logprob, entropy, lse, best, index);
+  check(sr_logprob_pair(&s, int32_t(top), logprob.data_ptr<float>(), entropy.data_ptr<float>(), lse.data_ptr<float>(),
+                        lse_low.data_ptr<float>(), top ? best.data_ptr<float>() : nullptr,
+                        top ? index.data_ptr<int64_t>() : nullptr, need ? work.data_ptr() : nullptr, need,
+                        stream_of(device)),
+        "sr_logprob_pair");
+  if (!top) return py::make_tuple(logprob, entropy, lse, py::none(), py::none(), lse_low);
+  return py::make_tuple(logprob, entropy, lse, best, index, lse_low);
 }
 
 const float* row_values(const at::Tensor& t, const char* what, const at::Tensor& targets) {
@@ -489,9 +490,10 @@ const float* row_values(const at::Tensor& t, const char* what, const at::Tensor&
 at::Tensor token_logprobs_grad(const at::Tensor& logits, const at::Tensor& targets, const at::Tensor& lse,
                                const at::Tensor& entropy, const c10::optional<at::Tensor>& grad_logprob,
                                const c10::optional<at::Tensor>& grad_entropy, const c10::optional<int64_t>& vocab,
-                               const c10::optional<at::Tensor>& out) {
+                               const c10::optional<at::Tensor>& out, const c10::optional<at::Tensor>& lse_low) {
   const sr_logprob_shape s = logprob_shape(logits, targets, vocab);
   const float* l = row_values(lse, "lse", targets);
+  const float* low = lse_low ? row_values(*lse_low, "lse_low", targets) : nullptr;
   const float* h = row_values(entropy, "entropy", targets);
   const float* gl = grad_logprob ? row_values(*grad_logprob, "grad_logprob", targets) : nullptr;
   const float* gh = grad_entropy ? row_values(*grad_entropy, "grad_entropy", targets) : nullptr;
@@ -503,7 +505,11 @@ at::Tensor token_logprobs_grad(const at::Tensor& logits, const at::Tensor& targe
   }
   at::Tensor to = out ? *out : at::empty(logits.sizes(), on(logits.device(), logits.scalar_type()));
   const uint64_t stride = row_stride(to, "out");
-  check(sr_logprob_grad(&s, l, h, gl, gh, to.data_ptr(), stride, stream_of(logits.device())), "sr_logprob_grad");
+  if (lse_low)
+    check(sr_logprob_pair_grad(&s, l, low, h, gl, gh, to.data_ptr(), stride, stream_of(logits.device())),
+          "sr_logprob_pair_grad");
+  else
+    check(sr_logprob_grad(&s, l, h, gl, gh, to.data_ptr(), stride, stream_of(logits.device())), "sr_logprob_grad");
   if (out) written(to);
   return to;
 }
@@ -529,7 +535,8 @@ void bind_step(py::module_& m) {
         py::arg("scale"), py::arg("vocab_start"), py::arg("dtype"), py::arg("out"), py::arg("accumulate"));
   m.def("token_logprobs", &token_logprobs, py::arg("logits"), py::arg("targets"), py::arg("top"), py::arg("vocab"));
   m.def("token_logprobs_grad", &token_logprobs_grad, py::arg("logits"), py::arg("targets"), py::arg("lse"),
-        py::arg("entropy"), py::arg("grad_logprob"), py::arg("grad_entropy"), py::arg("vocab"), py::arg("out"));
+        py::arg("entropy"), py::arg("grad_logprob"), py::arg("grad_entropy"), py::arg("vocab"), py::arg("out"),
+        py::arg("lse_low"));
 }
 
 }  // namespace suika_host

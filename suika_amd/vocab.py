@@ -75,14 +75,29 @@ class _Embedding(torch.autograd.Function):
         return None, grad, None, None
 
 
-class TokenLogprobs(NamedTuple):
-    """What ``token_logprobs`` returns: float32 tensors of the targets' shape,
-    and the alternatives (with one more dimension) or ``None``."""
+class _Results(NamedTuple):
     logprob: Tensor
     entropy: Tensor
     lse: Tensor
     top_logprob: Optional[Tensor]
     top_index: Optional[Tensor]
+
+
+class TokenLogprobs(_Results):
+    """What ``token_logprobs`` returns: float32 tensors of the targets' shape,
+    and the alternatives (with one more dimension) or ``None``.
+
+    ``lse_low``, which is not one of the tuple's items, is what the rounding
+    of ``lse`` to float32 lost: ``token_logprobs_grad`` takes both where the
+    logits have a large common offset.
+    """
+    lse_low: Optional[Tensor] = None
+
+    @classmethod
+    def _of(cls, results) -> "TokenLogprobs":
+        r = cls(*results[:5])
+        r.lse_low = results[5]
+        return r
 
 
 def token_logprobs(logits: Tensor, targets: Tensor, *, top: int = 0, vocab: Optional[int] = None) -> TokenLogprobs:
@@ -106,29 +121,33 @@ def token_logprobs(logits: Tensor, targets: Tensor, *, top: int = 0, vocab: Opti
     not.
     """
     if logits.requires_grad and torch.is_grad_enabled():
-        return TokenLogprobs(*_Logprobs.apply(logits, targets, top, vocab))
-    return TokenLogprobs(*_lib.host().token_logprobs(logits, targets, top, vocab))
+        return TokenLogprobs._of(_Logprobs.apply(logits, targets, top, vocab))
+    return TokenLogprobs._of(_lib.host().token_logprobs(logits, targets, top, vocab))
 
 
 def token_logprobs_grad(logits: Tensor, targets: Tensor, lse: Tensor, entropy: Tensor,
                         grad_logprob: Optional[Tensor], grad_entropy: Optional[Tensor] = None, *,
-                        vocab: Optional[int] = None, out: Optional[Tensor] = None) -> Tensor:
+                        vocab: Optional[int] = None, out: Optional[Tensor] = None,
+                        lse_low: Optional[Tensor] = None) -> Tensor:
     """The gradient of the logits from those of ``logprob`` and ``entropy``
     (float32 of the targets' shape, or ``None``), in the logits' type:
     ``grad_logprob ([j = target] - p_j) - grad_entropy p_j (ln p_j + entropy)``.
 
-    ``lse`` and ``entropy`` are what ``token_logprobs`` returned.  Padded
-    columns and rows that are all -inf get 0, and a row that is not scored has
-    no first term.  ``out`` may be ``logits`` itself.
+    ``lse`` and ``entropy`` are what ``token_logprobs`` returned, and so is
+    ``lse_low``; without it, p_j is off by up to ``|lse| 2^-24`` of itself, as
+    ``lse`` is rounded to float32.  Padded columns and rows that are all -inf
+    get 0, and a row that is not scored has no first term.  ``out`` may be
+    ``logits`` itself.
     """
-    return _lib.host().token_logprobs_grad(logits, targets, lse, entropy, grad_logprob, grad_entropy, vocab, out)
+    return _lib.host().token_logprobs_grad(logits, targets, lse, entropy, grad_logprob, grad_entropy, vocab, out,
+                                           lse_low)
 
 
 class _Logprobs(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, targets, top, vocab):
         r = _lib.host().token_logprobs(logits, targets, top, vocab)
-        ctx.save_for_backward(logits, targets, r[2], r[1])
+        ctx.save_for_backward(logits, targets, r[2], r[1], r[5])
         ctx.vocab = vocab
         ctx.set_materialize_grads(False)
         ctx.mark_non_differentiable(*[t for t in r[2:] if t is not None])
@@ -139,6 +158,7 @@ class _Logprobs(torch.autograd.Function):
     def backward(ctx, grad_logprob, grad_entropy, *others):
         if grad_logprob is None and grad_entropy is None:
             return None, None, None, None
-        logits, targets, lse, entropy = ctx.saved_tensors
+        logits, targets, lse, entropy, lse_low = ctx.saved_tensors
         grads = [None if g is None else g.contiguous() for g in (grad_logprob, grad_entropy)]
-        return token_logprobs_grad(logits, targets, lse, entropy, *grads, vocab=ctx.vocab), None, None, None
+        grad = token_logprobs_grad(logits, targets, lse, entropy, *grads, vocab=ctx.vocab, lse_low=lse_low)
+        return grad, None, None, None

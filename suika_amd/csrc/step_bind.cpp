@@ -68,6 +68,11 @@ void check_stored(const at::Tensor& t, const char* what) {
   if (!stored(t)) plan_error(std::string(what) + ": its storage has been released");
 }
 
+// These operators have no forward-mode derivatives: a tangent would be lost.
+void check_tangent(const at::Tensor& t, const char* what) {
+  if (t._fw_grad(0).defined()) plan_error(std::string(what) + ": forward-mode derivatives are not supported");
+}
+
 // Whether a tensor is what check_dense wants, but for its storage.
 bool dense(const at::Tensor& t, const c10::optional<at::Device>& device) {
   return t.layout() == at::kStrided && t.is_cuda() && device && t.device() == *device && t.is_contiguous();
@@ -150,6 +155,7 @@ std::vector<sr_array> arrays_of(const Fast& list, const char* what, c10::optiona
     if (list[i] == Py_None) continue;
     const at::Tensor& t = tensor_of(list[i], indexed(what, i));
     check_dense(t, indexed(what, i), device);
+    check_tangent(t, what);
     a.push_back(array_of(t, indexed(what, i)));
   }
   return a;
@@ -200,6 +206,7 @@ at::Tensor clip_grads(py::object grads, double max_norm, py::object outs, py::ob
     if (list[i] == Py_None) continue;
     const at::Tensor& t = tensor_of(list[i], indexed("grads", i));
     check_dense(t, indexed("grads", i), device);
+    check_tangent(t, "grads");
     src.push_back(array_of(t, indexed("grads", i)));
     if (in_place) {
       to.push_back(t);
@@ -383,6 +390,7 @@ at::Tensor vocab_embedding(const at::Tensor& tokens, const at::Tensor& weight, d
   const sr_embedding_shape s =
       embedding_shape(tokens, float_code(weight, "weight"), rows, cols, scale, vocab_start);
   check_device(weight, "weight", tokens.device());
+  check_tangent(weight, "weight");
   const uint64_t stride = row_stride(weight, "weight");
   const c10::DeviceGuard guard(tokens.device());
   std::vector<int64_t> shape(tokens.sizes().begin(), tokens.sizes().end());
@@ -409,6 +417,7 @@ at::Tensor vocab_embedding_grad(const at::Tensor& tokens, const at::Tensor& grad
   const sr_embedding_shape s =
       embedding_shape(tokens, float_code(grad_output, "grad_output"), rows, cols, scale, vocab_start);
   check_device(grad_output, "grad_output", tokens.device());
+  check_tangent(grad_output, "grad_output");
   const uint64_t stride = row_stride(grad_output, "grad_output");
   const c10::DeviceGuard guard(tokens.device());
   at::Tensor to;
@@ -443,6 +452,7 @@ sr_logprob_shape logprob_shape(const at::Tensor& logits, const at::Tensor& targe
   if (!logits.is_cuda() || !targets.is_contiguous()) plan_error("logits on the GPU and contiguous targets are wanted");
   check_device(targets, "targets", logits.device());
   check_stored(targets, "targets");
+  check_tangent(logits, "logits");
   const int64_t columns = logits.size(-1), v = vocab ? *vocab : columns;
   if (v < 1 || v > columns)
     plan_error("a vocabulary of " + std::to_string(v) + " in " + std::to_string(columns) + " columns");
@@ -484,6 +494,7 @@ const float* row_values(const at::Tensor& t, const char* what, const at::Tensor&
   if (t.scalar_type() != at::kFloat || t.sizes() != targets.sizes() || !t.is_contiguous())
     plan_error(std::string(what) + ": a contiguous float32 tensor of the targets' shape is wanted");
   check_stored(t, what);
+  check_tangent(t, what);
   return t.data_ptr<float>();
 }
 

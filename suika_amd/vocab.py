@@ -17,7 +17,8 @@ are whole, as the reference gathers them (lm_head is column parallel with
 padded, ``vocab`` says how many are tokens.
 
 The kernels run on the tensors' device, on its current stream, behind the C
-ABI of include/suika_step.h.  Refused arguments raise ``PlanError``.
+ABI of include/suika_step.h.  Refused arguments raise ``PlanError``, and so do
+forward-mode tangents, which the operators do not have.
 """
 from __future__ import annotations
 
@@ -27,6 +28,7 @@ import torch
 from torch import Tensor
 
 from . import _lib
+from ._lib import PlanError
 
 
 def vocab_embedding(tokens: Tensor, weight: Tensor, *, scale: float = 1.0, vocab_start: int = 0,
@@ -37,10 +39,11 @@ def vocab_embedding(tokens: Tensor, weight: Tensor, *, scale: float = 1.0, vocab
     ``tokens`` are int64 or int32 and contiguous, ``weight`` is float32,
     bfloat16 or float16 with dense rows at any distance.  Products are rounded
     once.  Where ``weight`` wants a gradient, the result is differentiable
-    (``vocab_embedding_grad``, in the weight's type); ``out`` is for calls
-    without.
+    (``vocab_embedding_grad``, in the weight's type), and ``out`` is refused.
     """
-    if out is None and weight.requires_grad and torch.is_grad_enabled():
+    if weight.requires_grad and torch.is_grad_enabled():
+        if out is not None:
+            raise PlanError("out: the weight wants a gradient, which rows in a given output do not have")
         return _Embedding.apply(tokens, weight, float(scale), int(vocab_start))
     return _lib.host().vocab_embedding(tokens, weight, scale, vocab_start, out)
 

@@ -142,7 +142,7 @@ typedef struct sr_embedding_shape {
   uint64_t n_tokens;
   uint64_t rows;         /* of the shard */
   uint64_t cols;
-  int64_t vocab_start;
+  int64_t vocab_start;   /* 0 or more */
   float scale;
   int32_t reserved;      /* must be 0 */
 } sr_embedding_shape;

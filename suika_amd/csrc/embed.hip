@@ -522,6 +522,8 @@ int check_shape(const char* who, const sr_embedding_shape* s) {
   if (s->n_tokens > SR_STEP_MAX_ROWS || s->rows > SR_STEP_MAX_ROWS || s->cols > SR_STEP_MAX_ROWS)
     return fail(SR_EBOUNDS, "%s: %llu tokens, %llu rows, %llu columns", who, (unsigned long long)s->n_tokens,
                 (unsigned long long)s->rows, (unsigned long long)s->cols);
+  // a negative start would make rows of negative tokens, which lie outside of every shard
+  if (s->vocab_start < 0) return fail(SR_EINVAL, "%s: vocab_start %lld", who, (long long)s->vocab_start);
   if (s->n_tokens && s->tokens == nullptr) return fail(SR_EINVAL, "%s: tokens is null", who);
   if (!aligned(s->tokens, s->token_dtype)) return fail(SR_EALIGN, "%s: tokens not aligned", who);
   return SR_OK;

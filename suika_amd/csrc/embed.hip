@@ -84,6 +84,7 @@ __global__ __launch_bounds__(kThreads) void embedding_kernel(const I* tokens, co
   const bool inside = row < rows;
   const T* src = weight + (inside ? row * stride : 0) + c;
   T* dst = out + uint64_t(i) * cols + c;
+  const float by = inside ? scale : 0.0f;      // rows outside are zeros whatever the scale is
   float x[U][N] = {};
 #pragma unroll
   for (int u = 0; u < U; ++u)
@@ -93,7 +94,7 @@ __global__ __launch_bounds__(kThreads) void embedding_kernel(const I* tokens, co
     const uint64_t at = c + u * step;
     if (at + N <= cols) {
 #pragma unroll
-      for (int k = 0; k < N; ++k) x[u][k] *= scale;
+      for (int k = 0; k < N; ++k) x[u][k] *= by;
       store_stream<T, N>(dst + u * step, x[u]);
     } else {
       for (uint64_t k = at; k < cols; ++k) dst[k - c] = inside ? T(float(src[k - c]) * scale) : T(0.0f);
@@ -463,7 +464,8 @@ __global__ __launch_bounds__(kThreads) void sum_kernel(const T* grad_out, uint64
       from += n < 2 ? n : 2;
     }
     sum_tokens<kWhole, T, N>(grad_out, stride, in.order, from, run.to, at, cols, acc);
-    put_row<G, N>(grad + uint64_t(row) * cols, own, at, cols, scale, accumulate, acc);
+    // a row without tokens is zeros whatever the scale is
+    put_row<G, N>(grad + uint64_t(row) * cols, own, at, cols, n ? scale : 0.0f, accumulate, acc);
   }
 }
 

@@ -360,15 +360,25 @@ int32_t index_code(const at::Tensor& t, const char* what) {
   plan_error(std::string(what) + ": dtype " + c10::toString(t.scalar_type()) + ", not int64 or int32");
 }
 
-// A tensor of rows of `cols` dense elements: their distance in elements.
+// A tensor of rows of dense elements, all of one distance from the next: that
+// distance, in elements.
 uint64_t row_stride(const at::Tensor& t, const std::string& what) {
   if (t.layout() != at::kStrided || t.dim() < 1) plan_error(what + ": a dense tensor of rows is wanted");
   if (!stored(t)) plan_error(what + ": its storage has been released");
   const int64_t cols = t.size(-1);
   if (t.is_contiguous()) return uint64_t(cols);
-  if (t.dim() != 2 || (t.stride(1) != 1 && cols > 1) || (t.stride(0) < cols && t.size(0) > 1))
-    plan_error(what + ": rows of dense elements are wanted, not strides of " + std::to_string(t.stride(-1)));
-  return uint64_t(t.size(0) > 1 ? t.stride(0) : cols);
+  int64_t distance = cols, next = -1;     // from row to row; what an outer dimension's stride has to be
+  bool ok = t.stride(-1) == 1 || cols <= 1;
+  for (int64_t d = t.dim() - 2; d >= 0; --d) {
+    if (t.size(d) <= 1) continue;
+    if (next < 0) distance = t.stride(d);
+    else if (t.stride(d) != next) ok = false;
+    next = t.stride(d) * t.size(d);
+  }
+  if (!ok || distance < cols)
+    plan_error(what + ": rows of dense elements, one distance apart, are wanted, not strides of " +
+               c10::str(t.strides()));
+  return uint64_t(distance);
 }
 
 void check_device(const at::Tensor& t, const char* what, const at::Device& device) {

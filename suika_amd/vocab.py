@@ -107,10 +107,11 @@ def token_logprobs(logits: Tensor, targets: Tensor, *, top: int = 0, vocab: Opti
     """Log probabilities of ``targets`` under ``logits``, with the entropy and
     the ``lse`` (log of the sum of the exponentials) of each row.
 
-    ``logits`` are float32, bfloat16 or float16 with dense rows at any
-    distance; their first ``vocab`` columns (default: all) are tokens.
-    ``targets`` (int64 or int32) has the other dimensions.  A negative target,
-    as ``ignore_index=-100``, is not scored: logprob 0.  A target of ``vocab``
+    ``logits`` are float32, bfloat16 or float16 with dense rows, all one
+    distance apart (``logits[..., :n]`` of a contiguous tensor, for example);
+    their first ``vocab`` columns (default: all) are tokens.  ``targets``
+    (int64 or int32) has the other dimensions.  A negative target, as
+    ``ignore_index=-100``, is not scored: logprob 0.  A target of ``vocab``
     or more has logprob -inf.  ``top`` (at most 64) asks for the largest log
     probabilities in falling order, int64 columns with them; equal logits come
     by column.  Statistics are formed in 32 bits.

@@ -61,7 +61,8 @@ typedef struct sr_array {
 /*
  * The sum of the squares of all elements, in 64 bits: *sum on the device, and
  * its root, *norm, where norm is not NULL.  Ranks that hold other shards add
- * their sums before clipping.  workspace: sr_square_sum_workspace bytes.
+ * their sums before clipping.  workspace: sr_square_sum_workspace bytes.  *sum,
+ * *norm and the workspace overlap nothing else (SR_EOVERLAP).
  */
 int sr_square_sum_workspace(const sr_array* arrays, int32_t count, uint64_t* bytes);
 int sr_square_sum(const sr_array* arrays, int32_t count, int32_t read_again, void* workspace, uint64_t workspace_bytes,
@@ -70,7 +71,7 @@ int sr_square_sum(const sr_array* arrays, int32_t count, int32_t read_again, voi
 /*
  * dst[i] = src[i] * min(1, max_norm / (sqrt(*square_sum) + 1e-6)), array by
  * array.  dst NULL: in place, where a factor of 1 leaves the memory as it is.
- * Arrays that are written overlap no others (SR_EOVERLAP).
+ * Arrays that are written overlap no others, nor *square_sum or *norm (SR_EOVERLAP).
  * norm (may be NULL) gets sqrt(*square_sum).
  */
 int sr_clip(const sr_array* src, const sr_array* dst, int32_t count, const double* square_sum, float max_norm,
@@ -120,7 +121,8 @@ typedef struct sr_adamw_options {
 /*
  * One AdamW update in place (decoupled weight decay, bias corrections of
  * `step`).  square_sum: the sum that clipping goes by, on the device; NULL: no
- * clipping.  Fields that are written overlap no others (SR_EOVERLAP).
+ * clipping.  Fields that are written overlap no others, nor *square_sum
+ * (SR_EOVERLAP).
  */
 int sr_adamw(const sr_adamw_tensor* tensors, int32_t count, const sr_adamw_options* options, const double* square_sum,
              hipStream_t stream);

@@ -564,6 +564,12 @@ int check_sum(const char* who, const sr_array* arrays, int32_t count, const void
   if (reinterpret_cast<uintptr_t>(workspace) % 16 || reinterpret_cast<uintptr_t>(sum) % 8 ||
       reinterpret_cast<uintptr_t>(norm) % 4)
     return fail(SR_EALIGN, "%s: the workspace or a result is not aligned", who);
+  const Extent written[3] = {{sum, sizeof(double)}, {norm, sizeof(float)}, {workspace, need}};
+  for (int k = 0; k < 3; ++k) {
+    bool meets = written[k].meets(written[(k + 1) % 3]);
+    for (int32_t i = 0; i < count && !meets; ++i) meets = written[k].meets({arrays[i].data, bytes_of(arrays[i])});
+    if (meets) return fail(SR_EOVERLAP, "%s: a result or the workspace overlaps other memory of the call", who);
+  }
   return SR_OK;
 }
 
@@ -611,6 +617,14 @@ int check_norm(const char* who, const sr_norm& n, const sr_array* grads, int32_t
   return SR_OK;
 }
 
+// The memory of a checked norm beside the gradients.
+void add_norm_spans(std::vector<Span>& spans, const sr_norm& n, const sr_array* grads, int32_t count) {
+  add_span(spans, n.norm, sizeof(float), true);
+  if (n.square_sum != nullptr) return add_span(spans, n.square_sum, sizeof(double), false);
+  add_span(spans, n.sum, sizeof(double), true);
+  add_span(spans, n.workspace, sum_workspace(grads, count), true);
+}
+
 // *norm = sqrt(*square_sum), with nothing to clip.
 int launch_norm(const char* who, const double* square_sum, float* norm, hipStream_t stream) {
   ClipTable t;
@@ -641,7 +655,8 @@ int clip(const char* who, const sr_array* src, const sr_array* dst, int32_t coun
     if (src[i].data != dst[i].data || src[i].dtype != dst[i].dtype)
       add_span(spans, src[i].data, bytes_of(src[i]), false);
   }
-  if (clash(spans)) return fail(SR_EOVERLAP, "%s: an array that is written overlaps another", who);
+  add_norm_spans(spans, n, src, count);
+  if (clash(spans)) return fail(SR_EOVERLAP, "%s: an array or a value that is written overlaps another", who);
   const double* square_sum = n.square_sum;
   if (square_sum == nullptr) {
     if (int rc = launch_square_sum(src, count, true, n.workspace, n.sum, nullptr, stream)) return rc;
@@ -728,8 +743,9 @@ int adamw(const char* who, const sr_adamw_tensor* tensors, const int64_t* steps,
   }
   if (n != nullptr) {
     if (int rc = check_norm(who, *n, grads.data(), int32_t(grads.size()))) return rc;
+    add_norm_spans(spans, *n, grads.data(), int32_t(grads.size()));
   }
-  if (clash(spans)) return fail(SR_EOVERLAP, "%s: a field that is written overlaps another", who);
+  if (clash(spans)) return fail(SR_EOVERLAP, "%s: a field or a value that is written overlaps another", who);
   hipStreamCaptureStatus capturing = hipStreamCaptureStatusNone;
   SR_STEP_TRY(hipStreamIsCapturing(stream, &capturing));
   if (capturing != hipStreamCaptureStatusNone)

@@ -112,7 +112,6 @@ constexpr uint32_t kSortRows = 512;       // most rows of one workgroup
 struct Owners {
   uint32_t log2;     // of the number of workgroups
   uint32_t range;    // rows of each
-
 };
 
 // One workgroup a compute unit, or more where that many rows have no room.
@@ -510,8 +509,6 @@ __global__ __launch_bounds__(kThreads) void join_kernel(G* grad, uint32_t cols, 
 }
 
 // ---------------------------------------------------------------------- host
-
-bool float_dtype(int32_t dt) { return dt == SR_DT_F32 || dt == SR_DT_BF16 || dt == SR_DT_F16; }
 
 bool aligned(const void* p, int32_t dt) { return reinterpret_cast<uintptr_t>(p) % sr_internal::dtype_size(dt) == 0; }
 

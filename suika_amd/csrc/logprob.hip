@@ -667,8 +667,7 @@ int check_shape(const char* who, const sr_logprob_shape* s) {
   if (s == nullptr) return fail(SR_EINVAL, "%s: null argument", who);
   if (s->target_dtype != SR_DT_I32 && s->target_dtype != SR_DT_I64)
     return fail(SR_EDTYPE, "%s: targets of dtype %d", who, s->target_dtype);
-  if (s->dtype != SR_DT_F32 && s->dtype != SR_DT_BF16 && s->dtype != SR_DT_F16)
-    return fail(SR_EDTYPE, "%s: logits of dtype %d", who, s->dtype);
+  if (!float_dtype(s->dtype)) return fail(SR_EDTYPE, "%s: logits of dtype %d", who, s->dtype);
   if (s->rows > SR_STEP_MAX_ROWS || s->columns > SR_STEP_MAX_ROWS)
     return fail(SR_EBOUNDS, "%s: %llu rows of %llu columns", who, (unsigned long long)s->rows,
                 (unsigned long long)s->columns);

@@ -337,7 +337,7 @@ template <typename W, typename M, typename G, typename P>
 __global__ __launch_bounds__(kAdamThreads) void adamw_kernel(uint32_t chunks,
                                                              AdamTable<!__is_same(P, NoCopy)> t) {
   constexpr int N = kAdamChunk / kAdamThreads;
-    const uint32_t c = xcd_order(blockIdx.x, chunks);
+  const uint32_t c = xcd_order(blockIdx.x, chunks);
   if (c >= chunks) return;
   const auto found = t.at.find(c);
   const uint32_t i = found.entry;
@@ -386,8 +386,6 @@ __global__ __launch_bounds__(kAdamThreads) void adamw_kernel(uint32_t chunks,
 
 // ---------------------------------------------------------------------- host
 
-bool float_dtype(int32_t dt) { return dt == SR_DT_F32 || dt == SR_DT_BF16 || dt == SR_DT_F16; }
-
 int check_arrays(const char* who, const sr_array* a, int32_t count) {
   if (count < 0 || (count > 0 && a == nullptr)) return fail(SR_EINVAL, "%s: no arrays", who);
   for (int32_t i = 0; i < count; ++i) {
@@ -426,7 +424,6 @@ bool clash(std::vector<Span>& spans) {
   }
   return false;
 }
-
 
 constexpr int32_t kFloatTypes[3] = {SR_DT_F32, SR_DT_BF16, SR_DT_F16};
 

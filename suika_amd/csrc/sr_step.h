@@ -108,6 +108,8 @@ __device__ __forceinline__ uint32_t xcd_order(uint32_t block, uint32_t items) {
   return block % kXcds * ((items + kXcds - 1) / kXcds) + block / kXcds;
 }
 
+inline bool float_dtype(int32_t dt) { return dt == SR_DT_F32 || dt == SR_DT_BF16 || dt == SR_DT_F16; }
+
 // Memory that a call reads or writes.
 struct Extent {
   const void* p;

@@ -622,12 +622,15 @@ __global__ __launch_bounds__(kThreads) void parts_kernel(const T* logits, const 
 // bf16 in 168 us (6.2 TB/s), 2047 x 50304 f32 in 123 (6.7), HBM bound (workgroups
 // in the order of rows, four vectors a lane: 176 and 124; stores streamed: 185
 // and 148).
-template <typename T, typename I>
+// PAIR: with lse_low, one more value of the row behind an address in memory
+// (8192 x 32000 bf16 under the profiler 176 us, without 174; decided at run time,
+// the single lse takes 176 as well).
+template <bool PAIR, typename T, typename I>
 __global__ __launch_bounds__(kThreads) void grad_kernel(const T* logits, const I* targets, uint64_t stride,
                                                         uint32_t vocab, uint32_t columns, uint32_t spans,
-                                                        const float* lse, const float* lse_low, const float* entropy,
+                                                        const float* lse, const float* entropy,
                                                         const float* g_logprob, const float* g_entropy, T* grad,
-                                                        uint64_t grad_stride) {
+                                                        uint64_t grad_stride, const float* lse_low) {
   constexpr int N = 16 / sizeof(T);
   const uint32_t i = blockIdx.x / spans;
   const uint32_t c = ((blockIdx.x - i * spans) * kThreads + threadIdx.x) * N;
@@ -637,16 +640,16 @@ __global__ __launch_bounds__(kThreads) void grad_kernel(const T* logits, const I
   Vec<T, N> x;
   if (whole) x = __builtin_nontemporal_load(reinterpret_cast<const Vec<T, N>*>(row + c));
   const int64_t target = target_at(targets, i);
-  const float l = lse[i], low = lse_low ? lse_low[i] : 0.0f, h = entropy[i];
+  const float l = lse[i], low = PAIR ? lse_low[i] : 0.0f, h = entropy[i];
   const float gl = g_logprob && target >= 0 ? g_logprob[i] : 0.0f;
   const float gh = g_entropy ? g_entropy[i] : 0.0f;
   // grad = [target] gl - p (gl + gh (ln p + h)) with ln p = d - low; d = x - l is exact where x is within a factor
   // of two of l
-  const float base = fmaf(-gh, low, fmaf(gh, h, gl)), low2 = low * kLog2e;
+  const float base = PAIR ? fmaf(-gh, low, fmaf(gh, h, gl)) : fmaf(gh, h, gl), low2 = low * kLog2e;
   const bool empty = l == -kInf;
   auto value = [&](float x, uint32_t c) {
     const float d = x - l;
-    const float p = exp2_fast(fmaf(d, kLog2e, -low2));             // NaN stays NaN
+    const float p = exp2_fast(PAIR ? fmaf(d, kLog2e, -low2) : d * kLog2e);             // NaN stays NaN
     float g = -p * fmaf(gh, fmaxf(d, -200.0f), base);
     if (int64_t(c) == target) g += gl;
     return empty || c >= vocab ? 0.0f : g;
@@ -798,9 +801,14 @@ int logprobs_grad(const char* who, const sr_logprob_shape* shape, const float* l
                 (unsigned long long)s.columns);
   with_types(s, [&](const auto* logits, const auto* targets) {
     typedef typename std::remove_cv<typename std::remove_reference<decltype(*logits)>::type>::type T;
-    grad_kernel<<<uint32_t(blocks), kThreads, 0, stream>>>(
-        logits, targets, s.stride, uint32_t(s.vocab), uint32_t(s.columns), uint32_t(spans), lse, lse_low,
-        entropy, g_logprob, g_entropy, static_cast<T*>(grad), grad_stride);
+    auto launch = [&](auto* kernel) {
+      kernel<<<uint32_t(blocks), kThreads, 0, stream>>>(
+          logits, targets, s.stride, uint32_t(s.vocab), uint32_t(s.columns), uint32_t(spans), lse, entropy, g_logprob,
+          g_entropy, static_cast<T*>(grad), grad_stride, lse_low);
+    };
+    typedef typename std::remove_cv<typename std::remove_reference<decltype(*targets)>::type>::type I;
+    if (pair) launch(grad_kernel<true, T, I>);
+    else launch(grad_kernel<false, T, I>);
   });
   return launched(who);
 }

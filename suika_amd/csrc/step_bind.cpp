@@ -57,11 +57,14 @@ const at::Tensor& tensor_of(PyObject* o, const std::string& what) {
 // released (forcefully_free_tensor), and then a view's address is its offset
 // alone.
 bool stored(const at::Tensor& t) {
-  if (t.numel() == 0) return true;
+  const int64_t n = t.numel();
+  if (n == 0) return true;
   if (!t.has_storage()) return false;
-  uint64_t last = uint64_t(t.storage_offset());
-  for (int64_t d = 0; d < t.dim(); ++d) last += uint64_t((t.size(d) - 1) * t.stride(d));
-  return (last + 1) * t.element_size() <= t.storage().nbytes();
+  uint64_t end = uint64_t(t.storage_offset()) + 1;
+  if (t.is_contiguous()) end += uint64_t(n) - 1;
+  else
+    for (int64_t d = 0; d < t.dim(); ++d) end += uint64_t((t.size(d) - 1) * t.stride(d));
+  return end * t.dtype().itemsize() <= t.storage().nbytes();
 }
 
 void check_stored(const at::Tensor& t, const char* what) {
@@ -153,10 +156,11 @@ std::vector<sr_array> arrays_of(const Fast& list, const char* what, c10::optiona
   a.reserve(list.size());
   for (size_t i = 0; i < list.size(); ++i) {
     if (list[i] == Py_None) continue;
-    const at::Tensor& t = tensor_of(list[i], indexed(what, i));
-    check_dense(t, indexed(what, i), device);
+    const std::string name = indexed(what, i);
+    const at::Tensor& t = tensor_of(list[i], name);
+    check_dense(t, name, device);
     check_tangent(t, what);
-    a.push_back(array_of(t, indexed(what, i)));
+    a.push_back(array_of(t, name));
   }
   return a;
 }
@@ -204,18 +208,20 @@ at::Tensor clip_grads(py::object grads, double max_norm, py::object outs, py::ob
     plan_error("out has " + std::to_string(out_list.size()) + " tensors, grads " + std::to_string(list.size()));
   for (size_t i = 0; i < list.size(); ++i) {
     if (list[i] == Py_None) continue;
-    const at::Tensor& t = tensor_of(list[i], indexed("grads", i));
-    check_dense(t, indexed("grads", i), device);
+    const std::string name = indexed("grads", i);
+    const at::Tensor& t = tensor_of(list[i], name);
+    check_dense(t, name, device);
     check_tangent(t, "grads");
-    src.push_back(array_of(t, indexed("grads", i)));
+    src.push_back(array_of(t, name));
     if (in_place) {
       to.push_back(t);
       continue;
     }
-    const at::Tensor& o = tensor_of(out_list[i], indexed("out", i));
-    check_dense(o, indexed("out", i), device);
-    if (o.sizes() != t.sizes()) plan_error(indexed("out", i) + ": shape differs from the gradient's");
-    dst.push_back(array_of(o, indexed("out", i)));
+    const std::string out_name = indexed("out", i);
+    const at::Tensor& o = tensor_of(out_list[i], out_name);
+    check_dense(o, out_name, device);
+    if (o.sizes() != t.sizes()) plan_error(out_name + ": shape differs from the gradient's");
+    dst.push_back(array_of(o, out_name));
     to.push_back(o);
   }
   if (!device) device = current_device();

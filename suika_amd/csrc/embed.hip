@@ -29,7 +29,8 @@
 //           memory, gradients read and written past the caches: 48.2 us for
 //           256 MB (5.3 TB/s; four tokens at once and indices as they are
 //           needed 51.8; with cached accesses 73; rows in the sort's order 78).
-//   join    The partial sums of such rows, added in order: 6.7 us.
+//   join    The partial sums of such rows, added in order: 6.7 us (30011
+//           tokens of 3584 columns 7.9).
 
 #include <hip/hip_runtime.h>
 
@@ -133,7 +134,8 @@ constexpr uint32_t kNoPiece = 0xffffffffu;
 
 // The tokens of a piece of a row of n: `least` or, of long rows, as many as the
 // row then has pieces, so that adding up a piece and joining them take the same
-// number of steps (with `least` for all: the join 11.8 us, not 8.9).
+// number of steps (16384 tokens of 4096 bf16 columns: sort and join 11.2 and
+// 6.7 us, with `least` for all 12.6 and 9.2).
 __device__ __forceinline__ uint32_t piece_of(uint32_t n, uint32_t least) {
   return max(least, (uint32_t(sqrtf(float(n))) + 3) / 4 * 4);
 }

@@ -325,9 +325,11 @@ static_assert(sizeof(AdamTable<true>) <= kTableBytes && sizeof(AdamTable<false>)
 struct NoCopy {};
 
 // One chunk a workgroup, one vector of every field a lane, all loads before the
-// first store.  Chunks go to the dies by eighths (xcd_order): 200 M to 900 M
-// elements run at 5.9 to 6.3 TB/s of the 28 bytes each that they read and
-// write, in plain order at 5.4 to 5.6.  Loads and stores stream: with stores that
+// first store.  Chunks go to the dies by eighths (xcd_order).  That pays for the
+// largest states and costs the smaller ones: TB/s of the 28 bytes an element
+// that are read and written, by eighths / in plain order, of 40, 200, 400 and 936 M
+// elements in 100 tensors: f32 5.5 / 6.1, 5.8 / 5.7, 5.8 / 5.6, 5.8 / 5.7; mixed
+// 5.6 / 6.0, 5.5 / 5.7, 5.6 / 5.6, 5.7 / 5.4.  Loads and stores stream: with stores that
 // write through the L2 the update itself is as fast or 3% faster, but the next
 // kernel's reads wait for what they left in the memory-side cache (GPT-125M's
 // share with clipping 238 us a step, streamed 212).

@@ -17,8 +17,9 @@
 // largest of 64 lane groups' maxima is a bound that at least k logits reach,
 // and only the groups whose maximum reaches it are read again, their vectors
 // dealt out to all lanes.  The logits that reach it are ranked against each
-// other; equal ones by column.  With 5 alternatives the bf16 rows take 112 us,
-// with 20 128 us (each lane reading its own group's vectors again: 217 and 231).
+// other; equal ones by column.  With 5 alternatives the bf16 rows take 102 to
+// 112 us, with 20 128 to 132 (each lane reading its own group's vectors again: 217
+// and 231).
 // A chain of loads and barriers a row, and the second reads, are what they cost.
 //
 // Rows that this arithmetic does not cover (NaN or +inf, a largest logit beyond

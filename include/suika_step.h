@@ -19,6 +19,10 @@
  *   sr_logprob, sr_logprob_grad, sr_logprob_pair, sr_logprob_pair_grad
  *       log probabilities of given tokens, entropy and the best alternatives
  *       from the head's logits, and the gradient of the logits
+ *   sr_ffn, sr_ffn_grad
+ *       the gated feed-forward block of a share and its gradients.  In the
+ *       reference it is the blocks' mlp, gate and up column parallel and down
+ *       row parallel (Suika/models/llama_model.py:16-35)
  *
  * Conventions
  *   - All device memory, workspaces included, belongs to the caller.
@@ -216,6 +220,65 @@ int sr_logprob_pair(const sr_logprob_shape* shape, int32_t top, float* logprob, 
 int sr_logprob_pair_grad(const sr_logprob_shape* shape, const float* lse, const float* lse_low, const float* entropy,
                          const float* g_logprob, const float* g_entropy, void* grad, uint64_t grad_stride,
                          hipStream_t stream);
+
+/* Activations: a s(a), a Phi(a) and a s(2 z) with z = sqrt(2/pi) (a + 0.044715
+ * a^3), where s(a) = 1 / (1 + exp(-a)) and Phi is the normal distribution. */
+#define SR_ACT_SILU 0
+#define SR_ACT_GELU 1
+#define SR_ACT_GELU_TANH 2
+
+/* A gated feed-forward block: x [tokens][hidden], this rank's rows of gate and
+ * up [ffn][hidden] and columns of down [hidden][ffn], of one type, with rows of
+ * dense elements `*_stride` apart.  hidden and ffn are at most 2^20, and any of
+ * the three sizes may be 0. */
+typedef struct sr_ffn_shape {
+  const void* x;
+  const void* gate;
+  const void* up;
+  const void* down;
+  uint64_t tokens;
+  uint64_t hidden;
+  uint64_t ffn;
+  uint64_t x_stride;
+  uint64_t gate_stride;
+  uint64_t up_stride;
+  uint64_t down_stride;
+  int32_t dtype;        /* SR_DT_F32, SR_DT_BF16 or SR_DT_F16 */
+  int32_t activation;   /* SR_ACT_* */
+} sr_ffn_shape;
+
+/*
+ * out = (act(x gate^T) * (x up^T)) down^T, dense [tokens][hidden]; the ranks'
+ * outputs add up.  The product in brackets is rounded to the operands' type on
+ * the way, sums are in 32 bits.  gate_out and up_out (both or neither, floats,
+ * dense [tokens][ffn]) keep x gate^T and x up^T for sr_ffn_grad.  workspace:
+ * sr_ffn_workspace bytes, for a call that keeps them or does not.  What is
+ * written overlaps nothing else (SR_EOVERLAP).
+ */
+int sr_ffn_workspace(const sr_ffn_shape* shape, int32_t keep, uint64_t* bytes);
+int sr_ffn(const sr_ffn_shape* shape, void* out, float* gate_out, float* up_out, void* workspace,
+           uint64_t workspace_bytes, hipStream_t stream);
+
+/* Where the gradients go, dense; NULL: not wanted. */
+typedef struct sr_ffn_grads {
+  void* x;        /* [tokens][hidden] */
+  void* gate;     /* [ffn][hidden] */
+  void* up;       /* [ffn][hidden] */
+  void* down;     /* [hidden][ffn] */
+} sr_ffn_grads;
+
+/*
+ * The gradients of a block from that of its output (grad_out, rows
+ * grad_out_stride apart) and what sr_ffn kept.  The gradients of the two
+ * projections are rounded to the operands' type on the way, sums are in 32
+ * bits.  workspace: sr_ffn_grad_workspace bytes for the same gradients.  What
+ * is written overlaps nothing else (SR_EOVERLAP).
+ */
+int sr_ffn_grad_workspace(const sr_ffn_shape* shape, const void* grad_out, uint64_t grad_out_stride,
+                          const sr_ffn_grads* grads, uint64_t* bytes);
+int sr_ffn_grad(const sr_ffn_shape* shape, const float* gate_out, const float* up_out, const void* grad_out,
+                uint64_t grad_out_stride, const sr_ffn_grads* grads, void* workspace, uint64_t workspace_bytes,
+                hipStream_t stream);
 
 #ifdef __cplusplus
 }

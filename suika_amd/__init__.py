@@ -20,6 +20,7 @@ from ._lib import PlanError, ReshardError
 from .checkpoint import checkpoint_load, checkpoint_save, migration_load, migration_save
 from .handoff import HandoffError, dummy_migration_IPC_state_dict
 from .optim import ShardAdamW, clip_grads, counted_names, grad_norm, grad_square_sum
+from .ffn import GatedFFN, gated_ffn, gated_ffn_grad
 from .vocab import TokenLogprobs, token_logprobs, token_logprobs_grad, vocab_embedding, vocab_embedding_grad
 
 __all__ = [
@@ -32,4 +33,5 @@ __all__ = [
     "migration_load", "forcefully_free_tensor", "cuda_gc", "dummy_migration_IPC_state_dict", "HandoffError",
     "ShardAdamW", "clip_grads", "counted_names", "grad_norm", "grad_square_sum",
     "vocab_embedding", "vocab_embedding_grad", "TokenLogprobs", "token_logprobs", "token_logprobs_grad",
+    "GatedFFN", "gated_ffn", "gated_ffn_grad",
 ]

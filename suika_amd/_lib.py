@@ -91,6 +91,10 @@ EXPORTED_SYMBOLS = (
     "sr_logprob_grad",
     "sr_logprob_pair",
     "sr_logprob_pair_grad",
+    "sr_ffn_workspace",
+    "sr_ffn",
+    "sr_ffn_grad_workspace",
+    "sr_ffn_grad",
 )
 
 # Largest hand-off allocation (SR_HANDOFF_MAX_BYTES, include/suika_handoff.h).

@@ -1,0 +1,846 @@
+// ffn.hip -- the gated feed-forward block of a tensor-parallel share and its
+// gradients (C ABI in include/suika_step.h).
+//
+//   a = x G^T   b = x U^T   h = act(a) b   y = h D^T
+//
+// Gate G and up U are this rank's rows, down D this rank's columns, so the
+// ranks' y add up.  Forward, both projections, the activation and the product
+// are one kernel: a tile has the rows of G and of U in turn, so a wave has a
+// and b of the same columns.  Backward, the product dy D ends in the gradients
+// of a and b; dx is one product over both pairs, and the three matrices'
+// gradients are one launch.
+//
+// h, da and db are rounded to the operands' type, as the next product takes
+// them; sums are in 32 bits.  a and b are kept for the gradients as floats: kept
+// in bf16 they would be two roundings more on the way to each gradient, whose
+// distance from the exact one grew from 1.4 to 2.1 roundings of its own; writing
+// and reading them costs 4 bytes more a value, 2% of a training step's time.
+
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <new>
+#include <vector>
+
+#include "suika_step.h"
+#include "sr_step.h"
+#include "sr_tile.h"
+
+namespace {
+
+using namespace sr_step;
+using sr_tile::Block;
+using sr_tile::COL;
+using sr_tile::f32x4;
+using sr_tile::Grid;
+using sr_tile::Operand;
+using sr_tile::Product;
+using sr_tile::ROW;
+using sr_tile::Shared;
+using sr_tile::Side;
+
+// -------------------------------------------------------------- activations
+
+struct Act {
+  float value, slope;
+};
+
+// All three are a times a weight between 0 and 1.  exp overflows to infinity
+// for far negative a, where the weight is then 0.
+__device__ __forceinline__ float weight_of(float z) { return 1.0f / (1.0f + __expf(-z)); }
+
+constexpr float kTanhScale = 1.5957691216057308f;     // 2 sqrt(2 / pi)
+constexpr float kTanhCube = 0.044715f;
+
+template <bool SLOPE>
+__device__ __forceinline__ Act act(float a, int32_t kind) {
+  Act r{0, 0};
+  if (kind == SR_ACT_GELU) {
+    const float p = 0.5f * erfcf(a * -0.70710678118654752f);
+    r.value = a * p;
+    if (SLOPE) r.slope = fmaf(a * 0.39894228040143268f, __expf(-0.5f * a * a), p);
+    return r;
+  }
+  float z = a, dz = 1.0f;
+  if (kind == SR_ACT_GELU_TANH) {
+    const float q = a * a;
+    z = kTanhScale * fmaf(kTanhCube * q, a, a);
+    dz = kTanhScale * fmaf(3 * kTanhCube, q, 1.0f);
+  }
+  const float p = weight_of(z);
+  r.value = a * p;
+  // the rest of the weight, 1 - p, from the other side: nothing cancels
+  if (SLOPE) r.slope = fmaf(r.value * weight_of(-z), dz, p);
+  return r;
+}
+
+// Eight values of a row, n of which exist.
+template <typename T>
+__device__ __forceinline__ void store_row(T* p, const float (&v)[8], uint32_t n) {
+  if (n >= 8) {
+    if constexpr (sizeof(T) == 2) {
+      store<T, 8>(p, v);
+    } else {
+      const float lo[4] = {v[0], v[1], v[2], v[3]}, hi[4] = {v[4], v[5], v[6], v[7]};
+      store<T, 4>(p, lo);
+      store<T, 4>(p + 4, hi);
+    }
+  } else {
+    for (uint32_t e = 0; e < n; ++e) p[e] = static_cast<T>(v[e]);
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void load_row(const T* p, float (&v)[8], uint32_t n) {
+  if (n >= 8) {
+    if constexpr (sizeof(T) == 2) {
+      load<T, 8>(p, v);
+    } else {
+      float lo[4], hi[4];
+      load<T, 4>(p, lo);
+      load<T, 4>(p + 4, hi);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = lo[e], v[4 + e] = hi[e];
+    }
+  } else {
+#pragma unroll
+    for (uint32_t e = 0; e < 8; ++e) v[e] = e < n ? static_cast<float>(p[e]) : 0.0f;
+  }
+}
+
+// ------------------------------------------------------------------ products
+
+// What a workgroup of these kernels has of shared memory: two halves of both
+// operands, arrays of their own (see sr_tile::run), then the waves' slabs.
+#define SR_TILE_MEMORY(Tile)                                                     \
+  __shared__ __attribute__((aligned(1024))) char a0[Tile::PartA::kBytes];        \
+  __shared__ __attribute__((aligned(1024))) char a1[Tile::PartA::kBytes];        \
+  __shared__ __attribute__((aligned(1024))) char b0[Tile::PartB::kBytes];        \
+  __shared__ __attribute__((aligned(1024))) char b1[Tile::PartB::kBytes]
+
+struct ForwardArgs {
+  Product p;
+  Grid grid;
+  uint64_t h, a, b;           // a and b: kept for the gradients, or 0
+  uint64_t h_stride;          // elements
+  uint32_t tokens, ffn, padded;     // columns of h: those behind ffn are zeros
+  int32_t activation;
+};
+
+template <typename T, int SIZE>
+__global__ __launch_bounds__(sr_tile::threads(SIZE), 2) void forward_kernel(ForwardArgs t) {
+  typedef sr_tile::Tile<T, false, SIZE, ROW, ROW, true> Tile;
+  SR_TILE_MEMORY(Tile);
+  const uint32_t item = t.grid.item();
+  if (item >= t.grid.items) return;
+  uint32_t row, column;
+  sr_tile::banded(item, t.grid.rows, t.grid.columns, row, column);
+  row *= SIZE;
+  column *= Tile::kColumns;
+  Tile tile;
+  sr_tile::run(tile, t.p, row, column, 0, (t.p.k + Tile::kK - 1) / Tile::kK, (Shared)a0, (Shared)a1, (Shared)b0,
+               (Shared)b1);
+  __syncthreads();
+  tile.template results<false>(Tile::slab((Shared)a0, (Shared)a1, (Shared)b0, (Shared)b1), [&](uint32_t r, uint32_t n, const float (&a)[8], const float (&b)[8]) {
+    r += row;
+    n += column;
+    if (r >= t.tokens || n >= t.padded) return;
+    float h[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) h[e] = act<false>(a[e], t.activation).value * b[e];
+    store_row(global<T>(t.h) + r * t.h_stride + n, h, t.padded - n);
+    if (t.a && n < t.ffn) {
+      store_row(global<float>(t.a) + uint64_t(r) * t.ffn + n, a, t.ffn - n);
+      store_row(global<float>(t.b) + uint64_t(r) * t.ffn + n, b, t.ffn - n);
+    }
+  });
+}
+
+// dh = dy D, and from it da, db and h again: the same h as forward's, which is
+// not kept.
+struct BackwardArgs {
+  Product p;
+  Grid grid;
+  uint64_t a, b;              // kept
+  uint64_t da, db, h;         // 0: not wanted
+  uint64_t stride;            // of da, db and h
+  uint32_t tokens, ffn, padded;
+  int32_t activation;
+};
+
+template <typename T, int SIZE>
+__global__ __launch_bounds__(sr_tile::threads(SIZE), 2) void backward_kernel(BackwardArgs t) {
+  typedef sr_tile::Tile<T, false, SIZE, ROW, COL> Tile;
+  SR_TILE_MEMORY(Tile);
+  const uint32_t item = t.grid.item();
+  if (item >= t.grid.items) return;
+  uint32_t row, column;
+  sr_tile::banded(item, t.grid.rows, t.grid.columns, row, column);
+  row *= SIZE;
+  column *= SIZE;
+  Tile tile;
+  sr_tile::run(tile, t.p, row, column, 0, (t.p.k + Tile::kK - 1) / Tile::kK, (Shared)a0, (Shared)a1, (Shared)b0,
+               (Shared)b1);
+  __syncthreads();
+  tile.template results<false>(Tile::slab((Shared)a0, (Shared)a1, (Shared)b0, (Shared)b1), [&](uint32_t r, uint32_t n, const float (&dh)[8]) {
+    r += row;
+    n += column;
+    if (r >= t.tokens || n >= t.padded) return;
+    float a[8], b[8], da[8], db[8], h[8];
+    const uint32_t have = n < t.ffn ? t.ffn - n : 0;
+    load_row(global<const float>(t.a) + uint64_t(r) * t.ffn + n, a, have);
+    load_row(global<const float>(t.b) + uint64_t(r) * t.ffn + n, b, have);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const Act f = act<true>(a[e], t.activation);
+      h[e] = f.value * b[e];
+      db[e] = dh[e] * f.value;
+      da[e] = dh[e] * b[e] * f.slope;
+    }
+    const uint64_t at = r * t.stride + n;
+    if (t.da) {
+      store_row(global<T>(t.da) + at, da, t.padded - n);
+      store_row(global<T>(t.db) + at, db, t.padded - n);
+    }
+    if (t.h) store_row(global<T>(t.h) + at, h, t.padded - n);
+  });
+}
+
+// Plain products, up to three in a launch, or one with its steps split over
+// `splits` workgroups a tile, whose parts are joined in order afterwards.
+struct Job {
+  Product p;
+  uint32_t rows, columns;     // of C
+  uint32_t tile_rows, tile_columns, first;     // its first item
+  uint64_t out;               // dense
+};
+
+constexpr int kMostJobs = 3;
+
+struct ProductArgs {
+  Job job[kMostJobs];
+  uint32_t items;
+  uint32_t splits, steps;     // of one workgroup, where splits > 1
+  uint64_t parts;             // splits x rows x columns floats
+};
+
+template <typename T, int SIZE, Side A, Side B>
+__global__ __launch_bounds__(sr_tile::threads(SIZE), 2) void product_kernel(ProductArgs t) {
+  typedef sr_tile::Tile<T, false, SIZE, A, B> Tile;
+  SR_TILE_MEMORY(Tile);
+  uint32_t item = xcd_order(blockIdx.x, t.items);
+  if (item >= t.items) return;
+  int j = 0;
+#pragma unroll
+  for (int i = 1; i < kMostJobs; ++i) j = item >= t.job[i].first ? i : j;
+  const Job& job = t.job[j];
+  item -= job.first;
+  const uint32_t split = item % t.splits;
+  uint32_t row, column;
+  sr_tile::banded(item / t.splits, job.tile_rows, job.tile_columns, row, column);
+  row *= SIZE;
+  column *= SIZE;
+  const uint32_t steps = (job.p.k + Tile::kK - 1) / Tile::kK * (job.p.a2.data ? 2 : 1);
+  const uint32_t from = split * t.steps, to = t.splits == 1 ? steps : min(steps, from + t.steps);
+  Tile tile;
+  sr_tile::run(tile, job.p, row, column, from, to, (Shared)a0, (Shared)a1, (Shared)b0, (Shared)b1);
+  __syncthreads();
+  tile.template results<false>(Tile::slab((Shared)a0, (Shared)a1, (Shared)b0, (Shared)b1), [&](uint32_t r, uint32_t n, const float (&v)[8]) {
+    r += row;
+    n += column;
+    if (r >= job.rows || n >= job.columns) return;
+    const uint64_t at = uint64_t(r) * job.columns + n;
+    if (t.splits == 1) store_row(global<T>(job.out) + at, v, job.columns - n);
+    else store_row(global<float>(t.parts) + uint64_t(split) * job.rows * job.columns + at, v, job.columns - n);
+  });
+}
+
+constexpr int kPlainThreads = 256;
+
+// The sum of the parts, in order.
+template <typename T>
+__global__ __launch_bounds__(kPlainThreads) void join_kernel(const float* parts, uint32_t splits, uint64_t n, T* out) {
+  const uint64_t at = (uint64_t(blockIdx.x) * kPlainThreads + threadIdx.x) * 4;
+  if (at >= n) return;
+  const uint32_t have = n - at < 4 ? uint32_t(n - at) : 4;
+  float sum[4] = {0, 0, 0, 0};
+  for (uint32_t s = 0; s < splits; ++s) {
+    const float* p = parts + s * n + at;
+    if (have == 4) {
+      float x[4];
+      load<float, 4>(p, x);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sum[e] += x[e];
+    } else {
+      for (uint32_t e = 0; e < have; ++e) sum[e] += p[e];
+    }
+  }
+  if (have == 4) store<T, 4>(out + at, sum);
+  else
+    for (uint32_t e = 0; e < have; ++e) out[at + e] = static_cast<T>(sum[e]);
+}
+
+// A copy of rows that tiles can be loaded from: each starts at a multiple of 16
+// bytes and ends in zeros.
+template <typename T>
+__global__ __launch_bounds__(kPlainThreads) void align_kernel(const T* from, uint64_t stride, uint32_t columns, T* to,
+                                                              uint32_t padded) {
+  const uint32_t n = (blockIdx.y * kPlainThreads + threadIdx.x) * 8;
+  if (n >= padded) return;
+  float v[8];
+  load_row(from + blockIdx.x * stride + n, v, n < columns ? columns - n : 0);
+  store_row(to + uint64_t(blockIdx.x) * padded + n, v, padded - n);
+}
+
+// ---------------------------------------------------------------- few tokens
+
+// Up to 64 tokens: the matrices' bytes bound it, so their rows go from memory
+// straight to the matrix cores.  A workgroup has 16 rows (of G and of U) for all
+// tokens; its waves share out the k, and their sums are joined in shared memory.
+template <typename T> struct Thin;
+template <> struct Thin<bf16> {
+  typedef __bf16 Frag __attribute__((ext_vector_type(8)));
+  __device__ static void add(const Frag& a, const Frag& b, f32x4& c) {
+    c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+  }
+};
+template <> struct Thin<f16> {
+  typedef _Float16 Frag __attribute__((ext_vector_type(8)));
+  __device__ static void add(const Frag& a, const Frag& b, f32x4& c) {
+    c = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+  }
+};
+template <> struct Thin<float> {
+  typedef f32x4 Frag;
+  __device__ static void add(const Frag& a, const Frag& b, f32x4& c) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[j], b[j], c, 0, 0, 0);
+  }
+};
+
+struct ThinArgs {
+  uint64_t x, m, m2, out;     // m2: up, or 0
+  uint64_t x_stride, m_stride, m2_stride;     // elements
+  uint32_t tokens, rows, k, out_stride;
+  int32_t activation;
+};
+
+constexpr int kThinRows = 16;
+
+// GROUPS: of 16 tokens; WAVES: of a workgroup; GATED: two matrices and the
+// activation.
+template <typename T, int GROUPS, int WAVES, bool GATED>
+__global__ __launch_bounds__(WAVES * kWave) void thin_kernel(ThinArgs t) {
+  typedef Thin<T> K;
+  typedef typename K::Frag Frag;
+  constexpr int kEach = 16 / sizeof(T);       // k of a lane
+  constexpr int kSpan = 4 * kEach;            // of a wave's 16 x 16 block
+  constexpr int kAhead = 4;                   // of them on their way at once
+  constexpr int kMatrices = GATED ? 2 : 1;
+  const uint32_t lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+  const uint32_t row = min(blockIdx.x * kThinRows + lane % 16, t.rows - 1);
+  const uint32_t mine = lane / 16 * kEach;
+  const T* m[kMatrices];
+  m[0] = global<const T>(t.m) + row * t.m_stride;
+  if (GATED) m[kMatrices - 1] = global<const T>(t.m2) + row * t.m2_stride;
+  const T* x[GROUPS];
+#pragma unroll
+  for (int g = 0; g < GROUPS; ++g)
+    x[g] = global<const T>(t.x) + min(uint32_t(16 * g) + lane % 16, t.tokens - 1) * t.x_stride;
+  f32x4 c[kMatrices][GROUPS];
+#pragma unroll
+  for (int i = 0; i < kMatrices; ++i)
+#pragma unroll
+    for (int g = 0; g < GROUPS; ++g) c[i][g] = f32x4(0.0f);
+  auto read = [&](const T* p) { return *reinterpret_cast<const Vec<T, kEach>*>(p); };
+  const uint32_t blocks = t.k / (kSpan * kAhead);
+  for (uint32_t b = wave; b < blocks; b += WAVES) {
+    const uint32_t k = b * (kSpan * kAhead) + mine;
+    Frag w[kMatrices][kAhead], v[GROUPS][kAhead];
+#pragma unroll
+    for (int a = 0; a < kAhead; ++a)
+#pragma unroll
+      for (int i = 0; i < kMatrices; ++i) w[i][a] = read(m[i] + k + a * kSpan);
+#pragma unroll
+    for (int a = 0; a < kAhead; ++a)
+#pragma unroll
+      for (int g = 0; g < GROUPS; ++g) v[g][a] = read(x[g] + k + a * kSpan);
+#pragma unroll
+    for (int a = 0; a < kAhead; ++a)
+#pragma unroll
+      for (int g = 0; g < GROUPS; ++g)
+#pragma unroll
+        for (int i = 0; i < kMatrices; ++i) K::add(w[i][a], v[g][a], c[i][g]);
+  }
+  // what is left of k, a block at a time
+  const uint32_t rest = blocks * kSpan * kAhead;
+  for (uint32_t k0 = rest + wave * kSpan; k0 < t.k; k0 += WAVES * kSpan) {
+    const uint32_t k = k0 + mine;
+    auto tail = [&](const T* p) {
+      if (k + kEach <= t.k) return Frag(read(p + k));
+      Frag f;
+#pragma unroll
+      for (int e = 0; e < kEach; ++e) f[e] = k + e < t.k ? p[k + e] : T(0);
+      return f;
+    };
+    Frag w[kMatrices];
+#pragma unroll
+    for (int i = 0; i < kMatrices; ++i) w[i] = tail(m[i]);
+#pragma unroll
+    for (int g = 0; g < GROUPS; ++g) {
+      const Frag v = tail(x[g]);
+#pragma unroll
+      for (int i = 0; i < kMatrices; ++i) K::add(w[i], v, c[i][g]);
+    }
+  }
+  // four rows of a token a lane; the waves' sums in order
+  __shared__ f32x4 part[WAVES][kMatrices][GROUPS][kWave];
+#pragma unroll
+  for (int i = 0; i < kMatrices; ++i)
+#pragma unroll
+    for (int g = 0; g < GROUPS; ++g) part[wave][i][g][lane] = c[i][g];
+  __syncthreads();
+  if (wave >= GROUPS) return;
+  const uint32_t token = wave * 16 + lane % 16, first = blockIdx.x * kThinRows + lane / 16 * 4;
+  f32x4 sum[kMatrices];
+#pragma unroll
+  for (int i = 0; i < kMatrices; ++i) {
+    sum[i] = part[0][i][wave][lane];
+#pragma unroll
+    for (int w = 1; w < WAVES; ++w) sum[i] += part[w][i][wave][lane];
+  }
+  if (token >= t.tokens) return;
+  T* out = global<T>(t.out) + uint64_t(token) * t.out_stride;
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    if (first + r >= t.rows) return;
+    const float v = GATED ? act<false>(sum[0][r], t.activation).value * sum[kMatrices - 1][r] : sum[0][r];
+    out[first + r] = static_cast<T>(v);
+  }
+}
+
+// ---------------------------------------------------------------------- host
+
+constexpr uint64_t kFewTokens = 64;
+constexpr uint64_t kMostSide = uint64_t(1) << 20;     // hidden, ffn: an aligned row is within kMostStride
+
+uint64_t padded(uint64_t n) { return (n + 7) / 8 * 8; }
+uint64_t ceil_div(uint64_t n, uint64_t d) { return (n + d - 1) / d; }
+
+// Parts of a workspace, each at a multiple of 256 bytes.
+struct Space {
+  char* base;
+  uint64_t used = 0;
+
+  uint64_t take(uint64_t bytes) {
+    const uint64_t at = used;
+    used += (bytes + 255) / 256 * 256;
+    return reinterpret_cast<uint64_t>(base) + at;
+  }
+};
+
+// A user's matrix: rows of `columns` dense elements.
+struct Matrix {
+  const void* data;
+  uint64_t rows, columns, stride;
+};
+
+// Whether tiles can be loaded from it as it is.
+bool loadable(const Matrix& m, int size) {
+  return reinterpret_cast<uintptr_t>(m.data) % 16 == 0 && m.stride * size % 16 == 0 && m.columns * size % 16 == 0 &&
+         m.stride * size <= sr_tile::kMostStride;
+}
+
+// Rows of at most this many workgroups' grids: hidden and ffn beyond 65535 x 2048 columns do not occur.
+template <typename T>
+void launch_align(const Matrix& m, uint64_t to, hipStream_t stream) {
+  const uint32_t wide = uint32_t(padded(m.columns));
+  const dim3 grid(uint32_t(m.rows), uint32_t(ceil_div(wide, 8 * kPlainThreads)));
+  align_kernel<T><<<grid, kPlainThreads, 0, stream>>>(static_cast<const T*>(m.data), m.stride, uint32_t(m.columns),
+                                                      reinterpret_cast<T*>(to), wide);
+}
+
+// A matrix as an operand with its rows (ROW) or columns (COL) as C's; copied
+// to the workspace first where tiles cannot be loaded from it.  `launch` false:
+// only the workspace is counted.
+template <typename T>
+struct Loader {
+  Space& space;
+  bool launch;
+  hipStream_t stream;
+
+  // The address and the distance of rows in bytes.
+  Matrix ready(const Matrix& m) {
+    if (loadable(m, sizeof(T)) || m.rows == 0 || m.columns == 0) return m;
+    const uint64_t wide = padded(m.columns), to = space.take(m.rows * wide * sizeof(T));
+    if (launch) launch_align<T>(m, to, stream);
+    return {reinterpret_cast<const void*>(to), m.rows, m.columns, wide};
+  }
+};
+
+template <typename T>
+Operand operand(const Matrix& m, Side side) {
+  return {reinterpret_cast<uint64_t>(m.data), m.stride * sizeof(T),
+          uint32_t(side == ROW ? m.rows : m.columns)};
+}
+
+// Large tiles where there are enough of them for most compute units.
+constexpr uint64_t kManyTiles = 192;
+int tile_size(uint64_t rows, uint64_t columns) {
+  return ceil_div(rows, 256) * ceil_div(columns, 256) >= kManyTiles ? 256 : 128;
+}
+
+// Work items that a long sum is split for, and the least steps of a part.
+constexpr uint64_t kSplitItems = 512, kLeastSteps = 4;
+
+template <typename T, int SIZE, Side A, Side B>
+void launch_products(const ProductArgs& t, hipStream_t stream) {
+  product_kernel<T, SIZE, A, B><<<xcd_blocks(t.items), sr_tile::threads(SIZE), 0, stream>>>(t);
+}
+
+struct Wanted {
+  Product p;
+  uint64_t rows, columns;
+  void* out;
+};
+
+// One product, or several of the same operands' sides.  Where there are few
+// tiles and long sums (SPLIT), their steps are dealt out to several workgroups.
+template <typename T, Side A, Side B>
+int products(const char* who, const Wanted* w, int count, bool split, Space& space, bool launch, hipStream_t stream) {
+  uint64_t large = 0;
+  for (int i = 0; i < count; ++i) large += ceil_div(w[i].rows, 256) * ceil_div(w[i].columns, 256);
+  const bool f32 = sizeof(T) == 4;
+  const int size = !f32 && large >= kManyTiles ? 256 : 128;
+  ProductArgs t{};
+  uint64_t items = 0, steps = 0;
+  int n = 0;
+  for (int i = 0; i < count; ++i) {
+    if (w[i].rows == 0 || w[i].columns == 0) continue;
+    Job& j = t.job[n++];
+    j.p = w[i].p;
+    j.rows = uint32_t(w[i].rows);
+    j.columns = uint32_t(w[i].columns);
+    j.tile_rows = uint32_t(ceil_div(w[i].rows, size));
+    j.tile_columns = uint32_t(ceil_div(w[i].columns, size));
+    j.first = uint32_t(items);
+    j.out = reinterpret_cast<uint64_t>(w[i].out);
+    items += uint64_t(j.tile_rows) * j.tile_columns;
+    steps = ceil_div(w[i].p.k, 128 / sizeof(T)) * (w[i].p.a2.data ? 2 : 1);
+    if (items > sr_tile::kMostItems) return fail(SR_EBOUNDS, "%s: a product of %llu x %llu", who,
+                                                 (unsigned long long)w[i].rows, (unsigned long long)w[i].columns);
+  }
+  if (n == 0) return SR_OK;
+  for (int i = n; i < kMostJobs; ++i) t.job[i].first = 0xffffffffu;
+  t.splits = 1;
+  if (split && n == 1 && items < kSplitItems) {
+    // two workgroups of a 128 x 128 tile are on a compute unit at once
+    const uint64_t most = std::max<uint64_t>(1, std::min<uint64_t>(kSplitItems / items, steps / kLeastSteps));
+    t.steps = uint32_t(ceil_div(steps, most));
+    t.splits = uint32_t(std::max<uint64_t>(1, ceil_div(steps, std::max<uint32_t>(1, t.steps))));
+  }
+  const uint64_t elements = uint64_t(t.job[0].rows) * t.job[0].columns;
+  if (t.splits > 1) t.parts = space.take(t.splits * elements * sizeof(float));
+  if (!launch) return SR_OK;
+  t.items = uint32_t(items) * t.splits;
+  if constexpr (sizeof(T) == 4) launch_products<T, 128, A, B>(t, stream);
+  else if (size == 256) launch_products<T, 256, A, B>(t, stream);
+  else launch_products<T, 128, A, B>(t, stream);
+  if (t.splits > 1)
+    join_kernel<T><<<uint32_t(ceil_div(elements, 4 * kPlainThreads)), kPlainThreads, 0, stream>>>(
+        reinterpret_cast<const float*>(t.parts), t.splits, elements, reinterpret_cast<T*>(t.job[0].out));
+  return launched(who);
+}
+
+template <typename T, int GROUPS, bool GATED>
+void launch_thin(const ThinArgs& t, hipStream_t stream) {
+  constexpr int kWaves = 8;
+  thin_kernel<T, GROUPS, kWaves, GATED><<<uint32_t(ceil_div(t.rows, kThinRows)), kWaves * kWave, 0, stream>>>(t);
+}
+
+template <typename T, bool GATED>
+void thin(const ThinArgs& t, hipStream_t stream) {
+  if (t.rows == 0) return;
+  if (t.tokens <= 16) launch_thin<T, 1, GATED>(t, stream);
+  else if (t.tokens <= 32) launch_thin<T, 2, GATED>(t, stream);
+  else launch_thin<T, 4, GATED>(t, stream);
+}
+
+Matrix matrix_x(const sr_ffn_shape& s) { return {s.x, s.tokens, s.hidden, s.x_stride}; }
+Matrix matrix_gate(const sr_ffn_shape& s) { return {s.gate, s.ffn, s.hidden, s.gate_stride}; }
+Matrix matrix_up(const sr_ffn_shape& s) { return {s.up, s.ffn, s.hidden, s.up_stride}; }
+Matrix matrix_down(const sr_ffn_shape& s) { return {s.down, s.hidden, s.ffn, s.down_stride}; }
+
+// The block, or (launch false) only its workspace.
+template <typename T>
+int forward(const sr_ffn_shape& s, void* out, void* a, void* b, Space& space, bool launch, hipStream_t stream) {
+  if (s.tokens == 0) return SR_OK;
+  const uint64_t wide = padded(s.ffn);
+  const uint64_t h = space.take(s.tokens * wide * sizeof(T));
+  if (s.tokens <= kFewTokens && a == nullptr) {
+    if (!launch) return SR_OK;
+    ThinArgs g{reinterpret_cast<uint64_t>(s.x), reinterpret_cast<uint64_t>(s.gate), reinterpret_cast<uint64_t>(s.up), h,
+               s.x_stride, s.gate_stride, s.up_stride, uint32_t(s.tokens), uint32_t(s.ffn), uint32_t(s.hidden),
+               uint32_t(wide), s.activation};
+    thin<T, true>(g, stream);
+    ThinArgs d{h, reinterpret_cast<uint64_t>(s.down), 0, reinterpret_cast<uint64_t>(out), wide, s.down_stride, 0,
+               uint32_t(s.tokens), uint32_t(s.hidden), uint32_t(s.ffn), uint32_t(s.hidden), 0};
+    thin<T, false>(d, stream);
+    return launched("sr_ffn");
+  }
+  Loader<T> loader{space, launch, stream};
+  const Matrix x = loader.ready(matrix_x(s)), gate = loader.ready(matrix_gate(s)), up = loader.ready(matrix_up(s)),
+               down = loader.ready(matrix_down(s));
+  if (s.ffn) {
+    ForwardArgs t{};
+    t.p = {operand<T>(x, ROW), operand<T>(gate, ROW), {}, operand<T>(up, ROW), uint32_t(s.hidden)};
+    const int size = sizeof(T) == 4 ? 128 : tile_size(s.tokens, 2 * s.ffn);
+    const uint64_t rows = ceil_div(s.tokens, size), columns = ceil_div(wide, size / 2);
+    if (rows * columns > sr_tile::kMostItems)
+      return fail(SR_EBOUNDS, "sr_ffn: %llu tokens of %llu columns", (unsigned long long)s.tokens, (unsigned long long)s.ffn);
+    t.grid = {uint32_t(rows), uint32_t(columns), uint32_t(rows * columns)};
+    t.h = h;
+    t.a = reinterpret_cast<uint64_t>(a);
+    t.b = reinterpret_cast<uint64_t>(b);
+    t.h_stride = wide;
+    t.tokens = uint32_t(s.tokens);
+    t.ffn = uint32_t(s.ffn);
+    t.padded = uint32_t(wide);
+    t.activation = s.activation;
+    if (launch) {
+      const uint32_t blocks = xcd_blocks(t.grid.items);
+      if constexpr (sizeof(T) == 4) forward_kernel<T, 128><<<blocks, sr_tile::threads(128), 0, stream>>>(t);
+      else if (size == 256) forward_kernel<T, 256><<<blocks, sr_tile::threads(256), 0, stream>>>(t);
+      else forward_kernel<T, 128><<<blocks, sr_tile::threads(128), 0, stream>>>(t);
+      if (int rc = launched("sr_ffn")) return rc;
+    }
+  }
+  const Matrix hm{reinterpret_cast<const void*>(h), s.tokens, s.ffn, wide};
+  const Wanted w{{operand<T>(hm, ROW), operand<T>(down, ROW), {}, {}, uint32_t(s.ffn)}, s.tokens, s.hidden, out};
+  return products<T, ROW, ROW>("sr_ffn", &w, 1, true, space, launch, stream);
+}
+
+template <typename T>
+int backward(const sr_ffn_shape& s, const void* a, const void* b, const void* dy, uint64_t dy_stride,
+             const sr_ffn_grads& g, Space& space, bool launch, hipStream_t stream) {
+  const char* who = "sr_ffn_grad";
+  const uint64_t wide = padded(s.ffn), bytes = s.tokens * wide * sizeof(T);
+  Loader<T> loader{space, launch, stream};
+  const Matrix dym = loader.ready({dy, s.tokens, s.hidden, dy_stride});
+  const bool inner = g.x || g.gate || g.up;
+  const uint64_t da = inner ? space.take(bytes) : 0, db = inner ? space.take(bytes) : 0, h = g.down ? space.take(bytes) : 0;
+  if (s.tokens && s.ffn && (inner || g.down)) {
+    const Matrix down = loader.ready(matrix_down(s));
+    BackwardArgs t{};
+    t.p = {operand<T>(dym, ROW), operand<T>(down, COL), {}, {}, uint32_t(s.hidden)};
+    const int size = sizeof(T) == 4 ? 128 : tile_size(s.tokens, s.ffn);
+    const uint64_t rows = ceil_div(s.tokens, size), columns = ceil_div(wide, size);
+    if (rows * columns > sr_tile::kMostItems)
+      return fail(SR_EBOUNDS, "%s: %llu tokens of %llu columns", who, (unsigned long long)s.tokens, (unsigned long long)s.ffn);
+    t.grid = {uint32_t(rows), uint32_t(columns), uint32_t(rows * columns)};
+    t.a = reinterpret_cast<uint64_t>(a);
+    t.b = reinterpret_cast<uint64_t>(b);
+    t.da = da;
+    t.db = db;
+    t.h = h;
+    t.stride = wide;
+    t.tokens = uint32_t(s.tokens);
+    t.ffn = uint32_t(s.ffn);
+    t.padded = uint32_t(wide);
+    t.activation = s.activation;
+    if (launch) {
+      const uint32_t blocks = xcd_blocks(t.grid.items);
+      if constexpr (sizeof(T) == 4) backward_kernel<T, 128><<<blocks, sr_tile::threads(128), 0, stream>>>(t);
+      else if (size == 256) backward_kernel<T, 256><<<blocks, sr_tile::threads(256), 0, stream>>>(t);
+      else backward_kernel<T, 128><<<blocks, sr_tile::threads(128), 0, stream>>>(t);
+      if (int rc = launched(who)) return rc;
+    }
+  }
+  auto rows_of = [&](uint64_t p) { return Matrix{reinterpret_cast<const void*>(p), s.tokens, s.ffn, wide}; };
+  if (g.x) {
+    // dx = da G + db U, one sum over both
+    const Matrix gate = loader.ready(matrix_gate(s)), up = loader.ready(matrix_up(s));
+    const Wanted w{{operand<T>(rows_of(da), ROW), operand<T>(gate, COL), operand<T>(rows_of(db), ROW), operand<T>(up, COL),
+                    uint32_t(s.ffn)},
+                   s.tokens, s.hidden, g.x};
+    if (int rc = products<T, ROW, COL>(who, &w, 1, true, space, launch, stream)) return rc;
+  }
+  Wanted w[kMostJobs];
+  int n = 0;
+  if (g.gate || g.up) {
+    const Operand x = operand<T>(loader.ready(matrix_x(s)), COL);
+    if (g.gate) w[n++] = {{operand<T>(rows_of(da), COL), x, {}, {}, uint32_t(s.tokens)}, s.ffn, s.hidden, g.gate};
+    if (g.up) w[n++] = {{operand<T>(rows_of(db), COL), x, {}, {}, uint32_t(s.tokens)}, s.ffn, s.hidden, g.up};
+  }
+  if (g.down)
+    w[n++] = {{operand<T>(dym, COL), operand<T>(rows_of(h), COL), {}, {}, uint32_t(s.tokens)}, s.hidden, s.ffn, g.down};
+  return products<T, COL, COL>(who, w, n, false, space, launch, stream);
+}
+
+
+uint64_t extent(const Matrix& m, int size) {
+  return m.rows && m.columns ? ((m.rows - 1) * m.stride + m.columns) * size : 0;
+}
+
+int check_matrix(const char* who, const char* what, const Matrix& m, int size) {
+  if (m.stride < m.columns || m.stride > SR_STEP_MAX_ELEMENTS)
+    return fail(SR_EINVAL, "%s: rows of %s %llu elements apart, %llu columns", who, what, (unsigned long long)m.stride,
+                (unsigned long long)m.columns);
+  if (m.rows && m.columns && m.data == nullptr) return fail(SR_EINVAL, "%s: %s is null", who, what);
+  if (reinterpret_cast<uintptr_t>(m.data) % size) return fail(SR_EALIGN, "%s: %s is not aligned to its elements", who, what);
+  return SR_OK;
+}
+
+int check_shape(const char* who, const sr_ffn_shape* s) {
+  if (s == nullptr) return fail(SR_EINVAL, "%s: no shape", who);
+  if (!float_dtype(s->dtype)) return fail(SR_EDTYPE, "%s: dtype %d", who, s->dtype);
+  if (s->activation != SR_ACT_SILU && s->activation != SR_ACT_GELU && s->activation != SR_ACT_GELU_TANH)
+    return fail(SR_EINVAL, "%s: activation %d", who, s->activation);
+  if (s->tokens > SR_STEP_MAX_ROWS || s->hidden > kMostSide || s->ffn > kMostSide)
+    return fail(SR_EBOUNDS, "%s: %llu tokens, hidden %llu, ffn %llu", who, (unsigned long long)s->tokens,
+                (unsigned long long)s->hidden, (unsigned long long)s->ffn);
+  const int size = sr_internal::dtype_size(s->dtype);
+  if (int rc = check_matrix(who, "x", matrix_x(*s), size)) return rc;
+  if (int rc = check_matrix(who, "gate", matrix_gate(*s), size)) return rc;
+  if (int rc = check_matrix(who, "up", matrix_up(*s), size)) return rc;
+  return check_matrix(who, "down", matrix_down(*s), size);
+}
+
+// The memory of a call: what it writes overlaps nothing else.
+struct Memory {
+  std::vector<Extent> read, written;
+
+  bool clash() const {
+    for (size_t i = 0; i < written.size(); ++i) {
+      for (const Extent& r : read)
+        if (written[i].meets(r)) return true;
+      for (size_t j = 0; j < i; ++j)
+        if (written[i].meets(written[j])) return true;
+    }
+    return false;
+  }
+};
+
+Memory inputs_of(const sr_ffn_shape& s, int size) {
+  Memory m;
+  for (const Matrix& x : {matrix_x(s), matrix_gate(s), matrix_up(s), matrix_down(s)}) m.read.push_back({x.data, extent(x, size)});
+  return m;
+}
+
+int check_workspace(const char* who, const void* workspace, uint64_t bytes, uint64_t need) {
+  if (bytes < need || (need && workspace == nullptr))
+    return fail(SR_EINVAL, "%s: a workspace of %llu bytes, %llu are needed", who, (unsigned long long)bytes,
+                (unsigned long long)need);
+  if (reinterpret_cast<uintptr_t>(workspace) % 16) return fail(SR_EALIGN, "%s: the workspace is not aligned", who);
+  return SR_OK;
+}
+
+int check_out(const char* who, const char* what, const void* p, uint64_t n, int size) {
+  if (n && p == nullptr) return fail(SR_EINVAL, "%s: %s is null", who, what);
+  if (reinterpret_cast<uintptr_t>(p) % size) return fail(SR_EALIGN, "%s: %s is not aligned to its elements", who, what);
+  return SR_OK;
+}
+
+template <typename F>
+int typed(int32_t dtype, F&& f) {
+  if (dtype == SR_DT_F32) return f(float());
+  if (dtype == SR_DT_BF16) return f(bf16());
+  return f(f16());
+}
+
+int forward_of(const sr_ffn_shape& s, void* out, void* a, void* b, Space& space, bool launch, hipStream_t stream) {
+  return typed(s.dtype, [&](auto t) { return forward<decltype(t)>(s, out, a, b, space, launch, stream); });
+}
+
+int backward_of(const sr_ffn_shape& s, const void* a, const void* b, const void* dy, uint64_t dy_stride,
+                const sr_ffn_grads& g, Space& space, bool launch, hipStream_t stream) {
+  return typed(s.dtype, [&](auto t) { return backward<decltype(t)>(s, a, b, dy, dy_stride, g, space, launch, stream); });
+}
+
+}  // namespace
+
+extern "C" {
+
+int sr_ffn_workspace(const sr_ffn_shape* s, int32_t keep, uint64_t* bytes) {
+  if (bytes == nullptr) return fail(SR_EINVAL, "sr_ffn_workspace: null argument");
+  if (int rc = check_shape("sr_ffn_workspace", s)) return rc;
+  Space space{nullptr};
+  void* kept = keep ? reinterpret_cast<void*>(16) : nullptr;
+  if (int rc = forward_of(*s, nullptr, kept, kept, space, false, nullptr)) return rc;
+  *bytes = space.used;
+  return SR_OK;
+}
+
+int sr_ffn(const sr_ffn_shape* s, void* out, float* gate_out, float* up_out, void* workspace, uint64_t workspace_bytes,
+           hipStream_t stream) try {
+  const char* who = "sr_ffn";
+  if (int rc = check_shape(who, s)) return rc;
+  const int size = sr_internal::dtype_size(s->dtype);
+  if ((gate_out == nullptr) != (up_out == nullptr)) return fail(SR_EINVAL, "%s: gate_out and up_out go together", who);
+  if (int rc = check_out(who, "out", out, s->tokens * s->hidden, size)) return rc;
+  if (int rc = check_out(who, "gate_out", gate_out, 0, 4)) return rc;
+  if (int rc = check_out(who, "up_out", up_out, 0, 4)) return rc;
+  Space space{nullptr};
+  if (int rc = forward_of(*s, out, gate_out, up_out, space, false, nullptr)) return rc;
+  if (int rc = check_workspace(who, workspace, workspace_bytes, space.used)) return rc;
+  Memory m = inputs_of(*s, size);
+  m.written = {{out, s->tokens * s->hidden * size},
+               {gate_out, s->tokens * s->ffn * 4},
+               {up_out, s->tokens * s->ffn * 4},
+               {workspace, space.used}};
+  if (m.clash()) return fail(SR_EOVERLAP, "%s: an output or the workspace overlaps other memory of the call", who);
+  space = {static_cast<char*>(workspace)};
+  return forward_of(*s, out, gate_out, up_out, space, true, stream);
+} catch (const std::bad_alloc&) {
+  return fail(SR_ENOMEM, "sr_ffn: out of host memory");
+}
+
+int sr_ffn_grad_workspace(const sr_ffn_shape* s, const void* grad_out, uint64_t grad_out_stride, const sr_ffn_grads* grads,
+                          uint64_t* bytes) {
+  const char* who = "sr_ffn_grad_workspace";
+  if (bytes == nullptr || grads == nullptr) return fail(SR_EINVAL, "%s: null argument", who);
+  if (int rc = check_shape(who, s)) return rc;
+  if (int rc = check_matrix(who, "grad_out", {grad_out, s->tokens, s->hidden, grad_out_stride},
+                            sr_internal::dtype_size(s->dtype)))
+    return rc;
+  Space space{nullptr};
+  if (int rc = backward_of(*s, nullptr, nullptr, grad_out, grad_out_stride, *grads, space, false, nullptr)) return rc;
+  *bytes = space.used;
+  return SR_OK;
+}
+
+int sr_ffn_grad(const sr_ffn_shape* s, const float* gate_out, const float* up_out, const void* grad_out,
+                uint64_t grad_out_stride, const sr_ffn_grads* grads, void* workspace, uint64_t workspace_bytes,
+                hipStream_t stream) try {
+  const char* who = "sr_ffn_grad";
+  if (grads == nullptr) return fail(SR_EINVAL, "%s: null argument", who);
+  if (int rc = check_shape(who, s)) return rc;
+  const int size = sr_internal::dtype_size(s->dtype);
+  const Matrix dy{grad_out, s->tokens, s->hidden, grad_out_stride}, kept{nullptr, s->tokens, s->ffn, s->ffn};
+  if (int rc = check_matrix(who, "grad_out", dy, size)) return rc;
+  for (const float* p : {gate_out, up_out})
+    if (int rc = check_matrix(who, p == gate_out ? "gate_out" : "up_out", {p, kept.rows, kept.columns, kept.stride}, 4))
+      return rc;
+  const uint64_t inner = s->hidden * s->ffn;
+  for (const void* p : {grads->x, grads->gate, grads->up, grads->down})
+    if (int rc = check_out(who, "a gradient", p, 0, size)) return rc;
+  Space space{nullptr};
+  if (int rc = backward_of(*s, gate_out, up_out, grad_out, grad_out_stride, *grads, space, false, nullptr)) return rc;
+  if (int rc = check_workspace(who, workspace, workspace_bytes, space.used)) return rc;
+  Memory m = inputs_of(*s, size);
+  m.read.push_back({grad_out, extent(dy, size)});
+  m.read.push_back({gate_out, extent(kept, 4)});
+  m.read.push_back({up_out, extent(kept, 4)});
+  m.written = {{grads->x, s->tokens * s->hidden * size},
+               {grads->gate, inner * size},
+               {grads->up, inner * size},
+               {grads->down, inner * size},
+               {workspace, space.used}};
+  if (m.clash()) return fail(SR_EOVERLAP, "%s: a gradient or the workspace overlaps other memory of the call", who);
+  space = {static_cast<char*>(workspace)};
+  return backward_of(*s, gate_out, up_out, grad_out, grad_out_stride, *grads, space, true, stream);
+} catch (const std::bad_alloc&) {
+  return fail(SR_ENOMEM, "sr_ffn_grad: out of host memory");
+}
+
+}  // extern "C"

@@ -1,0 +1,429 @@
+// sr_tile.h -- products of matrices in tiles on the matrix cores, shared by
+// the operators on a share's matrices (not part of the C ABI).
+//
+//   C[m][n] = sum over k of A[m][k] B[n][k]
+//
+// Each operand is stored either with its k side by side (a row a line: ROW) or
+// with its rows side by side (a k a line: COL), so every product of a forward
+// and a backward pass works on the tensors as they are.  One workgroup of four
+// waves forms one tile of C, 256 x 256 or 128 x 128, as 2 x 2 squares of a wave
+// each, in 32 x 32 blocks.
+//
+//   - A step takes 128 bytes of every row: 64 values of 16 bits or 32 floats.
+//     They go from memory straight into shared memory, 16 bytes a lane, into
+//     the half that the step before has left, while the matrix cores work on
+//     the other one: one barrier a step.
+//   - 16-byte pieces are permuted within a line (by the lanes' addresses in
+//     memory, as the lanes' places in shared memory are fixed), so that eight
+//     lanes which read one column of pieces meet eight different bank groups.
+//   - COL operands of 16 bits are transposed on the way to the registers, by
+//     the read of shared memory that does so.
+//   - What lies outside an operand is read as zero: such lanes ask for an
+//     address beyond the buffer resource.
+//
+// A 256 x 256 tile reads 1 byte of memory for 128 operations of bf16, a wave
+// of it 1 byte of shared memory for 64: at 128 bytes a clock that is half of
+// what the matrix cores take.  128 x 128 tiles need twice as much of both, but
+// two workgroups share a compute unit; they serve products with few tiles.
+//
+// Values of 22 bits (TWO): a matrix as two of f16, the values rounded and what
+// the rounding lost, 32 of the one and 32 of the other in turn in every row.
+// The product of two such matrices is three products of f16, the one of the two
+// remainders, below 2^-22, left out; sums are in f32.
+#ifndef SR_TILE_H
+#define SR_TILE_H
+
+#include "sr_step.h"
+
+namespace sr_tile {
+
+using sr_step::bf16;
+using sr_step::f16;
+using sr_step::kWave;
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+typedef __attribute__((address_space(3))) char* Shared;
+
+constexpr int kLine = 128;                       // bytes of a row in a step
+constexpr uint32_t kOutside = 0x80000000u;       // an offset beyond every resource
+constexpr uint32_t kResource = 0x7fffffffu;
+constexpr uint64_t kMostStride = uint64_t(1) << 22;     // bytes from row to row: 256 rows within a resource
+
+constexpr int threads(int size) { return size == 256 ? 512 : 256; }
+
+enum Side { ROW, COL };
+
+// A matrix with its rows or its k side by side, as a kernel takes it.
+struct Operand {
+  uint64_t data;
+  uint64_t stride;     // bytes from line to line
+  uint32_t rows;       // values of a COL operand's line, or lines of a ROW one (padded: see TWO)
+};
+
+// ------------------------------------------------------- blocks of 32 x 32
+
+template <typename T> struct Block;
+
+template <> struct Block<bf16> {
+  typedef __bf16 Frag __attribute__((ext_vector_type(8)));
+  __device__ static void add(const Frag& b, const Frag& a, f32x16& c) {
+    c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(b, a, c, 0, 0, 0);
+  }
+};
+
+template <> struct Block<f16> {
+  typedef _Float16 Frag __attribute__((ext_vector_type(8)));
+  __device__ static void add(const Frag& b, const Frag& a, f32x16& c) {
+    c = __builtin_amdgcn_mfma_f32_32x32x16_f16(b, a, c, 0, 0, 0);
+  }
+};
+
+// Four k a lane: which four does not matter as long as both operands agree.
+template <> struct Block<float> {
+  typedef f32x4 Frag;
+  __device__ static void add(const Frag& b, const Frag& a, f32x16& c) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_32x32x2f32(b[j], a[j], c, 0, 0, 0);
+  }
+};
+
+// ---------------------------------------------------------------- operands
+
+// One operand's part of a tile: ROWS rows, a step's k.  PAIR: the rows of two
+// matrices in turn, 32 * PAIR of the one and as many of the other.
+template <typename T, bool TWO, Side SIDE, int ROWS, int PAIR, int kThreads>
+struct Part {
+  static constexpr int kEach = 16 / sizeof(T);                       // values of a piece
+  static constexpr int kK = kLine / int(sizeof(T)) / (TWO ? 2 : 1);  // of a step
+  static constexpr int kBytes = ROWS * kLine;
+  static constexpr int kLoads = kBytes / (kThreads * 16);
+  // pieces of a line in shared memory
+  static constexpr int kPieces = SIDE == ROW ? kLine / 16 : ROWS * int(sizeof(T)) * (TWO ? 2 : 1) / 16;
+  static constexpr int kLines = kThreads / kPieces;                  // of one load
+  static_assert(kThreads % kPieces == 0 && (PAIR == 0 || SIDE == ROW), "whole lines a load");
+
+  uint64_t data[2];       // of both matrices
+  uint32_t at[kLoads];     // bytes from data, or kOutside
+  uint32_t piece;          // of a line: which of its pieces this lane loads
+  uint64_t step;           // bytes from step to step
+
+  // How a piece's place in its line is permuted.
+  __device__ static uint32_t turn(uint32_t line) { return SIDE == ROW ? line & 7 : (line & 3) << 2; }
+
+  // Which matrix a wave's lines of a load are of.
+  static constexpr int kTurn = PAIR ? 32 * PAIR : 1;
+  __device__ __forceinline__ static int half_of(int i) {
+    if (!PAIR) return 0;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    return (i * kLines + wave * (kWave / kPieces)) / kTurn % 2;
+  }
+
+  // Rows from `first` on, k from `k` on.
+  __device__ __forceinline__ void start(const Operand& o, const Operand& other, uint32_t first, uint32_t k) {
+    const uint32_t line = threadIdx.x / kPieces;
+    piece = threadIdx.x % kPieces;
+    static_assert(SIDE == COL || kLines % 8 == 0, "a lane's lines are permuted alike");
+    step = SIDE == ROW ? kLine : kK * o.stride;
+    const uint64_t along = (TWO ? 2 : 1) * sizeof(T);
+    data[0] = o.data + (SIDE == ROW ? first * o.stride + k * along : first * along + k * o.stride);
+    if (PAIR) data[1] = other.data + first * other.stride + k * along;
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const uint32_t l = i * kLines + line;
+      if (SIDE == ROW) {
+        const uint32_t r = PAIR ? l / (2 * kTurn) * kTurn + l % kTurn : l;
+        const uint64_t mine = o.stride, others = other.stride, stride = PAIR && half_of(i) ? others : mine;
+        at[i] = first + r < o.rows ? uint32_t(r * stride) + (piece ^ turn(l)) * 16 : kOutside;
+      } else {
+        const uint32_t p = piece ^ turn(l);
+        at[i] = first * (TWO ? 2 : 1) + p * kEach < o.rows ? uint32_t(l * o.stride) + p * 16 : kOutside;
+      }
+    }
+    if (SIDE == ROW) piece ^= turn(line);
+  }
+
+  // Loads a step into shared memory; `left`: k from here to the end.
+  __device__ __forceinline__ void load(Shared to, uint32_t left) const {
+    const Shared mine = to + threadIdx.x / kWave * (kWave * 16);
+    const bool whole = left >= kK;
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      uint32_t offset = at[i];
+      if (!whole) {
+        const bool in = SIDE == ROW ? piece * kEach < left : i * kLines + threadIdx.x / kPieces < left;
+        offset = in ? offset : kOutside;
+      }
+      const uint64_t first = data[0], second = data[1];
+      const sr_step::Region from = sr_step::region(reinterpret_cast<void*>(half_of(i) ? second : first), kResource);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(from, mine + i * kThreads * 16, 16, offset, 0, 0, 0);
+    }
+  }
+
+  __device__ __forceinline__ void next() {
+    data[0] += step;
+    if (PAIR) data[1] += step;
+  }
+
+  // The block of 32 rows from `first` on (a multiple of 32), k group `s` of the
+  // step; LOW: of the remainders.
+  template <bool LOW>
+  __device__ static __forceinline__ typename Block<T>::Frag frag(Shared from, int first, int s) {
+    const uint32_t lane = threadIdx.x % kWave;
+    if constexpr (SIDE == ROW) {
+      const uint32_t line = first + lane % 32;
+      const uint32_t p = (2 * s + lane / 32 + (LOW ? 4 : 0)) ^ turn(line);
+      typedef __attribute__((address_space(3))) const typename Block<T>::Frag* Source;
+      return *(Source)(from + line * kLine + p * 16);
+    } else if constexpr (sizeof(T) == 2) {
+      // Sixteen lanes read 4 lines of 16 values and get a column of 4 each.
+      const uint32_t column = (TWO ? 2 : 1) * first + (LOW ? 32 : 0) + lane / 16 % 2 * 16 + lane % 4 * 4;
+      s16x4 half[2];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const uint32_t line = 16 * s + lane / 32 * 8 + 4 * j + lane % 16 / 4;
+        const uint32_t p = (column / 8) ^ turn(line);
+        typedef __attribute__((address_space(3))) s16x4* Source;
+        half[j] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Source)(from + line * (kPieces * 16) + p * 16 + column % 8 * 2));
+      }
+      const s16x8 both = __builtin_shufflevector(half[0], half[1], 0, 1, 2, 3, 4, 5, 6, 7);
+      return __builtin_bit_cast(typename Block<T>::Frag, both);
+    } else {
+      typename Block<T>::Frag f;
+      const uint32_t column = first + lane % 32;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t line = 8 * s + lane / 32 * 4 + j;
+        const uint32_t p = (column / 4) ^ turn(line);
+        typedef __attribute__((address_space(3))) const float* Source;
+        f[j] = *(Source)(from + line * (kPieces * 16) + p * 16 + column % 4 * 4);
+      }
+      return f;
+    }
+  }
+};
+
+// ------------------------------------------------------------------- tiles
+
+// One tile: T: the operands' type, TWO: values of 22 bits, SIZE: rows and
+// columns, A, B: how they are stored, PAIR: B's rows are those of two matrices
+// in turn, so that a wave has both products of the same columns.
+template <typename T, bool TWO_, int SIZE_, Side A, Side B, bool PAIR_ = false, int WAVES = threads(SIZE_) / kWave>
+struct Tile {
+  static constexpr int SIZE = SIZE_;
+  static constexpr bool TWO = TWO_, PAIR = PAIR_;
+  static constexpr int kThreads = WAVES * kWave;
+  static constexpr int kRows = SIZE / 2, kSpan = SIZE / (WAVES / 2);     // of a wave
+  static constexpr int kI = kRows / 32, kJ = kSpan / 32;
+  static constexpr int kColumns = PAIR ? SIZE / 2 : SIZE;     // of C
+  typedef Part<T, TWO, A, SIZE, 0, kThreads> PartA;
+  typedef Part<T, TWO, B, SIZE, PAIR ? kSpan / 64 : 0, kThreads> PartB;
+  static constexpr int kK = PartA::kK;
+  static constexpr int kGroups = kLine / 32 / (TWO ? 2 : 1);       // k groups of a step
+  static constexpr int kWide = 64 + 4;              // floats of a slab's row; four more turn the banks of the next
+  static constexpr int kSlab = 32 * kWide * 4;
+  static_assert(kI % 2 == 0 && kJ % 2 == 0, "slabs of two blocks");
+  static constexpr int kSlabs = SIZE * kLine / kSlab;       // in the memory of an operand
+  static_assert(WAVES <= 4 * kSlabs, "the waves' slabs fit where the operands were");
+
+  f32x16 c[kI][kJ];
+
+  __device__ __forceinline__ static int wave() { return __builtin_amdgcn_readfirstlane(threadIdx.x / kWave); }
+  __device__ __forceinline__ static int wave_row() { return wave() % 2 * kRows; }
+  __device__ __forceinline__ static int wave_column() { return wave() / 2 * kSpan; }
+
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int i = 0; i < kI; ++i)
+#pragma unroll
+      for (int j = 0; j < kJ; ++j) c[i][j] = f32x16(0.0f);
+  }
+
+  // The operands of a k group, read while the group before is multiplied.
+  struct Group {
+    typename Block<T>::Frag a[kI], b[kJ], low_a[TWO ? kI : 1], low_b[TWO ? kJ : 1];
+
+    __device__ __forceinline__ void read(Shared sa, Shared sb, int s) {
+      const int row = wave_row(), column = wave_column();
+#pragma unroll
+      for (int j = 0; j < kJ; ++j) b[j] = PartB::template frag<false>(sb, column + 32 * j, s);
+#pragma unroll
+      for (int i = 0; i < kI; ++i) a[i] = PartA::template frag<false>(sa, row + 32 * i, s);
+      if constexpr (TWO) {
+#pragma unroll
+        for (int j = 0; j < kJ; ++j) low_b[j] = PartB::template frag<true>(sb, column + 32 * j, s);
+#pragma unroll
+        for (int i = 0; i < kI; ++i) low_a[i] = PartA::template frag<true>(sa, row + 32 * i, s);
+      }
+    }
+  };
+
+  // One step's products.
+  __device__ __forceinline__ void products(Shared sa, Shared sb) {
+    typedef Block<T> K;
+    Group g[2];
+    g[0].read(sa, sb, 0);
+#pragma unroll
+    for (int s = 0; s < kGroups; ++s) {
+      Group& x = g[s % 2];
+      if (s + 1 < kGroups) g[(s + 1) % 2].read(sa, sb, s + 1);
+#pragma unroll
+      for (int i = 0; i < kI; ++i)
+#pragma unroll
+        for (int j = 0; j < kJ; ++j) {
+          K::add(x.b[j], x.a[i], c[i][j]);
+          if constexpr (TWO) {
+            K::add(x.b[j], x.low_a[i], c[i][j]);
+            K::add(x.low_b[j], x.a[i], c[i][j]);
+          }
+        }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+
+  // This wave's slab, where the operands were.
+  __device__ __forceinline__ static Shared slab(Shared a0, Shared a1, Shared b0, Shared b1) {
+    const int in = wave() / kSlabs;
+    return (in == 0 ? a0 : in == 1 ? a1 : in == 2 ? b0 : b1) + wave() % kSlabs * kSlab;
+  }
+
+  // The rows and columns of this wave, eight values a lane: f(row, column,
+  // values) with the row and the first column in the tile.  FLIP: of the
+  // transpose of C.  With PAIR, f(row, column, values, values of the second
+  // matrix).  `slab`: the wave's, no longer read as operands.
+  template <bool FLIP, typename F>
+  __device__ __forceinline__ void results(Shared slab, F&& f) const {
+    static_assert(!(FLIP && PAIR), "");
+    const uint32_t lane = threadIdx.x % kWave;
+    const int row0 = FLIP ? wave_column() : wave_row();
+    const int column0 = PAIR ? wave_column() / 2 : FLIP ? wave_row() : wave_column();
+    typedef __attribute__((address_space(3))) float* Floats;
+    typedef __attribute__((address_space(3))) f32x4* Fours;
+    const Floats mine = (Floats)slab;
+    constexpr int kDown = FLIP ? kJ : kI, kAcross = FLIP ? kI : kJ;      // blocks
+#pragma unroll
+    for (int i = 0; i < kDown; ++i)
+#pragma unroll
+      for (int j = 0; j < kAcross / 2; ++j) {
+        // two blocks; a lane has the column lane % 32 of a block's transpose, four rows together
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int across = PAIR ? j + h * (kAcross / 2) : 2 * j + h;
+          const f32x16& x = FLIP ? c[across][i] : c[i][across];
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const int n = 8 * q + lane / 32 * 4;
+            if (!FLIP) {
+              *(Fours)(mine + lane % 32 * kWide + 32 * h + n) = f32x4{x[4 * q], x[4 * q + 1], x[4 * q + 2], x[4 * q + 3]};
+            } else {
+#pragma unroll
+              for (int r = 0; r < 4; ++r) mine[(n + r) * kWide + 32 * h + lane % 32] = x[4 * q + r];
+            }
+          }
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");     // the wave's own writes, read by other lanes
+        __builtin_amdgcn_wave_barrier();
+        constexpr int kLanes = (PAIR ? 32 : 64) / 8;     // of a row
+#pragma unroll 1
+        for (int p = 0; p < 32 * kLanes / kWave; ++p) {
+          const int r = p * (kWave / kLanes) + lane / kLanes, n = lane % kLanes * 8;
+          float v[8], w[8];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const f32x4 x = *(Fours)(mine + r * kWide + n + 4 * h);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[4 * h + e] = x[e];
+            if constexpr (PAIR) {
+              const f32x4 y = *(Fours)(mine + r * kWide + 32 + n + 4 * h);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) w[4 * h + e] = y[e];
+            }
+          }
+          const uint32_t to_row = row0 + 32 * i + r, to_column = column0 + (PAIR ? 32 : 64) * j + n;
+          if constexpr (PAIR) f(to_row, to_column, v, w);
+          else f(to_row, to_column, v);
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
+        __builtin_amdgcn_wave_barrier();
+      }
+  }
+};
+
+// Two operands, and a second pair whose products are added (its data 0: none)
+// or, with PAIR, whose B has the second matrix's rows.
+struct Product {
+  Operand a, b, a2, b2;
+  uint32_t k;          // of one pair
+};
+
+// All steps from `from` to `to` (steps of the second pair are counted on) of
+// the tile at (row, column).  A macro's worth of memory: the halves are arrays
+// of their own, so that a read of the one does not wait for loads to the other.
+template <typename Tile>
+__device__ __forceinline__ void run(Tile& tile, const Product& p, uint32_t row, uint32_t column, uint32_t from,
+                                    uint32_t to, Shared a0, Shared a1, Shared b0, Shared b1) {
+  typename Tile::PartA a;
+  typename Tile::PartB b;
+  const uint32_t each = (p.k + Tile::kK - 1) / Tile::kK;     // steps of a pair
+  uint32_t left = 0;
+  auto seek = [&](uint32_t s) {
+    const bool second = !Tile::PAIR && s >= each;
+    const uint32_t k = (second ? s - each : s) * Tile::kK;
+    a.start(second ? p.a2 : p.a, p.a2, row, k);
+    b.start(second ? p.b2 : p.b, p.b2, column, k);
+    left = p.k - k;
+  };
+  auto fetch = [&](uint32_t s, Shared to_a, Shared to_b) {
+    if (!Tile::PAIR && s == each) seek(s);
+    a.load(to_a, left);
+    b.load(to_b, left);
+    a.next();
+    b.next();
+    left -= Tile::kK;
+  };
+  tile.clear();
+  if (from >= to) return;
+  seek(from);
+  fetch(from, a0, b0);
+  uint32_t s = from;
+  for (; s + 2 <= to; s += 2) {
+    __syncthreads();      // the loads have arrived, and the other half is read
+    fetch(s + 1, a1, b1);
+    tile.products(a0, b0);
+    __syncthreads();
+    if (s + 2 < to) fetch(s + 2, a0, b0);
+    tile.products(a1, b1);
+  }
+  if (s < to) {
+    __syncthreads();
+    tile.products(a0, b0);
+  }
+}
+
+// Tiles of a product, items of a launch, and the order that workgroups take
+// them in: neighbours on one die, where they share rows and columns.
+struct Grid {
+  uint32_t rows, columns;
+  uint32_t items;
+
+  __device__ __forceinline__ uint32_t item() const { return sr_step::xcd_order(blockIdx.x, items); }
+};
+
+// Most workgroups of a launch: a grid has fewer than 2^32 threads, 512 a workgroup.
+constexpr uint64_t kMostItems = (uint64_t(1) << 23) - 2 * sr_step::kXcds;
+
+// The tile of a work item, in bands of 8 tiles' rows: the tiles of neighbouring
+// items share rows and columns.
+__device__ __forceinline__ void banded(uint32_t item, uint32_t rows, uint32_t columns, uint32_t& row, uint32_t& column) {
+  constexpr uint32_t kBand = 8;
+  const uint32_t band = item / (kBand * columns) * kBand, in = item - band * columns;
+  const uint32_t high = rows - band < kBand ? rows - band : kBand;
+  row = band + in % high;
+  column = in / high;
+}
+
+}  // namespace sr_tile
+
+#endif  // SR_TILE_H

@@ -541,6 +541,110 @@ at::Tensor token_logprobs_grad(const at::Tensor& logits, const at::Tensor& targe
   return to;
 }
 
+// --------------------------------------------------------- feed-forward block
+
+int32_t activation_code(const std::string& name) {
+  if (name == "silu") return SR_ACT_SILU;
+  if (name == "gelu") return SR_ACT_GELU;
+  if (name == "gelu_tanh") return SR_ACT_GELU_TANH;
+  plan_error("activation: " + name + ", not silu, gelu or gelu_tanh");
+}
+
+// A block's tensors; x and what has its shape may have any number of dimensions.
+sr_ffn_shape ffn_shape(const at::Tensor& x, const at::Tensor& gate, const at::Tensor& up, const at::Tensor& down,
+                       const std::string& activation) {
+  const struct { const at::Tensor& t; const char* what; } all[4] = {{x, "x"}, {gate, "gate"}, {up, "up"}, {down, "down"}};
+  if (x.dim() < 1) plan_error("x: rows of hidden elements are wanted");
+  if (!x.is_cuda()) plan_error("x is on " + x.device().str() + ", not on the GPU");
+  for (const auto& a : all) {
+    check_device(a.t, a.what, x.device());
+    check_tangent(a.t, a.what);
+    if (a.t.scalar_type() != x.scalar_type())
+      plan_error(std::string(a.what) + ": dtype " + c10::toString(a.t.scalar_type()) + ", x has " +
+                 c10::toString(x.scalar_type()));
+  }
+  const int32_t dtype = float_code(x, "x");
+  for (int i = 1; i < 4; ++i)
+    if (all[i].t.dim() != 2) plan_error(std::string(all[i].what) + ": a matrix is wanted");
+  const int64_t hidden = x.size(-1), ffn = gate.size(0);
+  if (gate.size(1) != hidden || up.size(0) != ffn || up.size(1) != hidden || down.size(0) != hidden || down.size(1) != ffn)
+    plan_error("gate and up of ffn x hidden and down of hidden x ffn are wanted, not " + c10::str(gate.sizes()) + ", " +
+               c10::str(up.sizes()) + " and " + c10::str(down.sizes()) + " for " + std::to_string(hidden));
+  int64_t tokens = 1;
+  for (int64_t d = 0; d + 1 < x.dim(); ++d) tokens *= x.size(d);
+  return {x.data_ptr(), gate.data_ptr(), up.data_ptr(), down.data_ptr(), uint64_t(tokens), uint64_t(hidden), uint64_t(ffn),
+          row_stride(x, "x"), row_stride(gate, "gate"), row_stride(up, "up"), row_stride(down, "down"), dtype,
+          activation_code(activation)};
+}
+
+py::tuple gated_ffn(const at::Tensor& x, const at::Tensor& gate, const at::Tensor& up, const at::Tensor& down,
+                    const std::string& activation, bool keep) {
+  const sr_ffn_shape s = ffn_shape(x, gate, up, down, activation);
+  const c10::DeviceGuard guard(x.device());
+  const at::TensorOptions like = on(x.device(), x.scalar_type());
+  uint64_t need = 0;
+  check(sr_ffn_workspace(&s, keep, &need), "sr_ffn");
+  const at::Tensor out = at::empty(x.sizes(), like), work = at::empty({int64_t(need)}, on(x.device(), at::kByte));
+  at::Tensor a, b;
+  if (keep) {
+    std::vector<int64_t> shape(x.sizes().begin(), x.sizes().end());
+    shape.back() = int64_t(s.ffn);
+    a = at::empty(shape, on(x.device(), at::kFloat));
+    b = at::empty(shape, on(x.device(), at::kFloat));
+  }
+  check(sr_ffn(&s, out.data_ptr(), keep ? a.data_ptr<float>() : nullptr, keep ? b.data_ptr<float>() : nullptr,
+               work.data_ptr(), need,
+               stream_of(x.device())),
+        "sr_ffn");
+  if (!keep) return py::make_tuple(out);
+  return py::make_tuple(out, a, b);
+}
+
+py::tuple gated_ffn_grad(const at::Tensor& x, const at::Tensor& gate, const at::Tensor& up, const at::Tensor& down,
+                         const at::Tensor& kept_gate, const at::Tensor& kept_up, const at::Tensor& grad_output,
+                         const std::string& activation, const std::vector<bool>& wanted) {
+  const sr_ffn_shape s = ffn_shape(x, gate, up, down, activation);
+  if (wanted.size() != 4) plan_error("wanted: one of each of x, gate, up and down");
+  std::vector<int64_t> shape(x.sizes().begin(), x.sizes().end());
+  shape.back() = int64_t(s.ffn);
+  const struct { const at::Tensor& t; const char* what; at::IntArrayRef shape; at::ScalarType type; } given[3] = {
+      {kept_gate, "kept_gate", shape, at::kFloat},
+      {kept_up, "kept_up", shape, at::kFloat},
+      {grad_output, "grad_output", x.sizes(), x.scalar_type()}};
+  for (const auto& g : given) {
+    check_device(g.t, g.what, x.device());
+    check_tangent(g.t, g.what);
+    if (g.t.scalar_type() != g.type || g.t.sizes() != g.shape)
+      plan_error(std::string(g.what) + ": " + c10::str(g.shape) + " of " + c10::toString(g.type) + " is wanted, not " +
+                 c10::str(g.t.sizes()) + " of " + c10::toString(g.t.scalar_type()));
+  }
+  for (const at::Tensor* t : {&kept_gate, &kept_up}) {
+    if (!t->is_contiguous()) plan_error("kept_gate and kept_up: contiguous tensors are wanted");
+    check_stored(*t, "kept_gate or kept_up");
+  }
+  const uint64_t stride = row_stride(grad_output, "grad_output");
+  const c10::DeviceGuard guard(x.device());
+  const at::Tensor* like[4] = {&x, &gate, &up, &down};
+  at::Tensor grad[4];
+  void* to[4] = {};
+  // an empty tensor has no address: what is wanted of it is nothing
+  for (int i = 0; i < 4; ++i) {
+    if (!wanted[i]) continue;
+    grad[i] = at::empty(like[i]->sizes(), on(x.device(), x.scalar_type()));
+    to[i] = grad[i].data_ptr();
+  }
+  const sr_ffn_grads g{to[0], to[1], to[2], to[3]};
+  uint64_t need = 0;
+  check(sr_ffn_grad_workspace(&s, grad_output.data_ptr(), stride, &g, &need), "sr_ffn_grad");
+  const at::Tensor work = at::empty({int64_t(need)}, on(x.device(), at::kByte));
+  check(sr_ffn_grad(&s, kept_gate.data_ptr<float>(), kept_up.data_ptr<float>(), grad_output.data_ptr(), stride, &g, work.data_ptr(), need,
+                    stream_of(x.device())),
+        "sr_ffn_grad");
+  py::tuple out(4);
+  for (int i = 0; i < 4; ++i) out[i] = wanted[i] ? py::cast(grad[i]) : py::none();
+  return out;
+}
+
 }  // namespace
 
 namespace suika_host {
@@ -564,6 +668,10 @@ void bind_step(py::module_& m) {
   m.def("token_logprobs_grad", &token_logprobs_grad, py::arg("logits"), py::arg("targets"), py::arg("lse"),
         py::arg("entropy"), py::arg("grad_logprob"), py::arg("grad_entropy"), py::arg("vocab"), py::arg("out"),
         py::arg("lse_low"));
+  m.def("gated_ffn", &gated_ffn, py::arg("x"), py::arg("gate"), py::arg("up"), py::arg("down"), py::arg("activation"),
+        py::arg("keep"));
+  m.def("gated_ffn_grad", &gated_ffn_grad, py::arg("x"), py::arg("gate"), py::arg("up"), py::arg("down"),
+        py::arg("kept_gate"), py::arg("kept_up"), py::arg("grad_output"), py::arg("activation"), py::arg("wanted"));
 }
 
 }  // namespace suika_host

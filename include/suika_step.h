@@ -23,6 +23,9 @@
  *       the gated feed-forward block of a share and its gradients.  In the
  *       reference it is the blocks' mlp, gate and up column parallel and down
  *       row parallel (Suika/models/llama_model.py:16-35)
+ *   sr_orthogonalize, sr_muon
+ *       matrices made orthogonal by Newton-Schulz products, and the Muon update
+ *       of a share's matrices, beside the reference's torch.optim.AdamW
  *
  * Conventions
  *   - All device memory, workspaces included, belongs to the caller.
@@ -279,6 +282,92 @@ int sr_ffn_grad_workspace(const sr_ffn_shape* shape, const void* grad_out, uint6
 int sr_ffn_grad(const sr_ffn_shape* shape, const float* gate_out, const float* up_out, const void* grad_out,
                 uint64_t grad_out_stride, const sr_ffn_grads* grads, void* workspace, uint64_t workspace_bytes,
                 hipStream_t stream);
+
+#define SR_MAX_NEWTON_SCHULZ 64
+
+/* Sums count values (SR_DT_F32 or SR_DT_F64) at data over the ranks, in place
+ * and in the order of the stream.  Not 0: the call ends with SR_EINVAL. */
+typedef int (*sr_reduce)(void* context, void* data, uint64_t count, int32_t dtype, hipStream_t stream);
+
+/* X = G / max(|G|, eps) with the norm of all elements, then steps times X <-
+ * a X + b (X X^T) X + c (X X^T)^2 X, with a, b and c from coefficients
+ * [steps][3].  The singular values of X, 1 at most at first, have to stay at
+ * 1.9 or less, and a + b s^2 + c s^4 within +-15 (SR_EINVAL).  Values of X below
+ * 2^-38 count as 0. */
+typedef struct sr_newton_schulz {
+  int32_t steps;                /* 1 to SR_MAX_NEWTON_SCHULZ */
+  int32_t reserved;             /* must be 0 */
+  const double* coefficients;   /* in host memory */
+  double eps;
+  sr_reduce reduce;             /* NULL: no matrix is split */
+  void* reduce_context;
+} sr_newton_schulz;
+
+/* A matrix with rows of dense elements.  split: -1, or the dimension (0: rows,
+ * 1: columns) that is cut over the ranks, of which this is one's part.  All
+ * ranks then call with the same list, and reduce is called equally often on
+ * each, also where a part has no elements. */
+typedef struct sr_matrix {
+  void* data;
+  uint64_t rows;
+  uint64_t cols;
+  uint64_t stride;    /* elements between rows */
+  int32_t dtype;      /* SR_DT_F32, SR_DT_BF16 or SR_DT_F16 */
+  int32_t split;
+} sr_matrix;
+
+/*
+ * dst[i] = the last X of G = src[i]; sides of at most 2^19.  Products are of 22
+ * bits a value in sums of 32 bits.  A matrix may be its own result; otherwise
+ * what is written overlaps nothing else (SR_EOVERLAP).  workspace:
+ * sr_orthogonalize_workspace bytes (16 for a value of X and 8 for a value of X
+ * X^T, of at most 8 GiB of matrices at a time or of one).  split of dst is not
+ * read.
+ */
+int sr_orthogonalize_workspace(const sr_matrix* src, const sr_matrix* dst, int32_t count, const sr_newton_schulz* ns,
+                               uint64_t* bytes);
+int sr_orthogonalize(const sr_matrix* src, const sr_matrix* dst, int32_t count, const sr_newton_schulz* ns, void* workspace,
+                     uint64_t workspace_bytes, hipStream_t stream);
+
+/* One parameter's fields, dense [rows][cols]; param as in sr_adamw_tensor. */
+typedef struct sr_muon_tensor {
+  void* weight;          /* master, or the parameter: f32 or bf16 */
+  void* exp_avg;
+  void* param;           /* bf16 copy, or NULL */
+  const void* grad;
+  uint64_t rows;
+  uint64_t cols;
+  double scale;          /* of this matrix's update, times lr */
+  int32_t weight_dtype;  /* SR_DT_F32 or SR_DT_BF16 (no param then) */
+  int32_t moment_dtype;  /* SR_DT_F32 or SR_DT_BF16 */
+  int32_t grad_dtype;    /* SR_DT_F32 or SR_DT_BF16 */
+  int32_t split;         /* as in sr_matrix */
+  int64_t reserved;      /* must be 0 */
+} sr_muon_tensor;
+
+typedef struct sr_muon_options {
+  double lr;
+  double weight_decay;
+  double momentum;
+  int32_t nesterov;
+  int32_t reserved;           /* must be 0 */
+  double max_norm;            /* with square_sum: the gradients are clipped to it */
+  const double* square_sum;   /* as for sr_adamw */
+} sr_muon_options;
+
+/*
+ * One Muon update in place: exp_avg = momentum exp_avg + (1 - momentum) g; G =
+ * momentum exp_avg + (1 - momentum) g with nesterov, else exp_avg, as it is
+ * stored; weight = weight (1 - lr weight_decay) - lr scale X with the last X of
+ * G.  Fields that are written overlap no others (SR_EOVERLAP).  It holds no
+ * step number and can be captured where reduce can.  A reduce that fails leaves
+ * the moments updated and the weights of its matrices as they were.  workspace:
+ * sr_muon_workspace bytes; that call makes all of sr_muon's checks.
+ */
+int sr_muon_workspace(const sr_muon_tensor* tensors, int32_t count, const sr_muon_options* options, const sr_newton_schulz* ns,
+                      uint64_t* bytes);
+int sr_muon(const sr_muon_tensor* tensors, int32_t count, const sr_muon_options* options, const sr_newton_schulz* ns,
+            void* workspace, uint64_t workspace_bytes, hipStream_t stream);
 
 #ifdef __cplusplus
 }

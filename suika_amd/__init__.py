@@ -19,6 +19,7 @@ from .plan import PlanOptions, ReshardPlan, SlotSpec
 from ._lib import PlanError, ReshardError
 from .checkpoint import checkpoint_load, checkpoint_save, migration_load, migration_save
 from .handoff import HandoffError, dummy_migration_IPC_state_dict
+from .muon import ShardMuon, orthogonalize, split_matrices
 from .optim import ShardAdamW, clip_grads, counted_names, grad_norm, grad_square_sum
 from .ffn import GatedFFN, gated_ffn, gated_ffn_grad
 from .vocab import TokenLogprobs, token_logprobs, token_logprobs_grad, vocab_embedding, vocab_embedding_grad
@@ -34,4 +35,5 @@ __all__ = [
     "ShardAdamW", "clip_grads", "counted_names", "grad_norm", "grad_square_sum",
     "vocab_embedding", "vocab_embedding_grad", "TokenLogprobs", "token_logprobs", "token_logprobs_grad",
     "GatedFFN", "gated_ffn", "gated_ffn_grad",
+    "ShardMuon", "orthogonalize", "split_matrices",
 ]

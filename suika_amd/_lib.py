@@ -95,6 +95,10 @@ EXPORTED_SYMBOLS = (
     "sr_ffn",
     "sr_ffn_grad_workspace",
     "sr_ffn_grad",
+    "sr_orthogonalize_workspace",
+    "sr_orthogonalize",
+    "sr_muon_workspace",
+    "sr_muon",
 )
 
 # Largest hand-off allocation (SR_HANDOFF_MAX_BYTES, include/suika_handoff.h).

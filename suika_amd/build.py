@@ -12,7 +12,8 @@ host memory, through pinned windows and a host thread pool), ``optim.hip``
 (gradient norm, clipping and the AdamW update of a share's state),
 ``embed.hip`` (rows of a vocabulary shard and their gradient),
 ``logprob.hip`` (token log probabilities and the gradient of the logits),
-``ffn.hip`` (the gated feed-forward block and its gradients).
+``ffn.hip`` (the gated feed-forward block and its gradients), ``muon.hip``
+(matrices made orthogonal and the Muon update).
 
 ``build_host`` compiles ``host_bind.cpp`` and ``step_bind.cpp`` into
 ``suika_amd/lib/_suika_host.so``, the CPython extension (on torch's C++ API)
@@ -34,7 +35,8 @@ REPO_DIR = PKG_DIR.parent
 SOURCES = [PKG_DIR / "csrc" / "reshard.hip", PKG_DIR / "csrc" / "schedule.cpp",
            PKG_DIR / "csrc" / "lower.cpp", PKG_DIR / "csrc" / "handoff.cpp", PKG_DIR / "csrc" / "stage.cpp",
            PKG_DIR / "csrc" / "optim.hip", PKG_DIR / "csrc" / "embed.hip",
-           PKG_DIR / "csrc" / "logprob.hip", PKG_DIR / "csrc" / "ffn.hip"]
+           PKG_DIR / "csrc" / "logprob.hip", PKG_DIR / "csrc" / "ffn.hip",
+           PKG_DIR / "csrc" / "muon.hip"]
 INCLUDE = REPO_DIR / "include"
 LIB_DIR = PKG_DIR / "lib"
 LIB = LIB_DIR / "libsuika_reshard.so"

@@ -74,49 +74,7 @@ __device__ __forceinline__ Act act(float a, int32_t kind) {
   return r;
 }
 
-// Eight values of a row, n of which exist.
-template <typename T>
-__device__ __forceinline__ void store_row(T* p, const float (&v)[8], uint32_t n) {
-  if (n >= 8) {
-    if constexpr (sizeof(T) == 2) {
-      store<T, 8>(p, v);
-    } else {
-      const float lo[4] = {v[0], v[1], v[2], v[3]}, hi[4] = {v[4], v[5], v[6], v[7]};
-      store<T, 4>(p, lo);
-      store<T, 4>(p + 4, hi);
-    }
-  } else {
-    for (uint32_t e = 0; e < n; ++e) p[e] = static_cast<T>(v[e]);
-  }
-}
-
-template <typename T>
-__device__ __forceinline__ void load_row(const T* p, float (&v)[8], uint32_t n) {
-  if (n >= 8) {
-    if constexpr (sizeof(T) == 2) {
-      load<T, 8>(p, v);
-    } else {
-      float lo[4], hi[4];
-      load<T, 4>(p, lo);
-      load<T, 4>(p + 4, hi);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = lo[e], v[4 + e] = hi[e];
-    }
-  } else {
-#pragma unroll
-    for (uint32_t e = 0; e < 8; ++e) v[e] = e < n ? static_cast<float>(p[e]) : 0.0f;
-  }
-}
-
 // ------------------------------------------------------------------ products
-
-// What a workgroup of these kernels has of shared memory: two halves of both
-// operands, arrays of their own (see sr_tile::run), then the waves' slabs.
-#define SR_TILE_MEMORY(Tile)                                                     \
-  __shared__ __attribute__((aligned(1024))) char a0[Tile::PartA::kBytes];        \
-  __shared__ __attribute__((aligned(1024))) char a1[Tile::PartA::kBytes];        \
-  __shared__ __attribute__((aligned(1024))) char b0[Tile::PartB::kBytes];        \
-  __shared__ __attribute__((aligned(1024))) char b1[Tile::PartB::kBytes]
 
 struct ForwardArgs {
   Product p;
@@ -131,7 +89,7 @@ template <typename T, int SIZE>
 __global__ __launch_bounds__(sr_tile::threads(SIZE), 2) void forward_kernel(ForwardArgs t) {
   typedef sr_tile::Tile<T, false, SIZE, ROW, ROW, true> Tile;
   SR_TILE_MEMORY(Tile);
-  const uint32_t item = t.grid.item();
+  const uint32_t item = sr_tile::item_of(blockIdx.x, t.grid.items, SIZE);
   if (item >= t.grid.items) return;
   uint32_t row, column;
   sr_tile::banded(item, t.grid.rows, t.grid.columns, row, column);
@@ -141,7 +99,8 @@ __global__ __launch_bounds__(sr_tile::threads(SIZE), 2) void forward_kernel(Forw
   sr_tile::run(tile, t.p, row, column, 0, (t.p.k + Tile::kK - 1) / Tile::kK, (Shared)a0, (Shared)a1, (Shared)b0,
                (Shared)b1);
   __syncthreads();
-  tile.template results<false>(Tile::slab((Shared)a0, (Shared)a1, (Shared)b0, (Shared)b1), [&](uint32_t r, uint32_t n, const float (&a)[8], const float (&b)[8]) {
+  tile.template results<false, false>(SR_TILE_SLAB(Tile), sr_tile::nothing, [&](uint32_t r, uint32_t n, const float (&a)[8],
+                                                                         const float (&b)[8], sr_tile::Nothing) {
     r += row;
     n += column;
     if (r >= t.tokens || n >= t.padded) return;
@@ -168,11 +127,15 @@ struct BackwardArgs {
   int32_t activation;
 };
 
+struct Kept {
+  float a[8], b[8];
+};
+
 template <typename T, int SIZE>
 __global__ __launch_bounds__(sr_tile::threads(SIZE), 2) void backward_kernel(BackwardArgs t) {
   typedef sr_tile::Tile<T, false, SIZE, ROW, COL> Tile;
   SR_TILE_MEMORY(Tile);
-  const uint32_t item = t.grid.item();
+  const uint32_t item = sr_tile::item_of(blockIdx.x, t.grid.items, SIZE);
   if (item >= t.grid.items) return;
   uint32_t row, column;
   sr_tile::banded(item, t.grid.rows, t.grid.columns, row, column);
@@ -182,20 +145,26 @@ __global__ __launch_bounds__(sr_tile::threads(SIZE), 2) void backward_kernel(Bac
   sr_tile::run(tile, t.p, row, column, 0, (t.p.k + Tile::kK - 1) / Tile::kK, (Shared)a0, (Shared)a1, (Shared)b0,
                (Shared)b1);
   __syncthreads();
-  tile.template results<false>(Tile::slab((Shared)a0, (Shared)a1, (Shared)b0, (Shared)b1), [&](uint32_t r, uint32_t n, const float (&dh)[8]) {
+  auto kept = [&](uint32_t r, uint32_t n) {
+    r += row;
+    n += column;
+    Kept k{};
+    if (r >= t.tokens || n >= t.ffn) return k;
+    load_row(global<const float>(t.a) + uint64_t(r) * t.ffn + n, k.a, t.ffn - n);
+    load_row(global<const float>(t.b) + uint64_t(r) * t.ffn + n, k.b, t.ffn - n);
+    return k;
+  };
+  tile.template results<false, true>(SR_TILE_SLAB(Tile), kept, [&](uint32_t r, uint32_t n, const float (&dh)[8], const Kept& k) {
     r += row;
     n += column;
     if (r >= t.tokens || n >= t.padded) return;
-    float a[8], b[8], da[8], db[8], h[8];
-    const uint32_t have = n < t.ffn ? t.ffn - n : 0;
-    load_row(global<const float>(t.a) + uint64_t(r) * t.ffn + n, a, have);
-    load_row(global<const float>(t.b) + uint64_t(r) * t.ffn + n, b, have);
+    float da[8], db[8], h[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const Act f = act<true>(a[e], t.activation);
-      h[e] = f.value * b[e];
+      const Act f = act<true>(k.a[e], t.activation);
+      h[e] = f.value * k.b[e];
       db[e] = dh[e] * f.value;
-      da[e] = dh[e] * b[e] * f.slope;
+      da[e] = dh[e] * k.b[e] * f.slope;
     }
     const uint64_t at = r * t.stride + n;
     if (t.da) {
@@ -228,7 +197,7 @@ template <typename T, int SIZE, Side A, Side B>
 __global__ __launch_bounds__(sr_tile::threads(SIZE), 2) void product_kernel(ProductArgs t) {
   typedef sr_tile::Tile<T, false, SIZE, A, B> Tile;
   SR_TILE_MEMORY(Tile);
-  uint32_t item = xcd_order(blockIdx.x, t.items);
+  uint32_t item = sr_tile::item_of(blockIdx.x, t.items, SIZE);
   if (item >= t.items) return;
   int j = 0;
 #pragma unroll
@@ -245,7 +214,8 @@ __global__ __launch_bounds__(sr_tile::threads(SIZE), 2) void product_kernel(Prod
   Tile tile;
   sr_tile::run(tile, job.p, row, column, from, to, (Shared)a0, (Shared)a1, (Shared)b0, (Shared)b1);
   __syncthreads();
-  tile.template results<false>(Tile::slab((Shared)a0, (Shared)a1, (Shared)b0, (Shared)b1), [&](uint32_t r, uint32_t n, const float (&v)[8]) {
+  tile.template results<false, false>(SR_TILE_SLAB(Tile), sr_tile::nothing, [&](uint32_t r, uint32_t n, const float (&v)[8],
+                                                                         sr_tile::Nothing) {
     r += row;
     n += column;
     if (r >= job.rows || n >= job.columns) return;
@@ -484,18 +454,25 @@ Operand operand(const Matrix& m, Side side) {
           uint32_t(side == ROW ? m.rows : m.columns)};
 }
 
-// Large tiles where there are enough of them for most compute units.
-constexpr uint64_t kManyTiles = 192;
-int tile_size(uint64_t rows, uint64_t columns) {
-  return ceil_div(rows, 256) * ceil_div(columns, 256) >= kManyTiles ? 256 : 128;
+// The tiles' size of a product of rows x columns over `steps` steps.
+template <typename T>
+int tile_size(uint64_t rows, uint64_t columns, uint64_t steps) {
+  if (sizeof(T) == 4) return 128;
+  sr_tile::Cost large(256), small(128);
+  large.add(ceil_div(rows, 256) * ceil_div(columns, 256), steps);
+  small.add(ceil_div(rows, 128) * ceil_div(columns, 128), steps);
+  return large.time() <= small.time() ? 256 : 128;
 }
+
+// Steps of a product over k values.
+template <typename T> uint64_t steps_of(uint64_t k) { return ceil_div(k, 128 / sizeof(T)); }
 
 // Work items that a long sum is split for, and the least steps of a part.
 constexpr uint64_t kSplitItems = 512, kLeastSteps = 4;
 
 template <typename T, int SIZE, Side A, Side B>
 void launch_products(const ProductArgs& t, hipStream_t stream) {
-  product_kernel<T, SIZE, A, B><<<xcd_blocks(t.items), sr_tile::threads(SIZE), 0, stream>>>(t);
+  product_kernel<T, SIZE, A, B><<<sr_tile::blocks_of(t.items, SIZE), sr_tile::threads(SIZE), 0, stream>>>(t);
 }
 
 struct Wanted {
@@ -508,10 +485,13 @@ struct Wanted {
 // tiles and long sums (SPLIT), their steps are dealt out to several workgroups.
 template <typename T, Side A, Side B>
 int products(const char* who, const Wanted* w, int count, bool split, Space& space, bool launch, hipStream_t stream) {
-  uint64_t large = 0;
-  for (int i = 0; i < count; ++i) large += ceil_div(w[i].rows, 256) * ceil_div(w[i].columns, 256);
-  const bool f32 = sizeof(T) == 4;
-  const int size = !f32 && large >= kManyTiles ? 256 : 128;
+  sr_tile::Cost large(256), small(128);
+  for (int i = 0; i < count; ++i) {
+    const uint64_t k = steps_of<T>(w[i].p.k) * (w[i].p.a2.data ? 2 : 1);
+    large.add(ceil_div(w[i].rows, 256) * ceil_div(w[i].columns, 256), k);
+    small.add(ceil_div(w[i].rows, 128) * ceil_div(w[i].columns, 128), k);
+  }
+  const int size = sizeof(T) == 2 && large.time() <= small.time() ? 256 : 128;
   ProductArgs t{};
   uint64_t items = 0, steps = 0;
   int n = 0;
@@ -526,7 +506,7 @@ int products(const char* who, const Wanted* w, int count, bool split, Space& spa
     j.first = uint32_t(items);
     j.out = reinterpret_cast<uint64_t>(w[i].out);
     items += uint64_t(j.tile_rows) * j.tile_columns;
-    steps = ceil_div(w[i].p.k, 128 / sizeof(T)) * (w[i].p.a2.data ? 2 : 1);
+    steps = steps_of<T>(w[i].p.k) * (w[i].p.a2.data ? 2 : 1);
     if (items > sr_tile::kMostItems) return fail(SR_EBOUNDS, "%s: a product of %llu x %llu", who,
                                                  (unsigned long long)w[i].rows, (unsigned long long)w[i].columns);
   }
@@ -594,7 +574,7 @@ int forward(const sr_ffn_shape& s, void* out, void* a, void* b, Space& space, bo
   if (s.ffn) {
     ForwardArgs t{};
     t.p = {operand<T>(x, ROW), operand<T>(gate, ROW), {}, operand<T>(up, ROW), uint32_t(s.hidden)};
-    const int size = sizeof(T) == 4 ? 128 : tile_size(s.tokens, 2 * s.ffn);
+    const int size = tile_size<T>(s.tokens, 2 * s.ffn, steps_of<T>(s.hidden));
     const uint64_t rows = ceil_div(s.tokens, size), columns = ceil_div(wide, size / 2);
     if (rows * columns > sr_tile::kMostItems)
       return fail(SR_EBOUNDS, "sr_ffn: %llu tokens of %llu columns", (unsigned long long)s.tokens, (unsigned long long)s.ffn);
@@ -608,7 +588,7 @@ int forward(const sr_ffn_shape& s, void* out, void* a, void* b, Space& space, bo
     t.padded = uint32_t(wide);
     t.activation = s.activation;
     if (launch) {
-      const uint32_t blocks = xcd_blocks(t.grid.items);
+      const uint32_t blocks = sr_tile::blocks_of(t.grid.items, size);
       if constexpr (sizeof(T) == 4) forward_kernel<T, 128><<<blocks, sr_tile::threads(128), 0, stream>>>(t);
       else if (size == 256) forward_kernel<T, 256><<<blocks, sr_tile::threads(256), 0, stream>>>(t);
       else forward_kernel<T, 128><<<blocks, sr_tile::threads(128), 0, stream>>>(t);
@@ -633,7 +613,7 @@ int backward(const sr_ffn_shape& s, const void* a, const void* b, const void* dy
     const Matrix down = loader.ready(matrix_down(s));
     BackwardArgs t{};
     t.p = {operand<T>(dym, ROW), operand<T>(down, COL), {}, {}, uint32_t(s.hidden)};
-    const int size = sizeof(T) == 4 ? 128 : tile_size(s.tokens, s.ffn);
+    const int size = tile_size<T>(s.tokens, s.ffn, steps_of<T>(s.hidden));
     const uint64_t rows = ceil_div(s.tokens, size), columns = ceil_div(wide, size);
     if (rows * columns > sr_tile::kMostItems)
       return fail(SR_EBOUNDS, "%s: %llu tokens of %llu columns", who, (unsigned long long)s.tokens, (unsigned long long)s.ffn);
@@ -649,7 +629,7 @@ int backward(const sr_ffn_shape& s, const void* a, const void* b, const void* dy
     t.padded = uint32_t(wide);
     t.activation = s.activation;
     if (launch) {
-      const uint32_t blocks = xcd_blocks(t.grid.items);
+      const uint32_t blocks = sr_tile::blocks_of(t.grid.items, size);
       if constexpr (sizeof(T) == 4) backward_kernel<T, 128><<<blocks, sr_tile::threads(128), 0, stream>>>(t);
       else if (size == 256) backward_kernel<T, 256><<<blocks, sr_tile::threads(256), 0, stream>>>(t);
       else backward_kernel<T, 128><<<blocks, sr_tile::threads(128), 0, stream>>>(t);

@@ -252,12 +252,6 @@ static_assert(sizeof(ClipTable) <= kTableBytes, "kernel arguments");
 static_assert(SR_STEP_MAX_ELEMENTS / kClipChunk <= kMostChunks, "an array fits into a launch");
 static_assert(uint64_t(kMostChunks) * kThreads < uint64_t(1) << 32, "a grid's threads");
 
-// min(1, max_norm / (norm + 1e-6)); NaN stays NaN.
-__device__ __forceinline__ float clip_factor(double square_sum, float max_norm) {
-  const double f = double(max_norm) / (sqrt(square_sum) + 1e-6);
-  return f > 1.0 ? 1.0f : float(f);
-}
-
 template <typename S, typename D>
 __global__ __launch_bounds__(kThreads) void clip_kernel(ClipTable t) {
   constexpr int N = 4;

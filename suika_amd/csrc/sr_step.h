@@ -99,6 +99,49 @@ __device__ __forceinline__ T wave_sum(T x) {
   return x;
 }
 
+// Eight values of a row, n of which exist.
+template <typename T>
+__device__ __forceinline__ void store_row(T* p, const float (&v)[8], uint32_t n) {
+  if (n >= 8) {
+    if constexpr (sizeof(T) == 2) {
+      store<T, 8>(p, v);
+    } else {
+      const float lo[4] = {v[0], v[1], v[2], v[3]}, hi[4] = {v[4], v[5], v[6], v[7]};
+      store<T, 4>(p, lo);
+      store<T, 4>(p + 4, hi);
+    }
+  } else {
+#pragma unroll
+    for (uint32_t e = 0; e < 8; ++e)
+      if (e < n) p[e] = static_cast<T>(v[e]);
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void load_row(const T* p, float (&v)[8], uint32_t n) {
+  if (n >= 8) {
+    if constexpr (sizeof(T) == 2) {
+      load<T, 8>(p, v);
+    } else {
+      float lo[4], hi[4];
+      load<T, 4>(p, lo);
+      load<T, 4>(p + 4, hi);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = lo[e], v[4 + e] = hi[e];
+    }
+  } else {
+#pragma unroll
+    for (uint32_t e = 0; e < 8; ++e) v[e] = e < n ? static_cast<float>(p[e]) : 0.0f;
+  }
+}
+
+// The factor that gradients are clipped by: min(1, max_norm / (norm + 1e-6));
+// NaN stays NaN.
+__device__ __forceinline__ float clip_factor(double square_sum, float max_norm) {
+  const double f = double(max_norm) / (sqrt(square_sum) + 1e-6);
+  return f > 1.0 ? 1.0f : float(f);
+}
+
 // Work items in the order of memory, an eighth of them for each of the 8 dies
 // that workgroups go to in turn: the items in flight then come from 8 distant
 // regions.  A grid of xcd_blocks(items), of which some have no item.

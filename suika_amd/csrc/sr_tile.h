@@ -52,6 +52,8 @@ constexpr uint32_t kOutside = 0x80000000u;       // an offset beyond every resou
 constexpr uint32_t kResource = 0x7fffffffu;
 constexpr uint64_t kMostStride = uint64_t(1) << 22;     // bytes from row to row: 256 rows within a resource
 
+constexpr int kAllLoads = 0x0f70;                // s_waitcnt vmcnt(0)
+
 constexpr int threads(int size) { return size == 256 ? 512 : 256; }
 
 enum Side { ROW, COL };
@@ -110,8 +112,10 @@ struct Part {
   uint32_t piece;          // of a line: which of its pieces this lane loads
   uint64_t step;           // bytes from step to step
 
-  // How a piece's place in its line is permuted.
-  __device__ static uint32_t turn(uint32_t line) { return SIDE == ROW ? line & 7 : (line & 3) << 2; }
+  // How a piece's place in its line is permuted: sixteen lanes that read a column
+  // of pieces (ROW), or four lines of two pieces and their neighbours' (COL), meet
+  // all 64 banks.
+  __device__ static uint32_t turn(uint32_t line) { return SIDE == ROW ? line / 2 & 7 : (line & 3) << 2; }
 
   // Which matrix a wave's lines of a load are of.
   static constexpr int kTurn = PAIR ? 32 * PAIR : 1;
@@ -153,7 +157,8 @@ struct Part {
     for (int i = 0; i < kLoads; ++i) {
       uint32_t offset = at[i];
       if (!whole) {
-        const bool in = SIDE == ROW ? piece * kEach < left : i * kLines + threadIdx.x / kPieces < left;
+        // (TWO: rows are padded to whole steps)
+        const bool in = SIDE == ROW ? TWO || piece * kEach < left : i * kLines + threadIdx.x / kPieces < left;
         offset = in ? offset : kOutside;
       }
       const uint64_t first = data[0], second = data[1];
@@ -241,7 +246,7 @@ struct Tile {
       for (int j = 0; j < kJ; ++j) c[i][j] = f32x16(0.0f);
   }
 
-  // The operands of a k group, read while the group before is multiplied.
+  // The operands of a k group.
   struct Group {
     typename Block<T>::Frag a[kI], b[kJ], low_a[TWO ? kI : 1], low_b[TWO ? kJ : 1];
 
@@ -260,27 +265,65 @@ struct Tile {
     }
   };
 
-  // One step's products.
-  __device__ __forceinline__ void products(Shared sa, Shared sb) {
+  // The products of a k group.  With 128 x 128 tiles a wave that multiplies goes
+  // before those of the other workgroup, whose loads and barriers fill its gaps
+  // (bf16 1.10 to 1.17 PFLOP/s, values of 22 bits 1.19 to 1.27; with 256 x 256
+  // tiles 1-2% slower).
+  __device__ __forceinline__ void multiply(const Group& x) {
     typedef Block<T> K;
-    Group g[2];
-    g[0].read(sa, sb, 0);
-#pragma unroll
-    for (int s = 0; s < kGroups; ++s) {
-      Group& x = g[s % 2];
-      if (s + 1 < kGroups) g[(s + 1) % 2].read(sa, sb, s + 1);
+    auto each = [&](const auto& fb, const auto& fa) {
 #pragma unroll
       for (int i = 0; i < kI; ++i)
 #pragma unroll
-        for (int j = 0; j < kJ; ++j) {
-          K::add(x.b[j], x.a[i], c[i][j]);
-          if constexpr (TWO) {
-            K::add(x.b[j], x.low_a[i], c[i][j]);
-            K::add(x.low_b[j], x.a[i], c[i][j]);
-          }
-        }
+        for (int j = 0; j < kJ; ++j) K::add(fb[j], fa[i], c[i][j]);
+    };
+    if (SIZE == 128) __builtin_amdgcn_s_setprio(1);
+    each(x.b, x.a);
+    if constexpr (TWO) {
+      each(x.b, x.low_a);
+      each(x.low_b, x.a);
+    }
+    if (SIZE == 128) __builtin_amdgcn_s_setprio(0);
+  }
+
+  // A step's products but for the last group's, which are left in `g`, as the
+  // first group's are at the start.
+  __device__ __forceinline__ void most_products(Group (&g)[2], Shared sa, Shared sb) {
+#pragma unroll
+    for (int s = 0; s + 1 < kGroups; ++s) {
+      g[(s + 1) % 2].read(sa, sb, s + 1);
+      multiply(g[s % 2]);
+      // reads of the next group between this one's products (3% for 256 x 256 of ROW)
+      constexpr int kReads = (kI + kJ) * (TWO ? 2 : 1), kProducts = kI * kJ * (TWO ? 3 : 1);
+#pragma unroll
+      for (int q = 0; q < kReads; ++q) {
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x8, kProducts / kReads, 0);
+      }
       __builtin_amdgcn_sched_barrier(0);
     }
+  }
+  __device__ __forceinline__ void last_products(const Group (&g)[2]) {
+    multiply(g[(kGroups - 1) % 2]);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+
+  // f(row, column, values) on this wave's values as they lie in its registers:
+  // four columns of a row a lane.
+  template <typename F>
+  __device__ __forceinline__ void values(F&& f) {
+    const uint32_t lane = threadIdx.x % kWave;
+#pragma unroll
+    for (int i = 0; i < kI; ++i)
+#pragma unroll
+      for (int j = 0; j < kJ; ++j)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          float v[4] = {c[i][j][4 * q], c[i][j][4 * q + 1], c[i][j][4 * q + 2], c[i][j][4 * q + 3]};
+          f(uint32_t(wave_row() + 32 * i) + lane % 32, uint32_t(wave_column() + 32 * j + 8 * q) + lane / 32 * 4, v);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) c[i][j][4 * q + e] = v[e];
+        }
   }
 
   // This wave's slab, where the operands were.
@@ -290,11 +333,15 @@ struct Tile {
   }
 
   // The rows and columns of this wave, eight values a lane: f(row, column,
-  // values) with the row and the first column in the tile.  FLIP: of the
-  // transpose of C.  With PAIR, f(row, column, values, values of the second
-  // matrix).  `slab`: the wave's, no longer read as operands.
-  template <bool FLIP, typename F>
-  __device__ __forceinline__ void results(Shared slab, F&& f) const {
+  // values, what load(row, column) has returned) with the row and the first column
+  // in the tile.  FLIP: of the transpose of C.  With PAIR, the values of the second
+  // matrix come behind the first one's.  What is loaded for 32 rows is on its way
+  // at once or, with ROLLED, for the next 8 while these are worked on, in a loop
+  // that stays one: for so much work a value that the compiler would not unroll the
+  // loop around it, without which C has no registers.  `slab`: the wave's, no
+  // longer read as operands.
+  template <bool FLIP, bool ROLLED, typename L, typename F>
+  __device__ __forceinline__ void results(Shared slab, L&& load, F&& f) const {
     static_assert(!(FLIP && PAIR), "");
     const uint32_t lane = threadIdx.x % kWave;
     const int row0 = FLIP ? wave_column() : wave_row();
@@ -307,6 +354,13 @@ struct Tile {
     for (int i = 0; i < kDown; ++i)
 #pragma unroll
       for (int j = 0; j < kAcross / 2; ++j) {
+        constexpr int kLanes = (PAIR ? 32 : 64) / 8;     // of a row
+        constexpr int kPasses = 32 * kLanes / kWave;
+        auto row_of = [&](int p) { return uint32_t(row0 + 32 * i + p * (kWave / kLanes)) + lane / kLanes; };
+        const uint32_t column = uint32_t(column0 + (PAIR ? 32 : 64) * j) + lane % kLanes * 8;
+        decltype(load(0u, 0u)) loaded[ROLLED ? 1 : kPasses];
+#pragma unroll
+        for (int p = 0; p < (ROLLED ? 1 : kPasses); ++p) loaded[p] = load(row_of(p), column);
         // two blocks; a lane has the column lane % 32 of a block's transpose, four rows together
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
@@ -325,9 +379,7 @@ struct Tile {
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");     // the wave's own writes, read by other lanes
         __builtin_amdgcn_wave_barrier();
-        constexpr int kLanes = (PAIR ? 32 : 64) / 8;     // of a row
-#pragma unroll 1
-        for (int p = 0; p < 32 * kLanes / kWave; ++p) {
+        auto pass = [&](int p, const auto& with) {
           const int r = p * (kWave / kLanes) + lane / kLanes, n = lane % kLanes * 8;
           float v[8], w[8];
 #pragma unroll
@@ -341,9 +393,19 @@ struct Tile {
               for (int e = 0; e < 4; ++e) w[4 * h + e] = y[e];
             }
           }
-          const uint32_t to_row = row0 + 32 * i + r, to_column = column0 + (PAIR ? 32 : 64) * j + n;
-          if constexpr (PAIR) f(to_row, to_column, v, w);
-          else f(to_row, to_column, v);
+          if constexpr (PAIR) f(row_of(p), column, v, w, with);
+          else f(row_of(p), column, v, with);
+        };
+        if constexpr (ROLLED) {
+#pragma unroll 1
+          for (int p = 0; p < kPasses; ++p) {
+            const auto now = loaded[0];
+            if (p + 1 < kPasses) loaded[0] = load(row_of(p + 1), column);
+            pass(p, now);
+          }
+        } else {
+#pragma unroll
+          for (int p = 0; p < kPasses; ++p) pass(p, loaded[p]);
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
         __builtin_amdgcn_wave_barrier();
@@ -386,33 +448,112 @@ __device__ __forceinline__ void run(Tile& tile, const Product& p, uint32_t row, 
   tile.clear();
   if (from >= to) return;
   seek(from);
+  typename Tile::Group g[2];
+  // The barrier: the next step has arrived, and this one's operands have all been
+  // read; its last group is still to be multiplied, which hides the first reads
+  // of the next step.
+  // The wait for this wave's own loads is written out: a barrier by itself orders
+  // shared memory's reads and writes, but not what loads write there.
+  auto turn_over = [&] {
+    __builtin_amdgcn_s_waitcnt(kAllLoads);
+    __syncthreads();
+    __builtin_amdgcn_sched_barrier(0);
+  };
   fetch(from, a0, b0);
+  turn_over();
+  if (from + 1 < to) fetch(from + 1, a1, b1);
+  g[0].read(a0, b0, 0);
   uint32_t s = from;
   for (; s + 2 <= to; s += 2) {
-    __syncthreads();      // the loads have arrived, and the other half is read
-    fetch(s + 1, a1, b1);
-    tile.products(a0, b0);
-    __syncthreads();
+    tile.most_products(g, a0, b0);
+    turn_over();
     if (s + 2 < to) fetch(s + 2, a0, b0);
-    tile.products(a1, b1);
+    g[0].read(a1, b1, 0);
+    tile.last_products(g);
+    tile.most_products(g, a1, b1);
+    turn_over();
+    if (s + 3 < to) fetch(s + 3, a1, b1);
+    if (s + 2 < to) g[0].read(a0, b0, 0);
+    tile.last_products(g);
   }
   if (s < to) {
-    __syncthreads();
-    tile.products(a0, b0);
+    tile.most_products(g, a0, b0);
+    tile.last_products(g);
   }
 }
 
-// Tiles of a product, items of a launch, and the order that workgroups take
-// them in: neighbours on one die, where they share rows and columns.
+// What a workgroup of these kernels has of shared memory: two halves of both
+// operands, arrays of their own (see sr_tile::run), then the waves' slabs.
+#define SR_TILE_MEMORY(Tile)                                                     \
+  __shared__ __attribute__((aligned(1024))) char a0[Tile::PartA::kBytes];        \
+  __shared__ __attribute__((aligned(1024))) char a1[Tile::PartA::kBytes];        \
+  __shared__ __attribute__((aligned(1024))) char b0[Tile::PartB::kBytes];        \
+  __shared__ __attribute__((aligned(1024))) char b1[Tile::PartB::kBytes]
+#define SR_TILE_SLAB(Tile) \
+  Tile::slab((sr_tile::Shared)a0, (sr_tile::Shared)a1, (sr_tile::Shared)b0, (sr_tile::Shared)b1)
+
+// Items of a launch in the order that workgroups take them: as many neighbours
+// on one die as run there at once, die after die, so that they share rows and
+// columns in its L2 and all dies have the same mix of long and short ones (an
+// eighth of the items each: where the long ones come first, 2.1 ms instead of
+// 1.6).  What is left behind whole rounds goes to the dies by eighths.
+constexpr uint32_t at_once(int size) { return size == 256 ? 32 : 64; }      // of a die's 32 compute units
+
+inline uint32_t blocks_of(uint32_t items, int size) {
+  const uint32_t round = at_once(size) * sr_step::kXcds;
+  return items / round * round + sr_step::xcd_blocks(items % round);
+}
+
+__device__ __forceinline__ uint32_t item_of(uint32_t block, uint32_t items, int size) {
+  const uint32_t round = at_once(size) * sr_step::kXcds, first = block / round * round, in = block - first;
+  if (first + round <= items) return first + in % sr_step::kXcds * at_once(size) + in / sr_step::kXcds;
+  return first + sr_step::xcd_order(in, items - first);
+}
+
+// A launch's tiles and items.
 struct Grid {
   uint32_t rows, columns;
   uint32_t items;
-
-  __device__ __forceinline__ uint32_t item() const { return sr_step::xcd_order(blockIdx.x, items); }
 };
 
 // Most workgroups of a launch: a grid has fewer than 2^32 threads, 512 a workgroup.
 constexpr uint64_t kMostItems = (uint64_t(1) << 23) - 2 * sr_step::kXcds;
+
+// For results that nothing is loaded for.
+struct Nothing {};
+__device__ __forceinline__ Nothing nothing(uint32_t, uint32_t) { return {}; }
+
+// How long a launch of tiles takes, in steps of a 128 x 128 tile that has a
+// compute unit to itself: the sum of the steps over the compute units and half of
+// the longest tile that ends last, or, of tiles alike, whole rounds.  A 256 x 256
+// tile's step takes as long as four, two workgroups of 128 x 128 tiles share a
+// compute unit and take 1.12 times as long for the same.  Six steps for a tile's first loads and its results.
+class Cost {
+ public:
+  explicit Cost(int size)
+      : slots_(size == 256 ? kUnits : 2 * kUnits), each_(size == 256 ? 4.0 : 2.25), large_(size == 256) {}
+
+  void add(uint64_t tiles, uint64_t steps) {
+    if (tiles == 0) return;
+    const double t = double(steps) + 6;
+    alike_ = alike_ && (tiles_ == 0 || t == longest_);
+    tiles_ += tiles;
+    sum_ += double(tiles) * t;
+    longest_ = t > longest_ ? t : longest_;
+  }
+  double time() const {
+    // with one workgroup a compute unit nothing is shared
+    if (!large_ && tiles_ <= kUnits) return 1.2 * longest_;
+    if (alike_) return double((tiles_ + slots_ - 1) / slots_) * each_ * longest_;
+    return (sum_ / double(slots_) + longest_ / 2) * each_;
+  }
+
+ private:
+  static constexpr uint64_t kUnits = 256;      // compute units
+  uint64_t slots_, tiles_ = 0;
+  double each_, sum_ = 0, longest_ = 0;
+  bool large_, alike_ = true;
+};
 
 // The tile of a work item, in bands of 8 tiles' rows: the tiles of neighbouring
 // items share rows and columns.

@@ -8,6 +8,7 @@
 #include <torch/csrc/DynamicTypes.h>
 
 #include <cstdint>
+#include <exception>
 #include <string>
 #include <unordered_map>
 #include <vector>
@@ -645,6 +646,228 @@ py::tuple gated_ffn_grad(const at::Tensor& x, const at::Tensor& gate, const at::
   return out;
 }
 
+// ------------------------------------------------------- orthogonal matrices
+
+// A sum over ranks by a Python callable, on views of the call's workspace.  What
+// it raises comes back once the library has returned.
+class Reduce {
+ public:
+  explicit Reduce(py::object callable) : callable_(std::move(callable)) {}
+
+  void over(const at::Tensor& work) { work_ = work; }
+  sr_reduce function() const { return callable_.is_none() ? nullptr : &Reduce::call; }
+  // The library's status, or what the callable raised.
+  void check_call(int rc, const char* what) {
+    if (raised_) {
+      std::exception_ptr e = raised_;
+      raised_ = nullptr;
+      std::rethrow_exception(e);
+    }
+    check(rc, what);
+  }
+
+ private:
+  static int call(void* context, void* data, uint64_t count, int32_t dtype, hipStream_t) {
+    Reduce& self = *static_cast<Reduce*>(context);
+    try {
+      const bool wide = dtype == SR_DT_F64;
+      const int64_t at = static_cast<char*>(data) - static_cast<char*>(self.work_.data_ptr());
+      const at::Tensor bytes = self.work_.narrow(0, at, int64_t(count) * (wide ? 8 : 4));
+      self.callable_(bytes.view(wide ? at::kDouble : at::kFloat));
+      return 0;
+    } catch (...) {
+      self.raised_ = std::current_exception();
+      return 1;
+    }
+  }
+
+  py::object callable_;
+  at::Tensor work_;
+  std::exception_ptr raised_;
+};
+
+int32_t split_code(py::handle dim, const std::string& what) {
+  if (dim.is_none()) return -1;
+  if (!PyLong_Check(dim.ptr())) plan_error(what + ": None, 0 or 1 is wanted");
+  const int64_t d = PyLong_AsLongLong(dim.ptr());
+  if (d != 0 && d != 1) {
+    PyErr_Clear();
+    plan_error(what + ": None, 0 or 1 is wanted");
+  }
+  return int32_t(d);
+}
+
+sr_matrix matrix_of(const at::Tensor& t, const std::string& what, int32_t split, c10::optional<at::Device>& device) {
+  if (!t.is_cuda()) plan_error(what + " is on " + t.device().str() + ", not on the GPU");
+  if (!device) device = t.device();
+  if (t.device() != *device) plan_error(what + " is on " + t.device().str() + ", not on " + device->str());
+  if (t.dim() != 2) plan_error(what + ": a matrix is wanted, not " + c10::str(t.sizes()));
+  const uint64_t stride = row_stride(t, what);
+  return {t.data_ptr(), uint64_t(t.size(0)), uint64_t(t.size(1)), stride, float_code(t, what), split};
+}
+
+py::list orthogonalize(py::object matrices, py::object outs, py::object splits, int32_t steps,
+                       const std::vector<double>& coefficients, double eps, py::object all_reduce) {
+  c10::optional<at::Device> device;
+  const Fast list(matrices, "matrices");
+  const bool fresh = outs.is_none();
+  const Fast out_list(fresh ? py::object(py::list()) : outs, "out"),
+      split_list(splits.is_none() ? py::object(py::list()) : splits, "split");
+  if (!fresh && out_list.size() != list.size())
+    plan_error("out has " + std::to_string(out_list.size()) + " tensors, matrices " + std::to_string(list.size()));
+  if (!splits.is_none() && split_list.size() != list.size())
+    plan_error("split has " + std::to_string(split_list.size()) + " entries, matrices " + std::to_string(list.size()));
+  std::vector<sr_matrix> src, dst;
+  std::vector<at::Tensor> to;
+  for (size_t i = 0; i < list.size(); ++i) {
+    const std::string name = indexed("matrices", i);
+    const at::Tensor& t = tensor_of(list[i], name);
+    check_tangent(t, name.c_str());
+    src.push_back(matrix_of(t, name, splits.is_none() ? -1 : split_code(split_list[i], indexed("split", i)), device));
+    if (fresh) continue;
+    const std::string out_name = indexed("out", i);
+    const at::Tensor& o = tensor_of(out_list[i], out_name);
+    dst.push_back(matrix_of(o, out_name, -1, device));
+    if (o.sizes() != t.sizes()) plan_error(out_name + ": shape differs from the matrix's");
+    to.push_back(o);
+  }
+  if (!device) device = current_device();
+  const c10::DeviceGuard guard(*device);
+  if (fresh) {
+    for (size_t i = 0; i < list.size(); ++i) {
+      const at::Tensor& t = THPVariable_Unpack(list[i]);
+      to.push_back(at::empty(t.sizes(), on(*device, t.scalar_type())));
+      dst.push_back({to[i].data_ptr(), src[i].rows, src[i].cols, src[i].cols, src[i].dtype, -1});
+    }
+  }
+  Reduce reduce(all_reduce);
+  const sr_newton_schulz ns{steps, 0, coefficients.data(), eps, reduce.function(), &reduce};
+  uint64_t need = 0;
+  check(sr_orthogonalize_workspace(src.data(), dst.data(), int32_t(src.size()), &ns, &need), "sr_orthogonalize");
+  const at::Tensor work = at::empty({int64_t(need)}, on(*device, at::kByte));
+  reduce.over(work);
+  const int rc = sr_orthogonalize(src.data(), dst.data(), int32_t(src.size()), &ns, work.data_ptr(), need, stream_of(*device));
+  if (!fresh)
+    for (const at::Tensor& t : to) written(t);
+  reduce.check_call(rc, "sr_orthogonalize");
+  py::list out;
+  for (const at::Tensor& t : to) out.append(t);
+  return out;
+}
+
+// The matrices that Muon steps, in the order of their names.
+class MuonState {
+ public:
+  MuonState(py::object weight, py::object exp_avg, py::object param, std::vector<std::string> names,
+            std::vector<int32_t> split, std::vector<double> scale)
+      : names_(std::move(names)), split_(std::move(split)), scale_(std::move(scale)) {
+    const Fast w(weight, "weight"), m(exp_avg, "exp_avg"), p(param, "param");
+    if (w.size() != names_.size() || m.size() != w.size() || p.size() != w.size() || split_.size() != w.size() ||
+        scale_.size() != w.size())
+      plan_error("state: lists of different lengths");
+    for (size_t i = 0; i < names_.size(); ++i) {
+      weight_.push_back(tensor_of(w[i], names_[i] + "/weight"));
+      exp_avg_.push_back(tensor_of(m[i], names_[i] + "/exp_avg"));
+      param_.push_back(p[i] == Py_None ? at::Tensor() : tensor_of(p[i], names_[i] + "/param"));
+      check_fields(i);
+      shapes_.push_back(weight_[i].sizes().vec());
+    }
+  }
+
+  py::object step(py::object grads, double lr, double momentum, bool nesterov, double weight_decay, int32_t steps,
+                  const std::vector<double>& coefficients, double eps, py::object max_norm, py::object square_sum,
+                  py::object all_reduce) {
+    const Fast list(grads, "grads");
+    if (list.size() != names_.size())
+      plan_error("grads: " + std::to_string(list.size()) + " tensors for a state of " + std::to_string(names_.size()));
+    std::vector<sr_muon_tensor> tensors;
+    std::vector<sr_array> arrays;
+    std::vector<size_t> stepped;
+    for (size_t i = 0; i < names_.size(); ++i) {
+      if (list[i] == Py_None) continue;
+      const at::Tensor& g = tensor_of(list[i], "gradient of " + names_[i]);
+      const at::Tensor &w = weight_[i], &m = exp_avg_[i], &p = param_[i];
+      check_fields(i);
+      if (w.sizes() != at::IntArrayRef(shapes_[i])) plan_error(names_[i] + ": another shape than the state was taken with");
+      if (g.layout() != at::kStrided || !g.is_contiguous() || g.device() != w.device() || g.sizes() != w.sizes())
+        plan_error("gradient of " + names_[i] + ": a dense tensor like the weight on " + w.device().str() + " is wanted");
+      const at::ScalarType gt = g.scalar_type();
+      if (gt != at::kFloat && gt != at::kBFloat16)
+        plan_error("gradient of " + names_[i] + ": dtype " + c10::toString(gt) + ", not float32 or bfloat16");
+      if (!stored(g)) plan_error("gradient of " + names_[i] + ": its storage has been released");
+      check_tangent(g, "grads");
+      tensors.push_back({w.data_ptr(), m.data_ptr(), p.defined() ? p.data_ptr() : nullptr, g.data_ptr(), uint64_t(w.size(0)),
+                         uint64_t(w.size(1)), scale_[i], float_code(w, names_[i]), float_code(m, names_[i]),
+                         float_code(g, names_[i]), split_[i], 0});
+      arrays.push_back(array_of(g, names_[i]));
+      stepped.push_back(i);
+    }
+    const at::Device device = device_ ? *device_ : current_device();
+    const c10::DeviceGuard guard(device);
+    Reduce reduce(all_reduce);
+    const sr_newton_schulz ns{steps, 0, coefficients.data(), eps, reduce.function(), &reduce};
+    sr_muon_options o{lr, weight_decay, momentum, nesterov, 0, 0.0, nullptr};
+    c10::optional<SumWork> work;
+    at::Tensor norm;
+    const double* given = nullptr;
+    if (!max_norm.is_none()) {
+      o.max_norm = max_norm.cast<double>();
+      given = given_sum(square_sum, device);
+      norm = at::empty({}, on(device, at::kFloat));
+      if (!given) work.emplace(arrays, device);
+      o.square_sum = given ? given : work->sum();
+    } else if (!square_sum.is_none()) {
+      plan_error("square_sum is given without max_norm");
+    }
+    // all checks, before the sum of squares is launched
+    uint64_t need = 0;
+    check(sr_muon_workspace(tensors.data(), int32_t(tensors.size()), &o, &ns, &need), "sr_muon");
+    const at::Tensor memory = at::empty({int64_t(need)}, on(device, at::kByte));
+    reduce.over(memory);
+    if (work)
+      check(sr_square_sum(arrays.data(), int32_t(arrays.size()), 1, work->parts(), work->bytes, work->sum(),
+                          norm.data_ptr<float>(), stream_of(device)),
+            "sr_square_sum");
+    else if (given)
+      check(sr_clip(nullptr, nullptr, 0, given, float(o.max_norm), norm.data_ptr<float>(), stream_of(device)), "sr_clip");
+    const int rc = sr_muon(tensors.data(), int32_t(tensors.size()), &o, &ns, memory.data_ptr(), need, stream_of(device));
+    for (size_t i : stepped)
+      for (const at::Tensor* t : {&weight_[i], &exp_avg_[i], &param_[i]})
+        if (t->defined()) written(*t);
+    reduce.check_call(rc, "sr_muon");
+    if (!norm.defined()) return py::none();
+    return py::cast(norm);
+  }
+
+ private:
+  // The fields as they are now, as AdamWState checks them.
+  void check_fields(size_t i) {
+    const at::Tensor &w = weight_[i], &m = exp_avg_[i], &p = param_[i];
+    const struct { const at::Tensor& t; const char* what; } field[3] = {{w, "weight"}, {m, "exp_avg"}, {p, "param"}};
+    for (const auto& f : field) {
+      if (!f.t.defined()) continue;
+      if (!dense(f.t, device_)) check_dense(f.t, names_[i] + "/" + f.what, device_);     // says what is wrong
+      if (!stored(f.t)) plan_error(names_[i] + ": a field's storage has been released");
+      if (f.t.sizes() != w.sizes()) plan_error(names_[i] + ": fields of different shapes");
+    }
+    const at::ScalarType wt = w.scalar_type(), mt = m.scalar_type();
+    if (w.dim() != 2) plan_error(names_[i] + ": a matrix is wanted, not " + c10::str(w.sizes()));
+    if (wt != at::kFloat && wt != at::kBFloat16)
+      plan_error(names_[i] + ": weight of dtype " + c10::toString(wt) + ", not float32 or bfloat16");
+    if (mt != at::kFloat && mt != at::kBFloat16)
+      plan_error(names_[i] + ": exp_avg of dtype " + c10::toString(mt) + ", not float32 or bfloat16");
+    if (p.defined() && (wt != at::kFloat || p.scalar_type() != at::kBFloat16))
+      plan_error(names_[i] + ": a master weight is float32 and its param bfloat16");
+  }
+
+  std::vector<std::string> names_;
+  std::vector<int32_t> split_;
+  std::vector<double> scale_;
+  std::vector<at::Tensor> weight_, exp_avg_, param_;
+  std::vector<std::vector<int64_t>> shapes_;      // what split and scale were formed for
+  c10::optional<at::Device> device_;
+};
+
 }  // namespace
 
 namespace suika_host {
@@ -668,6 +891,14 @@ void bind_step(py::module_& m) {
   m.def("token_logprobs_grad", &token_logprobs_grad, py::arg("logits"), py::arg("targets"), py::arg("lse"),
         py::arg("entropy"), py::arg("grad_logprob"), py::arg("grad_entropy"), py::arg("vocab"), py::arg("out"),
         py::arg("lse_low"));
+  m.def("orthogonalize", &orthogonalize, py::arg("matrices"), py::arg("out"), py::arg("split"), py::arg("steps"),
+        py::arg("coefficients"), py::arg("eps"), py::arg("all_reduce"));
+  py::class_<MuonState>(m, "MuonState", "The matrices of a state that Muon updates in place")
+      .def(py::init<py::object, py::object, py::object, std::vector<std::string>, std::vector<int32_t>, std::vector<double>>(),
+           py::arg("weight"), py::arg("exp_avg"), py::arg("param"), py::arg("names"), py::arg("split"), py::arg("scale"))
+      .def("step", &MuonState::step, py::arg("grads"), py::arg("lr"), py::arg("momentum"), py::arg("nesterov"),
+           py::arg("weight_decay"), py::arg("steps"), py::arg("coefficients"), py::arg("eps"), py::arg("max_norm"),
+           py::arg("square_sum"), py::arg("all_reduce"));
   m.def("gated_ffn", &gated_ffn, py::arg("x"), py::arg("gate"), py::arg("up"), py::arg("down"), py::arg("activation"),
         py::arg("keep"));
   m.def("gated_ffn_grad", &gated_ffn_grad, py::arg("x"), py::arg("gate"), py::arg("up"), py::arg("down"),

@@ -203,7 +203,7 @@ __global__ __launch_bounds__(kSheetThreads) void scale_kernel(Table<SourceEntry>
   const uint32_t sheet = blockIdx.x - e.from, across = (e.columns + kSheet - 1) / kSheet;
   const uint32_t row0 = sheet / across * kSheet, column0 = sheet % across * kSheet;
   const double norm = sqrt(sums[e.at]);
-  const double scale = double(kX) / (norm < eps ? eps : norm);      // a NaN stays one
+  const double scale = norm == 0 ? 0.0 : double(kX) / (norm < eps ? eps : norm);      // a NaN stays one
   const float factor = mix.square_sum ? clip_factor(*mix.square_sum, mix.max_norm) : 1.0f;
   __shared__ float turned[kSheet][kSheet + 1];
 #pragma unroll
@@ -468,6 +468,177 @@ __global__ __launch_bounds__(sr_tile::threads(SIZE), 2) void last_kernel(Table<L
   }
 }
 
+// ------------------------------------------------------------ small matrices
+
+// A small matrix goes through everything in one workgroup and one launch, its
+// values and products in shared memory and 32 bits: 8 matrices of up to 32 x 24
+// take SMALL_US us instead of 80 with tiles, whose 17 launches are most of that.
+// Up to about 64 x 64 x 64 operations a product a workgroup is as fast as tiles;
+// the rule looks at the matrix alone, so its result does not depend on the list.
+constexpr uint32_t kSmallSide = 64, kSmallValues = 64 * 196;
+constexpr uint64_t kSmallWork = uint64_t(1) << 18;
+
+struct SmallEntry {
+  uint64_t source, momentum, to, param;
+  uint64_t source_stride, to_stride;
+  uint32_t rows, columns;
+  int32_t source_type, momentum_type, to_type;
+  uint32_t flip, weight;
+  float decay, step;
+};
+
+constexpr int kSmallEntries = 32;
+
+struct SmallTable {
+  SmallEntry entry[kSmallEntries];
+  Polynomial step[SR_MAX_NEWTON_SCHULZ];
+  Mix mix;
+  double eps;
+  int32_t steps;
+};
+static_assert(sizeof(SmallTable) <= 3832, "kernel arguments");
+
+__device__ __forceinline__ float load_one(uint64_t p, uint64_t at, int32_t type) {
+  return type == SR_DT_F32 ? global<const float>(p)[at]
+                           : type == SR_DT_BF16 ? float(global<const bf16>(p)[at]) : float(global<const f16>(p)[at]);
+}
+
+__device__ __forceinline__ void store_one(uint64_t p, uint64_t at, int32_t type, float v) {
+  if (type == SR_DT_F32) global<float>(p)[at] = v;
+  else if (type == SR_DT_BF16) global<bf16>(p)[at] = bf16(v);
+  else global<f16>(p)[at] = f16(v);
+}
+
+__host__ __device__ inline uint32_t fours(uint32_t n) { return (n + 3) / 4 * 4; }
+
+// out(i, j, sum over k of P[i][k] Q[k][j], or of Q[j][k] with ROWS), R x R sums a
+// lane; sides are multiples of 4.
+template <int R, bool ROWS, typename F>
+__device__ __forceinline__ void small_squares(const float* p, uint32_t p_wide, const float* q, uint32_t q_wide, uint32_t rows,
+                                              uint32_t columns, uint32_t depth, F&& out) {
+  using sr_tile::f32x4;
+  typedef float Across __attribute__((ext_vector_type(R)));
+  const uint32_t across = columns / R;
+  for (uint32_t t = threadIdx.x; t < rows / R * across; t += kSheetThreads) {
+    const uint32_t i = t / across * R, j = t % across * R;
+    float sum[R][R] = {};
+    for (uint32_t k = 0; k < depth; k += 4) {
+      f32x4 a[R], b[R];
+      Across c[4];
+#pragma unroll
+      for (int r = 0; r < R; ++r) a[r] = *reinterpret_cast<const f32x4*>(p + (i + r) * p_wide + k);
+      if (ROWS) {
+#pragma unroll
+        for (int r = 0; r < R; ++r) b[r] = *reinterpret_cast<const f32x4*>(q + (j + r) * q_wide + k);
+      } else {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) c[r] = *reinterpret_cast<const Across*>(q + (k + r) * q_wide + j);
+      }
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int x = 0; x < R; ++x)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) sum[r][x] = fmaf(a[r][e], ROWS ? b[x][e] : c[e][x], sum[r][x]);
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+      for (int x = 0; x < R; ++x) out(i + r, j + x, sum[r][x]);
+  }
+}
+
+// Smaller squares where that gives more lanes work.
+template <bool ROWS, typename F>
+__device__ __forceinline__ void small_product(const float* p, uint32_t p_wide, const float* q, uint32_t q_wide, uint32_t rows,
+                                              uint32_t columns, uint32_t depth, F&& out) {
+  if (rows * columns <= 4 * kSheetThreads) small_squares<2, ROWS>(p, p_wide, q, q_wide, rows, columns, depth, out);
+  else small_squares<4, ROWS>(p, p_wide, q, q_wide, rows, columns, depth, out);
+}
+
+__global__ __launch_bounds__(kSheetThreads) void small_kernel(SmallTable t) {
+  constexpr uint32_t kGram = kSmallSide * (kSmallSide + 4);
+  __shared__ __attribute__((aligned(16))) float first[kSmallValues + kSmallSide * 4], second[kSmallValues + kSmallSide * 4],
+      gram[kGram], factor[kGram];
+  __shared__ double part[kSheetThreads / kWave];
+  const SmallEntry& e = t.entry[blockIdx.x];
+  const uint32_t m = e.flip ? e.columns : e.rows, n = e.flip ? e.rows : e.columns;
+  const uint32_t high = fours(m), wide = fours(n) + 4, side = fours(m) + 4;
+  for (uint32_t i = threadIdx.x; i < high * wide; i += kSheetThreads) first[i] = second[i] = 0;
+  __syncthreads();
+  const float clip = t.mix.square_sum ? clip_factor(*t.mix.square_sum, t.mix.max_norm) : 1.0f;
+  const uint32_t wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
+  const uint32_t values = e.rows * e.columns;
+  constexpr uint32_t kAhead = 4;      // values of a lane that are loaded at once
+  double squares = 0;
+  for (uint32_t i = threadIdx.x; i < values; i += kAhead * kSheetThreads) {
+    float v[kAhead], old[kAhead];
+    uint32_t row[kAhead], column[kAhead];
+#pragma unroll
+    for (uint32_t a = 0; a < kAhead; ++a) {
+      const uint32_t at = min(i + a * kSheetThreads, values - 1);
+      row[a] = at / e.columns;
+      column[a] = at % e.columns;
+      v[a] = load_one(e.source, row[a] * e.source_stride + column[a], e.source_type);
+      old[a] = e.momentum ? load_one(e.momentum, at, e.momentum_type) : 0.0f;
+    }
+#pragma unroll
+    for (uint32_t a = 0; a < kAhead; ++a) {
+      const uint32_t at = i + a * kSheetThreads;
+      if (at >= values) continue;
+      if (e.momentum) {
+        float m = fmaf(old[a], t.mix.keep, clip * v[a] * t.mix.add);
+        if (e.momentum_type == SR_DT_BF16) m = float(bf16(m));
+        store_one(e.momentum, at, e.momentum_type, m);
+        v[a] = t.mix.nesterov ? fmaf(m, t.mix.keep, clip * v[a] * t.mix.add) : m;
+      }
+      squares = fma(double(v[a]), double(v[a]), squares);
+      first[e.flip ? column[a] * wide + row[a] : row[a] * wide + column[a]] = v[a];
+    }
+  }
+  squares = wave_sum(squares);
+  if (lane == 0) part[wave] = squares;
+  __syncthreads();
+  const double norm = sqrt((part[0] + part[1]) + (part[2] + part[3]));
+  const double scale = 1.0 / (norm < t.eps ? t.eps : norm);
+  for (uint32_t i = threadIdx.x; i < high * wide; i += kSheetThreads) first[i] = norm == 0 ? 0.0f : float(double(first[i]) * scale);
+  __syncthreads();
+  float *x = first, *y = second;
+  for (int32_t k = 0; k < t.steps; ++k) {
+    const Polynomial p = t.step[k];
+    small_product<true>(x, wide, x, wide, high, high, wide - 4,
+                        [&](uint32_t i, uint32_t j, float v) { gram[i * side + j] = v; });
+    __syncthreads();
+    small_product<false>(gram, side, gram, side, high, high, high, [&](uint32_t i, uint32_t j, float v) {
+      factor[i * side + j] = fmaf(gram[i * side + j], p.b, p.c * v);
+    });
+    __syncthreads();
+    small_product<false>(factor, side, x, wide, high, wide - 4, high,
+                         [&](uint32_t i, uint32_t j, float v) { y[i * wide + j] = fmaf(x[i * wide + j], p.a, v); });
+    __syncthreads();
+    float* const z = x;
+    x = y;
+    y = z;
+  }
+  for (uint32_t i = threadIdx.x; i < values; i += kAhead * kSheetThreads) {
+    float v[kAhead];
+    uint64_t to[kAhead];
+#pragma unroll
+    for (uint32_t a = 0; a < kAhead; ++a) {
+      const uint32_t at = min(i + a * kSheetThreads, values - 1), row = at / e.columns, column = at % e.columns;
+      to[a] = row * e.to_stride + column;
+      v[a] = x[e.flip ? column * wide + row : row * wide + column];
+      if (e.weight) v[a] = fmaf(load_one(e.to, to[a], e.to_type), e.decay, -e.step * v[a]);
+    }
+#pragma unroll
+    for (uint32_t a = 0; a < kAhead; ++a) {
+      if (i + a * kSheetThreads >= values) continue;
+      if (e.param) global<bf16>(e.param)[to[a]] = bf16(v[a]);
+      store_one(e.to, to[a], e.to_type, v[a]);
+    }
+  }
+}
+
 static_assert(sizeof(Table<SourceEntry>) + 32 <= 4064 && sizeof(Table<Entry>) <= 3832 && sizeof(Table<LastEntry>) <= 4064,
               "kernel arguments");
 
@@ -489,6 +660,12 @@ struct Work {
   bool flip() const { return split < 0 ? rows > columns : split == 0; }
   uint32_t m() const { return uint32_t(flip() ? columns : rows); }
   uint32_t n() const { return uint32_t(flip() ? rows : columns); }
+  // Whether it goes through one workgroup: what does not fit shared memory, or is
+  // summed up over ranks, does not.
+  bool small() const {
+    return split < 0 && m() <= kSmallSide && uint64_t(fours(m())) * fours(n()) <= kSmallValues &&
+           uint64_t(m()) * m() * n() <= kSmallWork;
+  }
   bool empty() const { return split < 0 ? rows == 0 || columns == 0 : m() == 0; }
 };
 
@@ -521,7 +698,7 @@ std::vector<Group> groups_of(const std::vector<Work>& all) {
   for (bool split : {false, true}) {
     std::vector<const Work*> some;
     for (const Work& w : all)
-      if ((w.split >= 0) == split && !w.empty()) some.push_back(&w);
+      if ((w.split >= 0) == split && !w.empty() && !w.small()) some.push_back(&w);
     // long tiles first: what remains at a launch's end is short
     std::stable_sort(some.begin(), some.end(), [&](const Work* a, const Work* b) {
       return a->m() != b->m() ? a->m() > b->m() : !split && a->n() > b->n();
@@ -672,8 +849,41 @@ int run_group(const Group& g, const Steps& s, Space& space, bool launch, hipStre
   return SR_OK;
 }
 
+// The small ones.
+int run_small(const std::vector<Work>& all, const Steps& s, hipStream_t stream) {
+  SmallTable t;
+  t.mix = s.mix;
+  t.eps = s.ns->eps;
+  t.steps = s.ns->steps;
+  for (int32_t k = 0; k < s.ns->steps; ++k) {
+    const double* c = s.ns->coefficients + 3 * k;
+    t.step[k] = {float(c[0]), float(c[1]), float(c[2])};
+  }
+  int count = 0;
+  auto flush = [&]() -> int {
+    if (count == 0) return SR_OK;
+    small_kernel<<<count, kSheetThreads, 0, stream>>>(t);
+    count = 0;
+    return launched(s.who);
+  };
+  for (const Work& w : all) {
+    if (w.empty() || !w.small()) continue;
+    t.entry[count++] = {reinterpret_cast<uint64_t>(w.source), reinterpret_cast<uint64_t>(w.momentum),
+                        reinterpret_cast<uint64_t>(w.to), reinterpret_cast<uint64_t>(w.param), w.source_stride, w.to_stride,
+                        uint32_t(w.rows), uint32_t(w.columns), w.source_type, w.momentum_type, w.to_type, w.flip(), w.weight,
+                        w.decay, w.step};
+    if (count == kSmallEntries) {
+      if (int rc = flush()) return rc;
+    }
+  }
+  return flush();
+}
+
 // All groups, one after another in the same memory.
 int run_all(const std::vector<Work>& all, const Steps& s, Space& space, bool launch, hipStream_t stream) {
+  if (launch) {
+    if (int rc = run_small(all, s, stream)) return rc;
+  }
   for (const Group& g : groups_of(all)) {
     space.used = 0;
     if (int rc = run_group(g, s, space, launch, stream)) return rc;

@@ -38,7 +38,7 @@ def steps(n=5, coefficients=None, eps=1e-7, reduce=None, reserved=0):
     return Steps(n, reserved, (F64 * max(1, len(c)))(*c), eps, reduce or REDUCE(0), None)
 
 
-def matrix(rows=8, cols=16, at=0, dtype=_lib.SR_DT_F32, split=-1, stride=None):
+def matrix(rows=72, cols=80, at=0, dtype=_lib.SR_DT_F32, split=-1, stride=None):
     return Matrix(BASE + at, rows, cols, cols if stride is None else stride, dtype, split)
 
 
@@ -58,6 +58,9 @@ def test_workspace():
     rc, need = workspace([matrix(100, 200)])
     assert rc == 0 and 100 * 4 * (2 * 224 + 2 * 128) <= need <= 100 * 4 * (2 * 224 + 2 * 128) + 4096
     assert workspace([matrix(200, 100)]) == (rc, need)
+    # small ones stay in shared memory
+    assert workspace([matrix(16, 24), matrix(64, 64, 1 << 20), matrix(700, 16, 2 << 20)]) == (0, 0)
+    assert workspace([matrix(64, 65)])[1] > 0 and workspace([matrix(3200, 8)])[1] > 0
     # matrices beyond 8 GiB go one group after another, in the same memory
     big = [matrix(8192, 8192, i << 30, _lib.SR_DT_BF16) for i in range(12)]
     one, all_ = workspace(big[:8])[1], workspace(big, [matrix(8192, 8192, (100 + i) << 30, _lib.SR_DT_BF16) for i in range(12)])[1]
@@ -73,7 +76,7 @@ def test_bad_matrices(bad, code):
 
 
 def test_bad_destinations():
-    assert workspace([matrix()], [matrix(16, 8, 1 << 20)])[0] == _lib.SR_EINVAL
+    assert workspace([matrix()], [matrix(80, 72, 1 << 20)])[0] == _lib.SR_EINVAL
     assert workspace([matrix()], [matrix(at=64)])[0] == _lib.SR_EOVERLAP
     assert workspace([matrix()], [matrix()])[0] == 0                       # in place
     assert workspace([matrix(), matrix()], [matrix(), matrix()])[0] == _lib.SR_EOVERLAP
@@ -113,7 +116,7 @@ def muon(tensors, options=None, ns=None):
                                         ctypes.byref(ns), ctypes.byref(need)), need.value
 
 
-def tensor(i=0, rows=8, cols=16, **other):
+def tensor(i=0, rows=72, cols=80, **other):
     at = BASE + (i << 28)
     t = Tensor_(at, at + (1 << 24), at + (2 << 24), at + (3 << 24), rows, cols, 1.0, _lib.SR_DT_F32, _lib.SR_DT_F32,
                 _lib.SR_DT_BF16, -1, 0)

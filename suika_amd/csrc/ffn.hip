@@ -292,13 +292,16 @@ struct ThinArgs {
   uint64_t x, m, m2, out;     // m2: up, or 0
   uint64_t x_stride, m_stride, m2_stride;     // elements
   uint32_t tokens, rows, k, out_stride;
+  uint32_t each;              // rows of a workgroup, of each matrix
   int32_t activation;
 };
 
-constexpr int kThinRows = 16;
-
-// GROUPS: of 16 tokens; WAVES: of a workgroup; GATED: two matrices and the
-// activation.
+// GROUPS: of 16 tokens; WAVES: of a workgroup; GATED: rows of G and of U, and the
+// activation.  Up to 16 tokens a workgroup has 8 rows of each as the 16 of a block,
+// so that 4736 rows are 592 workgroups instead of 296 on 256 compute units (one
+// token and 3584 columns 17.0 us, 21.2 with 16 rows of each); with more tokens x is
+// read for 16 rows of each at once (24 tokens, 8192 rows of 4096 columns 36 us, 48
+// with 8 of each).
 template <typename T, int GROUPS, int WAVES, bool GATED>
 __global__ __launch_bounds__(WAVES * kWave) void thin_kernel(ThinArgs t) {
   typedef Thin<T> K;
@@ -306,31 +309,38 @@ __global__ __launch_bounds__(WAVES * kWave) void thin_kernel(ThinArgs t) {
   constexpr int kEach = 16 / sizeof(T);       // k of a lane
   constexpr int kSpan = 4 * kEach;            // of a wave's 16 x 16 block
   constexpr int kAhead = 4;                   // of them on their way at once
-  constexpr int kMatrices = GATED ? 2 : 1;
+  constexpr bool kPacked = GATED && GROUPS == 1;       // rows of both in a block
+  constexpr int kBlocks = GATED && !kPacked ? 2 : 1;
+  constexpr uint32_t kRows = kPacked ? 8 : 16;
   const uint32_t lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
-  const uint32_t row = min(blockIdx.x * kThinRows + lane % 16, t.rows - 1);
+  // (a lane without a row of its own loads its neighbour's)
+  const uint32_t first_row = blockIdx.x * t.each, end = min(first_row + t.each, t.rows);
+  const uint32_t row = min(first_row + lane % kRows, end - 1);
   const uint32_t mine = lane / 16 * kEach;
-  const T* m[kMatrices];
-  m[0] = global<const T>(t.m) + row * t.m_stride;
-  if (GATED) m[kMatrices - 1] = global<const T>(t.m2) + row * t.m2_stride;
+  const T* m[kBlocks];
+#pragma unroll
+  for (int i = 0; i < kBlocks; ++i) {
+    const bool second = kPacked ? lane % 16 >= 8 : i == 1;
+    m[i] = global<const T>(second ? t.m2 : t.m) + row * (second ? t.m2_stride : t.m_stride);
+  }
   const T* x[GROUPS];
 #pragma unroll
   for (int g = 0; g < GROUPS; ++g)
     x[g] = global<const T>(t.x) + min(uint32_t(16 * g) + lane % 16, t.tokens - 1) * t.x_stride;
-  f32x4 c[kMatrices][GROUPS];
+  f32x4 c[kBlocks][GROUPS];
 #pragma unroll
-  for (int i = 0; i < kMatrices; ++i)
+  for (int i = 0; i < kBlocks; ++i)
 #pragma unroll
     for (int g = 0; g < GROUPS; ++g) c[i][g] = f32x4(0.0f);
   auto read = [&](const T* p) { return *reinterpret_cast<const Vec<T, kEach>*>(p); };
   const uint32_t blocks = t.k / (kSpan * kAhead);
   for (uint32_t b = wave; b < blocks; b += WAVES) {
     const uint32_t k = b * (kSpan * kAhead) + mine;
-    Frag w[kMatrices][kAhead], v[GROUPS][kAhead];
+    Frag w[kBlocks][kAhead], v[GROUPS][kAhead];
 #pragma unroll
     for (int a = 0; a < kAhead; ++a)
 #pragma unroll
-      for (int i = 0; i < kMatrices; ++i) w[i][a] = read(m[i] + k + a * kSpan);
+      for (int i = 0; i < kBlocks; ++i) w[i][a] = read(m[i] + k + a * kSpan);
 #pragma unroll
     for (int a = 0; a < kAhead; ++a)
 #pragma unroll
@@ -340,7 +350,7 @@ __global__ __launch_bounds__(WAVES * kWave) void thin_kernel(ThinArgs t) {
 #pragma unroll
       for (int g = 0; g < GROUPS; ++g)
 #pragma unroll
-        for (int i = 0; i < kMatrices; ++i) K::add(w[i][a], v[g][a], c[i][g]);
+        for (int i = 0; i < kBlocks; ++i) K::add(w[i][a], v[g][a], c[i][g]);
   }
   // what is left of k, a block at a time
   const uint32_t rest = blocks * kSpan * kAhead;
@@ -353,39 +363,38 @@ __global__ __launch_bounds__(WAVES * kWave) void thin_kernel(ThinArgs t) {
       for (int e = 0; e < kEach; ++e) f[e] = k + e < t.k ? p[k + e] : T(0);
       return f;
     };
-    Frag w[kMatrices];
+    Frag w[kBlocks];
 #pragma unroll
-    for (int i = 0; i < kMatrices; ++i) w[i] = tail(m[i]);
+    for (int i = 0; i < kBlocks; ++i) w[i] = tail(m[i]);
 #pragma unroll
     for (int g = 0; g < GROUPS; ++g) {
       const Frag v = tail(x[g]);
 #pragma unroll
-      for (int i = 0; i < kMatrices; ++i) K::add(w[i], v, c[i][g]);
+      for (int i = 0; i < kBlocks; ++i) K::add(w[i], v, c[i][g]);
     }
   }
   // four rows of a token a lane; the waves' sums in order
-  __shared__ f32x4 part[WAVES][kMatrices][GROUPS][kWave];
+  __shared__ f32x4 part[WAVES][kBlocks][GROUPS][kWave];
 #pragma unroll
-  for (int i = 0; i < kMatrices; ++i)
+  for (int i = 0; i < kBlocks; ++i)
 #pragma unroll
     for (int g = 0; g < GROUPS; ++g) part[wave][i][g][lane] = c[i][g];
   __syncthreads();
-  if (wave >= GROUPS) return;
-  const uint32_t token = wave * 16 + lane % 16, first = blockIdx.x * kThinRows + lane / 16 * 4;
-  f32x4 sum[kMatrices];
+  if (wave >= GROUPS || lane >= 4 * kRows) return;
+  const uint32_t token = wave * 16 + lane % 16, first = first_row + lane / 16 * 4;
+  const uint32_t up_lane = kPacked ? (lane + 32) % kWave : lane;
+  f32x4 sum = part[0][0][wave][lane], up = part[0][kBlocks - 1][wave][up_lane];
 #pragma unroll
-  for (int i = 0; i < kMatrices; ++i) {
-    sum[i] = part[0][i][wave][lane];
-#pragma unroll
-    for (int w = 1; w < WAVES; ++w) sum[i] += part[w][i][wave][lane];
+  for (int w = 1; w < WAVES; ++w) {
+    sum += part[w][0][wave][lane];
+    if (GATED) up += part[w][kBlocks - 1][wave][up_lane];
   }
   if (token >= t.tokens) return;
   T* out = global<T>(t.out) + uint64_t(token) * t.out_stride;
 #pragma unroll
   for (int r = 0; r < 4; ++r) {
-    if (first + r >= t.rows) return;
-    const float v = GATED ? act<false>(sum[0][r], t.activation).value * sum[kMatrices - 1][r] : sum[0][r];
-    out[first + r] = static_cast<T>(v);
+    if (first + r >= end) return;
+    out[first + r] = static_cast<T>(GATED ? act<false>(sum[r], t.activation).value * up[r] : sum[r]);
   }
 }
 
@@ -532,10 +541,24 @@ int products(const char* who, const Wanted* w, int count, bool split, Space& spa
   return launched(who);
 }
 
+// Rows of a workgroup so that the compute unit with the most of them has few: of
+// the launch's rounds over 256 units, each its rows and about two more for the
+// tokens (5504 rows: 501 workgroups of 11, 344 of 16 would give some units 32).
+uint32_t rows_each(uint32_t rows, uint32_t most) {
+  uint32_t best = most;
+  uint64_t least = ~uint64_t(0);
+  for (uint32_t r = most; r >= 5; --r) {
+    const uint64_t time = ceil_div(ceil_div(rows, r), 256) * (r + 2);
+    if (time < least) best = r, least = time;
+  }
+  return best;
+}
+
 template <typename T, int GROUPS, bool GATED>
-void launch_thin(const ThinArgs& t, hipStream_t stream) {
-  constexpr int kWaves = 8;
-  thin_kernel<T, GROUPS, kWaves, GATED><<<uint32_t(ceil_div(t.rows, kThinRows)), kWaves * kWave, 0, stream>>>(t);
+void launch_thin(ThinArgs t, hipStream_t stream) {
+  t.each = rows_each(t.rows, GATED && GROUPS == 1 ? 8 : 16);
+  constexpr int kWaves = GATED ? 8 : 16;
+  thin_kernel<T, GROUPS, kWaves, GATED><<<uint32_t(ceil_div(t.rows, t.each)), kWaves * kWave, 0, stream>>>(t);
 }
 
 template <typename T, bool GATED>
@@ -561,10 +584,10 @@ int forward(const sr_ffn_shape& s, void* out, void* a, void* b, Space& space, bo
     if (!launch) return SR_OK;
     ThinArgs g{reinterpret_cast<uint64_t>(s.x), reinterpret_cast<uint64_t>(s.gate), reinterpret_cast<uint64_t>(s.up), h,
                s.x_stride, s.gate_stride, s.up_stride, uint32_t(s.tokens), uint32_t(s.ffn), uint32_t(s.hidden),
-               uint32_t(wide), s.activation};
+               uint32_t(wide), 0, s.activation};
     thin<T, true>(g, stream);
     ThinArgs d{h, reinterpret_cast<uint64_t>(s.down), 0, reinterpret_cast<uint64_t>(out), wide, s.down_stride, 0,
-               uint32_t(s.tokens), uint32_t(s.hidden), uint32_t(s.ffn), uint32_t(s.hidden), 0};
+               uint32_t(s.tokens), uint32_t(s.hidden), uint32_t(s.ffn), uint32_t(s.hidden), 0, 0};
     thin<T, false>(d, stream);
     return launched("sr_ffn");
   }

@@ -472,7 +472,7 @@ __global__ __launch_bounds__(sr_tile::threads(SIZE), 2) void last_kernel(Table<L
 
 // A small matrix goes through everything in one workgroup and one launch, its
 // values and products in shared memory and 32 bits: 8 matrices of up to 32 x 24
-// take SMALL_US us instead of 80 with tiles, whose 17 launches are most of that.
+// take 15 us instead of 80 with tiles, whose 17 launches are most of that.
 // Up to about 64 x 64 x 64 operations a product a workgroup is as fast as tiles;
 // the rule looks at the matrix alone, so its result does not depend on the list.
 constexpr uint32_t kSmallSide = 64, kSmallValues = 64 * 196;

@@ -20,6 +20,7 @@
 
 #include <algorithm>
 #include <new>
+#include <type_traits>
 #include <vector>
 
 #include "suika_step.h"
@@ -86,7 +87,7 @@ struct ForwardArgs {
 };
 
 template <typename T, int SIZE>
-__global__ __launch_bounds__(sr_tile::threads(SIZE), 2) void forward_kernel(ForwardArgs t) {
+__global__ __launch_bounds__(sr_tile::threads(SIZE), SIZE == 64 ? 3 : 2) void forward_kernel(ForwardArgs t) {
   typedef sr_tile::Tile<T, false, SIZE, ROW, ROW, true> Tile;
   SR_TILE_MEMORY(Tile);
   const uint32_t item = sr_tile::item_of(blockIdx.x, t.grid.items, SIZE);
@@ -132,7 +133,7 @@ struct Kept {
 };
 
 template <typename T, int SIZE>
-__global__ __launch_bounds__(sr_tile::threads(SIZE), 2) void backward_kernel(BackwardArgs t) {
+__global__ __launch_bounds__(sr_tile::threads(SIZE), SIZE == 64 ? 3 : 2) void backward_kernel(BackwardArgs t) {
   typedef sr_tile::Tile<T, false, SIZE, ROW, COL> Tile;
   SR_TILE_MEMORY(Tile);
   const uint32_t item = sr_tile::item_of(blockIdx.x, t.grid.items, SIZE);
@@ -194,7 +195,7 @@ struct ProductArgs {
 };
 
 template <typename T, int SIZE, Side A, Side B>
-__global__ __launch_bounds__(sr_tile::threads(SIZE), 2) void product_kernel(ProductArgs t) {
+__global__ __launch_bounds__(sr_tile::threads(SIZE), SIZE == 64 ? 3 : 2) void product_kernel(ProductArgs t) {
   typedef sr_tile::Tile<T, false, SIZE, A, B> Tile;
   SR_TILE_MEMORY(Tile);
   uint32_t item = sr_tile::item_of(blockIdx.x, t.items, SIZE);
@@ -463,26 +464,55 @@ Operand operand(const Matrix& m, Side side) {
           uint32_t(side == ROW ? m.rows : m.columns)};
 }
 
-// The tiles' size of a product of rows x columns over `steps` steps.
-template <typename T>
-int tile_size(uint64_t rows, uint64_t columns, uint64_t steps) {
-  if (sizeof(T) == 4) return 128;
-  sr_tile::Cost large(256), small(128);
-  large.add(ceil_div(rows, 256) * ceil_div(columns, 256), steps);
-  small.add(ceil_div(rows, 128) * ceil_div(columns, 128), steps);
-  return large.time() <= small.time() ? 256 : 128;
-}
-
 // Steps of a product over k values.
 template <typename T> uint64_t steps_of(uint64_t k) { return ceil_div(k, 128 / sizeof(T)); }
 
-// Work items that a long sum is split for, and the least steps of a part.
-constexpr uint64_t kSplitItems = 512, kLeastSteps = 4;
+// How a product goes: its tiles' size, and the workgroups that a tile's steps are
+// dealt out to.
+struct Way {
+  int size;
+  uint64_t splits;
+  double time;
+};
 
-template <typename T, int SIZE, Side A, Side B>
-void launch_products(const ProductArgs& t, hipStream_t stream) {
-  product_kernel<T, SIZE, A, B><<<sr_tile::blocks_of(t.items, SIZE), sr_tile::threads(SIZE), 0, stream>>>(t);
+// The fastest way for `count` products of rows x columns over `steps` steps each;
+// with `most` splits at most, of four steps or more, whose parts are written, read
+// and added up by another launch.
+template <typename T>
+Way way_of(const uint64_t (*sides)[2], int count, uint64_t steps, uint64_t most) {
+  constexpr bool kF32 = sizeof(T) == 4;
+  constexpr double kUnit = 0.4e-6, kLaunch = 10, kRate = 8e12;
+  Way best{128, 1, 1e30};
+  for (int size : {256, 128, 64}) {
+    if (kF32 && size == 256) continue;
+    for (uint64_t splits = 1; splits <= std::max<uint64_t>(1, std::min(most, steps / 4)); ++splits) {
+      sr_tile::Cost cost(size, kF32);
+      double join = 0;
+      for (int i = 0; i < count; ++i) {
+        cost.add(ceil_div(sides[i][0], size) * ceil_div(sides[i][1], size) * splits, ceil_div(steps, splits));
+        if (splits > 1) join += kLaunch + double(sides[i][0]) * double(sides[i][1]) * 8 * splits / (kRate * kUnit);
+      }
+      if (cost.time() + join < best.time) best = {size, splits, cost.time() + join};
+    }
+  }
+  return best;
 }
+
+template <typename T>
+int tile_size(uint64_t rows, uint64_t columns, uint64_t steps) {
+  const uint64_t sides[1][2] = {{rows, columns}};
+  return way_of<T>(sides, 1, steps, 1).size;
+}
+
+// f(size) with the size as a constant.
+template <typename T, typename F>
+void with_size(int size, F&& f) {
+  if (size == 64) f(std::integral_constant<int, 64>());
+  else if (sizeof(T) == 4 || size == 128) f(std::integral_constant<int, 128>());
+  else if constexpr (sizeof(T) == 2) f(std::integral_constant<int, 256>());
+}
+
+constexpr uint64_t kMostSplits = 24;
 
 struct Wanted {
   Product p;
@@ -490,19 +520,21 @@ struct Wanted {
   void* out;
 };
 
-// One product, or several of the same operands' sides.  Where there are few
-// tiles and long sums (SPLIT), their steps are dealt out to several workgroups.
+// One product, or several with the same sides of operands and as many steps.  Of one
+// with few tiles and a long sum (`split`) the steps may be dealt out.
 template <typename T, Side A, Side B>
 int products(const char* who, const Wanted* w, int count, bool split, Space& space, bool launch, hipStream_t stream) {
-  sr_tile::Cost large(256), small(128);
+  uint64_t sides[kMostJobs][2] = {};
+  uint64_t steps = 0;
   for (int i = 0; i < count; ++i) {
-    const uint64_t k = steps_of<T>(w[i].p.k) * (w[i].p.a2.data ? 2 : 1);
-    large.add(ceil_div(w[i].rows, 256) * ceil_div(w[i].columns, 256), k);
-    small.add(ceil_div(w[i].rows, 128) * ceil_div(w[i].columns, 128), k);
+    sides[i][0] = w[i].rows;
+    sides[i][1] = w[i].columns;
+    steps = steps_of<T>(w[i].p.k) * (w[i].p.a2.data ? 2 : 1);      // alike
   }
-  const int size = sizeof(T) == 2 && large.time() <= small.time() ? 256 : 128;
+  const Way way = way_of<T>(sides, count, steps, split && count == 1 ? kMostSplits : 1);
+  const int size = way.size;
   ProductArgs t{};
-  uint64_t items = 0, steps = 0;
+  uint64_t items = 0;
   int n = 0;
   for (int i = 0; i < count; ++i) {
     if (w[i].rows == 0 || w[i].columns == 0) continue;
@@ -515,26 +547,20 @@ int products(const char* who, const Wanted* w, int count, bool split, Space& spa
     j.first = uint32_t(items);
     j.out = reinterpret_cast<uint64_t>(w[i].out);
     items += uint64_t(j.tile_rows) * j.tile_columns;
-    steps = steps_of<T>(w[i].p.k) * (w[i].p.a2.data ? 2 : 1);
     if (items > sr_tile::kMostItems) return fail(SR_EBOUNDS, "%s: a product of %llu x %llu", who,
                                                  (unsigned long long)w[i].rows, (unsigned long long)w[i].columns);
   }
   if (n == 0) return SR_OK;
   for (int i = n; i < kMostJobs; ++i) t.job[i].first = 0xffffffffu;
-  t.splits = 1;
-  if (split && n == 1 && items < kSplitItems) {
-    // two workgroups of a 128 x 128 tile are on a compute unit at once
-    const uint64_t most = std::max<uint64_t>(1, std::min<uint64_t>(kSplitItems / items, steps / kLeastSteps));
-    t.steps = uint32_t(ceil_div(steps, most));
-    t.splits = uint32_t(std::max<uint64_t>(1, ceil_div(steps, std::max<uint32_t>(1, t.steps))));
-  }
+  t.steps = uint32_t(ceil_div(steps, way.splits));
+  t.splits = uint32_t(way.splits == 1 ? 1 : ceil_div(steps, t.steps));
   const uint64_t elements = uint64_t(t.job[0].rows) * t.job[0].columns;
   if (t.splits > 1) t.parts = space.take(t.splits * elements * sizeof(float));
   if (!launch) return SR_OK;
   t.items = uint32_t(items) * t.splits;
-  if constexpr (sizeof(T) == 4) launch_products<T, 128, A, B>(t, stream);
-  else if (size == 256) launch_products<T, 256, A, B>(t, stream);
-  else launch_products<T, 128, A, B>(t, stream);
+  with_size<T>(size, [&](auto z) {
+    product_kernel<T, z(), A, B><<<sr_tile::blocks_of(t.items, z()), sr_tile::threads(z()), 0, stream>>>(t);
+  });
   if (t.splits > 1)
     join_kernel<T><<<uint32_t(ceil_div(elements, 4 * kPlainThreads)), kPlainThreads, 0, stream>>>(
         reinterpret_cast<const float*>(t.parts), t.splits, elements, reinterpret_cast<T*>(t.job[0].out));
@@ -612,9 +638,7 @@ int forward(const sr_ffn_shape& s, void* out, void* a, void* b, Space& space, bo
     t.activation = s.activation;
     if (launch) {
       const uint32_t blocks = sr_tile::blocks_of(t.grid.items, size);
-      if constexpr (sizeof(T) == 4) forward_kernel<T, 128><<<blocks, sr_tile::threads(128), 0, stream>>>(t);
-      else if (size == 256) forward_kernel<T, 256><<<blocks, sr_tile::threads(256), 0, stream>>>(t);
-      else forward_kernel<T, 128><<<blocks, sr_tile::threads(128), 0, stream>>>(t);
+      with_size<T>(size, [&](auto z) { forward_kernel<T, z()><<<blocks, sr_tile::threads(z()), 0, stream>>>(t); });
       if (int rc = launched("sr_ffn")) return rc;
     }
   }
@@ -653,9 +677,7 @@ int backward(const sr_ffn_shape& s, const void* a, const void* b, const void* dy
     t.activation = s.activation;
     if (launch) {
       const uint32_t blocks = sr_tile::blocks_of(t.grid.items, size);
-      if constexpr (sizeof(T) == 4) backward_kernel<T, 128><<<blocks, sr_tile::threads(128), 0, stream>>>(t);
-      else if (size == 256) backward_kernel<T, 256><<<blocks, sr_tile::threads(256), 0, stream>>>(t);
-      else backward_kernel<T, 128><<<blocks, sr_tile::threads(128), 0, stream>>>(t);
+      with_size<T>(size, [&](auto z) { backward_kernel<T, z()><<<blocks, sr_tile::threads(z()), 0, stream>>>(t); });
       if (int rc = launched(who)) return rc;
     }
   }

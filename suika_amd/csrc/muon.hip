@@ -735,7 +735,7 @@ int number(Table<E>& t, uint64_t most, F&& items) {
 // steps.
 template <typename E, typename F, typename G>
 int number_tiles(Table<E>& t, int& size, F&& tiles_of, G&& depth_of) {
-  sr_tile::Cost large(256), small(128);
+  sr_tile::Cost large(256, false), small(128, false);
   for (uint32_t i = 0; i < t.count; ++i) {
     large.add(tiles_of(t.entry[i], 256), depth_of(t.entry[i]));
     small.add(tiles_of(t.entry[i], 128), depth_of(t.entry[i]));

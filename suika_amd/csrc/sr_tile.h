@@ -6,8 +6,7 @@
 // Each operand is stored either with its k side by side (a row a line: ROW) or
 // with its rows side by side (a k a line: COL), so every product of a forward
 // and a backward pass works on the tensors as they are.  One workgroup of four
-// waves forms one tile of C, 256 x 256 or 128 x 128, as 2 x 2 squares of a wave
-// each, in 32 x 32 blocks.
+// 
 //
 //   - A step takes 128 bytes of every row: 64 values of 16 bits or 32 floats.
 //     They go from memory straight into shared memory, 16 bytes a lane, into
@@ -54,7 +53,7 @@ constexpr uint64_t kMostStride = uint64_t(1) << 22;     // bytes from row to row
 
 constexpr int kAllLoads = 0x0f70;                // s_waitcnt vmcnt(0)
 
-constexpr int threads(int size) { return size == 256 ? 512 : 256; }
+constexpr int threads(int size) { return size == 256 ? 512 : size == 128 ? 256 : 128; }
 
 enum Side { ROW, COL };
 
@@ -115,7 +114,10 @@ struct Part {
   // How a piece's place in its line is permuted: sixteen lanes that read a column
   // of pieces (ROW), or four lines of two pieces and their neighbours' (COL), meet
   // all 64 banks.
-  __device__ static uint32_t turn(uint32_t line) { return SIDE == ROW ? line / 2 & 7 : (line & 3) << 2; }
+  __device__ static uint32_t turn(uint32_t line) {
+    static_assert(kPieces >= 8, "a permuted place is one of the line's");
+    return SIDE == ROW ? line / 2 & 7 : (line & 3) << (kPieces == 8 ? 1 : 2);
+  }
 
   // Which matrix a wave's lines of a load are of.
   static constexpr int kTurn = PAIR ? 32 * PAIR : 1;
@@ -227,9 +229,10 @@ struct Tile {
   typedef Part<T, TWO, B, SIZE, PAIR ? kSpan / 64 : 0, kThreads> PartB;
   static constexpr int kK = PartA::kK;
   static constexpr int kGroups = kLine / 32 / (TWO ? 2 : 1);       // k groups of a step
-  static constexpr int kWide = 64 + 4;              // floats of a slab's row; four more turn the banks of the next
+  // floats of a slab's row; four more, where there is room, turn the banks of the next
+  static constexpr int kWide = SIZE == 64 ? 64 : 64 + 4;
   static constexpr int kSlab = 32 * kWide * 4;
-  static_assert(kI % 2 == 0 && kJ % 2 == 0, "slabs of two blocks");
+  static_assert(kJ % 2 == 0, "slabs of two blocks");
   static constexpr int kSlabs = SIZE * kLine / kSlab;       // in the memory of an operand
   static_assert(WAVES <= 4 * kSlabs, "the waves' slabs fit where the operands were");
 
@@ -342,7 +345,7 @@ struct Tile {
   // longer read as operands.
   template <bool FLIP, bool ROLLED, typename L, typename F>
   __device__ __forceinline__ void results(Shared slab, L&& load, F&& f) const {
-    static_assert(!(FLIP && PAIR), "");
+    static_assert(!(FLIP && (PAIR || kI % 2)), "slabs of two blocks");
     const uint32_t lane = threadIdx.x % kWave;
     const int row0 = FLIP ? wave_column() : wave_row();
     const int column0 = PAIR ? wave_column() / 2 : FLIP ? wave_row() : wave_column();
@@ -497,7 +500,7 @@ __device__ __forceinline__ void run(Tile& tile, const Product& p, uint32_t row, 
 // columns in its L2 and all dies have the same mix of long and short ones (an
 // eighth of the items each: where the long ones come first, 2.1 ms instead of
 // 1.6).  What is left behind whole rounds goes to the dies by eighths.
-constexpr uint32_t at_once(int size) { return size == 256 ? 32 : 64; }      // of a die's 32 compute units
+constexpr uint32_t at_once(int size) { return size == 256 ? 32 : size == 128 ? 64 : 128; }      // of a die's 32 compute units
 
 inline uint32_t blocks_of(uint32_t items, int size) {
   const uint32_t round = at_once(size) * sr_step::kXcds;
@@ -523,15 +526,18 @@ constexpr uint64_t kMostItems = (uint64_t(1) << 23) - 2 * sr_step::kXcds;
 struct Nothing {};
 __device__ __forceinline__ Nothing nothing(uint32_t, uint32_t) { return {}; }
 
-// How long a launch of tiles takes, in steps of a 128 x 128 tile that has a
-// compute unit to itself: the sum of the steps over the compute units and half of
-// the longest tile that ends last, or, of tiles alike, whole rounds.  A 256 x 256
-// tile's step takes as long as four, two workgroups of 128 x 128 tiles share a
-// compute unit and take 1.12 times as long for the same.  Six steps for a tile's first loads and its results.
+// How long a launch of tiles takes, in units of 0.4 us, a quarter of a 256 x 256
+// tile's step of 16-bit operands.  Of tiles alike, the compute unit with the most of
+// them counts.  256 x 256 tiles run one after another on it; smaller ones share it,
+// and have its latencies to themselves where there are few.  Measured, n tiles a
+// unit: 4.0 n a step, 1.15 n + 0.8 for 128 x 128 (2.0, 3.1, 4.0 and 13.5 for 1, 2, 3 and
+// 13), 0.5 n + 0.8 for 64 x 64 (1.4, 1.5, 3.4 and 4.6 for 2, 3, 5 and 10); floats,
+// which the matrix cores take 16 times as long for, 3.1 n + 2 and n + 2.5.  Of a
+// mixture the sum counts, and half of the longest tile, which ends last.  Six steps
+// are added for a tile's first loads and its results.
 class Cost {
  public:
-  explicit Cost(int size)
-      : slots_(size == 256 ? kUnits : 2 * kUnits), each_(size == 256 ? 4.0 : 2.25), large_(size == 256) {}
+  Cost(int size, bool f32) : size_(size), f32_(f32) {}
 
   void add(uint64_t tiles, uint64_t steps) {
     if (tiles == 0) return;
@@ -542,17 +548,27 @@ class Cost {
     longest_ = t > longest_ ? t : longest_;
   }
   double time() const {
-    // with one workgroup a compute unit nothing is shared
-    if (!large_ && tiles_ <= kUnits) return 1.2 * longest_;
-    if (alike_) return double((tiles_ + slots_ - 1) / slots_) * each_ * longest_;
-    return (sum_ / double(slots_) + longest_ / 2) * each_;
+    if (!alike_) return (sum_ / kUnits + longest_ / 2) * shared();
+    const double each = double((tiles_ + kUnits - 1) / kUnits);
+    return (each * shared() + alone()) * longest_;
   }
 
  private:
   static constexpr uint64_t kUnits = 256;      // compute units
-  uint64_t slots_, tiles_ = 0;
-  double each_, sum_ = 0, longest_ = 0;
-  bool large_, alike_ = true;
+
+  double shared() const {
+    if (f32_) return size_ == 128 ? 3.1 : 1.0;
+    return size_ == 256 ? 4.0 : size_ == 128 ? 1.15 : 0.5;
+  }
+  double alone() const {
+    if (f32_) return size_ == 128 ? 2.0 : 2.5;
+    return size_ == 256 ? 0.0 : 0.8;
+  }
+
+  int size_;
+  bool f32_, alike_ = true;
+  uint64_t tiles_ = 0;
+  double sum_ = 0, longest_ = 0;
 };
 
 // The tile of a work item, in bands of 8 tiles' rows: the tiles of neighbouring

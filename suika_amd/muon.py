@@ -61,12 +61,17 @@ def orthogonalize(matrices: Sequence[Tensor], *, steps: int = 5,
     zeros stays zeros, one with NaN or infinity becomes NaN, and the others of
     the list are not touched by it.
 
+    Not differentiable: a matrix that wants a gradient is refused, as is a
+    forward-mode tangent.
+
     ``split`` gives for each matrix ``None``, or the dimension along which ranks
     hold parts of it: 0 where the rows are dealt out, 1 the columns.  All ranks
     call with the same list; ``all_reduce`` gets 1-dim float32 and float64
     tensors on the device and sums them over the ranks in place, in the current
     stream's order (``torch.distributed.all_reduce``, for example).
     """
+    if torch.is_grad_enabled() and any(isinstance(m, Tensor) and m.requires_grad for m in matrices):
+        raise PlanError("matrices: one wants a gradient, which orthogonalize does not have")
     return _lib.host().orthogonalize(matrices, out, split, steps, _schedule(steps, coefficients), float(eps), all_reduce)
 
 

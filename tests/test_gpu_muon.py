@@ -168,6 +168,10 @@ def test_refusals():
                      (dict(split=[0]), "no reduce"), (dict(split=[2], all_reduce=print), "None, 0 or 1")]:
         with pytest.raises(PlanError, match=word):
             orthogonalize([g], **kw)
+    with pytest.raises(PlanError, match="wants a gradient"):
+        orthogonalize([g.clone().requires_grad_()])
+    with torch.no_grad():
+        assert torch.equal(orthogonalize([g.clone().requires_grad_()])[0], orthogonalize([g])[0])
     with pytest.raises(PlanError, match="a matrix"):
         orthogonalize([g[0]])
     with pytest.raises(PlanError, match="dtype"):

@@ -64,7 +64,7 @@ __device__ __forceinline__ Act act(float a, int32_t kind) {
   }
   float z = a, dz = 1.0f;
   if (kind == SR_ACT_GELU_TANH) {
-    const float q = a * a;
+    const float q = fminf(a * a, 1e30f);      // finite, so that a weight of 0 makes the slope's term 0
     z = kTanhScale * fmaf(kTanhCube * q, a, a);
     dz = kTanhScale * fmaf(3 * kTanhCube, q, 1.0f);
   }
@@ -106,8 +106,9 @@ __global__ __launch_bounds__(sr_tile::threads(SIZE), SIZE == 64 ? 3 : 2) void fo
     n += column;
     if (r >= t.tokens || n >= t.padded) return;
     float h[8];
+    // (the columns behind ffn are zeros also where a row of x has an infinity)
 #pragma unroll
-    for (int e = 0; e < 8; ++e) h[e] = act<false>(a[e], t.activation).value * b[e];
+    for (int e = 0; e < 8; ++e) h[e] = n + e < t.ffn ? act<false>(a[e], t.activation).value * b[e] : 0.0f;
     store_row(global<T>(t.h) + r * t.h_stride + n, h, t.padded - n);
     if (t.a && n < t.ffn) {
       store_row(global<float>(t.a) + uint64_t(r) * t.ffn + n, a, t.ffn - n);
@@ -163,9 +164,10 @@ __global__ __launch_bounds__(sr_tile::threads(SIZE), SIZE == 64 ? 3 : 2) void ba
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const Act f = act<true>(k.a[e], t.activation);
+      const float d = n + e < t.ffn ? dh[e] : 0.0f;      // (0 also where a row of dy has an infinity)
       h[e] = f.value * k.b[e];
-      db[e] = dh[e] * f.value;
-      da[e] = dh[e] * k.b[e] * f.slope;
+      db[e] = d * f.value;
+      da[e] = d * k.b[e] * f.slope;
     }
     const uint64_t at = r * t.stride + n;
     if (t.da) {

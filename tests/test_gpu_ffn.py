@@ -302,3 +302,32 @@ def test_refusals():
     with fwd.dual_level():
         with pytest.raises(PlanError, match="forward-mode"):
             gated_ffn(fwd.make_dual(x, x), g, up, d)
+
+
+@pytest.mark.parametrize("tokens", [4, 150])
+@pytest.mark.parametrize("ffn", [13, 16])
+def test_an_infinity_does_not_meet_the_padding(ffn, tokens):
+    """With positive values a row's infinity gives infinities, whatever ffn is a multiple of."""
+    gen = torch.Generator(DEV).manual_seed(7)
+    x, g, up, d, dy = (torch.rand(s, generator=gen, device=DEV).add_(0.5).to(BF16)
+                       for s in ((tokens, 24), (ffn, 24), (ffn, 24), (24, ffn), (tokens, 24)))
+    clean = gated_ffn(x, g, up, d, keep=True)
+    before = gated_ffn_grad(x, g, up, d, clean.gate, clean.up, dy)[0]
+    dy[1, 3] = math.inf
+    dx = gated_ffn_grad(x, g, up, d, clean.gate, clean.up, dy)[0]
+    others = [i for i in range(tokens) if i != 1]
+    assert bool((dx[1] == math.inf).all()) and torch.equal(dx[others], before[others])
+    x[1, 5] = math.inf
+    kept = gated_ffn(x, g, up, d, keep=True).out
+    assert bool((kept[1] == math.inf).all()) and torch.equal(kept[others], clean.out[others])
+    assert bool((gated_ffn(x, g, up, d)[1] == math.inf).all())
+
+
+def test_slope_of_far_gelu_tanh_gates():
+    """A gate whose square is beyond float32 has a slope of 0 or 1."""
+    for far in (-1e20, 1e20):
+        x, gate = torch.ones(1, 1, device=DEV), torch.tensor([[far]], device=DEV)
+        up, down = torch.ones(1, 1, device=DEV), torch.ones(1, 1, device=DEV)
+        r = gated_ffn(x, gate, up, down, activation="gelu_tanh", keep=True)
+        grads = gated_ffn_grad(x, gate, up, down, r.gate, r.up, torch.ones(1, 1, device=DEV), activation="gelu_tanh")
+        assert float(grads[1]) == (far > 0)

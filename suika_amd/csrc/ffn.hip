@@ -268,8 +268,15 @@ __global__ __launch_bounds__(kPlainThreads) void align_kernel(const T* from, uin
 // ---------------------------------------------------------------- few tokens
 
 // Up to 64 tokens: the matrices' bytes bound it, so their rows go from memory
-// straight to the matrix cores.  A workgroup has 16 rows (of G and of U) for all
+// straight to the matrix cores.  A workgroup has some rows (of G and of U) for all
 // tokens; its waves share out the k, and their sums are joined in shared memory.
+// The tokens come from the L2 for every workgroup, which is what keeps more than a
+// few of them from the matrices' 6 TB/s: workgroups have as many rows as leave no
+// compute unit without work.
+//
+// Measured (bf16, us of both launches): 1 token, 3584 columns and 4736 rows 14.8 + 7.8
+// (15.3 at a copy's rate), 24 tokens, 4096 and 5504 22.1 + 16.2 (20.4), 64 tokens, 3584
+// and 4736 26.8 + 24 (15.4).
 template <typename T> struct Thin;
 template <> struct Thin<bf16> {
   typedef __bf16 Frag __attribute__((ext_vector_type(8)));
@@ -299,61 +306,57 @@ struct ThinArgs {
   int32_t activation;
 };
 
-// GROUPS: of 16 tokens; WAVES: of a workgroup; GATED: rows of G and of U, and the
-// activation.  Up to 16 tokens a workgroup has 8 rows of each as the 16 of a block,
-// so that 4736 rows are 592 workgroups instead of 296 on 256 compute units (one
-// token and 3584 columns 17.0 us, 21.2 with 16 rows of each); with more tokens x is
-// read for 16 rows of each at once (24 tokens, 8192 rows of 4096 columns 36 us, 48
-// with 8 of each).
-template <typename T, int GROUPS, int WAVES, bool GATED>
+// GROUPS: of 16 tokens; BLOCKS: of 16 rows, GATED: half of them of G, then the same of
+// U; WAVES: of a workgroup.
+template <typename T, int GROUPS, int BLOCKS, int WAVES, bool GATED>
 __global__ __launch_bounds__(WAVES * kWave) void thin_kernel(ThinArgs t) {
   typedef Thin<T> K;
   typedef typename K::Frag Frag;
   constexpr int kEach = 16 / sizeof(T);       // k of a lane
   constexpr int kSpan = 4 * kEach;            // of a wave's 16 x 16 block
   constexpr int kAhead = 4;                   // of them on their way at once
-  constexpr bool kPacked = GATED && GROUPS == 1;       // rows of both in a block
-  constexpr int kBlocks = GATED && !kPacked ? 2 : 1;
-  constexpr uint32_t kRows = kPacked ? 8 : 16;
+  constexpr uint32_t kRows = 16 * BLOCKS / (GATED ? 2 : 1);      // of each matrix
   const uint32_t lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
   // (a lane without a row of its own loads its neighbour's)
   const uint32_t first_row = blockIdx.x * t.each, end = min(first_row + t.each, t.rows);
-  const uint32_t row = min(first_row + lane % kRows, end - 1);
   const uint32_t mine = lane / 16 * kEach;
-  const T* m[kBlocks];
+  const T* m[BLOCKS];
 #pragma unroll
-  for (int i = 0; i < kBlocks; ++i) {
-    const bool second = kPacked ? lane % 16 >= 8 : i == 1;
-    m[i] = global<const T>(second ? t.m2 : t.m) + row * (second ? t.m2_stride : t.m_stride);
+  for (int i = 0; i < BLOCKS; ++i) {
+    const uint32_t place = i * 16 + lane % 16, row = min(first_row + place % kRows, end - 1);
+    m[i] = place < kRows ? global<const T>(t.m) + row * t.m_stride : global<const T>(t.m2) + row * t.m2_stride;
   }
   const T* x[GROUPS];
 #pragma unroll
   for (int g = 0; g < GROUPS; ++g)
     x[g] = global<const T>(t.x) + min(uint32_t(16 * g) + lane % 16, t.tokens - 1) * t.x_stride;
-  f32x4 c[kBlocks][GROUPS];
+  f32x4 c[BLOCKS][GROUPS];
 #pragma unroll
-  for (int i = 0; i < kBlocks; ++i)
+  for (int i = 0; i < BLOCKS; ++i)
 #pragma unroll
     for (int g = 0; g < GROUPS; ++g) c[i][g] = f32x4(0.0f);
   auto read = [&](const T* p) { return *reinterpret_cast<const Vec<T, kEach>*>(p); };
   const uint32_t blocks = t.k / (kSpan * kAhead);
   for (uint32_t b = wave; b < blocks; b += WAVES) {
     const uint32_t k = b * (kSpan * kAhead) + mine;
-    Frag w[kBlocks][kAhead], v[GROUPS][kAhead];
+    Frag w[BLOCKS][kAhead], v[GROUPS][kAhead];
 #pragma unroll
     for (int a = 0; a < kAhead; ++a)
 #pragma unroll
-      for (int i = 0; i < kBlocks; ++i) w[i][a] = read(m[i] + k + a * kSpan);
+      for (int i = 0; i < BLOCKS; ++i) w[i][a] = read(m[i] + k + a * kSpan);
 #pragma unroll
     for (int a = 0; a < kAhead; ++a)
 #pragma unroll
       for (int g = 0; g < GROUPS; ++g) v[g][a] = read(x[g] + k + a * kSpan);
+    // all loads on their way: left to itself the compiler has three to six of them
+    // there at a time (24 tokens, 5504 rows of 4096 columns 31 us instead of 22)
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int a = 0; a < kAhead; ++a)
 #pragma unroll
       for (int g = 0; g < GROUPS; ++g)
 #pragma unroll
-        for (int i = 0; i < kBlocks; ++i) K::add(w[i][a], v[g][a], c[i][g]);
+        for (int i = 0; i < BLOCKS; ++i) K::add(w[i][a], v[g][a], c[i][g]);
   }
   // what is left of k, a block at a time
   const uint32_t rest = blocks * kSpan * kAhead;
@@ -366,38 +369,41 @@ __global__ __launch_bounds__(WAVES * kWave) void thin_kernel(ThinArgs t) {
       for (int e = 0; e < kEach; ++e) f[e] = k + e < t.k ? p[k + e] : T(0);
       return f;
     };
-    Frag w[kBlocks];
+    Frag w[BLOCKS];
 #pragma unroll
-    for (int i = 0; i < kBlocks; ++i) w[i] = tail(m[i]);
+    for (int i = 0; i < BLOCKS; ++i) w[i] = tail(m[i]);
 #pragma unroll
     for (int g = 0; g < GROUPS; ++g) {
       const Frag v = tail(x[g]);
 #pragma unroll
-      for (int i = 0; i < kBlocks; ++i) K::add(w[i], v, c[i][g]);
+      for (int i = 0; i < BLOCKS; ++i) K::add(w[i], v, c[i][g]);
     }
   }
   // four rows of a token a lane; the waves' sums in order
-  __shared__ f32x4 part[WAVES][kBlocks][GROUPS][kWave];
+  __shared__ f32x4 part[WAVES][BLOCKS][GROUPS][kWave];
 #pragma unroll
-  for (int i = 0; i < kBlocks; ++i)
+  for (int i = 0; i < BLOCKS; ++i)
 #pragma unroll
     for (int g = 0; g < GROUPS; ++g) part[wave][i][g][lane] = c[i][g];
   __syncthreads();
-  if (wave >= GROUPS || lane >= 4 * kRows) return;
-  const uint32_t token = wave * 16 + lane % 16, first = first_row + lane / 16 * 4;
-  const uint32_t up_lane = kPacked ? (lane + 32) % kWave : lane;
-  f32x4 sum = part[0][0][wave][lane], up = part[0][kBlocks - 1][wave][up_lane];
+  for (uint32_t p = wave; p < (kRows + 15) / 16 * GROUPS; p += WAVES) {
+    const uint32_t i = p / GROUPS, g = p % GROUPS, place = i * 16 + lane / 16 * 4, other = place + kRows;
+    if (place >= kRows) continue;
+    const uint32_t i2 = other / 16, lane2 = other % 16 / 4 * 16 + lane % 16;      // U's sums
+    const uint32_t token = g * 16 + lane % 16, first = first_row + place;
+    f32x4 sum = part[0][i][g][lane], up{};
+    if (GATED) up = part[0][i2][g][lane2];
 #pragma unroll
-  for (int w = 1; w < WAVES; ++w) {
-    sum += part[w][0][wave][lane];
-    if (GATED) up += part[w][kBlocks - 1][wave][up_lane];
-  }
-  if (token >= t.tokens) return;
-  T* out = global<T>(t.out) + uint64_t(token) * t.out_stride;
+    for (int w = 1; w < WAVES; ++w) {
+      sum += part[w][i][g][lane];
+      if (GATED) up += part[w][i2][g][lane2];
+    }
+    if (token >= t.tokens) continue;
+    T* out = global<T>(t.out) + uint64_t(token) * t.out_stride;
 #pragma unroll
-  for (int r = 0; r < 4; ++r) {
-    if (first + r >= end) return;
-    out[first + r] = static_cast<T>(GATED ? act<false>(sum[r], t.activation).value * up[r] : sum[r]);
+    for (int r = 0; r < 4; ++r) {
+      if (first + r < end) out[first + r] = static_cast<T>(GATED ? act<false>(sum[r], t.activation).value * up[r] : sum[r]);
+    }
   }
 }
 
@@ -433,7 +439,7 @@ bool loadable(const Matrix& m, int size) {
          m.stride * size <= sr_tile::kMostStride;
 }
 
-// Rows of at most this many workgroups' grids: hidden and ffn beyond 65535 x 2048 columns do not occur.
+// (a row a block: at most SR_STEP_MAX_ROWS of them, and kMostSide / 2048 for its columns)
 template <typename T>
 void launch_align(const Matrix& m, uint64_t to, hipStream_t stream) {
   const uint32_t wide = uint32_t(padded(m.columns));
@@ -569,24 +575,38 @@ int products(const char* who, const Wanted* w, int count, bool split, Space& spa
   return launched(who);
 }
 
-// Rows of a workgroup so that the compute unit with the most of them has few: of
-// the launch's rounds over 256 units, each its rows and about two more for the
-// tokens (5504 rows: 501 workgroups of 11, 344 of 16 would give some units 32).
-uint32_t rows_each(uint32_t rows, uint32_t most) {
+// Rows of a workgroup (of each matrix) so that the compute unit with the most of them
+// has few: of the launch's rounds over 256 units, each its rows, and half of a token's
+// row for every token.  Measured for G and U of 4096 columns, at 1, 2 and 3 rounds:
+// 24 tokens, 5504 rows 22.1, 27.6 and 31.8 us with 22, 11 and 8 rows; 4096 rows 17.6 and
+// 22.5 with 16 and 8; 64 tokens, 4736 rows of 3584 columns 26.8, 39.8 and 50.7 with 19,
+// 10 and 8.  Up to 16 tokens two workgroups on a unit hide each other's start: 18.4 us
+// with 11 rows and 20.8 with 22 (one token, 5504 rows).
+uint32_t rows_each(uint32_t rows, bool gated, int groups) {
+  const uint32_t most = !gated ? 32 : groups == 1 ? 12 : 24;
   uint32_t best = most;
   uint64_t least = ~uint64_t(0);
   for (uint32_t r = most; r >= 5; --r) {
-    const uint64_t time = ceil_div(ceil_div(rows, r), 256) * (r + 2);
+    const uint64_t time = ceil_div(ceil_div(rows, r), 256) * ((gated ? 2 : 1) * r + 8 * groups);
     if (time < least) best = r, least = time;
   }
   return best;
 }
 
+template <typename T, int GROUPS, int BLOCKS, bool GATED>
+void launch_blocks(const ThinArgs& t, hipStream_t stream) {
+  // (24 tokens, 5504 rows of both 22.1 us with 4 waves, 23.5 with 8; 48 tokens 33.9 and 31.8)
+  constexpr int kWaves = GROUPS == 2 ? 4 : 8;
+  thin_kernel<T, GROUPS, BLOCKS, kWaves, GATED><<<uint32_t(ceil_div(t.rows, t.each)), kWaves * kWave, 0, stream>>>(t);
+}
+
 template <typename T, int GROUPS, bool GATED>
 void launch_thin(ThinArgs t, hipStream_t stream) {
-  t.each = rows_each(t.rows, GATED && GROUPS == 1 ? 8 : 16);
-  constexpr int kWaves = GATED ? 8 : 16;
-  thin_kernel<T, GROUPS, kWaves, GATED><<<uint32_t(ceil_div(t.rows, t.each)), kWaves * kWave, 0, stream>>>(t);
+  t.each = rows_each(t.rows, GATED, GROUPS);
+  const uint32_t blocks = ceil_div(t.each, GATED ? 8 : 16);
+  if (blocks == 1) launch_blocks<T, GROUPS, 1, GATED>(t, stream);
+  else if (blocks == 2) launch_blocks<T, GROUPS, 2, GATED>(t, stream);
+  else if constexpr (GATED && GROUPS > 1) launch_blocks<T, GROUPS, 3, GATED>(t, stream);
 }
 
 template <typename T, bool GATED>

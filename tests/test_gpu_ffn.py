@@ -304,6 +304,15 @@ def test_refusals():
             gated_ffn(fwd.make_dual(x, x), g, up, d)
 
 
+# Few tokens of enough rows that a workgroup has up to 12 or 24 of both projections' and
+# up to 32 of the last product's.
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("size", [(1, 4100, 40), (3, 40, 3005), (24, 72, 5001), (24, 6001, 40), (50, 72, 5000),
+                                  (50, 6000, 33), (40, 136, 3500), (31, 264, 9000)], ids=str)
+def test_few_tokens_of_many_rows(size, dtype):
+    check(*size, dtype)
+
+
 @pytest.mark.parametrize("tokens", [4, 150])
 @pytest.mark.parametrize("ffn", [13, 16])
 def test_an_infinity_does_not_meet_the_padding(ffn, tokens):

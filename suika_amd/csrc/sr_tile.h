@@ -238,6 +238,12 @@ struct Tile {
 
   f32x16 c[kI][kJ];
 
+  // Sums of floats are formed of sums over 256 k: one over 2120 k is 1.3e-6 of the
+  // result's size off, 5e-7 in parts.  What 16 bits round off hides that.
+  static constexpr bool kParts = sizeof(T) == 4;
+  static constexpr uint32_t kPart = 8;      // steps
+  f32x16 whole[kParts ? kI : 1][kParts ? kJ : 1];
+
   __device__ __forceinline__ static int wave() { return __builtin_amdgcn_readfirstlane(threadIdx.x / kWave); }
   __device__ __forceinline__ static int wave_row() { return wave() % 2 * kRows; }
   __device__ __forceinline__ static int wave_column() { return wave() / 2 * kSpan; }
@@ -246,7 +252,33 @@ struct Tile {
 #pragma unroll
     for (int i = 0; i < kI; ++i)
 #pragma unroll
-      for (int j = 0; j < kJ; ++j) c[i][j] = f32x16(0.0f);
+      for (int j = 0; j < kJ; ++j) {
+        c[i][j] = f32x16(0.0f);
+        if constexpr (kParts) whole[i][j] = f32x16(0.0f);
+      }
+  }
+
+  // The end of a part.
+  __device__ __forceinline__ void part() {
+    if constexpr (kParts) {
+#pragma unroll
+      for (int i = 0; i < kI; ++i)
+#pragma unroll
+        for (int j = 0; j < kJ; ++j) {
+          whole[i][j] += c[i][j];
+          c[i][j] = f32x16(0.0f);
+        }
+    }
+  }
+
+  // The sums, in `c`.
+  __device__ __forceinline__ void join() {
+    if constexpr (kParts) {
+#pragma unroll
+      for (int i = 0; i < kI; ++i)
+#pragma unroll
+        for (int j = 0; j < kJ; ++j) c[i][j] += whole[i][j];
+    }
   }
 
   // The operands of a k group.
@@ -478,11 +510,13 @@ __device__ __forceinline__ void run(Tile& tile, const Product& p, uint32_t row, 
     if (s + 3 < to) fetch(s + 3, a1, b1);
     if (s + 2 < to) g[0].read(a0, b0, 0);
     tile.last_products(g);
+    if (Tile::kParts && (s - from + 2) % Tile::kPart == 0) tile.part();
   }
   if (s < to) {
     tile.most_products(g, a0, b0);
     tile.last_products(g);
   }
+  tile.join();
 }
 
 // What a workgroup of these kernels has of shared memory: two halves of both

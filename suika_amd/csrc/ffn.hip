@@ -87,7 +87,7 @@ struct ForwardArgs {
 };
 
 template <typename T, int SIZE>
-__global__ __launch_bounds__(sr_tile::threads(SIZE), SIZE == 64 ? 3 : 2) void forward_kernel(ForwardArgs t) {
+__global__ __launch_bounds__(sr_tile::threads<T>(SIZE), SIZE == 64 ? 3 : 2) void forward_kernel(ForwardArgs t) {
   typedef sr_tile::Tile<T, false, SIZE, ROW, ROW, true> Tile;
   SR_TILE_MEMORY(Tile);
   const uint32_t item = sr_tile::item_of(blockIdx.x, t.grid.items, SIZE);
@@ -134,7 +134,7 @@ struct Kept {
 };
 
 template <typename T, int SIZE>
-__global__ __launch_bounds__(sr_tile::threads(SIZE), SIZE == 64 ? 3 : 2) void backward_kernel(BackwardArgs t) {
+__global__ __launch_bounds__(sr_tile::threads<T>(SIZE), SIZE == 64 ? 3 : 2) void backward_kernel(BackwardArgs t) {
   typedef sr_tile::Tile<T, false, SIZE, ROW, COL> Tile;
   SR_TILE_MEMORY(Tile);
   const uint32_t item = sr_tile::item_of(blockIdx.x, t.grid.items, SIZE);
@@ -197,7 +197,7 @@ struct ProductArgs {
 };
 
 template <typename T, int SIZE, Side A, Side B>
-__global__ __launch_bounds__(sr_tile::threads(SIZE), SIZE == 64 ? 3 : 2) void product_kernel(ProductArgs t) {
+__global__ __launch_bounds__(sr_tile::threads<T>(SIZE), SIZE == 64 ? 3 : 2) void product_kernel(ProductArgs t) {
   typedef sr_tile::Tile<T, false, SIZE, A, B> Tile;
   SR_TILE_MEMORY(Tile);
   uint32_t item = sr_tile::item_of(blockIdx.x, t.items, SIZE);
@@ -567,7 +567,7 @@ int products(const char* who, const Wanted* w, int count, bool split, Space& spa
   if (!launch) return SR_OK;
   t.items = uint32_t(items) * t.splits;
   with_size<T>(size, [&](auto z) {
-    product_kernel<T, z(), A, B><<<sr_tile::blocks_of(t.items, z()), sr_tile::threads(z()), 0, stream>>>(t);
+    product_kernel<T, z(), A, B><<<sr_tile::blocks_of(t.items, z()), sr_tile::threads<T>(z()), 0, stream>>>(t);
   });
   if (t.splits > 1)
     join_kernel<T><<<uint32_t(ceil_div(elements, 4 * kPlainThreads)), kPlainThreads, 0, stream>>>(
@@ -660,7 +660,7 @@ int forward(const sr_ffn_shape& s, void* out, void* a, void* b, Space& space, bo
     t.activation = s.activation;
     if (launch) {
       const uint32_t blocks = sr_tile::blocks_of(t.grid.items, size);
-      with_size<T>(size, [&](auto z) { forward_kernel<T, z()><<<blocks, sr_tile::threads(z()), 0, stream>>>(t); });
+      with_size<T>(size, [&](auto z) { forward_kernel<T, z()><<<blocks, sr_tile::threads<T>(z()), 0, stream>>>(t); });
       if (int rc = launched("sr_ffn")) return rc;
     }
   }
@@ -699,7 +699,7 @@ int backward(const sr_ffn_shape& s, const void* a, const void* b, const void* dy
     t.activation = s.activation;
     if (launch) {
       const uint32_t blocks = sr_tile::blocks_of(t.grid.items, size);
-      with_size<T>(size, [&](auto z) { backward_kernel<T, z()><<<blocks, sr_tile::threads(z()), 0, stream>>>(t); });
+      with_size<T>(size, [&](auto z) { backward_kernel<T, z()><<<blocks, sr_tile::threads<T>(z()), 0, stream>>>(t); });
       if (int rc = launched(who)) return rc;
     }
   }

@@ -273,7 +273,7 @@ __device__ __forceinline__ Operand columns_of(uint64_t data, uint32_t n) { retur
 // SQUARE false: A = X X^T, or its floats where ranks add them up.  SQUARE true:
 // B = b A + c A A.
 template <int SIZE, bool SQUARE>
-__global__ __launch_bounds__(sr_tile::threads(SIZE), 2) void symmetric_kernel(Table<Entry> t, Polynomial p) {
+__global__ __launch_bounds__(sr_tile::threads<f16>(SIZE), 2) void symmetric_kernel(Table<Entry> t, Polynomial p) {
   typedef sr_tile::Tile<f16, true, SIZE, ROW, ROW> Tile;
   SR_TILE_MEMORY(Tile);
   uint32_t item = sr_tile::item_of(blockIdx.x, t.items, SIZE);
@@ -365,7 +365,7 @@ __device__ __forceinline__ void add_scaled(Tile& tile, const E& e, uint32_t row,
 
 // X <- a X + B X.
 template <int SIZE>
-__global__ __launch_bounds__(sr_tile::threads(SIZE), 2) void update_kernel(Table<Entry> t, float a) {
+__global__ __launch_bounds__(sr_tile::threads<f16>(SIZE), 2) void update_kernel(Table<Entry> t, float a) {
   typedef sr_tile::Tile<f16, true, SIZE, ROW, COL> Tile;
   SR_TILE_MEMORY(Tile);
   uint32_t item = sr_tile::item_of(blockIdx.x, t.items, SIZE);
@@ -411,7 +411,7 @@ struct Eight {
 };
 
 template <int SIZE>
-__global__ __launch_bounds__(sr_tile::threads(SIZE), 2) void last_kernel(Table<LastEntry> t, float a) {
+__global__ __launch_bounds__(sr_tile::threads<f16>(SIZE), 2) void last_kernel(Table<LastEntry> t, float a) {
   typedef sr_tile::Tile<f16, true, SIZE, ROW, COL> Tile;
   SR_TILE_MEMORY(Tile);
   uint32_t item = sr_tile::item_of(blockIdx.x, t.items, SIZE);
@@ -820,20 +820,20 @@ int run_group(const Group& g, const Steps& s, Space& space, bool launch, hipStre
     const double* c = s.ns->coefficients + 3 * k;
     const Polynomial p{float(c[0]), float(c[1]), float(c[2])};
     const uint32_t blocks = sr_tile::blocks_of(gram.items, large);
-    if (large == 256) symmetric_kernel<256, false><<<blocks, sr_tile::threads(256), 0, stream>>>(gram, p);
-    else symmetric_kernel<128, false><<<blocks, sr_tile::threads(128), 0, stream>>>(gram, p);
+    if (large == 256) symmetric_kernel<256, false><<<blocks, sr_tile::threads<f16>(256), 0, stream>>>(gram, p);
+    else symmetric_kernel<128, false><<<blocks, sr_tile::threads<f16>(128), 0, stream>>>(gram, p);
     if (g.split) {
       if (int rc = launched(s.who)) return rc;
       if (int rc = reduce(s, grams, gram_floats, SR_DT_F32, stream)) return rc;
       halves_kernel<<<halves.items, kSheetThreads, 0, stream>>>(halves);
     }
-    if (large == 256) symmetric_kernel<256, true><<<blocks, sr_tile::threads(256), 0, stream>>>(gram, p);
-    else symmetric_kernel<128, true><<<blocks, sr_tile::threads(128), 0, stream>>>(gram, p);
+    if (large == 256) symmetric_kernel<256, true><<<blocks, sr_tile::threads<f16>(256), 0, stream>>>(gram, p);
+    else symmetric_kernel<128, true><<<blocks, sr_tile::threads<f16>(128), 0, stream>>>(gram, p);
     if (update.items == 0) continue;      // nothing of these matrices is here
     if (k + 1 < s.ns->steps) {
       const uint32_t many = sr_tile::blocks_of(update.items, wide);
-      if (wide == 256) update_kernel<256><<<many, sr_tile::threads(256), 0, stream>>>(update, p.a);
-      else update_kernel<128><<<many, sr_tile::threads(128), 0, stream>>>(update, p.a);
+      if (wide == 256) update_kernel<256><<<many, sr_tile::threads<f16>(256), 0, stream>>>(update, p.a);
+      else update_kernel<128><<<many, sr_tile::threads<f16>(128), 0, stream>>>(update, p.a);
       for (uint32_t i = 0; i < t.count; ++i) {
         std::swap(gram.entry[i].x, gram.entry[i].y);
         std::swap(update.entry[i].x, update.entry[i].y);
@@ -841,8 +841,8 @@ int run_group(const Group& g, const Steps& s, Space& space, bool launch, hipStre
     } else {
       for (uint32_t i = 0; i < t.count; ++i) last.entry[i].x = update.entry[i].x;
       const uint32_t many = sr_tile::blocks_of(last.items, wide);
-      if (wide == 256) last_kernel<256><<<many, sr_tile::threads(256), 0, stream>>>(last, p.a);
-      else last_kernel<128><<<many, sr_tile::threads(128), 0, stream>>>(last, p.a);
+      if (wide == 256) last_kernel<256><<<many, sr_tile::threads<f16>(256), 0, stream>>>(last, p.a);
+      else last_kernel<128><<<many, sr_tile::threads<f16>(128), 0, stream>>>(last, p.a);
     }
     if (int rc = launched(s.who)) return rc;
   }

@@ -5,8 +5,8 @@
 //
 // Each operand is stored either with its k side by side (a row a line: ROW) or
 // with its rows side by side (a k a line: COL), so every product of a forward
-// and a backward pass works on the tensors as they are.  One workgroup of four
-// 
+// and a backward pass works on the tensors as they are.  A tile is 256 x 256 with
+// 8 waves of 128 x 64, 128 x 128 with 4 of 64 x 64, or 64 x 64 with 2 of 32 x 64.
 //
 //   - A step takes 128 bytes of every row: 64 values of 16 bits or 32 floats.
 //     They go from memory straight into shared memory, 16 bytes a lane, into
@@ -20,10 +20,13 @@
 //   - What lies outside an operand is read as zero: such lanes ask for an
 //     address beyond the buffer resource.
 //
-// A 256 x 256 tile reads 1 byte of memory for 128 operations of bf16, a wave
-// of it 1 byte of shared memory for 64: at 128 bytes a clock that is half of
-// what the matrix cores take.  128 x 128 tiles need twice as much of both, but
-// two workgroups share a compute unit; they serve products with few tiles.
+// A 256 x 256 tile of 16 bits does 128 operations for a byte that it loads, and 85
+// for one that its waves read of shared memory.  The matrix cores alone reach 1.88
+// PFLOP/s of bf16 here, with these reads 1.54, with the loads and barriers of whole
+// products 1.25 to 1.28 (f16 pairs, below, 1.34 to 1.38): a step has one barrier, at
+// which the waves meet.  128 x 128 tiles load twice as much, but two workgroups fill
+// each other's gaps: 1.17 and 1.22.  They and 64 x 64 ones serve products with few
+// tiles; Cost, below, says which is taken.
 //
 // Values of 22 bits (TWO): a matrix as two of f16, the values rounded and what
 // the rounding lost, 32 of the one and 32 of the other in turn in every row.
@@ -53,7 +56,12 @@ constexpr uint64_t kMostStride = uint64_t(1) << 22;     // bytes from row to row
 
 constexpr int kAllLoads = 0x0f70;                // s_waitcnt vmcnt(0)
 
-constexpr int threads(int size) { return size == 256 ? 512 : size == 128 ? 256 : 128; }
+// Threads of a workgroup; `halves`: sets of waves that share out a step's k.  Two for
+// 64 x 64 tiles of floats, whose products take long where a compute unit has but one.
+template <typename T> constexpr int halves(int size) { return size == 64 && sizeof(T) == 4 ? 2 : 1; }
+template <typename T> constexpr int threads(int size) {
+  return size == 256 ? 512 : size == 128 ? 256 : 128 * halves<T>(64);
+}
 
 enum Side { ROW, COL };
 
@@ -217,18 +225,19 @@ struct Part {
 // One tile: T: the operands' type, TWO: values of 22 bits, SIZE: rows and
 // columns, A, B: how they are stored, PAIR: B's rows are those of two matrices
 // in turn, so that a wave has both products of the same columns.
-template <typename T, bool TWO_, int SIZE_, Side A, Side B, bool PAIR_ = false, int WAVES = threads(SIZE_) / kWave>
+template <typename T, bool TWO_, int SIZE_, Side A, Side B, bool PAIR_ = false>
 struct Tile {
   static constexpr int SIZE = SIZE_;
   static constexpr bool TWO = TWO_, PAIR = PAIR_;
-  static constexpr int kThreads = WAVES * kWave;
+  static constexpr int kThreads = threads<T>(SIZE), kHalves = halves<T>(SIZE);
+  static constexpr int WAVES = kThreads / kWave / kHalves;       // of a half
   static constexpr int kRows = SIZE / 2, kSpan = SIZE / (WAVES / 2);     // of a wave
   static constexpr int kI = kRows / 32, kJ = kSpan / 32;
   static constexpr int kColumns = PAIR ? SIZE / 2 : SIZE;     // of C
   typedef Part<T, TWO, A, SIZE, 0, kThreads> PartA;
   typedef Part<T, TWO, B, SIZE, PAIR ? kSpan / 64 : 0, kThreads> PartB;
   static constexpr int kK = PartA::kK;
-  static constexpr int kGroups = kLine / 32 / (TWO ? 2 : 1);       // k groups of a step
+  static constexpr int kGroups = kLine / 32 / (TWO ? 2 : 1) / kHalves;       // k groups of a step, of a half
   // floats of a slab's row; four more, where there is room, turn the banks of the next
   static constexpr int kWide = SIZE == 64 ? 64 : 64 + 4;
   static constexpr int kSlab = 32 * kWide * 4;
@@ -244,7 +253,8 @@ struct Tile {
   static constexpr uint32_t kPart = 8;      // steps
   f32x16 whole[kParts ? kI : 1][kParts ? kJ : 1];
 
-  __device__ __forceinline__ static int wave() { return __builtin_amdgcn_readfirstlane(threadIdx.x / kWave); }
+  __device__ __forceinline__ static int wave() { return __builtin_amdgcn_readfirstlane(threadIdx.x / kWave) % WAVES; }
+  __device__ __forceinline__ static int half() { return __builtin_amdgcn_readfirstlane(threadIdx.x / kWave) / WAVES; }
   __device__ __forceinline__ static int wave_row() { return wave() % 2 * kRows; }
   __device__ __forceinline__ static int wave_column() { return wave() / 2 * kSpan; }
 
@@ -271,13 +281,42 @@ struct Tile {
     }
   }
 
-  // The sums, in `c`.
-  __device__ __forceinline__ void join() {
+  // The sums, in `c` of the first half's waves; every wave comes by.  The second
+  // half's go through the slabs, of which its waves have none.
+  __device__ __forceinline__ void join(Shared a0, Shared a1, Shared b0, Shared b1) {
     if constexpr (kParts) {
 #pragma unroll
       for (int i = 0; i < kI; ++i)
 #pragma unroll
         for (int j = 0; j < kJ; ++j) c[i][j] += whole[i][j];
+    }
+    if constexpr (kHalves > 1) {
+      static_assert(kHalves == 2 && kI * kJ * 16 * kWave * 4 <= kSlab, "a wave's sums fit its slab");
+      typedef __attribute__((address_space(3))) f32x4* Fours;
+      const Fours mine = (Fours)slab(a0, a1, b0, b1) + threadIdx.x % kWave;
+      __syncthreads();
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        if (half() != r) {
+#pragma unroll
+          for (int i = 0; i < kI; ++i)
+#pragma unroll
+            for (int j = 0; j < kJ; ++j)
+#pragma unroll
+              for (int q = 0; q < 4; ++q) {
+                const Fours at = mine + ((i * kJ + j) * 4 + q) * kWave;
+                f32x16& x = c[i][j];
+                if (r == 0) {
+                  *at = f32x4{x[4 * q], x[4 * q + 1], x[4 * q + 2], x[4 * q + 3]};
+                } else {
+                  const f32x4 more = *at;
+#pragma unroll
+                  for (int e = 0; e < 4; ++e) x[4 * q + e] += more[e];
+                }
+              }
+        }
+        if (r == 0) __syncthreads();
+      }
     }
   }
 
@@ -287,6 +326,7 @@ struct Tile {
 
     __device__ __forceinline__ void read(Shared sa, Shared sb, int s) {
       const int row = wave_row(), column = wave_column();
+      if (kHalves > 1) s += half() * kGroups;
 #pragma unroll
       for (int j = 0; j < kJ; ++j) b[j] = PartB::template frag<false>(sb, column + 32 * j, s);
 #pragma unroll
@@ -378,6 +418,7 @@ struct Tile {
   template <bool FLIP, bool ROLLED, typename L, typename F>
   __device__ __forceinline__ void results(Shared slab, L&& load, F&& f) const {
     static_assert(!(FLIP && (PAIR || kI % 2)), "slabs of two blocks");
+    if (kHalves > 1 && half()) return;
     const uint32_t lane = threadIdx.x % kWave;
     const int row0 = FLIP ? wave_column() : wave_row();
     const int column0 = PAIR ? wave_column() / 2 : FLIP ? wave_row() : wave_column();
@@ -516,7 +557,7 @@ __device__ __forceinline__ void run(Tile& tile, const Product& p, uint32_t row, 
     tile.most_products(g, a0, b0);
     tile.last_products(g);
   }
-  tile.join();
+  tile.join(a0, a1, b0, b1);
 }
 
 // What a workgroup of these kernels has of shared memory: two halves of both
@@ -566,7 +607,8 @@ __device__ __forceinline__ Nothing nothing(uint32_t, uint32_t) { return {}; }
 // and have its latencies to themselves where there are few.  Measured, n tiles a
 // unit: 4.0 n a step, 1.15 n + 0.8 for 128 x 128 (2.0, 3.1, 4.0 and 13.5 for 1, 2, 3 and
 // 13), 0.5 n + 0.8 for 64 x 64 (1.4, 1.5, 3.4 and 4.6 for 2, 3, 5 and 10); floats,
-// which the matrix cores take 16 times as long for, 3.1 n + 2 and n + 2.5.  Of a
+// which the matrix cores take 16 times as long for, 3.1 n + 2 and n + 1 (with n + 2.5,
+// that larger tiles are then taken more often, 4096 x 1024 x 1024 782 us instead of 671).  Of a
 // mixture the sum counts, and half of the longest tile, which ends last.  Six steps
 // are added for a tile's first loads and its results.
 class Cost {
@@ -595,7 +637,7 @@ class Cost {
     return size_ == 256 ? 4.0 : size_ == 128 ? 1.15 : 0.5;
   }
   double alone() const {
-    if (f32_) return size_ == 128 ? 2.0 : 2.5;
+    if (f32_) return size_ == 128 ? 2.0 : 1.0;
     return size_ == 256 ? 0.0 : 0.8;
   }
 

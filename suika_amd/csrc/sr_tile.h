@@ -6,7 +6,8 @@
 // Each operand is stored either with its k side by side (a row a line: ROW) or
 // with its rows side by side (a k a line: COL), so every product of a forward
 // and a backward pass works on the tensors as they are.  A tile is 256 x 256 with
-// 8 waves of 128 x 64, 128 x 128 with 4 of 64 x 64, or 64 x 64 with 2 of 32 x 64.
+// 8 waves of 128 x 64, 128 x 128 with 4 of 64 x 64, or 64 x 64 with 2 of 32 x 64
+// (of floats with two sets of these).
 //
 //   - A step takes 128 bytes of every row: 64 values of 16 bits or 32 floats.
 //     They go from memory straight into shared memory, 16 bytes a lane, into
@@ -20,7 +21,7 @@
 //   - What lies outside an operand is read as zero: such lanes ask for an
 //     address beyond the buffer resource.
 //
-// A 256 x 256 tile of 16 bits does 128 operations for a byte that it loads, and 85
+// A 256 x 256 tile of 16 bits does 128 operations for a byte that it loads, and 43
 // for one that its waves read of shared memory.  The matrix cores alone reach 1.88
 // PFLOP/s of bf16 here, with these reads 1.54, with the loads and barriers of whole
 // products 1.25 to 1.28 (f16 pairs, below, 1.34 to 1.38): a step has one barrier, at

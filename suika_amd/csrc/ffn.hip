@@ -182,16 +182,17 @@ __global__ __launch_bounds__(sr_tile::threads<T>(SIZE), SIZE == 64 ? 3 : 2) void
   });
 }
 
-// Plain products, up to three in a launch, or one with its steps split over
-// `splits` workgroups a tile, whose parts are joined in order afterwards.  The shape
+// Plain products, up to three in a launch.  The steps of all their tiles, or of those
+// behind the last whole round of the compute units, may be split over `splits`
+// workgroups a tile, whose parts are joined in order afterwards.  The shape
 // above: y 369 GFLOP in 334 to 350 us, dx 739 in 642 to 677, the matrices' gradients
-// 1108 in 1110 to 1290 (both operands' rows side by side).  Steps split, and joined: y and
+// 1108 in 1005 (both operands' rows side by side).  Steps split, and joined: y and
 // dx of 1021 tokens, 3584 columns and 4736 rows 60 and 98 us, of one workgroup a tile 74 and
 // 119; of 509, 768 and 2050 in floats 29 and 46, 47 and 120.
 struct Job {
   Product p;
   uint32_t rows, columns;     // of C
-  uint32_t tile_rows, tile_columns, first;     // its first item
+  uint32_t tile_rows, tile_columns, first;     // its first tile
   uint64_t out;               // dense
 };
 
@@ -200,65 +201,69 @@ constexpr int kMostJobs = 3;
 struct ProductArgs {
   Job job[kMostJobs];
   uint32_t items;
-  uint32_t splits, steps;     // of one workgroup, where splits > 1
-  uint64_t parts;             // splits x rows x columns floats
+  uint32_t whole;             // tiles that are not split
+  uint32_t splits, steps;     // of the others, and of one workgroup
+  uint64_t parts;             // splits tiles of floats for each of them
 };
+
+// The job of a tile, and the tile's place in its C.
+template <int SIZE>
+__device__ __forceinline__ const Job& job_of(const ProductArgs& t, uint32_t tile, uint32_t& row, uint32_t& column) {
+  int j = 0;
+#pragma unroll
+  for (int i = 1; i < kMostJobs; ++i) j = tile >= t.job[i].first ? i : j;
+  const Job& job = t.job[j];
+  sr_tile::banded(tile - job.first, job.tile_rows, job.tile_columns, row, column);
+  row *= SIZE;
+  column *= SIZE;
+  return job;
+}
 
 template <typename T, int SIZE, Side A, Side B>
 __global__ __launch_bounds__(sr_tile::threads<T>(SIZE), SIZE == 64 ? 3 : 2) void product_kernel(ProductArgs t) {
   typedef sr_tile::Tile<T, false, SIZE, A, B> Tile;
   SR_TILE_MEMORY(Tile);
-  uint32_t item = sr_tile::item_of(blockIdx.x, t.items, SIZE);
+  const uint32_t item = sr_tile::item_of(blockIdx.x, t.items, SIZE);
   if (item >= t.items) return;
-  int j = 0;
-#pragma unroll
-  for (int i = 1; i < kMostJobs; ++i) j = item >= t.job[i].first ? i : j;
-  const Job& job = t.job[j];
-  item -= job.first;
-  const uint32_t split = item % t.splits;
+  const bool split = item >= t.whole;
+  const uint32_t part = split ? item - t.whole : 0;
   uint32_t row, column;
-  sr_tile::banded(item / t.splits, job.tile_rows, job.tile_columns, row, column);
-  row *= SIZE;
-  column *= SIZE;
+  const Job& job = job_of<SIZE>(t, split ? t.whole + part / t.splits : item, row, column);
   const uint32_t steps = (job.p.k + Tile::kK - 1) / Tile::kK * (job.p.a2.data ? 2 : 1);
-  const uint32_t from = split * t.steps, to = t.splits == 1 ? steps : min(steps, from + t.steps);
+  const uint32_t from = split ? part % t.splits * t.steps : 0, to = split ? min(steps, from + t.steps) : steps;
   Tile tile;
   sr_tile::run(tile, job.p, row, column, from, to, (Shared)a0, (Shared)a1, (Shared)b0, (Shared)b1);
   __syncthreads();
   tile.template results<false, false>(SR_TILE_SLAB(Tile), sr_tile::nothing, [&](uint32_t r, uint32_t n, const float (&v)[8],
                                                                          sr_tile::Nothing) {
-    r += row;
-    n += column;
-    if (r >= job.rows || n >= job.columns) return;
-    const uint64_t at = uint64_t(r) * job.columns + n;
-    if (t.splits == 1) store_row(global<T>(job.out) + at, v, job.columns - n);
-    else store_row(global<float>(t.parts) + uint64_t(split) * job.rows * job.columns + at, v, job.columns - n);
+    const uint32_t i = row + r, j = column + n;
+    if (i >= job.rows || j >= job.columns) return;
+    if (split) store_row(global<float>(t.parts) + (uint64_t(part) * SIZE + r) * SIZE + n, v, 8);
+    else store_row(global<T>(job.out) + uint64_t(i) * job.columns + j, v, job.columns - j);
   });
 }
 
 constexpr int kPlainThreads = 256;
 
-// The sum of the parts, in order.
-template <typename T>
-__global__ __launch_bounds__(kPlainThreads) void join_kernel(const float* parts, uint32_t splits, uint64_t n, T* out) {
-  const uint64_t at = (uint64_t(blockIdx.x) * kPlainThreads + threadIdx.x) * 4;
-  if (at >= n) return;
-  const uint32_t have = n - at < 4 ? uint32_t(n - at) : 4;
-  float sum[4] = {0, 0, 0, 0};
-  for (uint32_t s = 0; s < splits; ++s) {
-    const float* p = parts + s * n + at;
-    if (have == 4) {
-      float x[4];
-      load<float, 4>(p, x);
+// The sums of the parts, in order: eight values a lane.
+template <typename T, int SIZE>
+__global__ __launch_bounds__(kPlainThreads) void join_kernel(ProductArgs t) {
+  constexpr uint32_t kBlocks = SIZE * SIZE / 8 / kPlainThreads;      // of a tile
+  const uint32_t tile = blockIdx.x / kBlocks, at = (blockIdx.x % kBlocks * kPlainThreads + threadIdx.x) * 8;
+  uint32_t row, column;
+  const Job& job = job_of<SIZE>(t, t.whole + tile, row, column);
+  row += at / SIZE;
+  column += at % SIZE;
+  if (row >= job.rows || column >= job.columns) return;
+  float sum[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+  const float* p = global<const float>(t.parts) + uint64_t(tile) * t.splits * (SIZE * SIZE) + at;
+  for (uint32_t s = 0; s < t.splits; ++s) {
+    float x[8];
+    load_row(p + s * (SIZE * SIZE), x, 8);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) sum[e] += x[e];
-    } else {
-      for (uint32_t e = 0; e < have; ++e) sum[e] += p[e];
-    }
+    for (int e = 0; e < 8; ++e) sum[e] += x[e];
   }
-  if (have == 4) store<T, 4>(out + at, sum);
-  else
-    for (uint32_t e = 0; e < have; ++e) out[at + e] = static_cast<T>(sum[e]);
+  store_row(global<T>(job.out) + uint64_t(row) * job.columns + column, sum, job.columns - column);
 }
 
 // A copy of rows that tiles can be loaded from: each starts at a multiple of 16
@@ -483,35 +488,50 @@ Operand operand(const Matrix& m, Side side) {
 // Steps of a product over k values.
 template <typename T> uint64_t steps_of(uint64_t k) { return ceil_div(k, 128 / sizeof(T)); }
 
-// How a product goes: its tiles' size, and the workgroups that a tile's steps are
-// dealt out to.
+// How products go: their tiles' size, how many of them are not split, and the
+// workgroups that the steps of each other one are dealt out to.
 struct Way {
   int size;
-  uint64_t splits;
+  uint64_t whole, splits;
   double time;
 };
 
 // The fastest way for `count` products of rows x columns over `steps` steps each;
 // with `most` splits at most, of four steps or more, whose parts are written, read
-// and added up by another launch.
+// and added up by another launch.  Of 256 x 256 tiles, of which a compute unit has one
+// at a time, also those alone that would keep few units busy for a round (8192 tokens,
+// 4096 columns and 5504 rows, the matrices' gradients have 4 x 256 + 32 tiles: a training
+// step takes 3000 us instead of 3110).
 template <typename T>
 Way way_of(const uint64_t (*sides)[2], int count, uint64_t steps, uint64_t most) {
   constexpr bool kF32 = sizeof(T) == 4;
   constexpr double kUnit = 0.4e-6, kLaunch = 10, kRate = 8e12;
-  Way best{128, 1, 1e30};
+  // splitting has to gain a twentieth by the model (1021 tokens, 3584 columns, 4736 rows:
+  // the matrices' gradients 3% by it and 25 us of 430 slower, y 6% and 60 us instead of 75)
+  constexpr double kGain = 0.95;
+  Way best{128, 0, 1, 1e30}, split = best;
   for (int size : {256, 128, 64}) {
     if (kF32 && size == 256) continue;
-    for (uint64_t splits = 1; splits <= std::max<uint64_t>(1, std::min(most, steps / 4)); ++splits) {
+    uint64_t tiles = 0;
+    for (int i = 0; i < count; ++i) tiles += ceil_div(sides[i][0], size) * ceil_div(sides[i][1], size);
+    auto time = [&](uint64_t n, uint64_t each) {
       sr_tile::Cost cost(size, kF32);
-      double join = 0;
-      for (int i = 0; i < count; ++i) {
-        cost.add(ceil_div(sides[i][0], size) * ceil_div(sides[i][1], size) * splits, ceil_div(steps, splits));
-        if (splits > 1) join += kLaunch + double(sides[i][0]) * double(sides[i][1]) * 8 * splits / (kRate * kUnit);
-      }
-      if (cost.time() + join < best.time) best = {size, splits, cost.time() + join};
+      cost.add(n, each);
+      return cost.time();
+    };
+    auto consider = [&](uint64_t whole, uint64_t splits) {
+      const double join = splits == 1 ? 0 : kLaunch + double(tiles - whole) * size * size * 8 * splits / (kRate * kUnit);
+      const double all = time(whole, steps) + time((tiles - whole) * splits, ceil_div(steps, splits)) + join;
+      Way& least = splits == 1 ? best : split;
+      if (all < least.time) least = {size, whole, splits, all};
+    };
+    consider(tiles, 1);
+    for (uint64_t splits = 2; splits <= std::min(most, steps / 4); ++splits) {
+      consider(0, splits);
+      if (size == 256 && tiles > 256 && tiles % 256) consider(tiles / 256 * 256, splits);
     }
   }
-  return best;
+  return split.time < kGain * best.time ? split : best;
 }
 
 template <typename T>
@@ -536,10 +556,9 @@ struct Wanted {
   void* out;
 };
 
-// One product, or several with the same sides of operands and as many steps.  Of one
-// with few tiles and a long sum (`split`) the steps may be dealt out.
+// Products with the same sides of operands and as many steps.
 template <typename T, Side A, Side B>
-int products(const char* who, const Wanted* w, int count, bool split, Space& space, bool launch, hipStream_t stream) {
+int products(const char* who, const Wanted* w, int count, Space& space, bool launch, hipStream_t stream) {
   uint64_t sides[kMostJobs][2] = {};
   uint64_t steps = 0;
   for (int i = 0; i < count; ++i) {
@@ -547,10 +566,10 @@ int products(const char* who, const Wanted* w, int count, bool split, Space& spa
     sides[i][1] = w[i].columns;
     steps = steps_of<T>(w[i].p.k) * (w[i].p.a2.data ? 2 : 1);      // alike
   }
-  const Way way = way_of<T>(sides, count, steps, split && count == 1 ? kMostSplits : 1);
+  const Way way = way_of<T>(sides, count, steps, kMostSplits);
   const int size = way.size;
   ProductArgs t{};
-  uint64_t items = 0;
+  uint64_t tiles = 0;
   int n = 0;
   for (int i = 0; i < count; ++i) {
     if (w[i].rows == 0 || w[i].columns == 0) continue;
@@ -560,26 +579,26 @@ int products(const char* who, const Wanted* w, int count, bool split, Space& spa
     j.columns = uint32_t(w[i].columns);
     j.tile_rows = uint32_t(ceil_div(w[i].rows, size));
     j.tile_columns = uint32_t(ceil_div(w[i].columns, size));
-    j.first = uint32_t(items);
+    j.first = uint32_t(tiles);
     j.out = reinterpret_cast<uint64_t>(w[i].out);
-    items += uint64_t(j.tile_rows) * j.tile_columns;
-    if (items > sr_tile::kMostItems) return fail(SR_EBOUNDS, "%s: a product of %llu x %llu", who,
+    tiles += uint64_t(j.tile_rows) * j.tile_columns;
+    if (tiles > sr_tile::kMostItems) return fail(SR_EBOUNDS, "%s: a product of %llu x %llu", who,
                                                  (unsigned long long)w[i].rows, (unsigned long long)w[i].columns);
   }
   if (n == 0) return SR_OK;
   for (int i = n; i < kMostJobs; ++i) t.job[i].first = 0xffffffffu;
+  t.whole = uint32_t(way.splits == 1 ? tiles : way.whole);
   t.steps = uint32_t(ceil_div(steps, way.splits));
   t.splits = uint32_t(way.splits == 1 ? 1 : ceil_div(steps, t.steps));
-  const uint64_t elements = uint64_t(t.job[0].rows) * t.job[0].columns;
-  if (t.splits > 1) t.parts = space.take(t.splits * elements * sizeof(float));
+  const uint64_t parted = tiles - t.whole, items = t.whole + parted * t.splits;
+  if (items > sr_tile::kMostItems) return fail(SR_EBOUNDS, "%s: %llu parts", who, (unsigned long long)items);
+  t.parts = parted ? space.take(parted * t.splits * size * size * sizeof(float)) : 0;
   if (!launch) return SR_OK;
-  t.items = uint32_t(items) * t.splits;
+  t.items = uint32_t(items);
   with_size<T>(size, [&](auto z) {
     product_kernel<T, z(), A, B><<<sr_tile::blocks_of(t.items, z()), sr_tile::threads<T>(z()), 0, stream>>>(t);
+    if (parted) join_kernel<T, z()><<<uint32_t(parted * (z() * z() / 8 / kPlainThreads)), kPlainThreads, 0, stream>>>(t);
   });
-  if (t.splits > 1)
-    join_kernel<T><<<uint32_t(ceil_div(elements, 4 * kPlainThreads)), kPlainThreads, 0, stream>>>(
-        reinterpret_cast<const float*>(t.parts), t.splits, elements, reinterpret_cast<T*>(t.job[0].out));
   return launched(who);
 }
 
@@ -674,7 +693,7 @@ int forward(const sr_ffn_shape& s, void* out, void* a, void* b, Space& space, bo
   }
   const Matrix hm{reinterpret_cast<const void*>(h), s.tokens, s.ffn, wide};
   const Wanted w{{operand<T>(hm, ROW), operand<T>(down, ROW), {}, {}, uint32_t(s.ffn)}, s.tokens, s.hidden, out};
-  return products<T, ROW, ROW>("sr_ffn", &w, 1, true, space, launch, stream);
+  return products<T, ROW, ROW>("sr_ffn", &w, 1, space, launch, stream);
 }
 
 template <typename T>
@@ -718,7 +737,7 @@ int backward(const sr_ffn_shape& s, const void* a, const void* b, const void* dy
     const Wanted w{{operand<T>(rows_of(da), ROW), operand<T>(gate, COL), operand<T>(rows_of(db), ROW), operand<T>(up, COL),
                     uint32_t(s.ffn)},
                    s.tokens, s.hidden, g.x};
-    if (int rc = products<T, ROW, COL>(who, &w, 1, true, space, launch, stream)) return rc;
+    if (int rc = products<T, ROW, COL>(who, &w, 1, space, launch, stream)) return rc;
   }
   Wanted w[kMostJobs];
   int n = 0;
@@ -729,7 +748,7 @@ int backward(const sr_ffn_shape& s, const void* a, const void* b, const void* dy
   }
   if (g.down)
     w[n++] = {{operand<T>(dym, COL), operand<T>(rows_of(h), COL), {}, {}, uint32_t(s.tokens)}, s.hidden, s.ffn, g.down};
-  return products<T, COL, COL>(who, w, n, false, space, launch, stream);
+  return products<T, COL, COL>(who, w, n, space, launch, stream);
 }
 
 

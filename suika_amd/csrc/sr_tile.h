@@ -608,9 +608,9 @@ __device__ __forceinline__ Nothing nothing(uint32_t, uint32_t) { return {}; }
 // and have its latencies to themselves where there are few.  Measured, n tiles a
 // unit: 4.0 n a step, 1.15 n + 0.8 for 128 x 128 (2.0, 3.1, 4.0 and 13.5 for 1, 2, 3 and
 // 13), 0.5 n + 0.8 for 64 x 64 (1.4, 1.5, 3.4 and 4.6 for 2, 3, 5 and 10); floats,
-// which the matrix cores take 16 times as long for, 3.1 n + 2 and n + 1 (with n + 2.5,
-// that larger tiles are then taken more often, 4096 x 1024 x 1024 782 us instead of 671).  Of a
-// mixture the sum counts, and half of the longest tile, which ends last.  Six steps
+// which the matrix cores take 16 times as long for, 3.7 n + 1.4 and n + 1 (with 3.1 n + 2
+// and n + 2.5, that take larger tiles more often, 4096 x 1024 x 1024 782 us instead of
+// 675).  Of a mixture the sum counts, and half of the longest tile, which ends last.  Six steps
 // are added for a tile's first loads and its results.
 class Cost {
  public:
@@ -634,11 +634,11 @@ class Cost {
   static constexpr uint64_t kUnits = 256;      // compute units
 
   double shared() const {
-    if (f32_) return size_ == 128 ? 3.1 : 1.0;
+    if (f32_) return size_ == 128 ? 3.7 : 1.0;
     return size_ == 256 ? 4.0 : size_ == 128 ? 1.15 : 0.5;
   }
   double alone() const {
-    if (f32_) return size_ == 128 ? 2.0 : 1.0;
+    if (f32_) return size_ == 128 ? 1.4 : 1.0;
     return size_ == 256 ? 0.0 : 0.8;
   }
 

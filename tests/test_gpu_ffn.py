@@ -340,3 +340,10 @@ def test_slope_of_far_gelu_tanh_gates():
         r = gated_ffn(x, gate, up, down, activation="gelu_tanh", keep=True)
         grads = gated_ffn_grad(x, gate, up, down, r.gate, r.up, torch.ones(1, 1, device=DEV), activation="gelu_tanh")
         assert float(grads[1]) == (far > 0)
+
+
+@pytest.mark.parametrize("size, dtype", [((4096, 2560, 2300), BF16), ((4100, 2555, 2305), F16), ((2000, 40, 72), BF16),
+                                         ((3001, 33, 65), F32)], ids=str)
+def test_long_sums_of_several_products(size, dtype):
+    """The matrices' gradients over many tokens: the tiles behind whole rounds of 256, or all of few, in parts."""
+    check(*size, dtype)

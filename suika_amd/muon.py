@@ -59,7 +59,8 @@ def orthogonalize(matrices: Sequence[Tensor], *, steps: int = 5,
     to ``out``, which may be the matrices themselves.  Products are formed of 22
     bits a value in sums of 32 bits, and the result is rounded once.  A matrix of
     zeros stays zeros, one with NaN or infinity becomes NaN, and the others of
-    the list are not touched by it.
+    the list are not touched by it.  Where ``eps`` is far above a matrix's norm,
+    what is below 2^-38 after the division by it is lost.
 
     Not differentiable: a matrix that wants a gradient is refused, as is a
     forward-mode tangent.

@@ -20,7 +20,7 @@ of include/suika_step.h.  Refused arguments raise ``PlanError``.
 from __future__ import annotations
 
 import math
-from typing import Callable, Dict, List, Mapping, Optional, Sequence, Tuple, Union
+from typing import Callable, Dict, Iterable, List, Mapping, Optional, Sequence, Tuple, Union
 
 import torch
 from torch import Tensor
@@ -42,7 +42,16 @@ def _schedule(steps: int, coefficients: Union[Triple, Sequence[Triple]]) -> List
     return [float(x) for r in rows for x in r]
 
 
-def orthogonalize(matrices: Sequence[Tensor], *, steps: int = 5,
+def _tensors(given: Iterable[Tensor], what: str) -> List[Tensor]:
+    """What may be an iterator, which can be gone through once."""
+    try:
+        each = iter(given)
+    except TypeError:
+        raise PlanError(f"{what}: a sequence of tensors is wanted") from None
+    return list(each)
+
+
+def orthogonalize(matrices: Iterable[Tensor], *, steps: int = 5,
                   coefficients: Union[Triple, Sequence[Triple]] = COEFFICIENTS, eps: float = 1e-7,
                   out: Optional[Sequence[Tensor]] = None, split: Optional[Sequence[Optional[int]]] = None,
                   all_reduce: Optional[Callable[[Tensor], object]] = None) -> List[Tensor]:
@@ -71,6 +80,7 @@ def orthogonalize(matrices: Sequence[Tensor], *, steps: int = 5,
     tensors on the device and sums them over the ranks in place, in the current
     stream's order (``torch.distributed.all_reduce``, for example).
     """
+    matrices = _tensors(matrices, "matrices")
     if torch.is_grad_enabled() and any(isinstance(m, Tensor) and m.requires_grad for m in matrices):
         raise PlanError("matrices: one wants a gradient, which orthogonalize does not have")
     return _lib.host().orthogonalize(matrices, out, split, steps, _schedule(steps, coefficients), float(eps), all_reduce)

@@ -467,3 +467,13 @@ def test_refused_steps_change_nothing():
     assert all(torch.equal(t, before[n][f]) for n, e in list(state.items())[1:] for f, t in e.items())
     with pytest.raises(PlanError, match="a matrix"):
         ShardMuon({"b": {"param": torch.zeros(3, device=DEV), "exp_avg": torch.zeros(3, device=DEV)}})
+
+
+def test_matrices_from_an_iterator():
+    gs = [draw((20, 30)), draw((70, 90))]
+    want = orthogonalize(gs)
+    for mode in (torch.enable_grad, torch.no_grad):
+        with mode():
+            for given in (iter(gs), (g for g in gs), torch.stack([gs[0], gs[0]])):
+                got = orthogonalize(given)
+                assert len(got) == 2 and torch.equal(got[0], want[0])

@@ -193,3 +193,17 @@ def test_split_matrices():
     assert split_matrices(layout, 1) == {"wte.weight": (0, 100), "qkv.weight": (0, 32), "down.weight": (1, 64)}
     one = ParamLayout.from_metas({0: {"a": TensorMeta(name="a", dtype=bf16, shape=(4, 4))}})
     assert split_matrices(one, 0) == {}
+
+
+def test_matrices_from_an_iterator():
+    """What can be gone through once reaches the host whole, in either mode."""
+    for mode in (torch.enable_grad, torch.no_grad):
+        with mode():
+            with pytest.raises(PlanError, match=r"matrices\[0\] is on cpu"):
+                orthogonalize(iter([torch.zeros(3, 3)]))
+            with pytest.raises(PlanError, match="a sequence of tensors"):
+                orthogonalize(None)
+            with pytest.raises(PlanError, match="not a tensor"):
+                orthogonalize(x for x in (1, 2))
+    with pytest.raises(PlanError, match="wants a gradient"):
+        orthogonalize(iter([torch.zeros(3, 3), torch.zeros(3, 3, requires_grad=True)]))

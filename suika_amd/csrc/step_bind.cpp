@@ -727,6 +727,7 @@ py::list orthogonalize(py::object matrices, py::object outs, py::object splits, 
     if (fresh) continue;
     const std::string out_name = indexed("out", i);
     const at::Tensor& o = tensor_of(out_list[i], out_name);
+    check_tangent(o, out_name.c_str());
     dst.push_back(matrix_of(o, out_name, -1, device));
     if (o.sizes() != t.sizes()) plan_error(out_name + ": shape differs from the matrix's");
     to.push_back(o);

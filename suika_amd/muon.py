@@ -53,7 +53,7 @@ def _tensors(given: Iterable[Tensor], what: str) -> List[Tensor]:
 
 def orthogonalize(matrices: Iterable[Tensor], *, steps: int = 5,
                   coefficients: Union[Triple, Sequence[Triple]] = COEFFICIENTS, eps: float = 1e-7,
-                  out: Optional[Sequence[Tensor]] = None, split: Optional[Sequence[Optional[int]]] = None,
+                  out: Optional[Iterable[Tensor]] = None, split: Optional[Sequence[Optional[int]]] = None,
                   all_reduce: Optional[Callable[[Tensor], object]] = None) -> List[Tensor]:
     """Each matrix G of a list with its singular values moved towards 1.
 
@@ -71,8 +71,8 @@ def orthogonalize(matrices: Iterable[Tensor], *, steps: int = 5,
     the list are not touched by it.  Where ``eps`` is far above a matrix's norm,
     what is below 2^-38 after the division by it is lost.
 
-    Not differentiable: a matrix that wants a gradient is refused, as is a
-    forward-mode tangent.
+    Not differentiable: a matrix or an ``out`` that wants a gradient is refused,
+    as is a forward-mode tangent of either.
 
     ``split`` gives for each matrix ``None``, or the dimension along which ranks
     hold parts of it: 0 where the rows are dealt out, 1 the columns.  All ranks
@@ -80,9 +80,11 @@ def orthogonalize(matrices: Iterable[Tensor], *, steps: int = 5,
     tensors on the device and sums them over the ranks in place, in the current
     stream's order (``torch.distributed.all_reduce``, for example).
     """
-    matrices = _tensors(matrices, "matrices")
-    if torch.is_grad_enabled() and any(isinstance(m, Tensor) and m.requires_grad for m in matrices):
-        raise PlanError("matrices: one wants a gradient, which orthogonalize does not have")
+    matrices, out = _tensors(matrices, "matrices"), None if out is None else _tensors(out, "out")
+    if torch.is_grad_enabled():
+        for what, given in (("matrices", matrices), ("out", out or [])):
+            if any(isinstance(m, Tensor) and m.requires_grad for m in given):
+                raise PlanError(f"{what}: one wants a gradient, which orthogonalize does not have")
     return _lib.host().orthogonalize(matrices, out, split, steps, _schedule(steps, coefficients), float(eps), all_reduce)
 
 

@@ -477,3 +477,18 @@ def test_matrices_from_an_iterator():
             for given in (iter(gs), (g for g in gs), torch.stack([gs[0], gs[0]])):
                 got = orthogonalize(given)
                 assert len(got) == 2 and torch.equal(got[0], want[0])
+
+
+def test_outputs_that_want_a_gradient():
+    import torch.autograd.forward_ad as fwd
+    g, out = draw((8, 8)), draw((8, 8), seed=1).requires_grad_()
+    before = out.detach().clone()
+    with pytest.raises(PlanError, match="out: one wants a gradient"):
+        orthogonalize([g], out=[out])
+    with fwd.dual_level():
+        with pytest.raises(PlanError, match="forward-mode"):
+            orthogonalize([g], out=[fwd.make_dual(before.clone(), g)])
+    assert torch.equal(out, before)
+    with torch.no_grad():
+        orthogonalize([g], out=iter([out]))
+    assert torch.equal(out.detach(), orthogonalize([g])[0])

@@ -207,3 +207,14 @@ def test_matrices_from_an_iterator():
                 orthogonalize(x for x in (1, 2))
     with pytest.raises(PlanError, match="wants a gradient"):
         orthogonalize(iter([torch.zeros(3, 3), torch.zeros(3, 3, requires_grad=True)]))
+
+
+def test_outputs_that_want_a_gradient():
+    g, out = torch.zeros(3, 3), torch.zeros(3, 3, requires_grad=True)
+    for given in ([out], (out,), iter([out]), [out * 2]):
+        with pytest.raises(PlanError, match="out: one wants a gradient"):
+            orthogonalize([g], out=given)
+    with torch.no_grad(), pytest.raises(PlanError, match="not on the GPU"):
+        orthogonalize([g], out=[out])
+    with pytest.raises(PlanError, match="out: a sequence of tensors"):
+        orthogonalize([g], out=1)

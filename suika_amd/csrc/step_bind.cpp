@@ -814,6 +814,9 @@ class MuonState {
     if (!max_norm.is_none()) {
       o.max_norm = max_norm.cast<double>();
       given = given_sum(square_sum, device);
+      // each rank would clip its part of a matrix by a factor of its own
+      for (const sr_muon_tensor& t : tensors)
+        if (t.split >= 0 && !given) plan_error("max_norm: matrices that are split want the square_sum of all ranks");
       norm = at::empty({}, on(device, at::kFloat));
       if (!given) work.emplace(arrays, device);
       o.square_sum = given ? given : work->sum();

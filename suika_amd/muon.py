@@ -162,7 +162,8 @@ class ShardMuon:
 
         With ``max_norm`` the gradients count as clipped to it (``clip_grads``;
         they are not written) and their norm is returned, a 0-dim float32
-        tensor; ``square_sum`` is as for ``clip_grads``.  An ``all_reduce`` that
+        tensor; ``square_sum`` is as for ``clip_grads``, and wanted where a matrix
+        of ``splits`` is stepped: its parts are clipped alike.  An ``all_reduce`` that
         raises ends the step: momentum is updated then, and some weights.
         """
         if not isinstance(grads, (list, tuple)) and isinstance(grads, Mapping):

@@ -492,3 +492,20 @@ def test_outputs_that_want_a_gradient():
     with torch.no_grad():
         orthogonalize([g], out=iter([out]))
     assert torch.equal(out.detach(), orthogonalize([g])[0])
+
+
+def test_a_local_norm_does_not_clip_parts():
+    """Ranks would clip the parts of one matrix by factors of their own, whose Gram matrices do not add up to its own."""
+    shapes = {"cut": (16, 24), "whole": (70, 90)}
+    state = dict(zip(shapes, share("f32", list(shapes.values())).values()))
+    before = {n: {f: t.clone() for f, t in e.items()} for n, e in state.items()}
+    grads = {n: draw(s, seed=i) for i, (n, s) in enumerate(shapes.items())}
+    optimizer = ShardMuon(state, lr=LR, momentum=MU, splits={"cut": (0, 32)}, all_reduce=lambda t: None)
+    with pytest.raises(PlanError, match="square_sum"):
+        optimizer.step(grads, max_norm=1.0)
+    assert all(torch.equal(t, before[n][f]) for n, e in state.items() for f, t in e.items())
+    # of whole matrices alone it is theirs, and a sum over the ranks serves all
+    assert torch.equal(optimizer.step({"whole": grads["whole"]}, max_norm=1.0), grad_norm([grads["whole"]]))
+    q = grad_square_sum(list(grads.values()))
+    assert torch.equal(optimizer.step(grads, max_norm=1.0, square_sum=q), grad_norm(list(grads.values())))
+

@@ -360,9 +360,11 @@ typedef struct sr_muon_options {
  * momentum exp_avg + (1 - momentum) g with nesterov, else exp_avg, as it is
  * stored; weight = weight (1 - lr weight_decay) - lr scale X with the last X of
  * G.  Fields that are written overlap no others (SR_EOVERLAP).  It holds no
- * step number and can be captured where reduce can.  A reduce that fails leaves
- * the moments updated and the weights of its matrices as they were.  workspace:
- * sr_muon_workspace bytes; that call makes all of sr_muon's checks.
+ * step number and can be captured where reduce can.  Where a reduce fails, all
+ * moments are updated, and of the weights those of matrices that are not split
+ * and of groups of split ones that came before (at most 48 matrices go through
+ * the steps together), each as a whole.  workspace: sr_muon_workspace bytes; that
+ * call makes all of sr_muon's checks.
  */
 int sr_muon_workspace(const sr_muon_tensor* tensors, int32_t count, const sr_muon_options* options, const sr_newton_schulz* ns,
                       uint64_t* bytes);

@@ -765,15 +765,41 @@ int reduce(const Steps& s, uint64_t data, uint64_t count, int32_t dtype, hipStre
   return rc == 0 ? int(SR_OK) : fail(SR_EINVAL, "%s: the sum over the ranks failed (%d)", s.who, rc);
 }
 
-// One group; launch false: only the workspace is counted.
-int run_group(const Group& g, const Steps& s, Space& space, bool launch, hipStream_t stream) {
+// A group's matrices as they are given, in sheets; their X come later.
+int sources_of(const Group& g, Table<SourceEntry>& source) {
+  source.count = uint32_t(g.work.size());
+  uint64_t sheets = 0;
+  for (size_t i = 0; i < g.work.size(); ++i) {
+    const Work& w = *g.work[i];
+    source.entry[i] = {reinterpret_cast<uint64_t>(w.source), reinterpret_cast<uint64_t>(w.momentum), w.source_stride, 0,
+                       uint32_t(w.rows), uint32_t(w.columns), 0, uint32_t(i), w.source_type, w.momentum_type, w.flip(),
+                       uint32_t(sheets)};
+    sheets += uint64_t(tiles(uint32_t(w.rows), kSheet)) * tiles(uint32_t(w.columns), kSheet);
+  }
+  return number(source, (uint64_t(1) << 24) - 1,
+                [](const SourceEntry& e) { return uint64_t(tiles(e.rows, kSheet)) * tiles(e.columns, kSheet); });
+}
+
+// The momentum's update and the squares' sums of a group.
+int run_sums(const Group& g, const Steps& s, uint64_t sums, Space& space, bool launch, hipStream_t stream) {
   Table<SourceEntry> source{};
+  if (int rc = sources_of(g, source)) return rc;
+  double* const parts = reinterpret_cast<double*>(space.take(source.items * sizeof(double)));
+  if (!launch) return SR_OK;
+  if (source.items) sums_kernel<<<source.items, kSheetThreads, 0, stream>>>(source, s.mix, parts);
+  join_sums_kernel<<<source.count, kSheetThreads, 0, stream>>>(source, parts, reinterpret_cast<double*>(sums));
+  return launched(s.who);
+}
+
+// The steps of a group.
+int run_steps(const Group& g, const Steps& s, uint64_t sums, Space& space, bool launch, hipStream_t stream) {
+  Table<SourceEntry> source{};
+  if (int rc = sources_of(g, source)) return rc;
   Table<Entry> t{};
   Table<LastEntry> last{};
-  source.count = t.count = last.count = uint32_t(g.work.size());
-  uint64_t sheets = 0, gram_floats = 0;
+  t.count = last.count = uint32_t(g.work.size());
+  uint64_t gram_floats = 0;
   for (size_t i = 0; i < g.work.size(); ++i) gram_floats += uint64_t(g.work[i]->m()) * g.work[i]->m();
-  const uint64_t sums = space.take(kEntries * sizeof(double));
   const uint64_t grams = g.split ? space.take(gram_floats * sizeof(float)) : 0;
   gram_floats = 0;
   for (size_t i = 0; i < g.work.size(); ++i) {
@@ -790,16 +816,10 @@ int run_group(const Group& g, const Steps& s, Space& space, bool launch, hipStre
       e.gram = grams + gram_floats * sizeof(float);
       gram_floats += uint64_t(e.m) * e.m;
     }
-    source.entry[i] = {reinterpret_cast<uint64_t>(w.source), reinterpret_cast<uint64_t>(w.momentum), w.source_stride, e.x,
-                       uint32_t(w.rows), uint32_t(w.columns), 0, uint32_t(i), w.source_type, w.momentum_type, w.flip(),
-                       uint32_t(sheets)};
-    sheets += uint64_t(tiles(uint32_t(w.rows), kSheet)) * tiles(uint32_t(w.columns), kSheet);
+    source.entry[i].x = e.x;
     last.entry[i] = {0, e.b, reinterpret_cast<uint64_t>(w.to), reinterpret_cast<uint64_t>(w.param), w.to_stride, e.m, e.n, 0,
                      w.to_type, w.flip(), w.weight, w.decay, w.step};
   }
-  const uint64_t parts = space.take(sheets * sizeof(double));
-  auto sheets_of = [](const SourceEntry& e) { return uint64_t(tiles(e.rows, kSheet)) * tiles(e.columns, kSheet); };
-  if (int rc = number(source, (uint64_t(1) << 24) - 1, sheets_of)) return rc;
   int large = 0, wide = 0;
   Table<Entry> gram = t, update = t;
   // A and A A have the same tiles; the steps are counted of both
@@ -811,11 +831,7 @@ int run_group(const Group& g, const Steps& s, Space& space, bool launch, hipStre
   if (int rc = number(halves, (uint64_t(1) << 24) - 1, [](const Entry& e) { return uint64_t(tiles(e.m, kSheet)) * tiles(e.m, kSheet); })) return rc;
   if (!launch) return SR_OK;
 
-  double* const part = reinterpret_cast<double*>(parts);
   double* const sum = reinterpret_cast<double*>(sums);
-  if (source.items) sums_kernel<<<source.items, kSheetThreads, 0, stream>>>(source, s.mix, part);
-  join_sums_kernel<<<source.count, kSheetThreads, 0, stream>>>(source, part, sum);
-  if (int rc = launched(s.who)) return rc;
   if (g.split) {
     if (int rc = reduce(s, sums, source.count, SR_DT_F64, stream)) return rc;
   }
@@ -883,14 +899,22 @@ int run_small(const std::vector<Work>& all, const Steps& s, hipStream_t stream) 
   return flush();
 }
 
-// All groups, one after another in the same memory.
+// All groups, one after another in the same memory.  All momentum is updated before
+// the ranks' first sum, so that what a failing one leaves does not depend on the groups.
 int run_all(const std::vector<Work>& all, const Steps& s, Space& space, bool launch, hipStream_t stream) {
   if (launch) {
     if (int rc = run_small(all, s, stream)) return rc;
   }
-  for (const Group& g : groups_of(all)) {
-    space.used = 0;
-    if (int rc = run_group(g, s, space, launch, stream)) return rc;
+  const std::vector<Group> groups = groups_of(all);
+  constexpr uint64_t kSums = kEntries * sizeof(double);      // of a group
+  const uint64_t sums = space.take(groups.size() * kSums), shared = space.used;
+  for (size_t i = 0; i < groups.size(); ++i) {
+    space.used = shared;
+    if (int rc = run_sums(groups[i], s, sums + i * kSums, space, launch, stream)) return rc;
+  }
+  for (size_t i = 0; i < groups.size(); ++i) {
+    space.used = shared;
+    if (int rc = run_steps(groups[i], s, sums + i * kSums, space, launch, stream)) return rc;
   }
   return SR_OK;
 }

@@ -164,7 +164,8 @@ class ShardMuon:
         they are not written) and their norm is returned, a 0-dim float32
         tensor; ``square_sum`` is as for ``clip_grads``, and wanted where a matrix
         of ``splits`` is stepped: its parts are clipped alike.  An ``all_reduce`` that
-        raises ends the step: momentum is updated then, and some weights.
+        raises ends the step: all momentum is updated then, and the weights of
+        matrices outside ``splits``; of the others' some, each as a whole.
         """
         if not isinstance(grads, (list, tuple)) and isinstance(grads, Mapping):
             unknown = grads.keys() - self._state.keys()

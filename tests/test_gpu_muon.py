@@ -509,3 +509,33 @@ def test_a_local_norm_does_not_clip_parts():
     q = grad_square_sum(list(grads.values()))
     assert torch.equal(optimizer.step(grads, max_norm=1.0, square_sum=q), grad_norm(list(grads.values())))
 
+
+@pytest.mark.parametrize("fails_at", [0, 1, 5, 6, 9])
+def test_failing_reduce_of_a_step(fails_at):
+    """More cut matrices than go through the steps together (48, with a call for their norms and one each step), whole
+    and small ones: all moments are updated, the weights of uncut matrices too, and of cut ones all or none of a weight."""
+    shapes = [(8, 12)] * 50 + [(70, 90), (20, 16)]
+    state = share("mixed", shapes)
+    names = list(state)
+    grads = [draw(s, seed=300 + i, dtype=BF16) for i, s in enumerate(shapes)]
+    other = {n: {f: t.clone() for f, t in e.items()} for n, e in state.items()}
+    before = {n: e["master"].clone() for n, e in state.items()}
+    splits = {n: (0, 8) for n in names[:50]}
+    calls = []
+
+    def fails(t):
+        calls.append(t)
+        if len(calls) == fails_at + 1:
+            raise ZeroDivisionError("the network is down")
+
+    ShardMuon(other, lr=LR, momentum=MU, splits=splits, all_reduce=lambda t: None).step(grads)
+    with pytest.raises(ZeroDivisionError, match="the network is down"):
+        ShardMuon(state, lr=LR, momentum=MU, splits=splits, all_reduce=fails).step(grads)
+    assert len(calls) == fails_at + 1
+    stepped = {n for n in names if not torch.equal(state[n]["master"], before[n])}
+    assert stepped == set(names[50:]) | (set(names[:48]) if fails_at > 5 else set())
+    for n, e in state.items():
+        assert torch.equal(e["exp_avg"], other[n]["exp_avg"]), n
+        if n in stepped:
+            assert torch.equal(e["master"], other[n]["master"]) and torch.equal(e["param"], other[n]["param"]), n
+

@@ -77,17 +77,79 @@ __device__ __forceinline__ Act act(float a, int32_t kind) {
 
 // ------------------------------------------------------------------ products
 
+// Which tiles of a launch have their steps dealt out to several workgroups: those from
+// `whole` on, to `splits` of them with `steps` steps each.  A workgroup then leaves the
+// sums of its steps as floats, a tile a part, and a launch behind it joins the parts of a
+// tile in order.
+struct Cut {
+  uint32_t whole;
+  uint32_t splits, steps;
+  uint64_t parts;
+};
+
+// A workgroup's tile, and its steps of all.
+struct Turn {
+  uint32_t tile, from, to;
+  uint32_t part;              // where its sums go, if `split`
+  bool split;
+};
+
+__device__ __forceinline__ Turn turn_of(const Cut& c, uint32_t item) {
+  const bool split = item >= c.whole;
+  if (!split) return {item, 0, 0xffffffffu, 0, false};
+  const uint32_t part = item - c.whole, from = part % c.splits * c.steps;
+  return {c.whole + part / c.splits, from, from + c.steps, part, true};
+}
+
+// Eight sums of a part: of row r, from column n on.
+template <int SIZE>
+__device__ __forceinline__ void store_part(const Cut& c, uint32_t part, uint32_t r, uint32_t n, const float (&v)[8]) {
+  store_row(global<float>(c.parts) + (uint64_t(part) * SIZE + r) * SIZE + n, v, 8);
+}
+
+// The joined sums of the tile that is the `tile`th of the split ones.
+template <int SIZE>
+__device__ __forceinline__ void join_parts(const Cut& c, uint32_t tile, uint32_t r, uint32_t n, float (&sum)[8]) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) sum[e] = 0;
+  const float* p = global<const float>(c.parts) + (uint64_t(tile) * c.splits * SIZE + r) * SIZE + n;
+  for (uint32_t s = 0; s < c.splits; ++s) {
+    float x[8];
+    load_row(p + s * (SIZE * SIZE), x, 8);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sum[e] += x[e];
+  }
+}
+
+constexpr int kPlainThreads = 256;
+
 // Both projections.  Bound by the matrix cores, and by the results' bytes where a and
 // b are kept: 8192 tokens, 4096 columns, 5504 rows of both (bf16, 739 GFLOP) 776 to
-// 850 us with 0.45 GB written.
+// 850 us with 0.45 GB written.  Few tiles with long sums are split (kActivatedGain).
 struct ForwardArgs {
   Product p;
   Grid grid;
+  Cut cut;
   uint64_t h, a, b;           // a and b: kept for the gradients, or 0
   uint64_t h_stride;          // elements
   uint32_t tokens, ffn, padded;     // columns of h: those behind ffn are zeros
   int32_t activation;
 };
+
+template <typename T>
+__device__ __forceinline__ void store_forward(const ForwardArgs& t, uint32_t r, uint32_t n, const float (&a)[8],
+                                              const float (&b)[8]) {
+  if (r >= t.tokens || n >= t.padded) return;
+  float h[8];
+  // (the columns behind ffn are zeros also where a row of x has an infinity)
+#pragma unroll
+  for (int e = 0; e < 8; ++e) h[e] = n + e < t.ffn ? act<false>(a[e], t.activation).value * b[e] : 0.0f;
+  store_row(global<T>(t.h) + r * t.h_stride + n, h, t.padded - n);
+  if (t.a && n < t.ffn) {
+    store_row(global<float>(t.a) + uint64_t(r) * t.ffn + n, a, t.ffn - n);
+    store_row(global<float>(t.b) + uint64_t(r) * t.ffn + n, b, t.ffn - n);
+  }
+}
 
 template <typename T, int SIZE>
 __global__ __launch_bounds__(sr_tile::threads<T>(SIZE), SIZE == 64 ? 3 : 2) void forward_kernel(ForwardArgs t) {
@@ -95,29 +157,42 @@ __global__ __launch_bounds__(sr_tile::threads<T>(SIZE), SIZE == 64 ? 3 : 2) void
   SR_TILE_MEMORY(Tile);
   const uint32_t item = sr_tile::item_of(blockIdx.x, t.grid.items, SIZE);
   if (item >= t.grid.items) return;
+  const Turn turn = turn_of(t.cut, item);
   uint32_t row, column;
-  sr_tile::banded(item, t.grid.rows, t.grid.columns, row, column);
+  sr_tile::banded(turn.tile, t.grid.rows, t.grid.columns, row, column);
   row *= SIZE;
   column *= Tile::kColumns;
   Tile tile;
-  sr_tile::run(tile, t.p, row, column, 0, (t.p.k + Tile::kK - 1) / Tile::kK, (Shared)a0, (Shared)a1, (Shared)b0,
-               (Shared)b1);
+  sr_tile::run(tile, t.p, row, column, turn.from, min(turn.to, (t.p.k + Tile::kK - 1) / Tile::kK), (Shared)a0, (Shared)a1,
+               (Shared)b0, (Shared)b1);
   __syncthreads();
   tile.template results<false, false>(SR_TILE_SLAB(Tile), sr_tile::nothing, [&](uint32_t r, uint32_t n, const float (&a)[8],
                                                                          const float (&b)[8], sr_tile::Nothing) {
-    r += row;
-    n += column;
-    if (r >= t.tokens || n >= t.padded) return;
-    float h[8];
-    // (the columns behind ffn are zeros also where a row of x has an infinity)
-#pragma unroll
-    for (int e = 0; e < 8; ++e) h[e] = n + e < t.ffn ? act<false>(a[e], t.activation).value * b[e] : 0.0f;
-    store_row(global<T>(t.h) + r * t.h_stride + n, h, t.padded - n);
-    if (t.a && n < t.ffn) {
-      store_row(global<float>(t.a) + uint64_t(r) * t.ffn + n, a, t.ffn - n);
-      store_row(global<float>(t.b) + uint64_t(r) * t.ffn + n, b, t.ffn - n);
+    if (turn.split) {
+      if (row + r >= t.tokens) return;
+      store_part<SIZE>(t.cut, turn.part, r, n, a);
+      store_part<SIZE>(t.cut, turn.part, r, Tile::kColumns + n, b);
+    } else {
+      store_forward<T>(t, row + r, column + n, a, b);
     }
   });
+}
+
+// Both projections' sums joined: eight columns a lane.
+template <typename T, int SIZE>
+__global__ __launch_bounds__(kPlainThreads) void forward_join_kernel(ForwardArgs t) {
+  constexpr uint32_t kColumns = SIZE / 2, kBlocks = SIZE * kColumns / 8 / kPlainThreads;      // of a tile
+  const uint32_t tile = blockIdx.x / kBlocks, at = (blockIdx.x % kBlocks * kPlainThreads + threadIdx.x) * 8;
+  const uint32_t r = at / kColumns, n = at % kColumns;
+  uint32_t row, column;
+  sr_tile::banded(t.cut.whole + tile, t.grid.rows, t.grid.columns, row, column);
+  row = row * SIZE + r;
+  column = column * kColumns + n;
+  if (row >= t.tokens || column >= t.padded) return;
+  float a[8], b[8];
+  join_parts<SIZE>(t.cut, tile, r, n, a);
+  join_parts<SIZE>(t.cut, tile, r, kColumns + n, b);
+  store_forward<T>(t, row, column, a, b);
 }
 
 // dh = dy D, and from it da, db and h again: the same h as forward's, which is
@@ -126,6 +201,7 @@ __global__ __launch_bounds__(sr_tile::threads<T>(SIZE), SIZE == 64 ? 3 : 2) void
 struct BackwardArgs {
   Product p;
   Grid grid;
+  Cut cut;
   uint64_t a, b;              // kept
   uint64_t da, db, h;         // 0: not wanted
   uint64_t stride;            // of da, db and h
@@ -137,54 +213,81 @@ struct Kept {
   float a[8], b[8];
 };
 
+__device__ __forceinline__ Kept load_kept(const BackwardArgs& t, uint32_t r, uint32_t n) {
+  Kept k{};
+  if (r >= t.tokens || n >= t.ffn) return k;
+  load_row(global<const float>(t.a) + uint64_t(r) * t.ffn + n, k.a, t.ffn - n);
+  load_row(global<const float>(t.b) + uint64_t(r) * t.ffn + n, k.b, t.ffn - n);
+  return k;
+}
+
+template <typename T>
+__device__ __forceinline__ void store_backward(const BackwardArgs& t, uint32_t r, uint32_t n, const float (&dh)[8],
+                                               const Kept& k) {
+  if (r >= t.tokens || n >= t.padded) return;
+  float da[8], db[8], h[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const Act f = act<true>(k.a[e], t.activation);
+    const float d = n + e < t.ffn ? dh[e] : 0.0f;      // (0 also where a row of dy has an infinity)
+    h[e] = f.value * k.b[e];
+    db[e] = d * f.value;
+    da[e] = d * k.b[e] * f.slope;
+  }
+  const uint64_t at = r * t.stride + n;
+  if (t.da) {
+    store_row(global<T>(t.da) + at, da, t.padded - n);
+    store_row(global<T>(t.db) + at, db, t.padded - n);
+  }
+  if (t.h) store_row(global<T>(t.h) + at, h, t.padded - n);
+}
+
 template <typename T, int SIZE>
 __global__ __launch_bounds__(sr_tile::threads<T>(SIZE), SIZE == 64 ? 3 : 2) void backward_kernel(BackwardArgs t) {
   typedef sr_tile::Tile<T, false, SIZE, ROW, COL> Tile;
   SR_TILE_MEMORY(Tile);
   const uint32_t item = sr_tile::item_of(blockIdx.x, t.grid.items, SIZE);
   if (item >= t.grid.items) return;
+  const Turn turn = turn_of(t.cut, item);
   uint32_t row, column;
-  sr_tile::banded(item, t.grid.rows, t.grid.columns, row, column);
+  sr_tile::banded(turn.tile, t.grid.rows, t.grid.columns, row, column);
   row *= SIZE;
   column *= SIZE;
   Tile tile;
-  sr_tile::run(tile, t.p, row, column, 0, (t.p.k + Tile::kK - 1) / Tile::kK, (Shared)a0, (Shared)a1, (Shared)b0,
-               (Shared)b1);
+  sr_tile::run(tile, t.p, row, column, turn.from, min(turn.to, (t.p.k + Tile::kK - 1) / Tile::kK), (Shared)a0, (Shared)a1,
+               (Shared)b0, (Shared)b1);
   __syncthreads();
-  auto kept = [&](uint32_t r, uint32_t n) {
-    r += row;
-    n += column;
-    Kept k{};
-    if (r >= t.tokens || n >= t.ffn) return k;
-    load_row(global<const float>(t.a) + uint64_t(r) * t.ffn + n, k.a, t.ffn - n);
-    load_row(global<const float>(t.b) + uint64_t(r) * t.ffn + n, k.b, t.ffn - n);
-    return k;
-  };
-  tile.template results<false, true>(SR_TILE_SLAB(Tile), kept, [&](uint32_t r, uint32_t n, const float (&dh)[8], const Kept& k) {
-    r += row;
-    n += column;
-    if (r >= t.tokens || n >= t.padded) return;
-    float da[8], db[8], h[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const Act f = act<true>(k.a[e], t.activation);
-      const float d = n + e < t.ffn ? dh[e] : 0.0f;      // (0 also where a row of dy has an infinity)
-      h[e] = f.value * k.b[e];
-      db[e] = d * f.value;
-      da[e] = d * k.b[e] * f.slope;
-    }
-    const uint64_t at = r * t.stride + n;
-    if (t.da) {
-      store_row(global<T>(t.da) + at, da, t.padded - n);
-      store_row(global<T>(t.db) + at, db, t.padded - n);
-    }
-    if (t.h) store_row(global<T>(t.h) + at, h, t.padded - n);
-  });
+  if (turn.split) {
+    tile.template results<false, true>(SR_TILE_SLAB(Tile), sr_tile::nothing, [&](uint32_t r, uint32_t n, const float (&v)[8],
+                                                                            sr_tile::Nothing) {
+      if (row + r < t.tokens) store_part<SIZE>(t.cut, turn.part, r, n, v);
+    });
+    return;
+  }
+  tile.template results<false, true>(
+      SR_TILE_SLAB(Tile), [&](uint32_t r, uint32_t n) { return load_kept(t, row + r, column + n); },
+      [&](uint32_t r, uint32_t n, const float (&dh)[8], const Kept& k) { store_backward<T>(t, row + r, column + n, dh, k); });
+}
+
+// dh joined: eight columns a lane.
+template <typename T, int SIZE>
+__global__ __launch_bounds__(kPlainThreads) void backward_join_kernel(BackwardArgs t) {
+  constexpr uint32_t kBlocks = SIZE * SIZE / 8 / kPlainThreads;      // of a tile
+  const uint32_t tile = blockIdx.x / kBlocks, at = (blockIdx.x % kBlocks * kPlainThreads + threadIdx.x) * 8;
+  const uint32_t r = at / SIZE, n = at % SIZE;
+  uint32_t row, column;
+  sr_tile::banded(t.cut.whole + tile, t.grid.rows, t.grid.columns, row, column);
+  row = row * SIZE + r;
+  column = column * SIZE + n;
+  if (row >= t.tokens || column >= t.padded) return;
+  const Kept k = load_kept(t, row, column);
+  float dh[8];
+  join_parts<SIZE>(t.cut, tile, r, n, dh);
+  store_backward<T>(t, row, column, dh, k);
 }
 
 // Plain products, up to three in a launch.  The steps of all their tiles, or of those
-// behind the last whole round of the compute units, may be split over `splits`
-// workgroups a tile, whose parts are joined in order afterwards.  The shape
+// behind the last whole round of the compute units, may be split.  The shape
 // above: y 369 GFLOP in 334 to 350 us, dx 739 in 642 to 677, the matrices' gradients
 // 1108 in 1005 (both operands' rows side by side).  Steps split, and joined: y and
 // dx of 1021 tokens, 3584 columns and 4736 rows 60 and 98 us, of one workgroup a tile 74 and
@@ -201,9 +304,7 @@ constexpr int kMostJobs = 3;
 struct ProductArgs {
   Job job[kMostJobs];
   uint32_t items;
-  uint32_t whole;             // tiles that are not split
-  uint32_t splits, steps;     // of the others, and of one workgroup
-  uint64_t parts;             // splits tiles of floats for each of them
+  Cut cut;
 };
 
 // The job of a tile, and the tile's place in its C.
@@ -225,44 +326,35 @@ __global__ __launch_bounds__(sr_tile::threads<T>(SIZE), SIZE == 64 ? 3 : 2) void
   SR_TILE_MEMORY(Tile);
   const uint32_t item = sr_tile::item_of(blockIdx.x, t.items, SIZE);
   if (item >= t.items) return;
-  const bool split = item >= t.whole;
-  const uint32_t part = split ? item - t.whole : 0;
+  const Turn turn = turn_of(t.cut, item);
   uint32_t row, column;
-  const Job& job = job_of<SIZE>(t, split ? t.whole + part / t.splits : item, row, column);
+  const Job& job = job_of<SIZE>(t, turn.tile, row, column);
   const uint32_t steps = (job.p.k + Tile::kK - 1) / Tile::kK * (job.p.a2.data ? 2 : 1);
-  const uint32_t from = split ? part % t.splits * t.steps : 0, to = split ? min(steps, from + t.steps) : steps;
   Tile tile;
-  sr_tile::run(tile, job.p, row, column, from, to, (Shared)a0, (Shared)a1, (Shared)b0, (Shared)b1);
+  sr_tile::run(tile, job.p, row, column, turn.from, min(turn.to, steps), (Shared)a0, (Shared)a1, (Shared)b0, (Shared)b1);
   __syncthreads();
   tile.template results<false, false>(SR_TILE_SLAB(Tile), sr_tile::nothing, [&](uint32_t r, uint32_t n, const float (&v)[8],
                                                                          sr_tile::Nothing) {
     const uint32_t i = row + r, j = column + n;
     if (i >= job.rows || j >= job.columns) return;
-    if (split) store_row(global<float>(t.parts) + (uint64_t(part) * SIZE + r) * SIZE + n, v, 8);
+    if (turn.split) store_part<SIZE>(t.cut, turn.part, r, n, v);
     else store_row(global<T>(job.out) + uint64_t(i) * job.columns + j, v, job.columns - j);
   });
 }
 
-constexpr int kPlainThreads = 256;
-
-// The sums of the parts, in order: eight values a lane.
+// The products' sums joined: eight values a lane.
 template <typename T, int SIZE>
 __global__ __launch_bounds__(kPlainThreads) void join_kernel(ProductArgs t) {
   constexpr uint32_t kBlocks = SIZE * SIZE / 8 / kPlainThreads;      // of a tile
   const uint32_t tile = blockIdx.x / kBlocks, at = (blockIdx.x % kBlocks * kPlainThreads + threadIdx.x) * 8;
   uint32_t row, column;
-  const Job& job = job_of<SIZE>(t, t.whole + tile, row, column);
-  row += at / SIZE;
-  column += at % SIZE;
+  const Job& job = job_of<SIZE>(t, t.cut.whole + tile, row, column);
+  const uint32_t r = at / SIZE, n = at % SIZE;
+  row += r;
+  column += n;
   if (row >= job.rows || column >= job.columns) return;
-  float sum[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-  const float* p = global<const float>(t.parts) + uint64_t(tile) * t.splits * (SIZE * SIZE) + at;
-  for (uint32_t s = 0; s < t.splits; ++s) {
-    float x[8];
-    load_row(p + s * (SIZE * SIZE), x, 8);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) sum[e] += x[e];
-  }
+  float sum[8];
+  join_parts<SIZE>(t.cut, tile, r, n, sum);
   store_row(global<T>(job.out) + uint64_t(row) * job.columns + column, sum, job.columns - column);
 }
 
@@ -496,19 +588,28 @@ struct Way {
   double time;
 };
 
+constexpr uint64_t kMostSplits = 24;
+
 // The fastest way for `count` products of rows x columns over `steps` steps each;
-// with `most` splits at most, of four steps or more, whose parts are written, read
+// with kMostSplits splits at most, of four steps or more, whose parts are written, read
 // and added up by another launch.  Of 256 x 256 tiles, of which a compute unit has one
 // at a time, also those alone that would keep few units busy for a round (8192 tokens,
 // 4096 columns and 5504 rows, the matrices' gradients have 4 x 256 + 32 tiles: a training
 // step takes 3000 us instead of 3110).
+//
+// Splitting has to take `gain` of the time or less by the model.  Products 0.95 (1021
+// tokens, 3584 columns, 4736 rows: the matrices' gradients 0.97 by it and 25 us of 430
+// slower, y 0.94 and 60 us instead of 75).  The projections and dh, whose join has the
+// activation's reads and writes to itself, 0.75: trained in bf16, dh of that shape is 0.77
+// by it and 7 us of 446 slower; 512 tokens of 4096 and 5504, projections 0.88 and 6 us of
+// 98 slower; 24 tokens of these 0.74 and 0.53, together 125 us instead of 166; 82 tokens of
+// 4976 columns and 168 rows in floats 0.12, the forward pass 35 us instead of 113.
+constexpr double kProductGain = 0.95, kActivatedGain = 0.75;
+
 template <typename T>
-Way way_of(const uint64_t (*sides)[2], int count, uint64_t steps, uint64_t most) {
+Way way_of(const uint64_t (*sides)[2], int count, uint64_t steps, double gain) {
   constexpr bool kF32 = sizeof(T) == 4;
   constexpr double kUnit = 0.4e-6, kLaunch = 10, kRate = 8e12;
-  // splitting has to gain a twentieth by the model (1021 tokens, 3584 columns, 4736 rows:
-  // the matrices' gradients 3% by it and 25 us of 430 slower, y 6% and 60 us instead of 75)
-  constexpr double kGain = 0.95;
   Way best{128, 0, 1, 1e30}, split = best;
   for (int size : {256, 128, 64}) {
     if (kF32 && size == 256) continue;
@@ -526,18 +627,40 @@ Way way_of(const uint64_t (*sides)[2], int count, uint64_t steps, uint64_t most)
       if (all < least.time) least = {size, whole, splits, all};
     };
     consider(tiles, 1);
-    for (uint64_t splits = 2; splits <= std::min(most, steps / 4); ++splits) {
+    for (uint64_t splits = 2; splits <= std::min(kMostSplits, steps / 4); ++splits) {
       consider(0, splits);
       if (size == 256 && tiles > 256 && tiles % 256) consider(tiles / 256 * 256, splits);
     }
   }
-  return split.time < kGain * best.time ? split : best;
+  return split.time < gain * best.time ? split : best;
 }
 
-template <typename T>
-int tile_size(uint64_t rows, uint64_t columns, uint64_t steps) {
-  const uint64_t sides[1][2] = {{rows, columns}};
-  return way_of<T>(sides, 1, steps, 1).size;
+// The cut of a launch's tiles, with the parts' memory, and its items.
+int cut_of(const char* who, const Way& way, uint64_t tiles, uint64_t steps, Space& space, Cut& cut, uint32_t& items) {
+  cut.whole = uint32_t(way.splits == 1 ? tiles : way.whole);
+  cut.steps = uint32_t(ceil_div(steps, way.splits));
+  cut.splits = uint32_t(way.splits == 1 ? 1 : ceil_div(steps, cut.steps));
+  const uint64_t parted = tiles - cut.whole, all = cut.whole + parted * cut.splits;
+  if (all > sr_tile::kMostItems) return fail(SR_EBOUNDS, "%s: %llu parts", who, (unsigned long long)all);
+  cut.parts = parted ? space.take(parted * cut.splits * way.size * way.size * sizeof(float)) : 0;
+  items = uint32_t(all);
+  return SR_OK;
+}
+
+// The tiles of a projections' launch (tokens x ffn, `wide` of them a tile), their cut and items.
+int grid_of(const char* who, const Way& way, const sr_ffn_shape& s, uint64_t wide, uint64_t steps, Space& space, Grid& grid,
+            Cut& cut) {
+  const uint64_t rows = ceil_div(s.tokens, way.size), columns = ceil_div(padded(s.ffn), wide);
+  if (rows * columns > sr_tile::kMostItems)
+    return fail(SR_EBOUNDS, "%s: %llu tokens of %llu columns", who, (unsigned long long)s.tokens, (unsigned long long)s.ffn);
+  grid.rows = uint32_t(rows);
+  grid.columns = uint32_t(columns);
+  return cut_of(who, way, rows * columns, steps, space, cut, grid.items);
+}
+
+// Workgroups of a launch that joins parts, of `values` values a tile.
+uint32_t join_blocks(const Grid& grid, const Cut& cut, int values) {
+  return uint32_t((uint64_t(grid.rows) * grid.columns - cut.whole) * (values / 8 / kPlainThreads));
 }
 
 // f(size) with the size as a constant.
@@ -547,8 +670,6 @@ void with_size(int size, F&& f) {
   else if (sizeof(T) == 4 || size == 128) f(std::integral_constant<int, 128>());
   else if constexpr (sizeof(T) == 2) f(std::integral_constant<int, 256>());
 }
-
-constexpr uint64_t kMostSplits = 24;
 
 struct Wanted {
   Product p;
@@ -566,7 +687,7 @@ int products(const char* who, const Wanted* w, int count, Space& space, bool lau
     sides[i][1] = w[i].columns;
     steps = steps_of<T>(w[i].p.k) * (w[i].p.a2.data ? 2 : 1);      // alike
   }
-  const Way way = way_of<T>(sides, count, steps, kMostSplits);
+  const Way way = way_of<T>(sides, count, steps, kProductGain);
   const int size = way.size;
   ProductArgs t{};
   uint64_t tiles = 0;
@@ -587,14 +708,9 @@ int products(const char* who, const Wanted* w, int count, Space& space, bool lau
   }
   if (n == 0) return SR_OK;
   for (int i = n; i < kMostJobs; ++i) t.job[i].first = 0xffffffffu;
-  t.whole = uint32_t(way.splits == 1 ? tiles : way.whole);
-  t.steps = uint32_t(ceil_div(steps, way.splits));
-  t.splits = uint32_t(way.splits == 1 ? 1 : ceil_div(steps, t.steps));
-  const uint64_t parted = tiles - t.whole, items = t.whole + parted * t.splits;
-  if (items > sr_tile::kMostItems) return fail(SR_EBOUNDS, "%s: %llu parts", who, (unsigned long long)items);
-  t.parts = parted ? space.take(parted * t.splits * size * size * sizeof(float)) : 0;
+  if (int rc = cut_of(who, way, tiles, steps, space, t.cut, t.items)) return rc;
+  const uint64_t parted = tiles - t.cut.whole;
   if (!launch) return SR_OK;
-  t.items = uint32_t(items);
   with_size<T>(size, [&](auto z) {
     product_kernel<T, z(), A, B><<<sr_tile::blocks_of(t.items, z()), sr_tile::threads<T>(z()), 0, stream>>>(t);
     if (parted) join_kernel<T, z()><<<uint32_t(parted * (z() * z() / 8 / kPlainThreads)), kPlainThreads, 0, stream>>>(t);
@@ -672,11 +788,9 @@ int forward(const sr_ffn_shape& s, void* out, void* a, void* b, Space& space, bo
   if (s.ffn) {
     ForwardArgs t{};
     t.p = {operand<T>(x, ROW), operand<T>(gate, ROW), {}, operand<T>(up, ROW), uint32_t(s.hidden)};
-    const int size = tile_size<T>(s.tokens, 2 * s.ffn, steps_of<T>(s.hidden));
-    const uint64_t rows = ceil_div(s.tokens, size), columns = ceil_div(wide, size / 2);
-    if (rows * columns > sr_tile::kMostItems)
-      return fail(SR_EBOUNDS, "sr_ffn: %llu tokens of %llu columns", (unsigned long long)s.tokens, (unsigned long long)s.ffn);
-    t.grid = {uint32_t(rows), uint32_t(columns), uint32_t(rows * columns)};
+    const uint64_t sides[1][2] = {{s.tokens, 2 * s.ffn}}, steps = steps_of<T>(s.hidden);
+    const Way way = way_of<T>(sides, 1, steps, kActivatedGain);
+    if (int rc = grid_of("sr_ffn", way, s, way.size / 2, steps, space, t.grid, t.cut)) return rc;
     t.h = h;
     t.a = reinterpret_cast<uint64_t>(a);
     t.b = reinterpret_cast<uint64_t>(b);
@@ -686,8 +800,12 @@ int forward(const sr_ffn_shape& s, void* out, void* a, void* b, Space& space, bo
     t.padded = uint32_t(wide);
     t.activation = s.activation;
     if (launch) {
-      const uint32_t blocks = sr_tile::blocks_of(t.grid.items, size);
-      with_size<T>(size, [&](auto z) { forward_kernel<T, z()><<<blocks, sr_tile::threads<T>(z()), 0, stream>>>(t); });
+      const uint32_t blocks = sr_tile::blocks_of(t.grid.items, way.size);
+      with_size<T>(way.size, [&](auto z) {
+        forward_kernel<T, z()><<<blocks, sr_tile::threads<T>(z()), 0, stream>>>(t);
+        const uint32_t joins = join_blocks(t.grid, t.cut, z() * z() / 2);
+        if (joins) forward_join_kernel<T, z()><<<joins, kPlainThreads, 0, stream>>>(t);
+      });
       if (int rc = launched("sr_ffn")) return rc;
     }
   }
@@ -709,11 +827,9 @@ int backward(const sr_ffn_shape& s, const void* a, const void* b, const void* dy
     const Matrix down = loader.ready(matrix_down(s));
     BackwardArgs t{};
     t.p = {operand<T>(dym, ROW), operand<T>(down, COL), {}, {}, uint32_t(s.hidden)};
-    const int size = tile_size<T>(s.tokens, s.ffn, steps_of<T>(s.hidden));
-    const uint64_t rows = ceil_div(s.tokens, size), columns = ceil_div(wide, size);
-    if (rows * columns > sr_tile::kMostItems)
-      return fail(SR_EBOUNDS, "%s: %llu tokens of %llu columns", who, (unsigned long long)s.tokens, (unsigned long long)s.ffn);
-    t.grid = {uint32_t(rows), uint32_t(columns), uint32_t(rows * columns)};
+    const uint64_t sides[1][2] = {{s.tokens, s.ffn}}, steps = steps_of<T>(s.hidden);
+    const Way way = way_of<T>(sides, 1, steps, kActivatedGain);
+    if (int rc = grid_of(who, way, s, way.size, steps, space, t.grid, t.cut)) return rc;
     t.a = reinterpret_cast<uint64_t>(a);
     t.b = reinterpret_cast<uint64_t>(b);
     t.da = da;
@@ -725,8 +841,12 @@ int backward(const sr_ffn_shape& s, const void* a, const void* b, const void* dy
     t.padded = uint32_t(wide);
     t.activation = s.activation;
     if (launch) {
-      const uint32_t blocks = sr_tile::blocks_of(t.grid.items, size);
-      with_size<T>(size, [&](auto z) { backward_kernel<T, z()><<<blocks, sr_tile::threads<T>(z()), 0, stream>>>(t); });
+      const uint32_t blocks = sr_tile::blocks_of(t.grid.items, way.size);
+      with_size<T>(way.size, [&](auto z) {
+        backward_kernel<T, z()><<<blocks, sr_tile::threads<T>(z()), 0, stream>>>(t);
+        const uint32_t joins = join_blocks(t.grid, t.cut, z() * z());
+        if (joins) backward_join_kernel<T, z()><<<joins, kPlainThreads, 0, stream>>>(t);
+      });
       if (int rc = launched(who)) return rc;
     }
   }

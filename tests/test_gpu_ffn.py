@@ -347,3 +347,39 @@ def test_slope_of_far_gelu_tanh_gates():
 def test_long_sums_of_several_products(size, dtype):
     """The matrices' gradients over many tokens: the tiles behind whole rounds of 256, or all of few, in parts."""
     check(*size, dtype)
+
+
+def kernels_of(f):
+    """The kernels that a call launches."""
+    with torch.profiler.profile(activities=[torch.profiler.ProfilerActivity.CUDA]) as p:
+        f()
+        torch.cuda.synchronize()
+    return {e.key for e in p.key_averages()}
+
+
+# Long sums of few tiles: those of the projections and of dh are split too.
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("size", [(5, 4986, 88), (64, 4100, 33), (70, 4242, 40), (200, 3001, 300), (129, 8192, 64), (300, 2056, 520)],
+                         ids=str)
+def test_long_sums_of_projections(size, dtype):
+    names = kernels_of(lambda: check(*size, dtype))
+    for k in ("forward_join_kernel", "backward_join_kernel"):
+        assert any(k in n for n in names) or (k == "forward_join_kernel" and size[0] <= 64), k
+
+
+@pytest.mark.parametrize("tokens", [4, 150])
+@pytest.mark.parametrize("ffn", [13, 16])
+def test_an_infinity_in_split_sums(ffn, tokens):
+    """As in sums that are not split: it stays in its row, and does not meet the padding's zeros."""
+    gen = torch.Generator(DEV).manual_seed(8)
+    x, g, up, d, dy = (torch.rand(s, generator=gen, device=DEV).add_(0.5).mul_(1 / 64).to(BF16)
+                       for s in ((tokens, 4104), (ffn, 4104), (ffn, 4104), (4104, ffn), (tokens, 4104)))
+    clean = gated_ffn(x, g, up, d, keep=True)
+    before = gated_ffn_grad(x, g, up, d, clean.gate, clean.up, dy)[0]
+    dy[1, 3] = math.inf
+    dx = gated_ffn_grad(x, g, up, d, clean.gate, clean.up, dy)[0]
+    others = [i for i in range(tokens) if i != 1]
+    assert bool((dx[1] == math.inf).all()) and torch.equal(dx[others], before[others])
+    x[1, 5] = math.inf
+    kept = gated_ffn(x, g, up, d, keep=True).out
+    assert bool((kept[1] == math.inf).all()) and torch.equal(kept[others], clean.out[others])

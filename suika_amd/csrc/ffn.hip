@@ -405,6 +405,7 @@ template <> struct Thin<float> {
 
 struct ThinArgs {
   uint64_t x, m, m2, out;     // m2: up, or 0
+  uint64_t a, b;              // both projections kept for the gradients, or 0
   uint64_t x_stride, m_stride, m2_stride;     // elements
   uint32_t tokens, rows, k, out_stride;
   uint32_t each;              // rows of a workgroup, of each matrix
@@ -507,14 +508,25 @@ __global__ __launch_bounds__(WAVES * kWave) void thin_kernel(ThinArgs t) {
     T* out = global<T>(t.out) + uint64_t(token) * t.out_stride;
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      if (first + r < end) out[first + r] = static_cast<T>(GATED ? act<false>(sum[r], t.activation).value * up[r] : sum[r]);
+      if (first + r >= end) continue;
+      out[first + r] = static_cast<T>(GATED ? act<false>(sum[r], t.activation).value * up[r] : sum[r]);
+      if (GATED && t.a) {
+        const uint64_t at = uint64_t(token) * t.rows + first + r;
+        global<float>(t.a)[at] = sum[r];
+        global<float>(t.b)[at] = up[r];
+      }
     }
   }
 }
 
 // ---------------------------------------------------------------------- host
 
-constexpr uint64_t kFewTokens = 64;
+// Calls of so few tokens take the thin kernels: 64, or 32 where the projections are
+// kept, which tiles write in wider pieces (trained, 4096
+// columns and 5504 rows in bf16: 24 tokens 117 us instead of 123 in tiles, 48 tokens 139
+// instead of 127; 5 tokens of 1886 rows of 4986 columns in floats 176 instead of 254, which
+// tiles would have to copy first).
+constexpr uint64_t kFewTokens = 64, kFewKept = 32;
 constexpr uint64_t kMostSide = uint64_t(1) << 20;     // hidden, ffn: an aligned row is within kMostStride
 
 uint64_t padded(uint64_t n) { return (n + 7) / 8 * 8; }
@@ -771,13 +783,13 @@ int forward(const sr_ffn_shape& s, void* out, void* a, void* b, Space& space, bo
   if (s.tokens == 0) return SR_OK;
   const uint64_t wide = padded(s.ffn);
   const uint64_t h = space.take(s.tokens * wide * sizeof(T));
-  if (s.tokens <= kFewTokens && a == nullptr) {
+  if (s.tokens <= (a ? kFewKept : kFewTokens)) {
     if (!launch) return SR_OK;
     ThinArgs g{reinterpret_cast<uint64_t>(s.x), reinterpret_cast<uint64_t>(s.gate), reinterpret_cast<uint64_t>(s.up), h,
-               s.x_stride, s.gate_stride, s.up_stride, uint32_t(s.tokens), uint32_t(s.ffn), uint32_t(s.hidden),
-               uint32_t(wide), 0, s.activation};
+               reinterpret_cast<uint64_t>(a), reinterpret_cast<uint64_t>(b), s.x_stride, s.gate_stride, s.up_stride,
+               uint32_t(s.tokens), uint32_t(s.ffn), uint32_t(s.hidden), uint32_t(wide), 0, s.activation};
     thin<T, true>(g, stream);
-    ThinArgs d{h, reinterpret_cast<uint64_t>(s.down), 0, reinterpret_cast<uint64_t>(out), wide, s.down_stride, 0,
+    ThinArgs d{h, reinterpret_cast<uint64_t>(s.down), 0, reinterpret_cast<uint64_t>(out), 0, 0, wide, s.down_stride, 0,
                uint32_t(s.tokens), uint32_t(s.hidden), uint32_t(s.ffn), uint32_t(s.hidden), 0, 0};
     thin<T, false>(d, stream);
     return launched("sr_ffn");

@@ -383,3 +383,18 @@ def test_an_infinity_in_split_sums(ffn, tokens):
     x[1, 5] = math.inf
     kept = gated_ffn(x, g, up, d, keep=True).out
     assert bool((kept[1] == math.inf).all()) and torch.equal(kept[others], clean.out[others])
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("tokens", [1, 16, 17, 32, 33])
+def test_few_tokens_that_are_kept(tokens, dtype):
+    """Odd rows need no copies for few tokens, and the projections are those that the block's output is of."""
+    check(tokens, 1025, 333, dtype, pad=3)
+    x, g, up, d, _ = block(tokens, 1025, 333, dtype, 3)
+    names = kernels_of(lambda: gated_ffn(x, g, up, d, keep=True))
+    assert any("align_kernel" in n for n in names) == (tokens > 32), names
+    r = gated_ffn(x, g, up, d, keep=True)
+    off = (1025 + 2) * u
+    for got, w in ((r.gate, g), (r.up, up)):
+        want, size = x.double() @ w.double().t(), x.double().abs() @ w.double().abs().t()
+        assert bool(((got.double() - want).abs() <= off * size).all())

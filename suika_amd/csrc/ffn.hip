@@ -46,20 +46,30 @@ struct Act {
   float value, slope;
 };
 
+// exp(x) for results of T.  The fast one rounds x log2(e), which leaves x 2^-24 of the
+// result's size: 1e-5 where the weight below is 1e-38.  16 bits round that off, floats
+// would show it (a gate of -60 3e-6 off).
+template <typename T>
+__device__ __forceinline__ float exp_for(float x) {
+  if constexpr (sizeof(T) == 4) return expf(x);
+  else return __expf(x);
+}
+
 // All three are a times a weight between 0 and 1.  exp overflows to infinity
 // for far negative a, where the weight is then 0.
-__device__ __forceinline__ float weight_of(float z) { return 1.0f / (1.0f + __expf(-z)); }
+template <typename T>
+__device__ __forceinline__ float weight_of(float z) { return 1.0f / (1.0f + exp_for<T>(-z)); }
 
 constexpr float kTanhScale = 1.5957691216057308f;     // 2 sqrt(2 / pi)
 constexpr float kTanhCube = 0.044715f;
 
-template <bool SLOPE>
+template <typename T, bool SLOPE>
 __device__ __forceinline__ Act act(float a, int32_t kind) {
   Act r{0, 0};
   if (kind == SR_ACT_GELU) {
     const float p = 0.5f * erfcf(a * -0.70710678118654752f);
     r.value = a * p;
-    if (SLOPE) r.slope = fmaf(a * 0.39894228040143268f, __expf(-0.5f * a * a), p);
+    if (SLOPE) r.slope = fmaf(a * 0.39894228040143268f, exp_for<T>(-0.5f * a * a), p);
     return r;
   }
   float z = a, dz = 1.0f;
@@ -68,10 +78,10 @@ __device__ __forceinline__ Act act(float a, int32_t kind) {
     z = kTanhScale * fmaf(kTanhCube * q, a, a);
     dz = kTanhScale * fmaf(3 * kTanhCube, q, 1.0f);
   }
-  const float p = weight_of(z);
+  const float p = weight_of<T>(z);
   r.value = a * p;
   // the rest of the weight, 1 - p, from the other side: nothing cancels
-  if (SLOPE) r.slope = fmaf(r.value * weight_of(-z), dz, p);
+  if (SLOPE) r.slope = fmaf(r.value * weight_of<T>(-z), dz, p);
   return r;
 }
 
@@ -143,7 +153,7 @@ __device__ __forceinline__ void store_forward(const ForwardArgs& t, uint32_t r, 
   float h[8];
   // (the columns behind ffn are zeros also where a row of x has an infinity)
 #pragma unroll
-  for (int e = 0; e < 8; ++e) h[e] = n + e < t.ffn ? act<false>(a[e], t.activation).value * b[e] : 0.0f;
+  for (int e = 0; e < 8; ++e) h[e] = n + e < t.ffn ? act<T, false>(a[e], t.activation).value * b[e] : 0.0f;
   store_row(global<T>(t.h) + r * t.h_stride + n, h, t.padded - n);
   if (t.a && n < t.ffn) {
     store_row(global<float>(t.a) + uint64_t(r) * t.ffn + n, a, t.ffn - n);
@@ -228,7 +238,7 @@ __device__ __forceinline__ void store_backward(const BackwardArgs& t, uint32_t r
   float da[8], db[8], h[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
-    const Act f = act<true>(k.a[e], t.activation);
+    const Act f = act<T, true>(k.a[e], t.activation);
     const float d = n + e < t.ffn ? dh[e] : 0.0f;      // (0 also where a row of dy has an infinity)
     h[e] = f.value * k.b[e];
     db[e] = d * f.value;
@@ -509,7 +519,7 @@ __global__ __launch_bounds__(WAVES * kWave) void thin_kernel(ThinArgs t) {
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       if (first + r >= end) continue;
-      out[first + r] = static_cast<T>(GATED ? act<false>(sum[r], t.activation).value * up[r] : sum[r]);
+      out[first + r] = static_cast<T>(GATED ? act<T, false>(sum[r], t.activation).value * up[r] : sum[r]);
       if (GATED && t.a) {
         const uint64_t at = uint64_t(token) * t.rows + first + r;
         global<float>(t.a)[at] = sum[r];

@@ -398,3 +398,22 @@ def test_few_tokens_that_are_kept(tokens, dtype):
     for got, w in ((r.gate, g), (r.up, up)):
         want, size = x.double() @ w.double().t(), x.double().abs() @ w.double().abs().t()
         assert bool(((got.double() - want).abs() <= off * size).all())
+
+
+@pytest.mark.parametrize("way", [-1, 1])
+def test_far_silu_gates_in_32_bits(way):
+    """The weight's exponential is off by an ulp (2u) whatever its argument, the sum, the division and the product by u
+    each: 5u of the value, and 12u of a slope whose two terms are at most 1.5 times their sum."""
+    gate = (torch.linspace(5, 85, 161, device=DEV) * way).view(-1, 1)
+    n = gate.shape[0]
+    x, up, down = torch.ones(1, 1, device=DEV), torch.ones(n, 1, device=DEV), torch.ones(1, n, device=DEV)
+    value, slope, _ = act64(gate.double().view(-1), "silu")
+    r = gated_ffn(x, gate, up, down, keep=True)
+    assert torch.equal(r.gate.view(-1), gate.view(-1))
+    _, dgate, dup, _ = gated_ffn_grad(x, gate, up, down, r.gate, r.up, torch.ones(1, 1, device=DEV))
+    assert bool(((dup.view(-1) - value).abs() <= 5 * u * value.abs()).all())
+    assert bool(((dgate.view(-1) - slope).abs() <= 12 * u * slope.abs()).all())
+    for i in (0, 60, 110, n - 1):
+        out = float(gated_ffn(x, gate[i:i + 1], up[:1], down[:, :1]))
+        assert abs(out - float(value[i])) <= 5 * u * abs(float(value[i]))
+

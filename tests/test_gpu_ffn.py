@@ -417,3 +417,16 @@ def test_far_silu_gates_in_32_bits(way):
         out = float(gated_ffn(x, gate[i:i + 1], up[:1], down[:, :1]))
         assert abs(out - float(value[i])) <= 5 * u * abs(float(value[i]))
 
+
+
+# Two whole rounds of 128 x 128 tiles: of the projections and of dh, of y and dx, and of
+# the matrices' gradients.
+@pytest.mark.parametrize("size, kernels", [((4000, 40, 2001), ("forward_kernel<float, 128>", "backward_kernel<float, 128>")),
+                                           ((4000, 2001, 24), ("product_kernel<float, 128, (sr_tile::Side)0, (sr_tile::Side)0>",
+                                                               "product_kernel<float, 128, (sr_tile::Side)0, (sr_tile::Side)1>")),
+                                           ((30, 1901, 1400), ("product_kernel<float, 128, (sr_tile::Side)1, (sr_tile::Side)1>",))],
+                         ids=str)
+def test_large_tiles_of_floats(size, kernels):
+    names = kernels_of(lambda: check(*size, F32))
+    for k in kernels:
+        assert any(k in n for n in names), (k, sorted(n for n in names if "kernel<" in n))

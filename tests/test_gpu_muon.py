@@ -539,3 +539,95 @@ def test_failing_reduce_of_a_step(fails_at):
         if n in stepped:
             assert torch.equal(e["master"], other[n]["master"]) and torch.equal(e["param"], other[n]["param"]), n
 
+
+
+# --------------------------------------------------- products of large tiles
+
+# One matrix of 16 x 16 tiles of 256, with odd remainders: X goes through its steps in these,
+# and from 32 tiles of 128 a side on so do A and B.
+LARGE = [(3843, 3901), (3903, 3842), (4003, 4069), (4071, 4001)]
+
+
+def kernels_of(f):
+    """The kernels that a call launches."""
+    with torch.profiler.profile(activities=[torch.profiler.ProfilerActivity.CUDA]) as p:
+        f()
+        torch.cuda.synchronize()
+    return {e.key for e in p.key_averages()}
+
+
+def iterates(g, steps=5):
+    """The result in 64 bits, and the norms of the iterates after each step."""
+    x = g.double()
+    x = x / x.norm()
+    flip = x.shape[0] > x.shape[1]
+    x = (x.t() if flip else x).contiguous()
+    a, b, c = COEFFICIENTS
+    sizes = []
+    for _ in range(steps):
+        s = x @ x.t()
+        x = a * x + (b * s + c * (s @ s)) @ x
+        sizes.append(float(x.norm()))
+    return (x.t() if flip else x), sizes
+
+
+def near_everywhere(got, want, sizes, what=""):
+    """A step's roundings are 4 * 2^-22 of its result's size and grow by 3.4445 in each later one: together the bound on
+    the norm of all.  Rows, columns and elements of a normal matrix are alike, so no row's or column's share of that is
+    more than 4 times its part, and no element's more than 16 times the root of the mean square."""
+    dt, n = got.dtype, len(sizes)
+    bound = sum(4 * 2.0 ** -22 * s * COEFFICIENTS[0] ** (n - 1 - j) for j, s in enumerate(sizes))
+    off = got.double() - want
+    assert float(off.norm()) <= bound + U[dt] * float(want.norm()), f"{what}: {float(off.norm()):.2e}, {bound:.2e} allowed"
+    for d in (0, 1):
+        allowed = 4 * bound / math.sqrt(want.shape[1 - d]) + U[dt] * want.norm(dim=d)
+        assert bool((off.norm(dim=d) <= allowed).all()), f"{what}: along {d}"
+    assert bool((off.abs() <= 16 * bound / math.sqrt(want.numel()) + U[dt] * want.abs()).all()), f"{what}: an element"
+
+
+@pytest.mark.parametrize("shape", LARGE, ids=str)
+def test_large_tiles(shape):
+    g = draw(shape)
+    want, sizes = iterates(g)
+    for dtype in (F32, BF16):
+        out = torch.empty(shape[0], shape[1] + 3, dtype=dtype, device=DEV)[:, 1:-2]
+        names = kernels_of(lambda: orthogonalize([g], out=[out]))
+        wanted = ["update_kernel<256>", "last_kernel<256>"]
+        if min(shape) > 31 * 128:
+            wanted += ["symmetric_kernel<256, false>", "symmetric_kernel<256, true>"]
+        assert all(any(k in n for n in names) for k in wanted), sorted(n for n in names if "kernel<" in n)
+        near_everywhere(out, want, sizes, str(dtype))
+    # as a part of itself, whose Gram matrices go to the host program
+    for split in (0, 1):
+        got, = orthogonalize([g], split=[split], all_reduce=lambda t: None)
+        near_everywhere(got, want, sizes, f"split {split}")
+
+
+@pytest.mark.parametrize("shape", LARGE, ids=str)
+@pytest.mark.parametrize("fields", ["mixed", "bf16"])
+def test_large_tiles_of_weights(shape, fields):
+    state = share(fields, [shape])
+    entry = state["p0"]
+    key = "master" if "master" in entry else "param"
+    old = {f: t.clone() for f, t in entry.items()}
+    grad = draw(shape, seed=300, std=0.02, dtype=FIELDS[fields][3])
+    optimizer = ShardMuon(state, lr=LR, momentum=MU, weight_decay=DECAY, adjust_lr="none")
+    assert any("last_kernel<256>" in n for n in kernels_of(lambda: optimizer.step([grad])))
+    m64, off_m = muon64(old[key], old["exp_avg"], grad, moment=entry["exp_avg"].dtype)
+    assert bool(((entry["exp_avg"].double() - m64).abs() <= off_m).all())
+    x, sizes = iterates(MU * entry["exp_avg"].double() + (1 - MU) * grad.double())
+    want = old[key].double() * (1 - LR * DECAY) - LR * x
+    bound = LR * sum(4 * 2.0 ** -22 * s * COEFFICIENTS[0] ** (4 - j) for j, s in enumerate(sizes))
+    # the decay factor, the two products and the difference, and what is stored
+    off = (entry[key].double() - want).abs()
+    allowed = 16 * bound / math.sqrt(want.numel()) + 2 * u * (old[key].double().abs() + LR * x.abs()) + U[entry[key].dtype] * want.abs()
+    assert bool((off <= allowed + 2.0 ** -133).all())
+    if key == "master":
+        assert torch.equal(entry["param"], entry["master"].to(BF16))
+
+
+@pytest.mark.parametrize("shape", [(65, 64), (127, 130), (129, 257), (300, 299), (520, 530), (200, 1000), (1000, 200)], ids=str)
+def test_every_element(shape):
+    g = draw(shape)
+    want, sizes = iterates(g)
+    near_everywhere(orthogonalize([g])[0], want, sizes)

@@ -631,3 +631,31 @@ def test_every_element(shape):
     g = draw(shape)
     want, sizes = iterates(g)
     near_everywhere(orthogonalize([g])[0], want, sizes)
+
+
+# --------------------------------------------------------- torch.optim.Muon
+
+@pytest.mark.parametrize("adjust", ["original", "match_rms_adamw"])
+@pytest.mark.parametrize("nesterov", [True, False])
+@pytest.mark.parametrize("shape", [(96, 40), (40, 96)], ids=str)
+def test_steps_of_torch(shape, nesterov, adjust):
+    """Two steps beside torch.optim.Muon, whose one Newton-Schulz step is in bf16: X, A, A A, B, B X and the sum rounded
+    to 2^-8, each of at most |a| + |b| + |c| of X's norm of 1.  Its momentum is in 32 bits, as here."""
+    lr, decay = 0.1, 0.5
+    w = draw(shape, seed=1, std=0.5)
+    theirs = torch.nn.Parameter(w.clone())
+    torch_muon = torch.optim.Muon([theirs], lr=lr, weight_decay=decay, momentum=MU, nesterov=nesterov, ns_steps=1,
+                                  adjust_lr_fn=adjust)
+    state = {"w": {"param": w.clone(), "exp_avg": torch.zeros_like(w)}}
+    ours = ShardMuon(state, lr=lr, weight_decay=decay, momentum=MU, nesterov=nesterov, ns_steps=1, adjust_lr=adjust)
+    rate = lr * (math.sqrt(max(1.0, shape[0] / shape[1])) if adjust == "original" else 0.2 * math.sqrt(max(shape)))
+    for k in range(1, 3):
+        theirs.grad = draw(shape, seed=10 + k, std=0.02)
+        ours.step([theirs.grad])
+        torch_muon.step()
+        m = torch_muon.state[theirs]["momentum_buffer"]
+        assert bool(((state["w"]["exp_avg"] - m).abs() <= 8 * u * (m.abs() + theirs.grad.abs())).all())
+        allowed = k * (rate * 6 * U[BF16] * sum(map(abs, COEFFICIENTS)) + 8 * u * float(w.norm()))
+        assert float((state["w"]["param"] - theirs.detach()).norm()) <= allowed
+    # without the decay, or at the other rate, the weights would be farther away than that
+    assert 2 * lr * decay * float(w.norm()) > 4 * allowed

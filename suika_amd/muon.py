@@ -20,6 +20,7 @@ of include/suika_step.h.  Refused arguments raise ``PlanError``.
 from __future__ import annotations
 
 import math
+from numbers import Real
 from typing import Callable, Dict, Iterable, List, Mapping, Optional, Sequence, Tuple, Union
 
 import torch
@@ -36,10 +37,15 @@ COEFFICIENTS: Triple = (3.4445, -4.7750, 2.0315)
 
 def _schedule(steps: int, coefficients: Union[Triple, Sequence[Triple]]) -> List[float]:
     """The coefficients of all steps, one after another."""
-    rows = [coefficients] * steps if isinstance(coefficients[0], (int, float)) else list(coefficients)
-    if len(rows) != steps or any(len(r) != 3 for r in rows):
-        raise PlanError(f"coefficients: three numbers, or three for each of the {steps} steps")
-    return [float(x) for r in rows for x in r]
+    try:
+        len(coefficients)       # no iterator: ShardMuon goes through them at every step
+        rows = list(coefficients)
+        rows = [rows] * steps if rows and isinstance(rows[0], Real) else [list(r) for r in rows]
+        if len(rows) == steps and all(len(r) == 3 for r in rows):
+            return [float(x) for r in rows for x in r]
+    except (TypeError, ValueError):
+        pass
+    raise PlanError(f"coefficients: three numbers, or three for each of the {steps} steps")
 
 
 def _tensors(given: Iterable[Tensor], what: str) -> List[Tensor]:

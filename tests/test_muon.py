@@ -218,3 +218,15 @@ def test_outputs_that_want_a_gradient():
         orthogonalize([g], out=[out])
     with pytest.raises(PlanError, match="out: a sequence of tensors"):
         orthogonalize([g], out=1)
+
+
+def test_coefficients_of_any_kind():
+    import numpy as np
+    from suika_amd.muon import _schedule
+    triple = (1.5, -0.5, 0.0)
+    for given in (triple, list(triple), np.array(triple), np.array(triple, dtype=np.float32), [triple] * 2,
+                  np.array([triple] * 2, dtype=np.float32)):
+        assert _schedule(2, given) == list(triple) * 2
+    for bad in ([], (), None, 1.5, "abc", iter(triple), triple[:2], [triple], [triple, None], [triple, ("a", "b", "c")], [[]] * 2):
+        with pytest.raises(PlanError, match="three numbers"):
+            orthogonalize([], steps=2, coefficients=bad)

@@ -320,9 +320,10 @@ typedef struct sr_matrix {
  * dst[i] = the last X of G = src[i]; sides of at most 2^19.  Products are of 22
  * bits a value in sums of 32 bits.  A matrix may be its own result; otherwise
  * what is written overlaps nothing else (SR_EOVERLAP).  workspace:
- * sr_orthogonalize_workspace bytes (16 for a value of X and 8 for a value of X
- * X^T, of at most 8 GiB of matrices at a time or of one).  split of dst is not
- * read.
+ * sr_orthogonalize_workspace bytes: 8 for a value of X and 8 for one of X X^T, of as
+ * many matrices as go through the steps together, 48 with 8 GiB of these at most, or
+ * one.  Of split matrices 12 for a value of X X^T, the 8 GiB are of these alone and
+ * X's come on top.  split of dst is not read.
  */
 int sr_orthogonalize_workspace(const sr_matrix* src, const sr_matrix* dst, int32_t count, const sr_newton_schulz* ns,
                                uint64_t* bytes);

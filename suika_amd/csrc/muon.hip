@@ -13,8 +13,9 @@
 // and with them all that is rounded in X, grow by up to a factor of a = 3.4 a
 // step, 485 in five: what 16 bits round off would be percents of the result.
 // X, A and B are therefore held in 22 bits, as two f16 (sr_tile.h), scaled by
-// powers of two that keep both in f16's normal range: |X| and |A| are below 2
-// and stored times 2^14, |B| below 31 and stored times 2^11.  A product is three
+// powers of two with which they fit f16, whose largest value is 65504: singular
+// values of X are held to 1.9 (check_steps), so X and A, 3.61 at most, are stored times
+// 2^14, up to 59200, and B, 30 at most, times 2^11, up to 61440.  A product is three
 // of f16 on the matrix cores, a third of their rate and five times that of
 // 32-bit floats, and its result is nearer to the exact one than a product of
 // 32-bit floats in 32-bit sums: 4e-7 to 2e-6 of the result's size after five
@@ -59,7 +60,6 @@ struct Entry {
   uint64_t gram;           // floats, where ranks add them up, or 0
   uint32_t m, n;
   uint32_t from;           // its first work item
-  uint32_t at;             // its number in the list, for the sums
 };
 
 constexpr int kEntries = 48;
@@ -689,7 +689,8 @@ uint64_t x_bytes(const Work& w) { return uint64_t(w.m()) * whole(w.n()) * 4; }
 uint64_t gram_bytes(const Work& w) { return uint64_t(w.m()) * whole(w.m()) * 4; }
 
 // Matrices that go through the steps together.  Ranks that add Gram matrices up
-// have the same ones in a group: it goes by what is the same on all of them.
+// have the same ones in a group: it goes by what is the same on all of them, the Gram
+// matrices, and the memory of X comes on top.
 constexpr uint64_t kGroupBytes = uint64_t(8) << 30;
 
 struct Group {
@@ -811,7 +812,6 @@ int run_steps(const Group& g, const Steps& s, uint64_t sums, Space& space, bool 
     e.b = space.take(gram_bytes(w));
     e.m = w.m();
     e.n = w.n();
-    e.at = uint32_t(i);
     if (g.split) {
       e.gram = grams + gram_floats * sizeof(float);
       gram_floats += uint64_t(e.m) * e.m;

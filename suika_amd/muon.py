@@ -12,7 +12,10 @@ Where tensor parallelism cuts a matrix, its orthogonal update depends on all of
 it.  A polynomial of the matrix needs only the products of its rows (or columns)
 with each other, ``X^T X`` or ``X X^T``, and those of the parts add up: with
 ``split`` and ``all_reduce`` every rank keeps its part and exchanges these sums,
-so a step's result does not depend on the degree.
+so a step's result depends on the degree only by the order of 32-bit sums.  The
+products are then those of the side that is whole, whichever is shorter, and every
+rank forms ``B`` by itself: where the cut side is much the shorter one, a whole
+matrix takes fewer operations.
 
 The kernels run on the tensors' device, on its current stream, behind the C ABI
 of include/suika_step.h.  Refused arguments raise ``PlanError``.

@@ -230,3 +230,16 @@ def test_coefficients_of_any_kind():
     for bad in ([], (), None, 1.5, "abc", iter(triple), triple[:2], [triple], [triple, None], [triple, ("a", "b", "c")], [[]] * 2):
         with pytest.raises(PlanError, match="three numbers"):
             orthogonalize([], steps=2, coefficients=bad)
+
+
+def test_workspace_of_split_matrices():
+    """X twice, A and B as pairs of 16 bits, and A in floats; groups of 8 GiB are counted without X."""
+    ns = steps(reduce=REDUCE(lambda *a: 0))
+    rc, need = workspace([matrix(100, 200, split=0)], ns=ns)
+    exact = 4 * (2 * 200 * 128 + 2 * 200 * 224 + 200 * 200)
+    assert rc == 0 and exact <= need <= exact + 4096
+    rc, other = workspace([matrix(100, 200, split=1)], ns=ns)
+    assert rc == 0 and 4 * (2 * 100 * 224 + 2 * 100 * 128 + 100 * 100) <= other < need
+    wide = [matrix(4096, 65536, i << 32, split=1) for i in range(40)]
+    rc, need = workspace(wide, [matrix(4096, 65536, (100 + i) << 32) for i in range(40)], ns)
+    assert rc == 0 and need > 40 * 4 * (2 * 4096 * 65536 + 3 * 4096 * 4096)

@@ -415,17 +415,22 @@ template <> struct Thin<float> {
 
 struct ThinArgs {
   uint64_t x, m, m2, out;     // m2: up, or 0
-  uint64_t a, b;              // both projections kept for the gradients, or 0
   uint64_t x_stride, m_stride, m2_stride;     // elements
   uint32_t tokens, rows, k, out_stride;
   uint32_t each;              // rows of a workgroup, of each matrix
   int32_t activation;
 };
 
+// With both projections kept for the gradients.
+struct ThinKept : ThinArgs {
+  uint64_t a, b;
+};
+
 // GROUPS: of 16 tokens; BLOCKS: of 16 rows, GATED: half of them of G, then the same of
-// U; WAVES: of a workgroup.
-template <typename T, int GROUPS, int BLOCKS, int WAVES, bool GATED>
-__global__ __launch_bounds__(WAVES * kWave) void thin_kernel(ThinArgs t) {
+// U; WAVES: of a workgroup; Args: ThinKept where the projections are kept (a kernel of its
+// own: 16 more bytes of arguments take a launch 0.25 us, 6% of the smallest calls).
+template <typename T, int GROUPS, int BLOCKS, int WAVES, bool GATED, typename Args>
+__global__ __launch_bounds__(WAVES * kWave) void thin_kernel(Args t) {
   typedef Thin<T> K;
   typedef typename K::Frag Frag;
   constexpr int kEach = 16 / sizeof(T);       // k of a lane
@@ -520,7 +525,7 @@ __global__ __launch_bounds__(WAVES * kWave) void thin_kernel(ThinArgs t) {
     for (int r = 0; r < 4; ++r) {
       if (first + r >= end) continue;
       out[first + r] = static_cast<T>(GATED ? act<T, false>(sum[r], t.activation).value * up[r] : sum[r]);
-      if (GATED && t.a) {
+      if constexpr (std::is_same_v<Args, ThinKept>) {
         const uint64_t at = uint64_t(token) * t.rows + first + r;
         global<float>(t.a)[at] = sum[r];
         global<float>(t.b)[at] = up[r];
@@ -532,11 +537,12 @@ __global__ __launch_bounds__(WAVES * kWave) void thin_kernel(ThinArgs t) {
 // ---------------------------------------------------------------------- host
 
 // Calls of so few tokens take the thin kernels: 64, or 32 where the projections are
-// kept, which tiles write in wider pieces (trained, 4096
-// columns and 5504 rows in bf16: 24 tokens 117 us instead of 123 in tiles, 48 tokens 139
-// instead of 127; 5 tokens of 1886 rows of 4986 columns in floats 176 instead of 254, which
-// tiles would have to copy first).
-constexpr uint64_t kFewTokens = 64, kFewKept = 32;
+// kept, and then where tiles would have to copy rows first, or ffn is no more than four
+// times hidden: y's few rows of long sums are split only in tiles.  Trained: 5 tokens, 4986
+// columns and 1886 rows in floats, which tiles copy, 176 us instead of 254; 24 tokens, 4096
+// and 5504 in bf16 117 instead of 123, but 48 tokens 139 instead of 127; 32 tokens, 700 and
+// 11008 in floats would be 181 instead of 166.
+constexpr uint64_t kFewTokens = 64, kFewKept = 32, kNarrow = 4;
 constexpr uint64_t kMostSide = uint64_t(1) << 20;     // hidden, ffn: an aligned row is within kMostStride
 
 uint64_t padded(uint64_t n) { return (n + 7) / 8 * 8; }
@@ -758,15 +764,15 @@ uint32_t rows_each(uint32_t rows, bool gated, int groups) {
   return best;
 }
 
-template <typename T, int GROUPS, int BLOCKS, bool GATED>
-void launch_blocks(const ThinArgs& t, hipStream_t stream) {
+template <typename T, int GROUPS, int BLOCKS, bool GATED, typename Args>
+void launch_blocks(const Args& t, hipStream_t stream) {
   // (24 tokens, 5504 rows of both 22.1 us with 4 waves, 23.5 with 8; 48 tokens 33.9 and 31.8)
   constexpr int kWaves = GROUPS == 2 ? 4 : 8;
-  thin_kernel<T, GROUPS, BLOCKS, kWaves, GATED><<<uint32_t(ceil_div(t.rows, t.each)), kWaves * kWave, 0, stream>>>(t);
+  thin_kernel<T, GROUPS, BLOCKS, kWaves, GATED, Args><<<uint32_t(ceil_div(t.rows, t.each)), kWaves * kWave, 0, stream>>>(t);
 }
 
-template <typename T, int GROUPS, bool GATED>
-void launch_thin(ThinArgs t, hipStream_t stream) {
+template <typename T, int GROUPS, bool GATED, typename Args>
+void launch_thin(Args t, hipStream_t stream) {
   t.each = rows_each(t.rows, GATED, GROUPS);
   const uint32_t blocks = ceil_div(t.each, GATED ? 8 : 16);
   if (blocks == 1) launch_blocks<T, GROUPS, 1, GATED>(t, stream);
@@ -774,12 +780,13 @@ void launch_thin(ThinArgs t, hipStream_t stream) {
   else if constexpr (GATED && GROUPS > 1) launch_blocks<T, GROUPS, 3, GATED>(t, stream);
 }
 
-template <typename T, bool GATED>
-void thin(const ThinArgs& t, hipStream_t stream) {
+template <typename T, bool GATED, typename Args>
+void thin(const Args& t, hipStream_t stream) {
+  constexpr bool kKeep = std::is_same_v<Args, ThinKept>;
   if (t.rows == 0) return;
   if (t.tokens <= 16) launch_thin<T, 1, GATED>(t, stream);
-  else if (t.tokens <= 32) launch_thin<T, 2, GATED>(t, stream);
-  else launch_thin<T, 4, GATED>(t, stream);
+  else if (kKeep || t.tokens <= 32) launch_thin<T, 2, GATED>(t, stream);
+  else if constexpr (!kKeep) launch_thin<T, 4, GATED>(t, stream);
 }
 
 Matrix matrix_x(const sr_ffn_shape& s) { return {s.x, s.tokens, s.hidden, s.x_stride}; }
@@ -793,20 +800,23 @@ int forward(const sr_ffn_shape& s, void* out, void* a, void* b, Space& space, bo
   if (s.tokens == 0) return SR_OK;
   const uint64_t wide = padded(s.ffn);
   const uint64_t h = space.take(s.tokens * wide * sizeof(T));
-  if (s.tokens <= (a ? kFewKept : kFewTokens)) {
+  const Matrix given[4] = {matrix_x(s), matrix_gate(s), matrix_up(s), matrix_down(s)};
+  auto copies = [&] { return !std::all_of(given, given + 4, [](const Matrix& m) { return loadable(m, sizeof(T)); }); };
+  if (s.tokens <= kFewTokens && (!a || (s.tokens <= kFewKept && (s.ffn <= kNarrow * s.hidden || copies())))) {
     if (!launch) return SR_OK;
     ThinArgs g{reinterpret_cast<uint64_t>(s.x), reinterpret_cast<uint64_t>(s.gate), reinterpret_cast<uint64_t>(s.up), h,
-               reinterpret_cast<uint64_t>(a), reinterpret_cast<uint64_t>(b), s.x_stride, s.gate_stride, s.up_stride,
-               uint32_t(s.tokens), uint32_t(s.ffn), uint32_t(s.hidden), uint32_t(wide), 0, s.activation};
-    thin<T, true>(g, stream);
-    ThinArgs d{h, reinterpret_cast<uint64_t>(s.down), 0, reinterpret_cast<uint64_t>(out), 0, 0, wide, s.down_stride, 0,
+               s.x_stride, s.gate_stride, s.up_stride, uint32_t(s.tokens), uint32_t(s.ffn), uint32_t(s.hidden),
+               uint32_t(wide), 0, s.activation};
+    if (a) thin<T, true>(ThinKept{g, reinterpret_cast<uint64_t>(a), reinterpret_cast<uint64_t>(b)}, stream);
+    else thin<T, true>(g, stream);
+    ThinArgs d{h, reinterpret_cast<uint64_t>(s.down), 0, reinterpret_cast<uint64_t>(out), wide, s.down_stride, 0,
                uint32_t(s.tokens), uint32_t(s.hidden), uint32_t(s.ffn), uint32_t(s.hidden), 0, 0};
     thin<T, false>(d, stream);
     return launched("sr_ffn");
   }
   Loader<T> loader{space, launch, stream};
-  const Matrix x = loader.ready(matrix_x(s)), gate = loader.ready(matrix_gate(s)), up = loader.ready(matrix_up(s)),
-               down = loader.ready(matrix_down(s));
+  const Matrix x = loader.ready(given[0]), gate = loader.ready(given[1]), up = loader.ready(given[2]),
+               down = loader.ready(given[3]);
   if (s.ffn) {
     ForwardArgs t{};
     t.p = {operand<T>(x, ROW), operand<T>(gate, ROW), {}, operand<T>(up, ROW), uint32_t(s.hidden)};

@@ -430,3 +430,12 @@ def test_large_tiles_of_floats(size, kernels):
     names = kernels_of(lambda: check(*size, F32))
     for k in kernels:
         assert any(k in n for n in names), (k, sorted(n for n in names if "kernel<" in n))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("ffn, thin", [(256, True), (264, False)])
+def test_few_kept_tokens_of_wide_blocks(ffn, thin, dtype):
+    """Rows that tiles can be loaded from: the way of few tokens up to four times as many rows as columns."""
+    check(20, 64, ffn, dtype)
+    x, g, up, d, _ = block(20, 64, ffn, dtype)
+    assert any("thin_kernel" in n for n in kernels_of(lambda: gated_ffn(x, g, up, d, keep=True))) == thin

@@ -385,9 +385,9 @@ __global__ __launch_bounds__(kPlainThreads) void align_kernel(const T* from, uin
 // Up to 64 tokens: the matrices' bytes bound it, so their rows go from memory
 // straight to the matrix cores.  A workgroup has some rows (of G and of U) for all
 // tokens; its waves share out the k, and their sums are joined in shared memory.
-// The tokens come from the L2 for every workgroup, which is what keeps more than a
-// few of them from the matrices' 6 TB/s: workgroups have as many rows as leave no
-// compute unit without work.
+// The tokens come from the L2 for every workgroup, and a wave's loads and products take
+// turns, which is what keeps more than a few tokens from the matrices' 6 TB/s: workgroups
+// have as many rows as leave no compute unit without work.
 //
 // Measured (bf16, us of both launches): 1 token, 3584 columns and 4736 rows 14.8 + 7.8
 // (15.3 at a copy's rate), 24 tokens, 4096 and 5504 22.1 + 16.2 (20.4), 64 tokens, 3584

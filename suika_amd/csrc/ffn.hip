@@ -630,7 +630,7 @@ constexpr uint64_t kMostSplits = 24;
 // slower, y 0.94 and 60 us instead of 75).  The projections and dh, whose join has the
 // activation's reads and writes to itself, 0.75: trained in bf16, dh of that shape is 0.77
 // by it and 7 us of 446 slower; 512 tokens of 4096 and 5504, projections 0.88 and 6 us of
-// 98 slower; 24 tokens of these 0.74 and 0.53, together 125 us instead of 166; 82 tokens of
+// 98 slower; 64 tokens of these 0.74 and 0.53, together 133 us instead of 172; 82 tokens of
 // 4976 columns and 168 rows in floats 0.12, the forward pass 35 us instead of 113.
 constexpr double kProductGain = 0.95, kActivatedGain = 0.75;
 
